@@ -106,6 +106,44 @@ SIGNATURES = {
         + [_i64] * 8  # po_sb po_ss po_sh lse_sb lse_ss lse_sh o_sb o_sh
         + [_ptr],  # stream
     ),
+    "dmla_kv_append_q4": (
+        _int,
+        [_ptr] * 6  # kv_pool, block_table, cache_seqlens, new_lens, new_kv, bad_index_flag
+        + [_i64] * 4  # B, n_new, num_pages, max_pages_per_seq
+        + [_i64] * 4  # kv_sp bt_sb nk_sb nk_ss
+        + [_ptr],  # stream
+    ),
+    "dmla_kv_gather_q4": (
+        _int,
+        [_ptr] * 5  # kv_pool, block_table, cache_seqlens, starts, out
+        + [_i64] * 4  # B, n_out, num_pages, max_pages_per_seq
+        + [_i64] * 4  # kv_sp bt_sb o_sb o_ss
+        + [_ptr],  # stream
+    ),
+    "dmla_decode_q4_workspace_bytes": (_i64, [_i64, _i64]),  # B H
+    "dmla_decode_paged_q4": (
+        _int,
+        [_ptr] * 6  # q, kv_pool, block_table, cache_seqlens, o, lse
+        + [_i64] * 6  # B, H, d_qk, d_v, num_pages, max_pages_per_seq
+        + [_i64] * 6  # q_sb q_sh kv_sp bt_sb o_sb o_sh
+        + [_f32, _ptr, _i64, _ptr],  # scale, workspace, workspace_bytes, stream
+    ),
+    "dmla_attn_mass": (
+        _int,
+        [_ptr] * 6  # q, kv_pool, block_table, cache_seqlens, lse, mass
+        + [_i64] * 6  # B, H, d_qk, num_pages, max_pages_per_seq, mass_len
+        + [_i64] * 6  # q_sb q_sh kv_sp kv_ss bt_sb m_sb
+        + [_int, _f32, _ptr],  # q4, scale, stream
+    ),
+    "dmla_kv_evict_workspace_bytes": (_i64, [_i64] * 6),  # B row_bytes max_pages budget recent sink
+    "dmla_kv_evict": (
+        _int,
+        [_ptr] * 8  # kv_pool, block_table, cache_seqlens, mass, new_lens, src, mass_out, bad_index_flag
+        + [_i64] * 5  # B, row_bytes, num_pages, max_pages_per_seq, mass_len
+        + [_i64] * 6  # kv_sp kv_ss bt_sb m_sb mo_sb src_sb
+        + [_i64] * 3  # budget, recent, sink
+        + [_ptr, _i64, _ptr],  # workspace, workspace_bytes, stream
+    ),
     "dmla_bwd_workspace_bytes": (_i64, [_i64] * 6 + [_int]),  # B H Sq Sk d_qk d_v causal
     "dmla_bwd_cache_latent": (
         _int,

@@ -27,6 +27,7 @@ from . import _lib
 D_QK = 576
 D_V = 512
 PAGE_SIZE = 64
+ROW_BYTES_Q4 = 400   # a 4-bit cache row: 256 bytes of codes, 16 of scales, 64 rope values in bf16
 
 
 # The calls below run in the time a small kernel takes (10-20 us), so the checks build no message and
@@ -382,6 +383,253 @@ def flash_dmla_lse_combine(
         part_lse.stride(2), o.stride(0), o.stride(1), _stream(part_o),
     )
     return (o, lse) if return_lse else o
+
+
+def _check_index(name: str, t: torch.Tensor, ndim: int) -> None:
+    if (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype is torch.int32 and t.dim() == ndim
+            and (t.is_contiguous() if ndim == 1 else t.stride(-1) == 1 or t.shape[-1] <= 1)):
+        return
+    raise ValueError(f"{name} must be a {ndim}-D int32 GPU tensor, contiguous in its last dim")
+
+
+def _check_q4_pool(t: torch.Tensor) -> None:
+    if (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype is torch.uint8 and t.dim() == 3 and t.shape[1] == PAGE_SIZE
+            and t.shape[2] == ROW_BYTES_Q4 and t.stride(2) == 1 and t.stride(1) == ROW_BYTES_Q4):
+        return
+    raise ValueError(f"a 4-bit kv_pool must be a [num_pages, {PAGE_SIZE}, {ROW_BYTES_Q4}] uint8 GPU tensor whose rows "
+                     "follow each other")
+
+
+def _check_tables(block_table: torch.Tensor, cache_seqlens: torch.Tensor, B: int) -> None:
+    _check_index("block_table", block_table, 2)
+    _check_index("cache_seqlens", cache_seqlens, 1)
+    if block_table.shape[0] != B or cache_seqlens.shape[0] != B:
+        raise ValueError("batch size mismatch")
+
+
+def _check_page_indices(block_table: torch.Tensor, cache_seqlens: torch.Tensor, num_pages: int) -> None:
+    """Raises unless every length fits the table and every page in use exists (one device sync)."""
+    sl = cache_seqlens.cpu().long()
+    bt = block_table.cpu().long()
+    _require(bool((sl >= 0).all()), "cache_seqlens must be >= 0")
+    _require(bool((sl <= bt.shape[1] * PAGE_SIZE).all()), "a cache_seqlens entry exceeds the block table capacity")
+    used = torch.arange(bt.shape[1])[None, :] * PAGE_SIZE < sl[:, None]
+    _require(bool(((bt >= 0) & (bt < num_pages))[used].all()), f"block_table holds a page index outside [0, {num_pages})")
+
+
+@_on_tensor_device
+def flash_dmla_kv_append_q4(
+    kv_pool: torch.Tensor,
+    block_table: torch.Tensor,
+    cache_seqlens: torch.Tensor,
+    new_kv: torch.Tensor,
+    new_lens: Optional[torch.Tensor] = None,
+    check_indices: bool = False,
+) -> None:
+    """flash_dmla_kv_append into 4-bit pages: quantises new latent rows and writes them in place.
+
+    kv_pool [num_pages, 64, 400] uint8; the other arguments as for flash_dmla_kv_append, new_kv
+    [B, n_new, 576] bf16.  The 512 latent values become e2m1 codes with a power-of-two scale for
+    each 32 (include/flashdmla.h), the 64 rope values stay bf16.
+    """
+    _check_q4_pool(kv_pool)
+    _check_bf16("new_kv", new_kv, 3)
+    B, n_new, d = new_kv.shape
+    if d != D_QK:
+        raise ValueError(f"new_kv rows must hold {D_QK} values, got {d}")
+    _check_tables(block_table, cache_seqlens, B)
+    if new_lens is not None:
+        _check_index("new_lens", new_lens, 1)
+        _require(new_lens.shape[0] == B, "new_lens must hold B entries")
+    _same_device(kv_pool=kv_pool, block_table=block_table, cache_seqlens=cache_seqlens, new_kv=new_kv, new_lens=new_lens)
+    flag = torch.zeros(1, dtype=torch.int32, device=kv_pool.device) if check_indices else None
+    _lib.call(
+        "dmla_kv_append_q4",
+        _ptr(kv_pool), _ptr(block_table), _ptr(cache_seqlens), _ptr(new_lens), _ptr(new_kv), _ptr(flag),
+        B, n_new, kv_pool.shape[0], block_table.shape[1], kv_pool.stride(0), block_table.stride(0),
+        new_kv.stride(0), new_kv.stride(1), _stream(kv_pool),
+    )
+    if check_indices:
+        _require(int(flag.item()) == 0, "kv append: a row's page slot or page index was out of range (row skipped)")
+
+
+@_on_tensor_device
+def flash_dmla_kv_gather_q4(
+    kv_pool: torch.Tensor,
+    block_table: torch.Tensor,
+    cache_seqlens: torch.Tensor,
+    max_len: int,
+    starts: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """Reads 4-bit pages back as dense rows: [B, max_len, 576] bf16, what flash_dmla_fwd takes as k_lat.
+
+    Row i of sequence b is the token at starts[b] + i (starts [B] int32, zeros when None); rows at or
+    past cache_seqlens[b] are zeros, rows on a page outside the pool are NaN.
+    """
+    _check_q4_pool(kv_pool)
+    B = cache_seqlens.shape[0]
+    _check_tables(block_table, cache_seqlens, B)
+    if starts is not None:
+        _check_index("starts", starts, 1)
+        _require(starts.shape[0] == B, "starts must hold B entries")
+    _require(max_len >= 0, "max_len must be >= 0")
+    _same_device(kv_pool=kv_pool, block_table=block_table, cache_seqlens=cache_seqlens, starts=starts)
+    out = torch.empty((B, max_len, D_QK), dtype=torch.bfloat16, device=kv_pool.device)
+    if out.numel() == 0:
+        return out
+    _lib.call(
+        "dmla_kv_gather_q4",
+        _ptr(kv_pool), _ptr(block_table), _ptr(cache_seqlens), _ptr(starts), _ptr(out),
+        B, max_len, kv_pool.shape[0], block_table.shape[1], kv_pool.stride(0), block_table.stride(0),
+        out.stride(0), out.stride(1), _stream(kv_pool),
+    )
+    return out
+
+
+@_on_tensor_device
+def flash_dmla_decode_paged_q4(
+    q: torch.Tensor,
+    kv_pool: torch.Tensor,
+    block_table: torch.Tensor,
+    cache_seqlens: torch.Tensor,
+    d_v: int = D_V,
+    softmax_scale: Optional[float] = None,
+    return_lse: bool = False,
+    check_indices: bool = False,
+):
+    """flash_dmla_decode_paged over 4-bit pages: kv_pool [num_pages, 64, 400] uint8.
+
+    q [B, H, 576] bf16; block_table [B, max_pages] int32; cache_seqlens [B] int32.  Returns o
+    [B, H, d_v] bf16 (and lse [B, H] fp32 natural log with return_lse): attention over exactly the
+    values that flash_dmla_kv_gather_q4 reads back.  Empty sequences give o = 0 and lse = -inf, a
+    sequence with a page outside the pool NaN (check_indices=True raises instead, one device sync).
+    """
+    _check_bf16("q", q, 3)
+    _check_q4_pool(kv_pool)
+    B, H, Dqk = q.shape
+    _check_tables(block_table, cache_seqlens, B)
+    _same_device(q=q, kv_pool=kv_pool, block_table=block_table, cache_seqlens=cache_seqlens)
+    if check_indices:
+        _check_page_indices(block_table, cache_seqlens, kv_pool.shape[0])
+    o = torch.empty((B, H, d_v), dtype=torch.bfloat16, device=q.device)
+    lse = torch.empty((B, H), dtype=torch.float32, device=q.device) if return_lse else None
+    ws_bytes = int(_lib.lib().dmla_decode_q4_workspace_bytes(B, H))
+    ws = torch.empty((max(ws_bytes, 1),), dtype=torch.uint8, device=q.device)
+    _lib.call(
+        "dmla_decode_paged_q4",
+        _ptr(q), _ptr(kv_pool), _ptr(block_table), _ptr(cache_seqlens), _ptr(o), _ptr(lse),
+        B, H, Dqk, d_v, kv_pool.shape[0], block_table.shape[1],
+        q.stride(0), q.stride(1), kv_pool.stride(0), block_table.stride(0), o.stride(0), o.stride(1),
+        _scale(softmax_scale, Dqk), _ptr(ws), ws_bytes, _stream(q),
+    )
+    return (o, lse) if return_lse else o
+
+
+def _check_pool(kv_pool: torch.Tensor) -> Tuple[int, int, int]:
+    """(row bytes, page stride, row stride in bytes) of a bf16 or 4-bit pool."""
+    if isinstance(kv_pool, torch.Tensor) and kv_pool.dtype is torch.uint8:
+        _check_q4_pool(kv_pool)
+        return ROW_BYTES_Q4, kv_pool.stride(0), ROW_BYTES_Q4
+    _check_bf16("kv_pool", kv_pool, 3)
+    if kv_pool.shape[1] != PAGE_SIZE:
+        raise ValueError(f"page size must be {PAGE_SIZE}, got {kv_pool.shape[1]}")
+    return 2 * kv_pool.shape[2], 2 * kv_pool.stride(0), 2 * kv_pool.stride(1)
+
+
+def _check_mass(mass: torch.Tensor, B: int, max_pages: int) -> None:
+    if not (isinstance(mass, torch.Tensor) and mass.is_cuda and mass.dtype is torch.float32 and mass.dim() == 2
+            and mass.shape[0] == B and mass.shape[1] >= max_pages * PAGE_SIZE and mass.stride(1) == 1):
+        raise ValueError(f"mass must be a [B, >= {max_pages * PAGE_SIZE}] float32 GPU tensor, contiguous in its last dim")
+
+
+@_on_tensor_device
+def flash_dmla_attn_mass(
+    q: torch.Tensor,
+    kv_pool: torch.Tensor,
+    block_table: torch.Tensor,
+    cache_seqlens: torch.Tensor,
+    lse: torch.Tensor,
+    mass: torch.Tensor,
+    softmax_scale: Optional[float] = None,
+) -> None:
+    """Adds the attention weight that a decode step gave each cached token to its account, in place:
+    mass[b, t] += sum_h exp(scale * q[b, h] . k[b, t] - lse[b, h]) for t < cache_seqlens[b].
+
+    q, block_table, cache_seqlens and softmax_scale as the step's decode took them; lse [B, H] as it
+    returned it; kv_pool its bf16 [num_pages, 64, 576] or 4-bit [num_pages, 64, 400] pages; mass
+    [B, >= 64 * max_pages] fp32.  Heads with lse = -inf add nothing, and tokens on a page outside the pool get
+    nothing.  Deterministic.
+    """
+    _check_bf16("q", q, 3)
+    row_bytes, kv_sp, kv_ss = _check_pool(kv_pool)
+    B, H, Dqk = q.shape
+    q4 = kv_pool.dtype is torch.uint8
+    if not q4 and kv_pool.shape[2] != Dqk:
+        raise ValueError(f"kv_pool last dim {kv_pool.shape[2]} != q last dim {Dqk}")
+    _check_tables(block_table, cache_seqlens, B)
+    if not (isinstance(lse, torch.Tensor) and lse.dtype is torch.float32 and lse.is_cuda and lse.is_contiguous()
+            and tuple(lse.shape) == (B, H)):
+        raise ValueError("lse must be a contiguous [B, H] float32 GPU tensor")
+    _check_mass(mass, B, block_table.shape[1])
+    _same_device(q=q, kv_pool=kv_pool, block_table=block_table, cache_seqlens=cache_seqlens, lse=lse, mass=mass)
+    _lib.call(
+        "dmla_attn_mass",
+        _ptr(q), _ptr(kv_pool), _ptr(block_table), _ptr(cache_seqlens), _ptr(lse), _ptr(mass),
+        B, H, Dqk, kv_pool.shape[0], block_table.shape[1], mass.shape[1],
+        q.stride(0), q.stride(1), kv_sp, kv_ss, block_table.stride(0), mass.stride(0),
+        1 if q4 else 0, _scale(softmax_scale, Dqk), _stream(q),
+    )
+
+
+@_on_tensor_device
+def flash_dmla_kv_evict(
+    kv_pool: torch.Tensor,
+    block_table: torch.Tensor,
+    cache_seqlens: torch.Tensor,
+    mass: torch.Tensor,
+    budget: int,
+    recent: int = 0,
+    sink: int = 0,
+    check_indices: bool = False,
+) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Cuts every sequence longer than `budget` tokens back to it and compacts its pages in place.
+
+    kv_pool bf16 [num_pages, 64, d] or 4-bit [num_pages, 64, 400]; mass [B, >= 64 * max_pages] fp32
+    (flash_dmla_attn_mass).  The first `sink` and the newest `recent` tokens stay, and of the others
+    those with the largest mass (the lower index first among equals).  Returns
+      new_lens [B] int32 -- the lengths to go on with (cache_seqlens is not changed);
+      src [B, min(budget, 64 * max_pages)] int32 -- the old index of the token at each place, -1 past the end;
+      new_mass -- mass moved like the rows, 0 past the end.
+    The newest tokens keep their order and come last; among the others rows move only to fill gaps
+    (include/flashdmla.h), which attention does not see.  A page may belong to one sequence only.
+    check_indices=True raises (one device sync) when a sequence was left alone because one of its page indices
+    is outside the pool.
+    """
+    row_bytes, kv_sp, kv_ss = _check_pool(kv_pool)
+    B = cache_seqlens.shape[0]
+    _check_tables(block_table, cache_seqlens, B)
+    max_pages = block_table.shape[1]
+    _check_mass(mass, B, max_pages)
+    if not (budget > 0 and recent >= 0 and sink >= 0 and recent + sink <= budget):
+        raise ValueError("budget must be positive and cover recent + sink")
+    _same_device(kv_pool=kv_pool, block_table=block_table, cache_seqlens=cache_seqlens, mass=mass)
+    width = min(budget, max_pages * PAGE_SIZE)
+    new_lens = torch.empty((B,), dtype=torch.int32, device=mass.device)
+    src = torch.empty((B, width), dtype=torch.int32, device=mass.device)
+    new_mass = torch.empty((B, mass.shape[1]), dtype=torch.float32, device=mass.device)
+    flag = torch.zeros(1, dtype=torch.int32, device=mass.device) if check_indices else None
+    ws_bytes = int(_lib.lib().dmla_kv_evict_workspace_bytes(B, row_bytes, max_pages, budget, recent, sink))
+    ws = torch.empty((max(ws_bytes, 1),), dtype=torch.uint8, device=mass.device)
+    _lib.call(
+        "dmla_kv_evict",
+        _ptr(kv_pool), _ptr(block_table), _ptr(cache_seqlens), _ptr(mass), _ptr(new_lens), _ptr(src), _ptr(new_mass),
+        _ptr(flag), B, row_bytes, kv_pool.shape[0], max_pages, mass.shape[1],
+        kv_sp, kv_ss, block_table.stride(0), mass.stride(0), new_mass.stride(0), src.stride(0),
+        budget, recent, sink, _ptr(ws), ws_bytes, _stream(mass),
+    )
+    if check_indices:
+        _require(int(flag.item()) == 0, "kv evict: a sequence has a page index outside the pool (left as it was)")
+    return new_lens, src, new_mass
 
 
 class FlashDMLACacheLatent(torch.autograd.Function):

@@ -17,6 +17,12 @@ matching backward op.  Only GPU tensors have a kernel: CPU tensors raise, as eve
         -> (o, lse)
     torch.ops.flashdmla.kv_append(kv_pool, block_table, cache_seqlens, new_kv, new_lens) -> ()   (kv_pool in place)
     torch.ops.flashdmla.lse_combine(part_o, part_lse, num_splits) -> (o, lse)
+    torch.ops.flashdmla.kv_append_q4(kv_pool, block_table, cache_seqlens, new_kv, new_lens) -> ()   (kv_pool in place)
+    torch.ops.flashdmla.kv_gather_q4(kv_pool, block_table, cache_seqlens, max_len, starts) -> rows
+    torch.ops.flashdmla.decode_paged_q4(q, kv_pool, block_table, cache_seqlens, d_v, softmax_scale) -> (o, lse)
+    torch.ops.flashdmla.attn_mass(q, kv_pool, block_table, cache_seqlens, lse, mass, softmax_scale) -> ()   (mass in place)
+    torch.ops.flashdmla.kv_evict(kv_pool, block_table, cache_seqlens, mass, budget, recent, sink)
+        -> (new_lens, src, new_mass)   (kv_pool in place)
 
 Shapes and conventions are those of python/ops.py.  m and l are outputs without a gradient;
 the backwards return dk_lat and dwk / dwv in float32 (the autograd formulas cast them to the
@@ -175,3 +181,63 @@ def lse_combine(part_o: Tensor, part_lse: Tensor, num_splits: Optional[Tensor]) 
 def _(part_o, part_lse, num_splits):
     B, _, H, d = part_o.shape
     return part_o.new_empty((B, H, d), dtype=_BF16), part_o.new_empty((B, H), dtype=_F32)
+
+
+# ---- the 4-bit cache, the accounts of attention weight and the eviction ------------------------
+@custom_op("flashdmla::kv_append_q4", mutates_args=("kv_pool",), device_types="cuda")
+def kv_append_q4(kv_pool: Tensor, block_table: Tensor, cache_seqlens: Tensor, new_kv: Tensor,
+                 new_lens: Optional[Tensor]) -> None:
+    ops.flash_dmla_kv_append_q4(kv_pool, block_table, cache_seqlens, new_kv, new_lens)
+
+
+@kv_append_q4.register_fake
+def _(kv_pool, block_table, cache_seqlens, new_kv, new_lens):
+    return None
+
+
+@custom_op("flashdmla::kv_gather_q4", mutates_args=(), device_types="cuda")
+def kv_gather_q4(kv_pool: Tensor, block_table: Tensor, cache_seqlens: Tensor, max_len: int,
+                 starts: Optional[Tensor]) -> Tensor:
+    return ops.flash_dmla_kv_gather_q4(kv_pool, block_table, cache_seqlens, max_len, starts)
+
+
+@kv_gather_q4.register_fake
+def _(kv_pool, block_table, cache_seqlens, max_len, starts):
+    return kv_pool.new_empty((cache_seqlens.shape[0], max_len, ops.D_QK), dtype=_BF16)
+
+
+@custom_op("flashdmla::decode_paged_q4", mutates_args=(), device_types="cuda")
+def decode_paged_q4(q: Tensor, kv_pool: Tensor, block_table: Tensor, cache_seqlens: Tensor, d_v: int,
+                    softmax_scale: Optional[float]) -> Tuple[Tensor, Tensor]:
+    o, lse = ops.flash_dmla_decode_paged_q4(q, kv_pool, block_table, cache_seqlens, d_v, softmax_scale, return_lse=True)
+    return o, lse
+
+
+@decode_paged_q4.register_fake
+def _(q, kv_pool, block_table, cache_seqlens, d_v, softmax_scale):
+    B, H, _ = q.shape
+    return q.new_empty((B, H, d_v), dtype=_BF16), q.new_empty((B, H), dtype=_F32)
+
+
+@custom_op("flashdmla::attn_mass", mutates_args=("mass",), device_types="cuda")
+def attn_mass(q: Tensor, kv_pool: Tensor, block_table: Tensor, cache_seqlens: Tensor, lse: Tensor, mass: Tensor,
+              softmax_scale: Optional[float]) -> None:
+    ops.flash_dmla_attn_mass(q, kv_pool, block_table, cache_seqlens, lse, mass, softmax_scale)
+
+
+@attn_mass.register_fake
+def _(q, kv_pool, block_table, cache_seqlens, lse, mass, softmax_scale):
+    return None
+
+
+@custom_op("flashdmla::kv_evict", mutates_args=("kv_pool",), device_types="cuda")
+def kv_evict(kv_pool: Tensor, block_table: Tensor, cache_seqlens: Tensor, mass: Tensor, budget: int, recent: int,
+             sink: int) -> Tuple[Tensor, Tensor, Tensor]:
+    return ops.flash_dmla_kv_evict(kv_pool, block_table, cache_seqlens, mass, budget, recent, sink)
+
+
+@kv_evict.register_fake
+def _(kv_pool, block_table, cache_seqlens, mass, budget, recent, sink):
+    B, width = mass.shape[0], min(budget, block_table.shape[1] * ops.PAGE_SIZE)
+    return (cache_seqlens.new_empty((B,), dtype=torch.int32), cache_seqlens.new_empty((B, width), dtype=torch.int32),
+            mass.new_empty((B, mass.shape[1])))

@@ -242,6 +242,105 @@ int dmla_lse_combine(const float* part_o, const float* part_lse, const int32_t* 
                      int64_t o_sb, int64_t o_sh, dmla_stream_t stream);
 
 /*
+ * The 4-bit paged latent cache.  No reference counterpart.
+ *
+ *   kv_pool [num_pages, 64, 400] uint8, the rows of a page following each other, page stride kv_sp
+ *   bytes (a multiple of 16).  A row is one token:
+ *     bytes 0..255    e2m1 codes of its 512 latent values, value 2i in the low half of byte i (sign in
+ *                     bit 3; 0, 0.5, 1, 1.5, 2, 3, 4, 6)
+ *     bytes 256..271  a scale byte for each 32 values: 2^(byte - 127); 255: not a number
+ *     bytes 272..399  its 64 rope values in bf16
+ *   A value is code x scale, exact in bf16; the page tables are those of dmla_decode_paged.
+ *
+ * Append: new_kv [B, n_new, 576] bf16, strides (nk_sb, nk_ss), else as dmla_kv_append with
+ * page_size = 64.  A block's scale is the least power of two with which none of its values exceeds 6
+ * (2^-125 at least, 2^125 at most), its values are rounded to the nearest code, the even one when two
+ * are as near; a block that holds an infinity or a NaN reads back as NaN.  Of rows that land in one place (two table
+ * entries with the same page), any one byte may be any of theirs.
+ *
+ * Gather: out [B, n_out, 576] bf16, strides (o_sb, o_ss).  Row i of sequence b is the value of the
+ * token at starts[b] + i (starts NULL: i; negative: 0), zeros at or past cache_seqlens[b] (at most
+ * 64 max_pages_per_seq), NaN where the token's page index is outside [0, num_pages).
+ */
+int dmla_kv_append_q4(void* kv_pool, const int32_t* block_table, const int32_t* cache_seqlens,
+                      const int32_t* new_lens, const void* new_kv, int32_t* bad_index_flag, int64_t B,
+                      int64_t n_new, int64_t num_pages, int64_t max_pages_per_seq, int64_t kv_sp,
+                      int64_t bt_sb, int64_t nk_sb, int64_t nk_ss, dmla_stream_t stream);
+int dmla_kv_gather_q4(const void* kv_pool, const int32_t* block_table, const int32_t* cache_seqlens,
+                      const int32_t* starts, void* out, int64_t B, int64_t n_out, int64_t num_pages,
+                      int64_t max_pages_per_seq, int64_t kv_sp, int64_t bt_sb, int64_t o_sb,
+                      int64_t o_ss, dmla_stream_t stream);
+
+/*
+ * dmla_decode_paged over 4-bit pages: same arguments, results and treatment of lengths and page
+ * indices, without the page and row sizes (64 tokens of 400 bytes).
+ *   Codes become bf16 values exactly; scores are bf16 products summed in fp32, the probabilities enter
+ *   the value product as bf16, and the parts of a sequence that is split are rounded to bf16.
+ * The workspace (16-byte aligned, contents ignored) holds the partial outputs; its size depends on
+ * the current device.  Supported: d_qk = 576, d_v = 512.
+ */
+int64_t dmla_decode_q4_workspace_bytes(int64_t B, int64_t H);
+int dmla_decode_paged_q4(const void* q, const void* kv_pool, const int32_t* block_table,
+                         const int32_t* cache_seqlens, void* o, float* lse, int64_t B, int64_t H,
+                         int64_t d_qk, int64_t d_v, int64_t num_pages, int64_t max_pages_per_seq,
+                         int64_t q_sb, int64_t q_sh, int64_t kv_sp, int64_t bt_sb, int64_t o_sb,
+                         int64_t o_sh, float softmax_scale, void* workspace, int64_t workspace_bytes,
+                         dmla_stream_t stream);
+
+/*
+ * Accounts of attention weight: mass[b, t] += sum_h exp(softmax_scale q[b, h] . k[b, t] - lse[b, h])
+ * for the tokens t < cache_seqlens[b] (at most 64 max_pages_per_seq), from a decode step's queries and
+ * its log-sum-exps.  No reference counterpart.
+ *
+ *   q        [B, H, 576] bf16   strides (q_sb, q_sh)
+ *   kv_pool  pages of 64 tokens, bf16 rows of 576 (q4 = 0) or 4-bit rows of 400 bytes (q4 != 0, rows
+ *            following each other); strides (kv_sp, kv_ss) in BYTES, multiples of 16
+ *   lse      [B, H] fp32 contiguous, as dmla_decode_paged[_q4] wrote it; a head with lse = -inf adds 0
+ *   mass     [B, mass_len] fp32 row stride m_sb, mass_len >= 64 max_pages_per_seq; added to in place,
+ *            untouched from the sequence's length on and for tokens whose page index is outside
+ *            [0, num_pages)
+ * The result is deterministic (no atomics).  Sequences may share pages.
+ */
+int dmla_attn_mass(const void* q, const void* kv_pool, const int32_t* block_table,
+                   const int32_t* cache_seqlens, const float* lse, float* mass, int64_t B, int64_t H,
+                   int64_t d_qk, int64_t num_pages, int64_t max_pages_per_seq, int64_t mass_len,
+                   int64_t q_sb, int64_t q_sh, int64_t kv_sp, int64_t kv_ss, int64_t bt_sb, int64_t m_sb,
+                   int q4, float softmax_scale, dmla_stream_t stream);
+
+/*
+ * Eviction from a paged cache by accumulated attention weight, in place.  No reference counterpart.
+ *
+ * A sequence of N = cache_seqlens[b] tokens (at most 64 max_pages_per_seq) above `budget` keeps its
+ * first `sink` tokens, its newest `recent`, and of those between the budget - sink - recent with the
+ * largest mass (the lower index first among equals, -0 equal to 0, NaN above everything).  In the
+ * pages the first `sink` rows stay; a kept row between them and place budget - recent stays; the
+ * other kept rows, in order, fill the places left there, in order; the newest rows follow in order.
+ * Rows from `budget` on are left as they were.  Sequences within the budget are untouched, and so is one
+ * with a page index outside [0, num_pages) among its pages (*bad_index_flag is then set to 1).
+ *
+ *   kv_pool   pages of 64 tokens of row_bytes bytes (a multiple of 16: 1152 for bf16 rows of 576, 400
+ *             for 4-bit ones); strides (kv_sp, kv_ss) in BYTES, multiples of 16.  A page may belong to one
+ *             sequence only.
+ *   mass      [B, mass_len] fp32 row stride m_sb, mass_len >= 64 max_pages_per_seq
+ *   new_lens  [B] int32: min(N, budget), or N where the sequence was left alone (cache_seqlens is not changed)
+ *   src       [B, min(budget, 64 max_pages_per_seq)] int32 row stride src_sb: the old index of the
+ *             token at each place, -1 from new_lens[b] on
+ *   mass_out  [B, mass_len] fp32 row stride mo_sb: mass moved like the rows, 0 from new_lens[b] on;
+ *             must not overlap mass
+ *   bad_index_flag  int32 device word; may be NULL; the caller clears it
+ *   workspace dmla_kv_evict_workspace_bytes bytes, 16-byte aligned, contents ignored
+ */
+int64_t dmla_kv_evict_workspace_bytes(int64_t B, int64_t row_bytes, int64_t max_pages_per_seq,
+                                      int64_t budget, int64_t recent, int64_t sink);
+int dmla_kv_evict(void* kv_pool, const int32_t* block_table, const int32_t* cache_seqlens,
+                  const float* mass, int32_t* new_lens, int32_t* src, float* mass_out,
+                  int32_t* bad_index_flag, int64_t B, int64_t row_bytes, int64_t num_pages,
+                  int64_t max_pages_per_seq, int64_t mass_len, int64_t kv_sp, int64_t kv_ss,
+                  int64_t bt_sb, int64_t m_sb, int64_t mo_sb, int64_t src_sb, int64_t budget,
+                  int64_t recent, int64_t sink, void* workspace, int64_t workspace_bytes,
+                  dmla_stream_t stream);
+
+/*
  * Cache-latent DMLA backward from the forward's saved statistics.
  * Replaces: fa2_backward (csrc/attention/fa2_bwd.cu:319-356, math of :198-310) specialised
  * to the cache-latent mode of README.md:12,15 -- the role of the absent

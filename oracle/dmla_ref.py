@@ -401,3 +401,101 @@ def dmla_grads_autograd(q: Tensor, k_lat: Tensor, do: Tensor, d_v: int, scale: O
     o, _, _ = dmla_fwd_cache_latent(qx, kx, d_v, scale, causal, dtype)
     (o * do.to(dtype)).sum().backward()
     return qx.grad, kx.grad
+
+
+# ---- the 4-bit latent cache, the accounts of attention weight and the eviction ------------------
+E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+
+
+def q4_pack(x: Tensor) -> Tensor:
+    """bf16 rows [..., 576] as 4-bit rows [..., 400] uint8 (no reference counterpart).
+
+    Each block of 32 of the 512 latent values: the scale is the least 2^e, -125 <= e <= 125, with
+    6 2^e >= max |x| (125 where there is none), the code the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 (the
+    even code of two as near; past 6: 6) with the sign in bit 3.  Bytes: 256 of codes (value 2i
+    low), 16 of e + 127 (255 and zero codes for a block with an infinity or a NaN), 64 rope values."""
+    lat = x[..., :512].double().reshape(-1, 16, 32)
+    rows = lat.shape[0]
+    codes = torch.zeros(rows, 16, 32, dtype=torch.uint8)
+    scales = torch.zeros(rows, 16, dtype=torch.uint8)
+    finite = torch.isfinite(lat).all(-1)
+    safe = torch.where(finite[..., None], lat, torch.zeros_like(lat))
+    top = safe.abs().amax(-1)
+    exps = torch.arange(-125, 126, dtype=torch.float64)
+    fits = 6.0 * torch.exp2(exps) >= top[..., None]
+    e = torch.where(fits.any(-1), fits.to(torch.uint8).argmax(-1), torch.tensor(250)).double() - 125.0
+    y = safe.abs() / torch.exp2(e)[..., None]
+    even_first = torch.tensor([0, 2, 4, 6, 1, 3, 5, 7])
+    dist = (y[..., None] - torch.tensor(E2M1, dtype=torch.float64)[even_first]).abs()
+    codes = even_first[dist.argmin(-1)] + 8 * torch.signbit(safe)
+    scales = torch.where(finite, e + 127.0, torch.tensor(255.0, dtype=torch.float64)).to(torch.uint8)
+    codes = torch.where(finite[..., None], codes, torch.zeros_like(codes)).to(torch.uint8).reshape(rows, 512)
+    packed = codes[:, 0::2] | (codes[:, 1::2] << 4)
+    rope = x[..., 512:].reshape(rows, 64).contiguous().view(torch.uint8)
+    return torch.cat((packed, scales, rope), dim=1).reshape(*x.shape[:-1], 400)
+
+
+def q4_unpack(rows: Tensor, dtype: torch.dtype = torch.float64) -> Tensor:
+    """4-bit rows [..., 400] as the values [..., 576] that they stand for."""
+    flat = rows.reshape(-1, 400)
+    lut = torch.tensor(E2M1 + tuple(-v for v in E2M1), dtype=torch.float64, device=rows.device)
+    lat = torch.empty(flat.shape[0], 512, dtype=torch.float64, device=rows.device)
+    lat[:, 0::2] = lut[(flat[:, :256] & 15).long()]
+    lat[:, 1::2] = lut[(flat[:, :256] >> 4).long()]
+    sb = flat[:, 256:272].long()
+    scale = torch.where(sb == 255, torch.full(sb.shape, float("nan"), dtype=torch.float64, device=rows.device),
+                        torch.exp2(sb.double() - 127.0))
+    lat = (lat.reshape(-1, 16, 32) * scale[..., None]).reshape(-1, 512)
+    rope = flat[:, 272:].contiguous().view(torch.bfloat16).double()
+    return torch.cat((lat, rope), dim=1).reshape(*rows.shape[:-1], 576).to(dtype)
+
+
+def attn_mass(q: Tensor, kv_pool: Tensor, block_table: Tensor, cache_seqlens: Tensor, lse: Tensor, mass: Tensor,
+              scale: float) -> Tensor:
+    """mass[b, t] + sum_h exp(scale q[b, h] . k[b, t] - lse[b, h]) in float64; heads with lse = -inf add 0."""
+    out = mass.double().clone()
+    for b in range(q.shape[0]):
+        n = int(cache_seqlens[b])
+        k = gather_pages(kv_pool, block_table[b], n, kv_pool.shape[1])
+        k = q4_unpack(k) if k.dtype == torch.uint8 else k.double()
+        heads = ~torch.isneginf(lse[b])
+        s = q[b].double()[heads] @ k.T * scale
+        out[b, :n] += torch.exp(s - lse[b].double()[heads][:, None]).sum(0)
+    return out
+
+
+def kv_evict_order(mass: Tensor, n: int, budget: int, recent: int, sink: int):
+    """The old index of the token at each place after the eviction of one sequence of n tokens."""
+    if n <= budget:
+        return list(range(n))
+    import math as _m
+    val = [float(v) for v in mass[:n]]
+    rank = [(0 if _m.isnan(v) else 1, 0.0 if _m.isnan(v) else -v, t) for t, v in enumerate(val)]
+    low_end = budget - recent
+    stay = set(sorted(range(sink, n - recent), key=lambda t: rank[t])[:low_end - sink])
+    at = list(range(low_end))
+    free = [t for t in range(sink, low_end) if t not in stay]
+    late = [t for t in range(low_end, n - recent) if t in stay]
+    for place, t in zip(free, late):
+        at[place] = t
+    return at + list(range(n - recent, n))
+
+
+def kv_evict(kv_pool: Tensor, block_table: Tensor, cache_seqlens: Tensor, mass: Tensor, budget: int, recent: int, sink: int):
+    """(pool, new_lens, src, mass) after the eviction: see kv_evict_order; rows from the budget on stay."""
+    pool, new_mass = kv_pool.clone(), torch.zeros_like(mass)
+    B, page = mass.shape[0], kv_pool.shape[1]
+    width = min(budget, block_table.shape[1] * page)
+    new_lens = torch.zeros(B, dtype=torch.int32)
+    src = torch.full((B, width), -1, dtype=torch.int32)
+    for b in range(B):
+        n = int(cache_seqlens[b])
+        at = kv_evict_order(mass[b], n, budget, recent, sink)
+        new_lens[b] = len(at)
+        src[b, :len(at)] = torch.tensor(at, dtype=torch.int32)
+        new_mass[b, :len(at)] = mass[b, torch.tensor(at, dtype=torch.long)]
+        rows = gather_pages(kv_pool, block_table[b], n, page)
+        for i, t in enumerate(at):
+            if i != t:
+                pool[int(block_table[b, i // page]), i % page] = rows[t]
+    return pool, new_lens, src, new_mass
