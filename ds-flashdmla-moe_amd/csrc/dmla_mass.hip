@@ -7,9 +7,10 @@
 // 128 heads the rows' bytes bound it (1152 bytes at 6.2 TB/s 0.19 ns, 147 kflop at 2.1 PFLOP/s 0.07 ns).
 // One workgroup of four waves per CU streams key tiles through LDS; a wave holds up to 32 heads' queries
 // in registers as the MFMA's row operand, keys are its columns, so a lane ends with one key's scores of
-// 4 heads per block and the sum over heads is in-lane adds and two lane swaps.  Every token belongs to
+// 16 heads and the sum over heads is in-lane adds and a lane swap.  Every token belongs to
 // one workgroup and its sum to one thread: no atomics, the same bits every time.
 #include <algorithm>
+#include <type_traits>
 
 #include "dmla_host.h"
 #include "dmla_q4.h"
@@ -41,60 +42,57 @@ template <bool kQ4>
 struct Tile {
   static constexpr int kTokens = kQ4 ? 64 : 32;
   static constexpr int kBytes = kQ4 ? kTokens * kQ4RowBytes : 9 * kGroupBytes;
-  static constexpr int kBlocks = kTokens / 16;
+  static constexpr int kBlocks = kTokens / 32;
   static constexpr int kSlots = kQ4 ? 5 : 3;
   static constexpr int kCost = kQ4 ? 3 : 4;   // a segment's start and end, in tiles
 };
 
+// One step of the score product of 32 heads (rows) with 32 keys: the query operand, and the keys' from
+// the tile's rows 32 kb .. +31.
+__device__ __forceinline__ bf16x8 query_operand_bf16(const bf16* q, int hl, int c) {
+  return *reinterpret_cast<const bf16x8*>(q + 16 * c + 8 * hl);
+}
 template <bool kQ4>
-struct Query;
-template <>
-struct Query<true> {
-  bf16x8 v[kQ4KeySteps];
-  __device__ __forceinline__ void load(const bf16* q, int g) { q4_load_query(q, g, v); }
-  // S[head 4 g + i][key l16] of the 16 keys from row block kb of the tile.
-  __device__ __forceinline__ f32x4 scores(const DMLA_LDS char* tile, int kb, int lane) const {
-    Q4Key key;
-    key.load(tile + (16 * kb + (lane & 15)) * kQ4RowBytes, lane >> 4);
-    f32x4 s = {0.f, 0.f, 0.f, 0.f};
-    step<0>(key, s);
-    step<1>(key, s);
-    step<2>(key, s);
-    step<3>(key, s);
-    s = mfma_bf16(v[16], key.rope[0], s);
-    return mfma_bf16(v[17], key.rope[1], s);
-  }
-  template <int kA>
-  __device__ __forceinline__ void step(const Q4Key& key, f32x4& s) const {
-    bf16x8 k[4];
-    key.octets<kA>(k);
+__device__ __forceinline__ f32x16 scores(const bf16x8 (&q)[kQ4Steps], const DMLA_LDS char* tile, int kb, int lane) {
+  const int l32 = lane & 31, hl = lane >> 5;
+  f32x16 s;
 #pragma unroll
-    for (int b = 0; b < 4; ++b) s = mfma_bf16(v[4 * kA + b], k[b], s);
-  }
-};
-template <>
-struct Query<false> {
-  bf16x8 v[18];
-  __device__ __forceinline__ void load(const bf16* q, int g) {
+  for (int i = 0; i < 16; ++i) s[i] = 0.f;
+  if constexpr (kQ4) {
+    const DMLA_LDS char* row = tile + (32 * kb + l32) * kQ4RowBytes;
+    const u32x2 scales = q4_key_scales(row, hl);
+    auto block = [&](auto a_tag) {
+      constexpr int kA = decltype(a_tag)::value;
+      const u32x4 w = q4_key_codes(row, hl, kA);
+      const float sc = q4_key_scale<kA>(scales);
 #pragma unroll
-    for (int c = 0; c < 18; ++c) v[c] = *reinterpret_cast<const bf16x8*>(q + 32 * c + 8 * g);
-  }
-  __device__ __forceinline__ f32x4 scores(const DMLA_LDS char* tile, int kb, int lane) const {
-    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+      for (int j = 0; j < 4; ++j) s = mfma32_bf16(q[4 * kA + j], q4_octet(w[j], sc), s);
+    };
+    block(std::integral_constant<int, 0>{});
+    block(std::integral_constant<int, 1>{});
+    block(std::integral_constant<int, 2>{});
+    block(std::integral_constant<int, 3>{});
+    block(std::integral_constant<int, 4>{});
+    block(std::integral_constant<int, 5>{});
+    block(std::integral_constant<int, 6>{});
+    block(std::integral_constant<int, 7>{});
 #pragma unroll
-    for (int c = 0; c < 18; ++c)
-      s = mfma_bf16(v[c], lds_read_b128(reinterpret_cast<const DMLA_LDS bf16x8*>(tile + row_operand_off(lane, kb, c))), s);
-    return s;
+    for (int c = 0; c < 4; ++c) s = mfma32_bf16(q[kQ4LatentSteps + c], q4_key_rope(row, hl, c), s);
+  } else {
+#pragma unroll
+    for (int c = 0; c < kQ4Steps; ++c)
+      s = mfma32_bf16(q[c], lds_read_b128(reinterpret_cast<const DMLA_LDS bf16x8*>(tile + tile_chunk_off(l32, 2 * c + hl))), s);
   }
-};
+  return s;
+}
 
-template <bool kQ4, int kNH, int kHW>
+template <bool kQ4, int kHW>
 __device__ __forceinline__ void mass_segment(const MassParams& p, int b, int t0, int t1, int ctx, DMLA_LDS char* ring,
                                              DMLA_LDS float* sums) {
   using T = Tile<kQ4>;
   constexpr int kKP = kWaves / kHW;
   const int lane = fresh_lane_id();
-  const int l16 = lane & 15, g = lane >> 4;
+  const int l32 = lane & 31, hl = lane >> 5;
   const int wave = uniform(threadIdx.x >> 6);
   const int hw = wave % kHW, kp = wave / kHW;
   const unsigned ring_addr = lds_addr(ring);
@@ -138,19 +136,18 @@ __device__ __forceinline__ void mass_segment(const MassParams& p, int b, int t0,
   constexpr int kFlight = T::kSlots - 2;
   constexpr int kTotal = kQ4 ? T::kBytes / 1024 : 9 * kWaves;   // copies of a tile, all waves
 
-  for (int h0 = 0; h0 < p.H; h0 += kHW * kNH * 16) {
-    Query<kQ4> q[kNH];
-    float lse2[kNH][4];
+  for (int h0 = 0; h0 < p.H; h0 += 32 * kHW) {
+    const int hb = h0 + 32 * hw;
+    const bf16* q_row = p.q + b * p.q_sb + min(hb + l32, p.H - 1) * p.q_sh;
+    bf16x8 q[kQ4Steps];
 #pragma unroll
-    for (int h = 0; h < kNH; ++h) {
-      const int hb = h0 + (hw * kNH + h) * 16;
-      q[h].load(p.q + b * p.q_sb + min(hb + l16, p.H - 1) * p.q_sh, g);
+    for (int c = 0; c < kQ4Steps; ++c) q[c] = kQ4 ? q4_query_operand(q_row, hl, c) : query_operand_bf16(q_row, hl, c);
+    float lse2[16];   // of the lane's rows, in log2 units; a head with no keys, or none at all, has weight 0
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int head = hb + 4 * g + i;
-        const float v = head < p.H ? p.lse[(int64_t)b * p.H + head] : kNegInf;
-        lse2[h][i] = v == kNegInf ? -kNegInf : v * kLog2e;   // a head with no keys, or none at all: weight 0
-      }
+    for (int i = 0; i < 16; ++i) {
+      const int head = hb + 8 * (i >> 2) + 4 * hl + (i & 3);
+      const float v = head < p.H ? p.lse[(int64_t)b * p.H + head] : kNegInf;
+      lse2[i] = v == kNegInf ? -kNegInf : v * kLog2e;
     }
     fetch_pages(t0 / kPerPage);
     for (int t = t0; t < t0 + T::kSlots - 1 && t < t1; ++t) copy_tile(t);
@@ -172,18 +169,14 @@ __device__ __forceinline__ void mass_segment(const MassParams& p, int b, int t0,
       const bool bad = page < 0 || page >= p.num_pages;
       const DMLA_LDS char* tile = ring + ((t - t0) % T::kSlots) * T::kBytes;
 #pragma unroll
-      for (int kb0 = 0; kb0 < T::kBlocks; kb0 += kKP) {
-        const int kb = kb0 + kp;
-        if (kb >= T::kBlocks) break;
+      for (int kb = 0; kb < T::kBlocks; ++kb) {
+        if ((t * T::kBlocks + kb) % kKP != kp) continue;   // the waves with the same heads take turns
+        const f32x16 s = scores<kQ4>(q, tile, kb, lane);
         float sum = 0.f;
 #pragma unroll
-        for (int h = 0; h < kNH; ++h) {
-          const f32x4 s = q[h].scores(tile, kb, lane);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) sum += fast_exp2(__builtin_fmaf(s[i], p.scale_log2, -lse2[h][i]));
-        }
-        sum = group_sum(sum);
-        if (g == 0) sums[hw * kChunk + (t - chunk0) * T::kTokens + 16 * kb + l16] = bad ? 0.f : sum;
+        for (int i = 0; i < 16; ++i) sum += fast_exp2(__builtin_fmaf(s[i], p.scale_log2, -lse2[i]));
+        sum = half_sum(sum);
+        if (hl == 0) sums[hw * kChunk + (t - chunk0) * T::kTokens + 32 * kb + l32] = bad ? 0.f : sum;
       }
       if (t + 1 == t1 || (t + 1 - chunk0) * T::kTokens == kChunk) {
         __syncthreads();
@@ -201,7 +194,7 @@ __device__ __forceinline__ void mass_segment(const MassParams& p, int b, int t0,
   }
 }
 
-template <bool kQ4, int kNH, int kHW>
+template <bool kQ4, int kHW>
 __global__ __launch_bounds__(kThreads, 1) void mass_kernel(MassParams p) {
   using T = Tile<kQ4>;
   __shared__ __attribute__((aligned(1024))) char smem[T::kSlots * T::kBytes];
@@ -210,7 +203,7 @@ __global__ __launch_bounds__(kThreads, 1) void mass_kernel(MassParams p) {
   for_each_segment<T::kTokens, T::kCost>(
       p.seqlens, p.B, p.max_pages * kPage, p.n_ranges, p.min_width, blockIdx.x, ranges,
       [&](int b, int t0, int t1, int ctx, int) {
-        mass_segment<kQ4, kNH, kHW>(p, b, t0, t1, ctx, (DMLA_LDS char*)smem, (DMLA_LDS float*)sum_mem);
+        mass_segment<kQ4, kHW>(p, b, t0, t1, ctx, (DMLA_LDS char*)smem, (DMLA_LDS float*)sum_mem);
       },
       [](int, int, int) {});
 }
@@ -266,15 +259,13 @@ extern "C" int dmla_attn_mass(const void* q, const void* kv_pool, const int32_t*
   const dim3 grid((unsigned)p.n_ranges);
   auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, (hipStream_t)stream, p); };
   if (q4) {
-    if (H <= 16) launch(mass_kernel<true, 1, 1>);
-    else if (H <= 32) launch(mass_kernel<true, 2, 1>);
-    else if (H <= 64) launch(mass_kernel<true, 2, 2>);
-    else launch(mass_kernel<true, 2, 4>);
+    if (H <= 32) launch(mass_kernel<true, 1>);
+    else if (H <= 64) launch(mass_kernel<true, 2>);
+    else launch(mass_kernel<true, 4>);
   } else {
-    if (H <= 16) launch(mass_kernel<false, 1, 1>);
-    else if (H <= 32) launch(mass_kernel<false, 2, 1>);
-    else if (H <= 64) launch(mass_kernel<false, 2, 2>);
-    else launch(mass_kernel<false, 2, 4>);
+    if (H <= 32) launch(mass_kernel<false, 1>);
+    else if (H <= 64) launch(mass_kernel<false, 2>);
+    else launch(mass_kernel<false, 4>);
   }
   return check_launch("dmla_attn_mass");
 }

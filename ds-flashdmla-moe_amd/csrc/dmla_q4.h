@@ -54,38 +54,32 @@ __device__ __forceinline__ bf16x8 q4_octet(unsigned w, float scale) {
   return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// ---- a key row as an MFMA operand --------------------------------------------------------------
-// Score product of 16 keys: 16 bf16 MFMAs of 32 latent dims and 2 of 32 rope dims.  Which dims a lane
-// group holds is free as long as the queries agree: group g takes the dims 128 g + 8 c + x in MFMA c, so
-// its codes are 64 contiguous bytes of the row (four LDS reads) and its scales one word.  Rows of
-// 400 bytes put the 16 rows of such a read into 16 different 16-byte columns of the LDS banks.
-struct Q4Key {
-  u32x4 w[4];
-  unsigned scales;
-  bf16x8 rope[2];
-  __device__ __forceinline__ void load(const DMLA_LDS char* row, int g) {
-    scales = *reinterpret_cast<const DMLA_LDS unsigned*>(row + kQ4ScaleOff + 4 * g);
-#pragma unroll
-    for (int a = 0; a < 4; ++a) w[a] = *reinterpret_cast<const DMLA_LDS u32x4*>(row + 64 * g + 16 * a);
-#pragma unroll
-    for (int c = 0; c < 2; ++c) rope[c] = lds_read_b128(reinterpret_cast<const DMLA_LDS bf16x8*>(row + kQ4RopeOff + 64 * c + 16 * g));
-  }
-  // Operands of MFMAs 4 kA .. 4 kA + 3.
-  template <int kA>
-  __device__ __forceinline__ void octets(bf16x8 (&k)[4]) const {
-    const float s = q4_scale_of<kA>(scales);
-#pragma unroll
-    for (int b = 0; b < 4; ++b) k[b] = q4_octet(w[kA][b], s);
-  }
-};
+// ---- key rows as an MFMA operand ----------------------------------------------------------------
+// Score product of 32 keys with 32 queries: 32 bf16 MFMAs (32x32x16) of the latent dims and 4 of the rope
+// dims, lane l holding key l % 32.  Which dims the two lane halves hold is free as long as the queries
+// agree: half h takes the dims 256 h + 8 c + x in MFMA c, so its codes are 128 contiguous bytes of the row
+// (eight LDS reads, a scale block each) and its scales two words.  Rows of 400 bytes put 16 consecutive rows
+// of such a read into 16 different 16-byte columns of the LDS banks.
+constexpr int kQ4Steps = 36;        // MFMAs of a 32-key tile
+constexpr int kQ4LatentSteps = 32;
 
-constexpr int kQ4KeySteps = 18;   // MFMAs of a key block: 16 latent, 2 rope
-// The query operand that goes with it.
-__device__ __forceinline__ void q4_load_query(const bf16* q, int g, bf16x8 (&v)[kQ4KeySteps]) {
-#pragma unroll
-  for (int c = 0; c < 16; ++c) v[c] = *reinterpret_cast<const bf16x8*>(q + 128 * g + 8 * c);
-#pragma unroll
-  for (int c = 0; c < 2; ++c) v[16 + c] = *reinterpret_cast<const bf16x8*>(q + 512 + 32 * c + 8 * g);
+// Query operand of MFMA c for lane half h.
+__device__ __forceinline__ bf16x8 q4_query_operand(const bf16* q, int h, int c) {
+  return *reinterpret_cast<const bf16x8*>(c < kQ4LatentSteps ? q + 256 * h + 8 * c : q + 512 + 16 * (c - kQ4LatentSteps) + 8 * h);
+}
+// Codes of MFMAs 4 a .. 4 a + 3, all scales, and rope operand c of this lane's row.
+__device__ __forceinline__ u32x4 q4_key_codes(const DMLA_LDS char* row, int h, int a) {
+  return *reinterpret_cast<const DMLA_LDS u32x4*>(row + 128 * h + 16 * a);
+}
+__device__ __forceinline__ u32x2 q4_key_scales(const DMLA_LDS char* row, int h) {
+  return *reinterpret_cast<const DMLA_LDS u32x2*>(row + kQ4ScaleOff + 8 * h);
+}
+__device__ __forceinline__ bf16x8 q4_key_rope(const DMLA_LDS char* row, int h, int c) {
+  return lds_read_b128(reinterpret_cast<const DMLA_LDS bf16x8*>(row + kQ4RopeOff + 32 * c + 16 * h));
+}
+template <int kA>
+__device__ __forceinline__ float q4_key_scale(const u32x2& scales) {
+  return q4_scale_of<kA % 4>(scales[kA / 4]);
 }
 
 // Wait until at most N vector-memory operations of this wave are outstanding.

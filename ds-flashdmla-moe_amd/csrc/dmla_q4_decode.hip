@@ -20,11 +20,13 @@
 //    4 / kHW such groups work on different tiles and meet in LDS at the end of a segment.
 //  * The value product of a tile runs one step behind its scores: one barrier per step, and the two
 //    products of a step are independent.
-//  * The softmax reference of a head rises only when a score passes it by 2^8 (kLazy), so outputs are
-//    rarely rescaled; P keeps bf16's relative precision whatever its size, sums stay in fp32.
+//  * The softmax reference of a head is its largest score in the segment's first tile; P may grow to 2^32
+//    past it (bf16 keeps its relative precision whatever the size, sums stay in fp32), and a segment
+//    whose scores climb further starts over from their exact maximum.
 //  * Sequences are cut over the chip's workgroups by weight (dmla_ranges.h); sequences in several parts
 //    are merged by the split-KV combine.
 #include <algorithm>
+#include <type_traits>
 
 #include "dmla_host.h"
 #include "dmla_q4.h"
@@ -39,7 +41,7 @@ constexpr int kTileBytes = kTile * kQ4RowBytes;      // 12800
 constexpr int kCopies = (kTileBytes + 1023) / 1024;  // wave copies of a tile, the last one half
 constexpr int kWaves = 4, kThreads = 64 * kWaves;
 static_assert(kThreads == kRangeThreads, "one workgroup cuts the ranges");
-constexpr float kLazy = 8.0f;
+constexpr float kHeadroom = 32.0f;   // log2 headroom of P over a head's reference
 
 struct Q4DecodeParams {
   const bf16* q;
@@ -58,17 +60,60 @@ struct Q4DecodeParams {
   float scale_log2;
 };
 
-template <int kNH, int kHW>
+// The output accumulators fill the AGPR file.  Where ordinary code touches them, the compiler gives them a
+// home among the VGPRs as well and spills the queries; these accesses leave them where they are.  The
+// compiler does not see into the assembly, so agpr_settle() keeps them clear of MFMAs on the same register.
+__device__ __forceinline__ float agpr_zero() {
+  float x;
+  asm volatile("v_accvgpr_write_b32 %0, 0" : "=a"(x));
+  return x;
+}
+__device__ __forceinline__ float agpr_read(float x) {
+  float v;
+  asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(v) : "a"(x));
+  return v;
+}
+// Longer than any MFMA takes to write its result, or a write to reach one.
+__device__ __forceinline__ void agpr_settle() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
+
+// Four steps of the score product, x += k[i] q[i], x = 0 before the first of a tile.  In assembly because
+// the AGPRs have no room for x beside the accumulators and the compiler gives every MFMA of a kernel the
+// same register file.  It does not see the waits that its operands need, so they are here: two states
+// after a VALU write of an operand or another step on x (both pass while the matrix core is busy), and
+// after the last step enough for x to be read.
+template <bool kFirst, bool kLast>
+__device__ __forceinline__ void score_steps(f32x16& x, const bf16x8 (&k)[4], const bf16x8& q0, const bf16x8& q1, const bf16x8& q2,
+                                            const bf16x8& q3) {
+  if constexpr (kFirst)
+    asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %5, 0\n\t"
+                 "s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %2, %6, %0\n\t"
+                 "s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %3, %7, %0\n\t"
+                 "s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %4, %8, %0"
+                 : "=&v"(x)
+                 : "v"(k[0]), "v"(k[1]), "v"(k[2]), "v"(k[3]), "v"(q0), "v"(q1), "v"(q2), "v"(q3));
+  else
+    asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %5, %0\n\t"
+                 "s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %2, %6, %0\n\t"
+                 "s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %3, %7, %0\n\t"
+                 "s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %4, %8, %0"
+                 : "+v"(x)
+                 : "v"(k[0]), "v"(k[1]), "v"(k[2]), "v"(k[3]), "v"(q0), "v"(q1), "v"(q2), "v"(q3));
+  if constexpr (kLast) asm volatile("s_nop 15\n\ts_nop 7" : "+v"(x));
+}
+
+template <int kHW>
 struct Shape {
   static constexpr int kKP = kWaves / kHW;              // tiles in work at once
   static constexpr int kSlotBytes = kKP * kTileBytes;
-  static constexpr int kSlots = kHW == 1 ? 3 : kHW == 2 ? 5 : 8;
+  static constexpr int kSlots = kHW == 1 ? 3 : kHW == 2 ? 4 : 6;
   static constexpr int kRingBytes = kSlots * kSlotBytes;
-  static constexpr int kNB = kHW * kNH;                 // head blocks of 16 of a workgroup
-  static constexpr int kHeads = kNB * 16;
-  static constexpr int kCols = 32 / kHW;                // neighbouring columns of a lane
+  static constexpr int kHeads = 32 * kHW;               // heads of a workgroup
+  static constexpr int kCols = 16 / kHW;                // neighbouring columns of a lane
   static constexpr int kLag = kHW > 1 ? 1 : 0;          // steps the value product runs behind
-  static constexpr int kXBytes = kHW > 1 ? 2 * kKP * kNB * 1024 : 16;   // P of two steps
+  static constexpr int kQRegs = kHW == 1 ? kQ4Steps : 24;   // query operands in registers, the others in LDS
+  static constexpr int kQLds = kQ4Steps - kQRegs;
+  static constexpr int kQBytes = kQLds > 0 ? kHW * kQLds * 1024 : 16;
+  static constexpr int kXBytes = kHW > 1 ? 2 * kWaves * 2048 : 16;   // P of two steps
   static constexpr int kMergeRow = 128 / kHW + 4;       // floats, padded against bank conflicts
   static constexpr int kMergeBytes = kWaves * kHeads * kMergeRow * 4;
   static constexpr int kSegCost = kHW == 1 ? 16 : kHW == 2 ? 10 : 5;
@@ -81,40 +126,36 @@ struct Segment {
 
 struct Lds {
   DMLA_LDS char* ring;
-  DMLA_LDS char* p;        // [2][kKP][kNB][64 lanes] x 16 bytes
-  DMLA_LDS float* alpha;   // [2][kKP][kHeads]: what a step multiplies the outputs by; after the last step
-                           // [kKP][kHeads][2], references and sums
+  DMLA_LDS char* q;        // [kHW][kQLds][64 lanes] x 16 bytes
+  DMLA_LDS char* p;        // [2][kKP][kHW][2][64 lanes] x 16 bytes
+  DMLA_LDS float* stat;    // [kKP][kHeads][2]: references and sums
   DMLA_LDS int* flag;      // [kWaves]
 };
 
 // One segment: the tiles [t0, t1) of a sequence.
-template <int kNH, int kHW>
+template <int kHW>
 __device__ __forceinline__ void run_segment(const Q4DecodeParams& p, const Segment& sg, const Lds& lds, int head0) {
-  using S = Shape<kNH, kHW>;
-  constexpr int kKP = S::kKP, kNB = S::kNB, kCols = S::kCols;
+  using S = Shape<kHW>;
+  constexpr int kKP = S::kKP, kCols = S::kCols;
   const int lane = fresh_lane_id();
-  const int l16 = lane & 15, g = lane >> 4;
+  const int l32 = lane & 31, hl = lane >> 5;
   const int wave = uniform(threadIdx.x >> 6);
   const int hw = wave % kHW, kp = wave / kHW;
   const int n_steps = (sg.t1 - sg.t0 + kKP - 1) / kKP;
   bool bad_page = false;
 
   // Pages of this wave's tiles, 64 at a time in a register (lane i: page page0 + i).
-  int page0 = sg.t0 / 2, pages = 0;
-  auto fetch_pages = [&]() {
+  int page0 = 0, pages = 0;
+  auto fetch_pages = [&](int from) {
+    page0 = from;
     const int i = page0 + lane;
     pages = i < (sg.t1 + 1) / 2 ? p.block_table[sg.b * p.bt_sb + i] : 0;
   };
-  fetch_pages();
   const unsigned ring_addr = lds_addr(lds.ring);
   // This wave's share of the copies of step s's tile kp: pieces hw, hw + kHW, ...
   auto copy_step = [&](int s) {
-    const int t = sg.t0 + s * kKP + kp;
-    if (t >= sg.t1) return;
-    if (t / 2 - page0 >= 64) {
-      page0 += 64;
-      fetch_pages();
-    }
+    const int t = min(sg.t0 + s * kKP + kp, sg.t1 - 1);   // past the end: the last tile, all masked
+    if (t / 2 - page0 >= 64) fetch_pages(page0 + 64);
     int page = __builtin_amdgcn_readlane(pages, (t / 2 - page0) & 63);
     const bool bad = page < 0 || page >= p.num_pages;
     bad_page = bad_page || bad;
@@ -122,216 +163,223 @@ __device__ __forceinline__ void run_segment(const Q4DecodeParams& p, const Segme
     const char* src = p.kv + page * p.kv_sp + (t & 1) * kTileBytes;
     const unsigned dst = ring_addr + (unsigned)((s % S::kSlots) * S::kSlotBytes + kp * kTileBytes);
     const int valid = sg.ctx - t * kTile;
-    if (valid >= kTile) {
+    const int ln = fresh_lane_id();   // nothing of this is kept across the loop
 #pragma unroll
-      for (int k = 0; k < kCopies; ++k) {
-        if (k % kHW != hw) continue;
-        if (k < kCopies - 1 || lane < 32) dma16(src + k * 1024, 16u * lane, dst + k * 1024);
+    for (int i = 0; i < (kCopies + kHW - 1) / kHW; ++i) {
+      const int k = i * kHW + hw;
+      if (k >= kCopies) continue;
+      const int c = k * 64 + ln;
+      unsigned off = 16u * c;
+      if (valid < kTile) {   // rows past the sequence's end re-read the tile's first row: finite data, masked below
+        const int row = c / kQ4Chunks;
+        off = row < valid ? off : 16u * (c - row * kQ4Chunks);
       }
-    } else {   // rows past the sequence's end re-read the tile's first row: finite data, masked below
-#pragma unroll
-      for (int k = 0; k < kCopies; ++k) {
-        if (k % kHW != hw) continue;
-        const int i = k * 64 + lane, row = i / kQ4Chunks, col = i - row * kQ4Chunks;
-        if (k < kCopies - 1 || lane < 32) dma16(src, 16u * (row < valid ? i : col), dst + k * 1024);
-      }
+      if (k < kCopies - 1 || ln < 32) dma16(src, off, dst + k * 1024);
     }
   };
+  // Copies run kAhead steps ahead: at step s the slot of step s - 1 - kLag is refilled.
+  constexpr int kAhead = S::kSlots - 1 - S::kLag;
+  auto start_copies = [&]() {
+    fetch_pages(sg.t0 / 2);
+    for (int s = 0; s < kAhead && s < n_steps; ++s) copy_step(s);
+  };
+  start_copies();
 
-  bf16x8 q[kNH][kQ4KeySteps];
+  bf16x8 q[S::kQRegs];
+  DMLA_LDS char* q_lds = lds.q + hw * S::kQLds * 1024 + lane * 16;
+  {
+    const bf16* src = p.q + sg.b * p.q_sb + min(head0 + hw * 32 + l32, p.H - 1) * p.q_sh;
 #pragma unroll
-  for (int h = 0; h < kNH; ++h) {
-    const int head = min(head0 + (hw * kNH + h) * 16 + l16, p.H - 1);
-    q4_load_query(p.q + sg.b * p.q_sb + head * p.q_sh, g, q[h]);
+    for (int c = 0; c < kQ4Steps; ++c) {
+      const bf16x8 v = q4_query_operand(src, hl, c);
+      if (c < S::kQRegs) q[c] = v;
+      else *reinterpret_cast<DMLA_LDS bf16x8*>(q_lds + (c - S::kQRegs) * 1024) = v;   // the same from every kp
+    }
   }
+  auto query = [&](int c) {
+    return c < S::kQRegs ? q[c < S::kQRegs ? c : 0]
+                         : lds_read_b128(reinterpret_cast<const DMLA_LDS bf16x8*>(q_lds + (c - S::kQRegs) * 1024));
+  };
 
-  f32x4 acc[kNB][kCols];   // O^T: row m = 4 g + i is column (512 / kHW) hw + kCols m + j, for head l16
-  float mref[kNH], lsum[kNH];
-#pragma unroll
-  for (int h = 0; h < kNH; ++h) {
-    mref[h] = kNegInf;
-    lsum[h] = 0.f;
-  }
-#pragma unroll
-  for (int n = 0; n < kNB; ++n)
-#pragma unroll
-    for (int j = 0; j < kCols; ++j) acc[n][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  bf16x8 pv[kNH];          // P of the wave's own heads
-  float alpha[kNH];
+  f32x16 acc[kHW][kCols];   // O^T of 32 heads and 32 columns: row m is column (512 / kHW) hw + kCols m + j
+  float mref = kNegInf, mtrue = kNegInf, lsum = 0.f;   // reference, largest score seen, sum
+  bf16x8 pv[2];             // P of the wave's own heads, 16 keys each
 
-  // S^T[key 16 kb + 4 g + i][head l16] of a tile, then P and alpha.
-  auto scores = [&](int s, int t) {
-    const DMLA_LDS char* tile = lds.ring + (s % S::kSlots) * S::kSlotBytes + kp * kTileBytes;
-    f32x4 sc[kNH][2];
+  // S^T[key 8 (i / 4) + 4 hl + i % 4][head l32] of a tile.
+  auto scores = [&](int s, int t) -> f32x16 {
+    const DMLA_LDS char* row = lds.ring + (s % S::kSlots) * S::kSlotBytes + kp * kTileBytes + l32 * kQ4RowBytes;
+    f32x16 x;
+    const u32x2 scales = q4_key_scales(row, hl);
+    auto block = [&](auto a_tag) {
+      constexpr int kA = decltype(a_tag)::value;
+      const u32x4 w = q4_key_codes(row, hl, kA);
+      const float sc = q4_key_scale<kA>(scales);
+      const bf16x8 k[4] = {q4_octet(w[0], sc), q4_octet(w[1], sc), q4_octet(w[2], sc), q4_octet(w[3], sc)};
+      score_steps<kA == 0, false>(x, k, query(4 * kA), query(4 * kA + 1), query(4 * kA + 2), query(4 * kA + 3));
+    };
+    block(std::integral_constant<int, 0>{});
+    block(std::integral_constant<int, 1>{});
+    block(std::integral_constant<int, 2>{});
+    block(std::integral_constant<int, 3>{});
+    block(std::integral_constant<int, 4>{});
+    block(std::integral_constant<int, 5>{});
+    block(std::integral_constant<int, 6>{});
+    block(std::integral_constant<int, 7>{});
+    const bf16x8 k[4] = {q4_key_rope(row, hl, 0), q4_key_rope(row, hl, 1), q4_key_rope(row, hl, 2), q4_key_rope(row, hl, 3)};
+    score_steps<false, true>(x, k, query(32), query(33), query(34), query(35));
+    const int left = t < sg.t1 ? sg.ctx - t * kTile : 0;   // keys of the tile
+    if (left < kTile) {
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-      Q4Key key;
-      key.load(tile + (16 * kb + l16) * kQ4RowBytes, g);
-#pragma unroll
-      for (int h = 0; h < kNH; ++h) sc[h][kb] = f32x4{0.f, 0.f, 0.f, 0.f};
-      auto step = [&](auto a_tag) {
-        constexpr int kA = decltype(a_tag)::value;
-        bf16x8 k[4];
-        key.octets<kA>(k);
-#pragma unroll
-        for (int b = 0; b < 4; ++b)
-#pragma unroll
-          for (int h = 0; h < kNH; ++h) sc[h][kb] = mfma_bf16(k[b], q[h][4 * kA + b], sc[h][kb]);
-      };
-      step(std::integral_constant<int, 0>{});
-      step(std::integral_constant<int, 1>{});
-      step(std::integral_constant<int, 2>{});
-      step(std::integral_constant<int, 3>{});
-#pragma unroll
-      for (int c = 0; c < 2; ++c)
-#pragma unroll
-        for (int h = 0; h < kNH; ++h) sc[h][kb] = mfma_bf16(key.rope[c], q[h][16 + c], sc[h][kb]);
+      for (int i = 0; i < 16; ++i) x[i] = 8 * (i >> 2) + 4 * hl + (i & 3) < left ? x[i] : kNegInf;
     }
-    const int left = sg.ctx - t * kTile;   // keys of the tile
+    return x;
+  };
+  auto tile_max = [&](const f32x16& x) {
+    float mx = x[0];
 #pragma unroll
-    for (int h = 0; h < kNH; ++h) {
-      float x[8], mx = kNegInf;
+    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, x[i]);
+    return half_max(mx) * p.scale_log2;   // scale > 0
+  };
+  auto softmax = [&](const f32x16& x) {
+    mtrue = fmaxf(mtrue, tile_max(x));
+    const float ms = mref == kNegInf ? 0.f : mref;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        x[j] = sc[h][j >> 2][j & 3] * p.scale_log2;
-        x[j] = 16 * (j >> 2) + 4 * g + (j & 3) < left ? x[j] : kNegInf;
-        mx = fmaxf(mx, x[j]);
-      }
-      mx = group_max(mx);
-      const bool rise = mx > mref[h] + kLazy || mref[h] == kNegInf;
-      const float mnew = rise ? fmaxf(mx, mref[h]) : mref[h];
-      alpha[h] = rise && mnew != kNegInf ? fast_exp2(mref[h] - mnew) : 1.f;
-      mref[h] = mnew;
-      lsum[h] *= alpha[h];
-      const float ms = mnew == kNegInf ? 0.f : mnew;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float e = fast_exp2(x[j] - ms);
-        lsum[h] += e;
-        pv[h][j] = (bf16)e;
-      }
+    for (int i = 0; i < 16; ++i) {
+      const float e = fast_exp2(__builtin_fmaf(x[i], p.scale_log2, -ms));
+      lsum += e;
+      pv[i >> 3][i & 7] = (bf16)e;
     }
   };
-  auto rescale = [&](int n, float al) {
-    if (__any(al != 1.f)) {
-#pragma unroll
-      for (int j = 0; j < kCols; ++j) acc[n][j] *= al;
-    }
-  };
-  // O^T += V^T P of step s's tile; pb(n): P of head block n.
+  // O^T += V^T P of step s's tile; pb(n, u): P of head block n and the keys from 16 u on.
   auto values = [&](int s, auto pb) {
     const DMLA_LDS char* tile = lds.ring + (s % S::kSlots) * S::kSlotBytes + kp * kTileBytes;
-    unsigned vc[8][kCols / 8];
-    float vs[8];
+    constexpr int kWords = kCols >= 8 ? kCols / 8 : 1;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {   // the keys of the scores: 4 g + j, then 16 + 4 g + j - 4
-      const DMLA_LDS char* row = tile + (16 * (j >> 2) + 4 * g + (j & 3)) * kQ4RowBytes;
-      const DMLA_LDS char* at = row + (256 / kHW) * hw + (kCols / 2) * l16;
-      if constexpr (kCols == 32) {
-        const u32x4 w = *reinterpret_cast<const DMLA_LDS u32x4*>(at);
+    for (int u = 0; u < 2; ++u) {
+      unsigned vc[8][kWords];
+      float vs[8];
 #pragma unroll
-        for (int d = 0; d < 4; ++d) vc[j][d] = w[d];
-      } else if constexpr (kCols == 16) {
-        const u32x2 w = *reinterpret_cast<const DMLA_LDS u32x2*>(at);
-        vc[j][0] = w[0];
-        vc[j][1] = w[1];
-      } else {
-        vc[j][0] = *reinterpret_cast<const DMLA_LDS unsigned*>(at);
+      for (int j = 0; j < 8; ++j) {   // the keys of the lane's scores
+        const DMLA_LDS char* row = tile + (16 * u + 8 * (j >> 2) + 4 * hl + (j & 3)) * kQ4RowBytes;
+        const DMLA_LDS char* at = row + (256 / kHW) * hw + (kCols / 2) * l32;
+        if constexpr (kCols == 16) {
+          const u32x2 w = *reinterpret_cast<const DMLA_LDS u32x2*>(at);
+          vc[j][0] = w[0];
+          vc[j][1] = w[1];
+        } else if constexpr (kCols == 8) {
+          vc[j][0] = *reinterpret_cast<const DMLA_LDS unsigned*>(at);
+        } else {
+          vc[j][0] = *reinterpret_cast<const DMLA_LDS uint16_t*>(at);
+        }
+        vs[j] = q4_scale(*reinterpret_cast<const DMLA_LDS uint8_t*>(row + kQ4ScaleOff + (16 / kHW) * hw + l32 / (2 * kHW)));
       }
-      vs[j] = q4_scale(*reinterpret_cast<const DMLA_LDS uint8_t*>(row + kQ4ScaleOff + (16 / kHW) * hw + l16 / kHW));
-    }
-    auto column_pair = [&](auto byte_tag, int d) {
-      constexpr int kB = decltype(byte_tag)::value;
-      unsigned e[8];
+      auto column_pair = [&](auto byte_tag, int d) {
+        constexpr int kB = decltype(byte_tag)::value;
+        unsigned e[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) e[j] = __builtin_bit_cast(unsigned, q4_pair<kB>(vc[j][d], vs[j]));
-      u32x4 even, odd;
+        for (int j = 0; j < 8; ++j) e[j] = __builtin_bit_cast(unsigned, q4_pair<kB>(vc[j][d], vs[j]));
+        u32x4 even, odd;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        even[r] = __builtin_amdgcn_perm(e[2 * r + 1], e[2 * r], 0x05040100u);
-        odd[r] = __builtin_amdgcn_perm(e[2 * r + 1], e[2 * r], 0x07060302u);
+        for (int r = 0; r < 4; ++r) {
+          even[r] = __builtin_amdgcn_perm(e[2 * r + 1], e[2 * r], 0x05040100u);
+          odd[r] = __builtin_amdgcn_perm(e[2 * r + 1], e[2 * r], 0x07060302u);
+        }
+#pragma unroll
+        for (int n = 0; n < kHW; ++n) {
+          const int j = 8 * d + 2 * kB;
+          acc[n][j] = mfma32_bf16(__builtin_bit_cast(bf16x8, even), pb(n, u), acc[n][j]);
+          acc[n][j + 1] = mfma32_bf16(__builtin_bit_cast(bf16x8, odd), pb(n, u), acc[n][j + 1]);
+        }
+      };
+#pragma unroll
+      for (int d = 0; d < kWords; ++d) {
+        column_pair(std::integral_constant<int, 0>{}, d);
+        column_pair(std::integral_constant<int, 1>{}, d);
+        if constexpr (kCols >= 8) {
+          column_pair(std::integral_constant<int, 2>{}, d);
+          column_pair(std::integral_constant<int, 3>{}, d);
+        }
       }
-#pragma unroll
-      for (int n = 0; n < kNB; ++n) {
-        const int j = 8 * d + 2 * kB;
-        acc[n][j] = mfma_bf16(__builtin_bit_cast(bf16x8, even), pb(n), acc[n][j]);
-        acc[n][j + 1] = mfma_bf16(__builtin_bit_cast(bf16x8, odd), pb(n), acc[n][j + 1]);
-      }
-    };
-#pragma unroll
-    for (int d = 0; d < kCols / 8; ++d) {
-      column_pair(std::integral_constant<int, 0>{}, d);
-      column_pair(std::integral_constant<int, 1>{}, d);
-      column_pair(std::integral_constant<int, 2>{}, d);
-      column_pair(std::integral_constant<int, 3>{}, d);
     }
   };
-  // P and alpha of step s through LDS, between the waves of a group.
+  // P of step s through LDS, between the waves of a group.
   auto post = [&](int s) {
+    const int at = (s & 1) * kWaves + kp * kHW + hw;
 #pragma unroll
-    for (int h = 0; h < kNH; ++h) {
-      const int n = hw * kNH + h, at = (s & 1) * kKP + kp;
-      *reinterpret_cast<DMLA_LDS bf16x8*>(lds.p + (at * kNB + n) * 1024 + lane * 16) = pv[h];
-      if (g == 0) lds.alpha[(at * kNB + n) * 16 + l16] = alpha[h];
-    }
+    for (int u = 0; u < 2; ++u) *reinterpret_cast<DMLA_LDS bf16x8*>(lds.p + (2 * at + u) * 1024 + lane * 16) = pv[u];
   };
   auto shared_values = [&](int s) {
-    const int at = (s & 1) * kKP + kp;
-    bf16x8 pall[kNB];
-#pragma unroll
-    for (int n = 0; n < kNB; ++n) {
-      pall[n] = lds_read_b128(reinterpret_cast<const DMLA_LDS bf16x8*>(lds.p + (at * kNB + n) * 1024 + lane * 16));
-      rescale(n, lds.alpha[(at * kNB + n) * 16 + l16]);
-    }
-    values(s, [&](int n) { return pall[n]; });
+    const int at = (s & 1) * kWaves + kp * kHW;
+    values(s, [&](int n, int u) {
+      return lds_read_b128(reinterpret_cast<const DMLA_LDS bf16x8*>(lds.p + (2 * (at + n) + u) * 1024 + lane * 16));
+    });
   };
 
-  // Copies run kSlots - 1 - kLag steps ahead: at step s the slot of step s - 1 - kLag is refilled.
-  constexpr int kAhead = S::kSlots - 1 - S::kLag;
-  for (int s = 0; s < kAhead && s < n_steps; ++s) copy_step(s);
-  for (int s = 0; s < n_steps; ++s) {
+  auto arrive = [&](int s, bool copy) {
     // This wave's copies of step s have landed; those of the kAhead - 1 steps after it stay in flight.
     constexpr int kFlight = kAhead - 1;
     constexpr int kMost = (kCopies + kHW - 1) / kHW, kLeast = kCopies / kHW;
-    if (s + kFlight >= n_steps - 1) wait_vm<0>();   // the last steps' tiles need not exist
+    if (s + kFlight >= n_steps) wait_vm<0>();   // the last steps have fewer behind them
     else if (hw < kCopies % kHW || kCopies % kHW == 0) wait_vm<kFlight * kMost>();
     else wait_vm<kFlight * kLeast>();
     wait_lds();   // this wave's reads of the slot that is refilled below are done
     if constexpr (kHW > 1) __syncthreads();   // and everybody's; all copies of step s have landed
-    if (s + kAhead < n_steps) copy_step(s + kAhead);
-    const int t = sg.t0 + s * kKP + kp;
+    if (copy && s + kAhead < n_steps) copy_step(s + kAhead);
+  };
+  // The reference of a head is its first tile's largest score.  Where scores have climbed more than
+  // kHeadroom above it, the segment starts over from the largest that was seen: rare, and the loop holds
+  // no rescaling of the outputs.
+  for (bool again = false;; again = true) {
+    arrive(0, true);
+    const f32x16 x0 = scores(0, sg.t0 + kp);
+    mref = again ? mtrue : tile_max(x0);
+    lsum = 0.f;
     if constexpr (kHW > 1) {
-      if (s > 0) shared_values(s - 1);
-      if (t < sg.t1) {
-        scores(s, t);
+      softmax(x0);
+      post(0);
+    }
+#pragma unroll
+    for (int n = 0; n < kHW; ++n)
+#pragma unroll
+      for (int j = 0; j < kCols; ++j)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[n][j][i] = agpr_zero();
+    agpr_settle();
+    if constexpr (kHW > 1) {
+      // One step more than there are tiles, whose scores are all masked: no branch in the loop.
+#pragma nounroll
+      for (int s = 1; s <= n_steps; ++s) {
+        arrive(s, true);
+        shared_values(s - 1);
+        softmax(scores(s, sg.t0 + s * kKP + kp));
         post(s);
       }
     } else {
-      if (t >= sg.t1) continue;
-      scores(s, t);
-#pragma unroll
-      for (int h = 0; h < kNH; ++h) rescale(h, alpha[h]);
-      values(s, [&](int n) { return pv[n]; });
+#pragma nounroll
+      for (int s = 0; s < n_steps; ++s) {
+        arrive(s, s > 0);
+        softmax(scores(s, sg.t0 + s * kKP + kp));
+        values(s, [&](int, int u) { return pv[u]; });
+      }
     }
-  }
-  if constexpr (kHW > 1) {
-    __syncthreads();
-    if (sg.t0 + (n_steps - 1) * kKP + kp < sg.t1) shared_values(n_steps - 1);
+    const bool over = __any(mtrue > mref + kHeadroom);
+    if (lane == 0) lds.flag[wave] = over ? 1 : 0;
+    wait_vm<0>();
+    wait_lds();
+    __syncthreads();   // flags posted; the ring and the exchange are free
+    const bool repeat = (lds.flag[0] | lds.flag[1] | lds.flag[2] | lds.flag[3]) != 0;
+    __syncthreads();   // flags read
+    if (again || !repeat) break;
+    start_copies();
   }
 
   // ---- the segment's output ----
-#pragma unroll
-  for (int h = 0; h < kNH; ++h) lsum[h] = group_sum(lsum[h]);
-  wait_vm<0>();
-  wait_lds();
-  __syncthreads();   // the ring and the exchange are free
-  if (g == 0) {
-#pragma unroll
-    for (int h = 0; h < kNH; ++h) {
-      const int at = (kp * S::kHeads + (hw * kNH + h) * 16 + l16) * 2;
-      lds.alpha[at] = mref[h];
-      lds.alpha[at + 1] = lsum[h];
-    }
+  lsum = half_sum(lsum);
+  agpr_settle();
+  if (hl == 0) {
+    const int at = (kp * S::kHeads + hw * 32 + l32) * 2;
+    lds.stat[at] = mref;
+    lds.stat[at + 1] = lsum;
   }
   if (lane == 0) lds.flag[wave] = bad_page ? 1 : 0;
   __syncthreads();
@@ -342,10 +390,10 @@ __device__ __forceinline__ void run_segment(const Q4DecodeParams& p, const Segme
     top = kNegInf;
     sum = 0.f;
 #pragma unroll
-    for (int k = 0; k < kKP; ++k) top = fmaxf(top, lds.alpha[(k * S::kHeads + hd) * 2]);
+    for (int k = 0; k < kKP; ++k) top = fmaxf(top, lds.stat[(k * S::kHeads + hd) * 2]);
 #pragma unroll
     for (int k = 0; k < kKP; ++k) {
-      const float m = lds.alpha[(k * S::kHeads + hd) * 2], l = lds.alpha[(k * S::kHeads + hd) * 2 + 1];
+      const float m = lds.stat[(k * S::kHeads + hd) * 2], l = lds.stat[(k * S::kHeads + hd) * 2 + 1];
       sum += m == kNegInf ? l : l * fast_exp2(m - top);   // no finite reference: 0, or NaN
     }
     if (poison) sum = nanv;
@@ -358,48 +406,50 @@ __device__ __forceinline__ void run_segment(const Q4DecodeParams& p, const Segme
     if (sg.nsplit > 1) p.part_lse[(int64_t)sg.slot * p.H + head] = lse;
     else if (p.lse != nullptr) p.lse[sg.b * p.H + head] = lse;
   };
+  // A lane holds, for each q = 0..3, 4 kCols neighbouring columns from kCols (8 q + 4 hl) of its wave's
+  // 512 / kHW on: value n of them is accumulator n % kCols, register 4 q + n / kCols.
   if constexpr (kKP == 1) {
 #pragma unroll
-    for (int n = 0; n < kNB; ++n) {
-      const int head = head0 + 16 * n + l16;
+    for (int n = 0; n < kHW; ++n) {
+      const int head = head0 + 32 * n + l32;
       if (head >= p.H) continue;
       float top, sum;
-      joined(16 * n + l16, top, sum);
+      joined(32 * n + l32, top, sum);
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
       bf16* orow = out_row(head) + (kDv / kHW) * hw;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int q4 = 0; q4 < 4; ++q4)
 #pragma unroll
-        for (int d = 0; d < kCols / 8; ++d) {
+        for (int d = 0; d < kCols / 2; ++d) {
           bf16x8 v;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = (bf16)(acc[n][8 * d + j][i] * inv);
-          *reinterpret_cast<bf16x8*>(orow + kCols * (4 * g + i) + 8 * d) = v;
+          for (int j = 0; j < 8; ++j) v[j] = (bf16)(agpr_read(acc[n][(8 * d + j) % kCols][4 * q4 + (8 * d + j) / kCols]) * inv);
+          *reinterpret_cast<bf16x8*>(orow + kCols * (8 * q4 + 4 * hl) + 8 * d) = v;
         }
-      if (g == 0 && hw == n % kHW) put_lse(head, top, sum);
+      if (hl == 0 && hw == n) put_lse(head, top, sum);
     }
   } else {
-    // The tile groups' outputs meet in LDS, one row index i of the accumulators a round (512 / 4
-    // columns of all heads): each group's at the common reference.
+    // The tile groups' outputs meet in LDS, one q a round (a quarter of the columns of all heads),
+    // each group's at the common reference.
     DMLA_LDS float* merge = reinterpret_cast<DMLA_LDS float*>(lds.ring);
-    float fac[kNB];
+    float fac[kHW];
 #pragma unroll
-    for (int n = 0; n < kNB; ++n) {
+    for (int n = 0; n < kHW; ++n) {
       float top, sum;
-      joined(16 * n + l16, top, sum);
-      const float m = lds.alpha[(kp * S::kHeads + 16 * n + l16) * 2];
+      joined(32 * n + l32, top, sum);
+      const float m = lds.stat[(kp * S::kHeads + 32 * n + l32) * 2];
       fac[n] = m == kNegInf ? 0.f : fast_exp2(m - top);
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int q4 = 0; q4 < 4; ++q4) {
 #pragma unroll
-      for (int n = 0; n < kNB; ++n) {
-        DMLA_LDS float* at = merge + ((wave * kNB + n) * 16 + l16) * S::kMergeRow + kCols * g;
+      for (int n = 0; n < kHW; ++n) {
+        DMLA_LDS float* at = merge + (wave * S::kHeads + 32 * n + l32) * S::kMergeRow + 4 * kCols * hl;
 #pragma unroll
-        for (int d = 0; d < kCols / 4; ++d) {
+        for (int d = 0; d < kCols; ++d) {
           f32x4 v;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) v[j] = acc[n][4 * d + j][i] * fac[n];
+          for (int j = 0; j < 4; ++j) v[j] = agpr_read(acc[n][(4 * d + j) % kCols][4 * q4 + (4 * d + j) / kCols]) * fac[n];
           *reinterpret_cast<DMLA_LDS f32x4*>(at + 4 * d) = v;
         }
       }
@@ -427,8 +477,9 @@ __device__ __forceinline__ void run_segment(const Q4DecodeParams& p, const Segme
             v[j] = (bf16)(v0[j] * inv);
             v[4 + j] = (bf16)(v1[j] * inv);
           }
-          *reinterpret_cast<bf16x8*>(out_row(head) + (kDv / kHW) * w0 + kCols * (4 * (lc / kCols) + i) + lc % kCols) = v;
-          if (i == 0 && cc == 0) put_lse(head, top, sum);
+          const int half = lc / (4 * kCols);
+          *reinterpret_cast<bf16x8*>(out_row(head) + (kDv / kHW) * w0 + kCols * (8 * q4 + 4 * half) + lc % (4 * kCols)) = v;
+          if (q4 == 0 && cc == 0) put_lse(head, top, sum);
         }
       }
       __syncthreads();   // read out before the next round writes
@@ -437,15 +488,16 @@ __device__ __forceinline__ void run_segment(const Q4DecodeParams& p, const Segme
 }
 
 // One workgroup per range (dmla_ranges.h) and head group.
-template <int kNH, int kHW>
+template <int kHW>
 __global__ __launch_bounds__(kThreads, 1) void q4_decode_kernel(Q4DecodeParams p) {
-  using S = Shape<kNH, kHW>;
+  using S = Shape<kHW>;
   __shared__ __attribute__((aligned(1024))) char ring[S::kRingBytes];
+  __shared__ __attribute__((aligned(1024))) char q_mem[S::kQBytes];
   __shared__ __attribute__((aligned(1024))) char p_mem[S::kXBytes];
-  __shared__ __attribute__((aligned(16))) float alpha[2 * S::kKP * S::kHeads];
+  __shared__ __attribute__((aligned(16))) float stat[2 * kWaves * 32];
   __shared__ __attribute__((aligned(16))) int flag[kWaves];
   __shared__ __attribute__((aligned(16))) RangeLds ranges;
-  const Lds lds = {(DMLA_LDS char*)ring, (DMLA_LDS char*)p_mem, (DMLA_LDS float*)alpha, (DMLA_LDS int*)flag};
+  const Lds lds = {(DMLA_LDS char*)ring, (DMLA_LDS char*)q_mem, (DMLA_LDS char*)p_mem, (DMLA_LDS float*)stat, (DMLA_LDS int*)flag};
   // The head groups of a range run 8 ids apart, on one XCD: the second read of its pages hits that L2.
   const int id = blockIdx.x;
   const int hg = (id / 8) % p.head_groups;
@@ -454,7 +506,7 @@ __global__ __launch_bounds__(kThreads, 1) void q4_decode_kernel(Q4DecodeParams p
   for_each_segment<kTile, S::kSegCost>(
       p.seqlens, p.B, p.max_pages * kPage, p.n_ranges, p.min_width, r, ranges,
       [&](int b, int t0, int t1, int ctx, int nsplit) {
-        run_segment<kNH, kHW>(p, Segment{b, t0, t1, ctx, nsplit, r + b}, lds, hg * S::kHeads);
+        run_segment<kHW>(p, Segment{b, t0, t1, ctx, nsplit, r + b}, lds, hg * S::kHeads);
       },
       [&](int b, int first_range, int nsplit) {
         if (hg != 0) return;
@@ -463,8 +515,7 @@ __global__ __launch_bounds__(kThreads, 1) void q4_decode_kernel(Q4DecodeParams p
       });
 }
 
-// Heads of a workgroup, by the number of heads: see kShapes' use in the launch.
-int wg_heads(int64_t H) { return H <= 16 ? 16 : H <= 32 ? 32 : H <= 64 ? 64 : 128; }
+int wg_heads(int64_t H) { return H <= 32 ? 32 : H <= 64 ? 64 : 128; }
 int64_t q4_ranges(int64_t H) {
   const int64_t hg = (H + wg_heads(H) - 1) / wg_heads(H);
   return std::max<int64_t>(1, device_cu_count() / hg);
@@ -536,10 +587,9 @@ extern "C" int dmla_decode_paged_q4(const void* q, const void* kv_pool, const in
   p.scale_log2 = softmax_scale * kLog2e;
   const dim3 grid((unsigned)((R + 7) / 8 * 8 * p.head_groups));
   switch (wg_heads(H)) {
-    case 16: p.min_width = 32; hipLaunchKernelGGL((q4_decode_kernel<1, 1>), grid, dim3(kThreads), 0, (hipStream_t)stream, p); break;
-    case 32: p.min_width = 32; hipLaunchKernelGGL((q4_decode_kernel<2, 1>), grid, dim3(kThreads), 0, (hipStream_t)stream, p); break;
-    case 64: p.min_width = 16; hipLaunchKernelGGL((q4_decode_kernel<2, 2>), grid, dim3(kThreads), 0, (hipStream_t)stream, p); break;
-    default: p.min_width = 8; hipLaunchKernelGGL((q4_decode_kernel<2, 4>), grid, dim3(kThreads), 0, (hipStream_t)stream, p); break;
+    case 32: p.min_width = 32; hipLaunchKernelGGL(q4_decode_kernel<1>, grid, dim3(kThreads), 0, (hipStream_t)stream, p); break;
+    case 64: p.min_width = 16; hipLaunchKernelGGL(q4_decode_kernel<2>, grid, dim3(kThreads), 0, (hipStream_t)stream, p); break;
+    default: p.min_width = 8; hipLaunchKernelGGL(q4_decode_kernel<4>, grid, dim3(kThreads), 0, (hipStream_t)stream, p); break;
   }
   const int rc = check_launch("dmla_decode_paged_q4");
   if (rc != DMLA_OK) return rc;
