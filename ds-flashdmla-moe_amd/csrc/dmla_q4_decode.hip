@@ -63,11 +63,6 @@ struct Q4DecodeParams {
 // The output accumulators fill the AGPR file.  Where ordinary code touches them, the compiler gives them a
 // home among the VGPRs as well and spills the queries; these accesses leave them where they are.  The
 // compiler does not see into the assembly, so agpr_settle() keeps them clear of MFMAs on the same register.
-__device__ __forceinline__ float agpr_zero() {
-  float x;
-  asm volatile("v_accvgpr_write_b32 %0, 0" : "=a"(x));
-  return x;
-}
 __device__ __forceinline__ float agpr_read(float x) {
   float v;
   asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(v) : "a"(x));
@@ -76,30 +71,29 @@ __device__ __forceinline__ float agpr_read(float x) {
 // Longer than any MFMA takes to write its result, or a write to reach one.
 __device__ __forceinline__ void agpr_settle() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
 
-// Four steps of the score product, x += k[i] q[i], x = 0 before the first of a tile.  In assembly because
-// the AGPRs have no room for x beside the accumulators and the compiler gives every MFMA of a kernel the
-// same register file.  It does not see the waits that its operands need, so they are here: two states
-// after a VALU write of an operand or another step on x (both pass while the matrix core is busy), and
-// after the last step enough for x to be read.
-template <bool kFirst, bool kLast>
-__device__ __forceinline__ void score_steps(f32x16& x, const bf16x8 (&k)[4], const bf16x8& q0, const bf16x8& q1, const bf16x8& q2,
-                                            const bf16x8& q3) {
-  if constexpr (kFirst)
-    asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %5, 0\n\t"
-                 "s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %2, %6, %0\n\t"
-                 "s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %3, %7, %0\n\t"
-                 "s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %4, %8, %0"
-                 : "=&v"(x)
-                 : "v"(k[0]), "v"(k[1]), "v"(k[2]), "v"(k[3]), "v"(q0), "v"(q1), "v"(q2), "v"(q3));
-  else
-    asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %5, %0\n\t"
-                 "s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %2, %6, %0\n\t"
-                 "s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %3, %7, %0\n\t"
-                 "s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %4, %8, %0"
-                 : "+v"(x)
-                 : "v"(k[0]), "v"(k[1]), "v"(k[2]), "v"(k[3]), "v"(q0), "v"(q1), "v"(q2), "v"(q3));
-  if constexpr (kLast) asm volatile("s_nop 15\n\ts_nop 7" : "+v"(x));
+// One step of the score product, x += k q (x = k q for the first of a tile).  In assembly because the
+// AGPRs have no room for x beside the accumulators and the compiler gives every MFMA of a kernel the same
+// register file.  It does not see the waits that such an operand needs, so they are here: two states after
+// a VALU write of an operand or another step on x (both pass while the matrix core is busy).  score_done()
+// stands between the last step and the first read of x.
+template <bool kFirst>
+__device__ __forceinline__ void score_step(f32x16& x, const bf16x8& k, const bf16x8& q) {
+  if constexpr (kFirst) asm("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(x) : "v"(k), "v"(q));
+  else asm("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(x) : "v"(k), "v"(q));
 }
+__device__ __forceinline__ void score_done(f32x16& x) { asm("s_nop 15\n\ts_nop 7" : "+v"(x)); }
+
+// f(0), f(1), .., f(kN - 1) with compile-time arguments.
+template <int kN, typename F, int kI = 0>
+__device__ __forceinline__ void static_for(F f) {
+  if constexpr (kI < kN) {
+    f(std::integral_constant<int, kI>{});
+    static_for<kN, F, kI + 1>(f);
+  }
+}
+
+// Nothing moves across: the order of a pipelined loop body is the source's.
+__device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); }
 
 template <int kHW>
 struct Shape {
@@ -147,21 +141,35 @@ __device__ __forceinline__ void run_segment(const Q4DecodeParams& p, const Segme
   // Pages of this wave's tiles, 64 at a time in a register (lane i: page page0 + i).
   int page0 = 0, pages = 0;
   auto fetch_pages = [&](int from) {
-    page0 = from;
-    const int i = page0 + lane;
+    page0 = uniform(from);
+    const int i = page0 + fresh_lane_id();
     pages = i < (sg.t1 + 1) / 2 ? p.block_table[sg.b * p.bt_sb + i] : 0;
+    asm volatile("" : "+v"(pages));   // waited for here, in the rare branch, and not by every reader
   };
   const unsigned ring_addr = lds_addr(lds.ring);
+  // LDS address of this wave's tile of step s, a scalar that the compiler cannot see through: it would keep
+  // an address per read up to date in the loop otherwise.
+  auto tile_addr = [&](int s) {
+    unsigned a = ring_addr + (unsigned)((s % S::kSlots) * S::kSlotBytes + kp * kTileBytes);
+    asm("" : "+s"(a));
+    return a;
+  };
+  // Address lane_off + add as one register; the reads through it carry their constant parts as offsets.
+  auto lds_at = [&](int lane_off, unsigned add) {
+    unsigned a;
+    asm("v_add_u32 %0, %1, %2" : "=v"(a) : "v"(lane_off), "s"(add));
+    return reinterpret_cast<const DMLA_LDS char*>(static_cast<uintptr_t>(a));
+  };
   // This wave's share of the copies of step s's tile kp: pieces hw, hw + kHW, ...
   auto copy_step = [&](int s) {
     const int t = min(sg.t0 + s * kKP + kp, sg.t1 - 1);   // past the end: the last tile, all masked
     if (t / 2 - page0 >= 64) fetch_pages(page0 + 64);
-    int page = __builtin_amdgcn_readlane(pages, (t / 2 - page0) & 63);
+    int page = __builtin_amdgcn_readlane(pages, uniform((t / 2 - page0) & 63));
     const bool bad = page < 0 || page >= p.num_pages;
     bad_page = bad_page || bad;
     page = bad ? 0 : page;
     const char* src = p.kv + page * p.kv_sp + (t & 1) * kTileBytes;
-    const unsigned dst = ring_addr + (unsigned)((s % S::kSlots) * S::kSlotBytes + kp * kTileBytes);
+    const unsigned dst = tile_addr(s);
     const int valid = sg.ctx - t * kTile;
     const int ln = fresh_lane_id();   // nothing of this is kept across the loop
 #pragma unroll
@@ -196,9 +204,8 @@ __device__ __forceinline__ void run_segment(const Q4DecodeParams& p, const Segme
       else *reinterpret_cast<DMLA_LDS bf16x8*>(q_lds + (c - S::kQRegs) * 1024) = v;   // the same from every kp
     }
   }
-  auto query = [&](int c) {
-    return c < S::kQRegs ? q[c < S::kQRegs ? c : 0]
-                         : lds_read_b128(reinterpret_cast<const DMLA_LDS bf16x8*>(q_lds + (c - S::kQRegs) * 1024));
+  auto query_lds = [&](int c) {
+    return lds_read_b128(reinterpret_cast<const DMLA_LDS bf16x8*>(q_lds + (c - S::kQRegs) * 1024));
   };
 
   f32x16 acc[kHW][kCols];   // O^T of 32 heads and 32 columns: row m is column (512 / kHW) hw + kCols m + j
@@ -206,27 +213,62 @@ __device__ __forceinline__ void run_segment(const Q4DecodeParams& p, const Segme
   bf16x8 pv[2];             // P of the wave's own heads, 16 keys each
 
   // S^T[key 8 (i / 4) + 4 hl + i % 4][head l32] of a tile.
-  auto scores = [&](int s, int t) -> f32x16 {
-    const DMLA_LDS char* row = lds.ring + (s % S::kSlots) * S::kSlotBytes + kp * kTileBytes + l32 * kQ4RowBytes;
+  // before_end runs while the last steps are in the matrix core.
+  auto scores = [&](int s, int t, auto before_end) -> f32x16 {
+    const unsigned tile = tile_addr(s);
+    const DMLA_LDS char* codes = lds_at(l32 * kQ4RowBytes + 128 * hl, tile);
+    const DMLA_LDS char* rope = lds_at(l32 * kQ4RowBytes + kQ4RopeOff + 16 * hl, tile);
+    // Blocks of four steps: codes are read two blocks ahead and converted one block ahead, a quarter of
+    // the next block's beside each MFMA; the queries kept in LDS are read one block ahead.
+    constexpr int kBlocks = kQ4LatentSteps / 4;
     f32x16 x;
-    const u32x2 scales = q4_key_scales(row, hl);
-    auto block = [&](auto a_tag) {
-      constexpr int kA = decltype(a_tag)::value;
-      const u32x4 w = q4_key_codes(row, hl, kA);
-      const float sc = q4_key_scale<kA>(scales);
-      const bf16x8 k[4] = {q4_octet(w[0], sc), q4_octet(w[1], sc), q4_octet(w[2], sc), q4_octet(w[3], sc)};
-      score_steps<kA == 0, false>(x, k, query(4 * kA), query(4 * kA + 1), query(4 * kA + 2), query(4 * kA + 3));
+    u32x4 w[3];
+    bf16x8 k[2][4], qx[2][4];
+    const u32x2 scales = *reinterpret_cast<const DMLA_LDS u32x2*>(lds_at(l32 * kQ4RowBytes + kQ4ScaleOff + 8 * hl, tile));
+    auto codes_of = [&](int a) { return *reinterpret_cast<const DMLA_LDS u32x4*>(codes + 16 * a); };
+    w[0] = codes_of(0);
+    w[1] = codes_of(1);
+    auto fetch_queries = [&](int a) {
+      if (4 * a >= S::kQRegs && a <= kBlocks) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) qx[a & 1][j] = query_lds(4 * a + j);
+      }
     };
-    block(std::integral_constant<int, 0>{});
-    block(std::integral_constant<int, 1>{});
-    block(std::integral_constant<int, 2>{});
-    block(std::integral_constant<int, 3>{});
-    block(std::integral_constant<int, 4>{});
-    block(std::integral_constant<int, 5>{});
-    block(std::integral_constant<int, 6>{});
-    block(std::integral_constant<int, 7>{});
-    const bf16x8 k[4] = {q4_key_rope(row, hl, 0), q4_key_rope(row, hl, 1), q4_key_rope(row, hl, 2), q4_key_rope(row, hl, 3)};
-    score_steps<false, true>(x, k, query(32), query(33), query(34), query(35));
+    auto query = [&](int a, int j) { return 4 * a < S::kQRegs ? q[4 * a < S::kQRegs ? 4 * a + j : 0] : qx[a & 1][j]; };
+    {
+      const float sc = q4_key_scale<0>(scales);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) k[0][j] = q4_octet(w[0][j], sc);
+    }
+    fetch_queries(0);
+    in_order();
+    auto block = [&](auto a_tag) {
+      constexpr int a = decltype(a_tag)::value;
+      if constexpr (a + 2 < kBlocks) w[(a + 2) % 3] = codes_of(a + 2);
+      fetch_queries(a + 1);
+      float sc = 0.f;
+      if constexpr (a + 1 < kBlocks) {
+        sc = q4_key_scale<a + 1>(scales);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) k[(a + 1) & 1][j] = lds_read_b128(reinterpret_cast<const DMLA_LDS bf16x8*>(rope + 32 * j));
+      }
+      in_order();
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (a == 0 && j == 0) score_step<true>(x, k[0][0], query(0, 0));
+        else score_step<false>(x, k[a & 1][j], query(a, j));
+        if constexpr (a + 1 < kBlocks) k[(a + 1) & 1][j] = q4_octet(w[(a + 1) % 3][j], sc);
+        in_order();
+      }
+    };
+    static_for<kBlocks>(block);
+    before_end();
+    in_order();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) score_step<false>(x, k[kBlocks & 1][j], query(kBlocks, j));
+    in_order();
+    score_done(x);
     const int left = t < sg.t1 ? sg.ctx - t * kTile : 0;   // keys of the tile
     if (left < kTile) {
 #pragma unroll
@@ -240,67 +282,96 @@ __device__ __forceinline__ void run_segment(const Q4DecodeParams& p, const Segme
     for (int i = 1; i < 16; ++i) mx = fmaxf(mx, x[i]);
     return half_max(mx) * p.scale_log2;   // scale > 0
   };
-  auto softmax = [&](const f32x16& x) {
-    mtrue = fmaxf(mtrue, tile_max(x));
-    const float ms = mref == kNegInf ? 0.f : mref;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float e = fast_exp2(__builtin_fmaf(x[i], p.scale_log2, -ms));
-      lsum += e;
-      pv[i >> 3][i & 7] = (bf16)e;
+  // The softmax of a tile in kPieces pieces, which the value product of another tile takes between its
+  // MFMAs: the maximum, then an element at a time.
+  constexpr int kPieces = 21;
+  float mx_part[4];
+  float ms = 0.f;
+  auto softmax_piece = [&](const f32x16& x, auto i_tag) {
+    constexpr int i = decltype(i_tag)::value;
+    if constexpr (i < 4) {
+      mx_part[i] = fmaxf(fmaxf(x[4 * i], x[4 * i + 1]), fmaxf(x[4 * i + 2], x[4 * i + 3]));
+    } else if constexpr (i == 4) {
+      const float mx = half_max(fmaxf(fmaxf(mx_part[0], mx_part[1]), fmaxf(mx_part[2], mx_part[3])));
+      mtrue = fmaxf(mtrue, mx * p.scale_log2);   // scale > 0
+      ms = mref == kNegInf ? 0.f : mref;
+    } else if constexpr (i < kPieces) {
+      constexpr int e = i - 5;
+      const float v = fast_exp2(__builtin_fmaf(x[e], p.scale_log2, -ms));
+      lsum += v;
+      pv[e >> 3][e & 7] = (bf16)v;
     }
   };
-  // O^T += V^T P of step s's tile; pb(n, u): P of head block n and the keys from 16 u on.
-  auto values = [&](int s, auto pb) {
-    const DMLA_LDS char* tile = lds.ring + (s % S::kSlots) * S::kSlotBytes + kp * kTileBytes;
-    constexpr int kWords = kCols >= 8 ? kCols / 8 : 1;
+  auto softmax = [&](const f32x16& x) {
+    static_for<kPieces>([&](auto i) { softmax_piece(x, i); });
+  };
+
+  // O^T += V^T P of step s's tile, in groups of a column pair: while a group's MFMAs run, the next group's
+  // codes are converted and between(i) is called after MFMA i, i = 0 .. 31.
+  constexpr int kWords = kCols >= 8 ? kCols / 8 : 1;   // words of codes per key
+  constexpr int kPairs = kCols / 2;                    // groups per 16 keys
+  struct Codes {
+    unsigned c[8][kWords];
+    float s[8];
+    bf16x8 p[kHW];
+  };
+  Codes cv[2];
+  // Codes, scales and probabilities of the keys from 16 u on; read_p(n, u): P of head block n.
+  auto read_codes = [&](int s, int u, auto read_p) {
+    const unsigned tile = tile_addr(s);
+    const DMLA_LDS char* codes = lds_at(4 * hl * kQ4RowBytes + (256 / kHW) * hw + (kCols / 2) * l32, tile);
+    const DMLA_LDS char* scales = lds_at(4 * hl * kQ4RowBytes + kQ4ScaleOff + (16 / kHW) * hw + l32 / (2 * kHW), tile);
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      unsigned vc[8][kWords];
-      float vs[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {   // the keys of the lane's scores
-        const DMLA_LDS char* row = tile + (16 * u + 8 * (j >> 2) + 4 * hl + (j & 3)) * kQ4RowBytes;
-        const DMLA_LDS char* at = row + (256 / kHW) * hw + (kCols / 2) * l32;
-        if constexpr (kCols == 16) {
-          const u32x2 w = *reinterpret_cast<const DMLA_LDS u32x2*>(at);
-          vc[j][0] = w[0];
-          vc[j][1] = w[1];
-        } else if constexpr (kCols == 8) {
-          vc[j][0] = *reinterpret_cast<const DMLA_LDS unsigned*>(at);
-        } else {
-          vc[j][0] = *reinterpret_cast<const DMLA_LDS uint16_t*>(at);
-        }
-        vs[j] = q4_scale(*reinterpret_cast<const DMLA_LDS uint8_t*>(row + kQ4ScaleOff + (16 / kHW) * hw + l32 / (2 * kHW)));
+    for (int j = 0; j < 8; ++j) {   // the keys of the lane's scores
+      const int row = (16 * u + 8 * (j >> 2) + (j & 3)) * kQ4RowBytes;
+      const DMLA_LDS char* at = codes + row;
+      if constexpr (kCols == 16) {
+        const u32x2 w = *reinterpret_cast<const DMLA_LDS u32x2*>(at);
+        cv[u].c[j][0] = w[0];
+        cv[u].c[j][1] = w[1];
+      } else if constexpr (kCols == 8) {
+        cv[u].c[j][0] = *reinterpret_cast<const DMLA_LDS unsigned*>(at);
+      } else {
+        cv[u].c[j][0] = *reinterpret_cast<const DMLA_LDS uint16_t*>(at);
       }
-      auto column_pair = [&](auto byte_tag, int d) {
-        constexpr int kB = decltype(byte_tag)::value;
-        unsigned e[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) e[j] = __builtin_bit_cast(unsigned, q4_pair<kB>(vc[j][d], vs[j]));
-        u32x4 even, odd;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          even[r] = __builtin_amdgcn_perm(e[2 * r + 1], e[2 * r], 0x05040100u);
-          odd[r] = __builtin_amdgcn_perm(e[2 * r + 1], e[2 * r], 0x07060302u);
-        }
-#pragma unroll
-        for (int n = 0; n < kHW; ++n) {
-          const int j = 8 * d + 2 * kB;
-          acc[n][j] = mfma32_bf16(__builtin_bit_cast(bf16x8, even), pb(n, u), acc[n][j]);
-          acc[n][j + 1] = mfma32_bf16(__builtin_bit_cast(bf16x8, odd), pb(n, u), acc[n][j + 1]);
-        }
-      };
-#pragma unroll
-      for (int d = 0; d < kWords; ++d) {
-        column_pair(std::integral_constant<int, 0>{}, d);
-        column_pair(std::integral_constant<int, 1>{}, d);
-        if constexpr (kCols >= 8) {
-          column_pair(std::integral_constant<int, 2>{}, d);
-          column_pair(std::integral_constant<int, 3>{}, d);
-        }
-      }
+      cv[u].s[j] = q4_scale(*reinterpret_cast<const DMLA_LDS uint8_t*>(scales + row));
     }
+#pragma unroll
+    for (int n = 0; n < kHW; ++n) cv[u].p[n] = read_p(n, u);
+  };
+  u32x4 even[2], odd[2];   // operands of two groups
+  // Keys 2 r and 2 r + 1 of group gi's operands.
+  auto convert = [&](auto g_tag, int r) {
+    constexpr int gi = decltype(g_tag)::value, u = gi / kPairs, cp = gi % kPairs;
+    const unsigned a = __builtin_bit_cast(unsigned, q4_pair<cp % 4>(cv[u].c[2 * r][cp / 4], cv[u].s[2 * r]));
+    const unsigned b = __builtin_bit_cast(unsigned, q4_pair<cp % 4>(cv[u].c[2 * r + 1][cp / 4], cv[u].s[2 * r + 1]));
+    even[gi & 1][r] = __builtin_amdgcn_perm(b, a, 0x05040100u);
+    odd[gi & 1][r] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+  };
+  auto values = [&](int s, auto read_p, auto between) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) convert(std::integral_constant<int, 0>{}, r);
+    read_codes(s, 1, read_p);
+    in_order();
+    static_for<2 * kPairs>([&](auto g_tag) {
+      constexpr int gi = decltype(g_tag)::value, u = gi / kPairs, cp = gi % kPairs;
+      static_for<2 * kHW>([&](auto i_tag) {
+        constexpr int i = decltype(i_tag)::value, n = i / 2, j = 2 * cp + (i & 1);
+        acc[n][j] = mfma32_bf16(__builtin_bit_cast(bf16x8, (i & 1) ? odd[gi & 1] : even[gi & 1]), cv[u].p[n], acc[n][j]);
+        if constexpr (gi + 1 < 2 * kPairs) {   // four quarters over the group's MFMAs
+          if constexpr (kHW == 4) {
+            if constexpr (i % 2 == 0) convert(std::integral_constant<int, gi + 1>{}, i / 2);
+          } else if constexpr (kHW == 2) {
+            convert(std::integral_constant<int, gi + 1>{}, i);
+          } else {
+            convert(std::integral_constant<int, gi + 1>{}, 2 * i);
+            convert(std::integral_constant<int, gi + 1>{}, 2 * i + 1);
+          }
+        }
+        between(std::integral_constant<int, gi * 2 * kHW + i>{});
+        in_order();
+      });
+    });
   };
   // P of step s through LDS, between the waves of a group.
   auto post = [&](int s) {
@@ -308,11 +379,10 @@ __device__ __forceinline__ void run_segment(const Q4DecodeParams& p, const Segme
 #pragma unroll
     for (int u = 0; u < 2; ++u) *reinterpret_cast<DMLA_LDS bf16x8*>(lds.p + (2 * at + u) * 1024 + lane * 16) = pv[u];
   };
-  auto shared_values = [&](int s) {
-    const int at = (s & 1) * kWaves + kp * kHW;
-    values(s, [&](int n, int u) {
-      return lds_read_b128(reinterpret_cast<const DMLA_LDS bf16x8*>(lds.p + (2 * (at + n) + u) * 1024 + lane * 16));
-    });
+  auto shared_p = [&](int s) {
+    const unsigned at = (unsigned)(2048 * ((s & 1) * kWaves + kp * kHW));
+    const DMLA_LDS char* from = lds_at(lane * 16, lds_addr(lds.p) + at);
+    return [from](int n, int u) { return lds_read_b128(reinterpret_cast<const DMLA_LDS bf16x8*>(from + 2048 * n + 1024 * u)); };
   };
 
   auto arrive = [&](int s, bool copy) {
@@ -331,35 +401,38 @@ __device__ __forceinline__ void run_segment(const Q4DecodeParams& p, const Segme
   // no rescaling of the outputs.
   for (bool again = false;; again = true) {
     arrive(0, true);
-    const f32x16 x0 = scores(0, sg.t0 + kp);
+    const f32x16 x0 = scores(0, sg.t0 + kp, [] {});
     mref = again ? mtrue : tile_max(x0);
     lsum = 0.f;
     if constexpr (kHW > 1) {
       softmax(x0);
       post(0);
     }
+    // Zeros by the matrix core, a whole accumulator at a time: element by element the compiler would
+    // assemble them elsewhere and move them.
 #pragma unroll
     for (int n = 0; n < kHW; ++n)
 #pragma unroll
-      for (int j = 0; j < kCols; ++j)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc[n][j][i] = agpr_zero();
-    agpr_settle();
+      for (int j = 0; j < kCols; ++j) acc[n][j] = mfma32_bf16(bf16x8{}, bf16x8{}, f32x16{});
+    wait_vm<0>();   // whatever the compiler has in flight, so that it does not wait for it in the loop
     if constexpr (kHW > 1) {
       // One step more than there are tiles, whose scores are all masked: no branch in the loop.
 #pragma nounroll
       for (int s = 1; s <= n_steps; ++s) {
         arrive(s, true);
-        shared_values(s - 1);
-        softmax(scores(s, sg.t0 + s * kKP + kp));
+        const auto read_p = shared_p(s - 1);
+        const f32x16 x = scores(s, sg.t0 + s * kKP + kp, [&] { read_codes(s - 1, 0, read_p); });
+        values(s - 1, read_p, [&](auto i) { softmax_piece(x, i); });
         post(s);
       }
     } else {
 #pragma nounroll
       for (int s = 0; s < n_steps; ++s) {
         arrive(s, s > 0);
-        softmax(scores(s, sg.t0 + s * kKP + kp));
-        values(s, [&](int, int u) { return pv[u]; });
+        softmax(scores(s, sg.t0 + s * kKP + kp, [] {}));
+        const auto own_p = [&](int, int u) { return pv[u]; };
+        read_codes(s, 0, own_p);
+        values(s, own_p, [](auto) {});
       }
     }
     const bool over = __any(mtrue > mref + kHeadroom);
