@@ -82,12 +82,21 @@ __device__ __forceinline__ float q4_key_scale(const u32x2& scales) {
   return q4_scale_of<kA % 4>(scales[kA / 4]);
 }
 
-// Wait until at most N vector-memory operations of this wave are outstanding.
+// Wait until at most N vector-memory (LDS) operations of this wave are outstanding; they end in order, and no
+// memory access moves across.
 template <int N>
 __device__ __forceinline__ void wait_vm() {
   static_assert(N >= 0 && N < 64, "vmcnt field");
+  asm volatile("" ::: "memory");
   __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | 0x0f70);
+  asm volatile("" ::: "memory");
 }
-__device__ __forceinline__ void wait_lds() { __builtin_amdgcn_s_waitcnt(0xc07f); }
+template <int N = 0>
+__device__ __forceinline__ void wait_lds() {
+  static_assert(N >= 0 && N < 16, "lgkmcnt field");
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xc07f | (N << 8));
+  asm volatile("" ::: "memory");
+}
 
 }  // namespace dmla
