@@ -45,7 +45,7 @@ __device__ __forceinline__ int key_swz(int r) { return (r & 3) << 2 | (r >> 2 & 
 
 struct Lds {
   unsigned keys, codes, rope, prob;   // addresses
-  DMLA_LDS float* stat;               // [kHeads][2]: references and sums
+  DMLA_LDS float* stat;               // [kHeads]: sums
   DMLA_LDS int* flag;                 // [kWaves]
 };
 
@@ -372,20 +372,27 @@ __device__ __forceinline__ void run_segment(const Q4DecodeParams& p, const Q4Seg
   // ---- the segment's output ----
   lsum = half_sum(lsum);
   agpr_settle();
-  if (hl == 0) {
-    lds.stat[2 * (wave * 32 + l32)] = mref;
-    lds.stat[2 * (wave * 32 + l32) + 1] = lsum;
-  }
+  if (hl == 0) lds.stat[wave * 32 + l32] = lsum;
   if (lane == 0) lds.flag[wave] = pages.bad ? 1 : 0;
   __syncthreads();
   const bool poison = (lds.flag[0] | lds.flag[1] | lds.flag[2] | lds.flag[3]) != 0;
-  // Through LDS, so that a store covers 256 bytes of each of 4 heads: stored as they lie in the registers,
-  // 32 bytes of 32 heads at a time, the outputs took 4.7 us of a segment.
+  if (hl == 0 && head0 + wave * 32 + l32 < p.H) {
+    const int head = head0 + wave * 32 + l32;
+    const float sum = poison ? __builtin_nanf("") : lsum;
+    const float lse = sum == 0.f ? kNegInf : (mref + __log2f(sum)) * kLn2;
+    if (sg.nsplit > 1) p.part_lse[(int64_t)sg.slot * p.H + head] = lse;
+    else if (p.lse != nullptr) p.lse[sg.b * p.H + head] = lse;
+  }
+  // Through LDS, so that a store covers 256 bytes of each of 4 heads.
   const unsigned unit = lds_sum(256 * l32, mine);   // 16-byte unit u of row r at u ^ r % 16
+  const unsigned from = lds_sum(256 * (lane >> 4) + 16 * ((lane & 15) ^ (lane >> 4)), mine);
+  const int64_t stride = sg.nsplit == 1 ? p.o_sh : kQ4Dv;
+  bf16* out = (sg.nsplit == 1 ? p.o + sg.b * p.o_sb : p.part_o + (int64_t)sg.slot * p.H * kQ4Dv) +
+              (head0 + (lane >> 4)) * stride + 128 * wave + 8 * (lane & 15);
+  const int heads = p.H - head0 - (lane >> 4);
 #pragma unroll
   for (int n = 0; n < kHeadBlocks; ++n) {
-    const float top = lds.stat[2 * (32 * n + l32)];
-    const float sum = poison ? __builtin_nanf("") : lds.stat[2 * (32 * n + l32) + 1];
+    const float sum = poison ? __builtin_nanf("") : lds.stat[32 * n + l32];
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
     for (int j = 0; j < kColBlocks; ++j)
@@ -396,18 +403,11 @@ __device__ __forceinline__ void run_segment(const Q4DecodeParams& p, const Q4Seg
         for (int i = 0; i < 8; ++i) v[i] = (bf16)(agpr_read(acc[n][j][8 * d + i]) * inv);
         *lds_ptr<bf16x8>(unit + 16 * ((4 * j + 2 * hl + d) ^ (l32 & 15))) = v;
       }
-    if (hl == 0 && wave == n && head0 + 32 * n + l32 < p.H) {
-      const int head = head0 + 32 * n + l32;
-      const float lse = sum == 0.f ? kNegInf : (top + __log2f(sum)) * kLn2;
-      if (sg.nsplit > 1) p.part_lse[(int64_t)sg.slot * p.H + head] = lse;
-      else if (p.lse != nullptr) p.lse[sg.b * p.H + head] = lse;
-    }
 #pragma unroll
-    for (int r = 0; r < 8; ++r) {
-      const int row = 4 * r + (lane >> 4), head = head0 + 32 * n + row;
-      const bf16x8 v = *lds_ptr<const bf16x8>(mine + 256 * row + 16 * ((lane & 15) ^ (row & 15)));
-      bf16* orow = sg.nsplit == 1 ? p.o + sg.b * p.o_sb + head * p.o_sh : p.part_o + ((int64_t)sg.slot * p.H + head) * kQ4Dv;
-      if (head < p.H) *reinterpret_cast<bf16x8*>(orow + 128 * wave + 8 * (lane & 15)) = v;
+    for (int r = 0; r < 8; ++r) {   // row 4 r + lane / 16
+      const bf16x8 v = *lds_ptr<const bf16x8>((from ^ (64 * (r & 3))) + 1024 * r);
+      if (32 * n + 4 * r < heads) *reinterpret_cast<bf16x8*>(out) = v;
+      out += 4 * stride;
     }
   }
 }
@@ -418,7 +418,7 @@ __global__ __launch_bounds__(kThreads, 1) void q4_wide_kernel(Q4DecodeParams p) 
   __shared__ __attribute__((aligned(1024))) char rope[kRopeSlots * kRopeBytes];
   __shared__ __attribute__((aligned(1024))) char prob[kProbBytes];
   __shared__ __attribute__((aligned(1024))) char codes[kCodeSlots * kCodeBytes];
-  __shared__ __attribute__((aligned(16))) float stat[2 * kHeads];
+  __shared__ __attribute__((aligned(16))) float stat[kHeads];
   __shared__ __attribute__((aligned(16))) int flag[kWaves];
   __shared__ __attribute__((aligned(16))) RangeLds ranges;
   const Lds lds = {lds_addr((DMLA_LDS char*)keys), lds_addr((DMLA_LDS char*)codes), lds_addr((DMLA_LDS char*)rope),

@@ -20,6 +20,17 @@ struct RangeLds {   // the segments of one chunk of kRangeThreads sequences
   int tmp[kRangeWaves];
 };
 
+// Sum over the lanes up to and including this one.
+__device__ __forceinline__ int lane_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);   // the lane 1, 2, 4, 8 before, in rows of 16
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);   // a row's last lane to the row after it
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);   // lane 31 to the upper half
+  return x;
+}
+
 // Calls segment(b, t0, t1, ctx, nsplit) for every piece of range r, with a barrier after each, and
 // owner(b, first_range, nsplit) on one thread for every sequence whose first tile lies in r (the empty
 // ones: r = 0).  All kRangeThreads threads take part.  ctx is the length, at most max_tokens.
@@ -30,40 +41,44 @@ __device__ __forceinline__ void for_each_segment(const int32_t* seqlens, int B, 
   const int tid = threadIdx.x;
   const int lane = tid & 63, wave = uniform(tid >> 6);
   auto length_of = [&](int b) { return b < B ? min(max(seqlens[b], 0), max_tokens) : 0; };
+  auto tiles_of = [&](int len) { return (len + kTokens - 1) / kTokens; };
   auto weight_of = [&](int nt) { return nt > 0 ? nt + kCost : 0; };
-  int ctx = length_of(tid);
-  int total = 0;
-  for (int c0 = 0; c0 < B; c0 += kRangeThreads)
-    total += weight_of(((c0 == 0 ? ctx : length_of(c0 + tid)) + kTokens - 1) / kTokens);
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) total += __shfl_xor(total, o, 64);
-  if (lane == 0) lds.tmp[wave] = total;
-  __syncthreads();
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < kRangeWaves; ++w) total += lds.tmp[w];
-  const int width = max(min_width, (total + n_ranges - 1) / n_ranges);
-  int carry = 0;
-  for (int c0 = 0; c0 < B; c0 += kRangeThreads) {
-    const int b = c0 + tid;
-    if (c0 > 0) ctx = length_of(b);
-    const int nt = (ctx + kTokens - 1) / kTokens, w = weight_of(nt);
-    int x = w;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int y = __shfl_up(x, o, 64);
-      if (lane >= o) x += y;
-    }
-    __syncthreads();   // tmp has been read
+  // Sum of the threads' w up to this one; sum: over all.  The first use of lds.tmp, or after a barrier.
+  auto scan = [&](int w, int& sum) {
+    int x = lane_scan(w);
     if (lane == 63) lds.tmp[wave] = x;
     __syncthreads();
-    int before = carry;
+    sum = 0;
 #pragma unroll
     for (int v = 0; v < kRangeWaves; ++v) {
-      if (v < wave) before += lds.tmp[v];
-      carry += lds.tmp[v];
+      if (v < wave) x += lds.tmp[v];
+      sum += lds.tmp[v];
     }
-    const int first_tile = before + x - w + kCost;   // weighted position of the sequence's first tile
+    return x;
+  };
+  int ctx = length_of(tid);
+  int chunk = 0;   // weight of the chunk
+  int x = scan(weight_of(tiles_of(ctx)), chunk);
+  int total = chunk;
+  if (B > kRangeThreads) {
+    int w = 0, rest = 0;
+    for (int c0 = kRangeThreads; c0 < B; c0 += kRangeThreads) w += weight_of(tiles_of(length_of(c0 + tid)));
+    __syncthreads();   // tmp has been read
+    scan(w, rest);
+    total += rest;
+  }
+  const int width = max(min_width, (total + n_ranges - 1) / n_ranges);
+  int carry = 0;   // weight of the chunks before
+  for (int c0 = 0; c0 < B; c0 += kRangeThreads) {
+    const int b = c0 + tid;
+    if (c0 > 0) {
+      ctx = length_of(b);
+      __syncthreads();   // tmp has been read
+      x = scan(weight_of(tiles_of(ctx)), chunk);
+    }
+    const int nt = tiles_of(ctx), w = weight_of(nt);
+    const int first_tile = carry + x - w + kCost;   // weighted position of the sequence's first tile
+    carry += chunk;
     const int fr = first_tile / width;
     const int ns = nt > 0 ? (first_tile + nt - 1) / width - fr + 1 : 0;
     const int64_t at = (int64_t)r * width - first_tile;   // 64 bits: the last ranges may start past the total
