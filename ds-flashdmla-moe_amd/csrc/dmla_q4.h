@@ -9,6 +9,8 @@
 // held as that), so code x scale is exact in bf16 and reading a row back rounds nothing.  The rope
 // values carry the position and stay in bf16.  A block that holds an infinity or a NaN is all NaN.
 #pragma once
+#include <type_traits>
+
 #include "dmla_common.h"
 
 namespace dmla {
@@ -57,29 +59,57 @@ __device__ __forceinline__ bf16x8 q4_octet(unsigned w, float scale) {
 // ---- key rows as an MFMA operand ----------------------------------------------------------------
 // Score product of 32 keys with 32 queries: 32 bf16 MFMAs (32x32x16) of the latent dims and 4 of the rope
 // dims, lane l holding key l % 32.  Which dims the two lane halves hold is free as long as the queries
-// agree: half h takes the dims 256 h + 8 c + x in MFMA c, so its codes are 128 contiguous bytes of the row
-// (eight LDS reads, a scale block each) and its scales two words.  Rows of 400 bytes put 16 consecutive rows
-// of such a read into 16 different 16-byte columns of the LDS banks.
+// agree: in MFMA 4 a + j half h takes the dims 64 a + 32 h + 8 j + x, so a lane reads 16 bytes of codes, a
+// scale block, for four MFMAs.  Rows of 400 bytes put 16 consecutive rows of such a read into 16 different
+// 16-byte columns of the LDS banks.
 constexpr int kQ4Steps = 36;        // MFMAs of a 32-key tile
 constexpr int kQ4LatentSteps = 32;
 
-// Query operand of MFMA c for lane half h.
+// First dim of half h in MFMA c, in units of 8 dims.
+__host__ __device__ constexpr int q4_operand_unit(int h, int c) {
+  return c < kQ4LatentSteps ? 8 * (c / 4) + 4 * h + c % 4 : 2 * c + h;
+}
 __device__ __forceinline__ bf16x8 q4_query_operand(const bf16* q, int h, int c) {
-  return *reinterpret_cast<const bf16x8*>(c < kQ4LatentSteps ? q + 256 * h + 8 * c : q + 512 + 16 * (c - kQ4LatentSteps) + 8 * h);
+  return *reinterpret_cast<const bf16x8*>(q + 8 * q4_operand_unit(h, c));
 }
-// Codes of MFMAs 4 a .. 4 a + 3, all scales, and rope operand c of this lane's row.
+// Codes of MFMAs 4 a .. 4 a + 3, all scales of the half (byte 2 (a % 2) of word a / 2), and rope operand c of
+// this lane's row.
 __device__ __forceinline__ u32x4 q4_key_codes(const DMLA_LDS char* row, int h, int a) {
-  return *reinterpret_cast<const DMLA_LDS u32x4*>(row + 128 * h + 16 * a);
+  return *reinterpret_cast<const DMLA_LDS u32x4*>(row + 32 * a + 16 * h);
 }
-__device__ __forceinline__ u32x2 q4_key_scales(const DMLA_LDS char* row, int h) {
-  return *reinterpret_cast<const DMLA_LDS u32x2*>(row + kQ4ScaleOff + 8 * h);
+__device__ __forceinline__ u32x4 q4_key_scales(const DMLA_LDS char* row, int h) {
+  return *reinterpret_cast<const DMLA_LDS u32x4*>(row + kQ4ScaleOff) >> (unsigned)(8 * h);
 }
 __device__ __forceinline__ bf16x8 q4_key_rope(const DMLA_LDS char* row, int h, int c) {
   return lds_read_b128(reinterpret_cast<const DMLA_LDS bf16x8*>(row + kQ4RopeOff + 32 * c + 16 * h));
 }
 template <int kA>
-__device__ __forceinline__ float q4_key_scale(const u32x2& scales) {
-  return q4_scale_of<kA % 4>(scales[kA / 4]);
+__device__ __forceinline__ float q4_key_scale(const u32x4& scales) {
+  return q4_scale_of<2 * (kA % 2)>(scales[kA / 2]);
+}
+
+// f(0), f(1), .., f(kN - 1) with compile-time arguments.
+template <int kN, typename F, int kI = 0>
+__device__ __forceinline__ void static_for(F f) {
+  if constexpr (kI < kN) {
+    f(std::integral_constant<int, kI>{});
+    static_for<kN, F, kI + 1>(f);
+  }
+}
+
+// Nothing moves across: the order of a pipelined loop body is the source's.
+__device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); }
+
+// Address lane_off + add as one register that the compiler does not see into: it would keep an address per
+// read up to date in a loop otherwise.
+__device__ __forceinline__ unsigned lds_sum(int lane_off, unsigned add) {
+  unsigned a;
+  asm("v_add_u32 %0, %1, %2" : "=v"(a) : "v"(lane_off), "s"(add));
+  return a;
+}
+template <typename T>
+__device__ __forceinline__ DMLA_LDS T* lds_ptr(unsigned addr) {
+  return reinterpret_cast<DMLA_LDS T*>(static_cast<uintptr_t>(addr));
 }
 
 // Wait until at most N vector-memory (LDS) operations of this wave are outstanding; they end in order, and no

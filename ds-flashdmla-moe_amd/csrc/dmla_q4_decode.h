@@ -1,8 +1,6 @@
 // What the two kernels of the 4-bit decode share (dmla_q4_decode.hip up to 32 heads a workgroup,
 // dmla_q4_wide.hip up to 128).
 #pragma once
-#include <type_traits>
-
 #include "dmla_q4.h"
 #include "dmla_ranges.h"
 
@@ -61,30 +59,6 @@ __device__ __forceinline__ void score_step(f32x16& x, const bf16x8& k, const bf1
   else asm("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(x) : "v"(k), "v"(q));
 }
 __device__ __forceinline__ void score_done(f32x16& x) { asm("s_nop 15\n\ts_nop 7" : "+v"(x)); }
-
-// f(0), f(1), .., f(kN - 1) with compile-time arguments.
-template <int kN, typename F, int kI = 0>
-__device__ __forceinline__ void static_for(F f) {
-  if constexpr (kI < kN) {
-    f(std::integral_constant<int, kI>{});
-    static_for<kN, F, kI + 1>(f);
-  }
-}
-
-// Nothing moves across: the order of a pipelined loop body is the source's.
-__device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); }
-
-// Address lane_off + add as one register that the compiler does not see into: it would keep an address per
-// read up to date in a loop otherwise.
-__device__ __forceinline__ unsigned lds_sum(int lane_off, unsigned add) {
-  unsigned a;
-  asm("v_add_u32 %0, %1, %2" : "=v"(a) : "v"(lane_off), "s"(add));
-  return a;
-}
-template <typename T>
-__device__ __forceinline__ DMLA_LDS T* lds_ptr(unsigned addr) {
-  return reinterpret_cast<DMLA_LDS T*>(static_cast<uintptr_t>(addr));
-}
 
 // The pages of a segment, 64 at a time in a register (lane i: page first + i).
 struct Q4Pages {

@@ -38,7 +38,7 @@ constexpr int kSlotBytes = kWaves * kTileBytes, kSlots = 3;
 constexpr int kRingBytes = kSlots * kSlotBytes;
 constexpr int kMergeRow = 128 + 4;             // floats, padded against bank conflicts
 static_assert(kWaves * kHeads * kMergeRow * 4 <= kRingBytes, "the merge reuses the ring");
-constexpr int kSegCost = 16;
+constexpr int kSegCost = 24;
 
 struct Lds {
   DMLA_LDS char* ring;
@@ -100,7 +100,7 @@ __device__ __forceinline__ void run_segment(const Q4DecodeParams& p, const Q4Seg
   // S^T[key 8 (i / 4) + 4 hl + i % 4][head l32] of a tile.
   auto scores = [&](int s, int t) -> f32x16 {
     const unsigned tile = tile_addr(s);
-    const DMLA_LDS char* codes = lds_at(l32 * kQ4RowBytes + 128 * hl, tile);
+    const DMLA_LDS char* codes = lds_at(l32 * kQ4RowBytes + 16 * hl, tile);
     const DMLA_LDS char* rope = lds_at(l32 * kQ4RowBytes + kQ4RopeOff + 16 * hl, tile);
     // Blocks of four steps: codes are read two blocks ahead and converted one block ahead, a quarter of
     // the next block's beside each MFMA.
@@ -108,8 +108,8 @@ __device__ __forceinline__ void run_segment(const Q4DecodeParams& p, const Q4Seg
     f32x16 x;
     u32x4 w[3];
     bf16x8 k[2][4];
-    const u32x2 scales = *reinterpret_cast<const DMLA_LDS u32x2*>(lds_at(l32 * kQ4RowBytes + kQ4ScaleOff + 8 * hl, tile));
-    auto codes_of = [&](int a) { return *reinterpret_cast<const DMLA_LDS u32x4*>(codes + 16 * a); };
+    const u32x4 scales = q4_key_scales(lds_at(l32 * kQ4RowBytes, tile), hl);
+    auto codes_of = [&](int a) { return *reinterpret_cast<const DMLA_LDS u32x4*>(codes + 32 * a); };
     w[0] = codes_of(0);
     w[1] = codes_of(1);
     {
@@ -427,7 +427,7 @@ extern "C" int dmla_decode_paged_q4(const void* q, const void* kv_pool, const in
     p.min_width = 32;
     hipLaunchKernelGGL(q4_decode_kernel, dim3((unsigned)grid), dim3(kThreads), 0, (hipStream_t)stream, p);
   } else {
-    p.min_width = 8;
+    p.min_width = 4;
     launch_q4_wide(p, grid, (hipStream_t)stream);
   }
   const int rc = check_launch("dmla_decode_paged_q4");

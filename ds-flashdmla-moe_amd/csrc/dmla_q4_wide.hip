@@ -38,7 +38,7 @@ constexpr int kRopeBytes = kTile * 128, kRopeSlots = 4;
 constexpr int kProbBytes = kWaves * 2048;      // P of a step
 constexpr int kAhead = 4;                      // tiles between a copy's start and its step
 constexpr int kCopies = 4;                     // copies of a wave and step
-constexpr int kSegCost = 5;
+constexpr int kSegCost = 8;
 
 // Unit permutation of row r: 16 consecutive rows differ, and rows r .. r + 3 differ in the upper two bits.
 __device__ __forceinline__ int key_swz(int r) { return (r & 3) << 2 | (r >> 2 & 3); }

@@ -15,7 +15,8 @@ namespace dmla {
 constexpr int kRangeThreads = 256, kRangeWaves = kRangeThreads / 64;
 
 struct RangeLds {   // the segments of one chunk of kRangeThreads sequences
-  int lo[kRangeThreads], hi[kRangeThreads], ctx[kRangeThreads], nsplit[kRangeThreads];
+  int lo[kRangeThreads], hi[kRangeThreads], ctx[kRangeThreads];
+  unsigned short nsplit[kRangeThreads];   // at most a part per workgroup
   unsigned long long live[kRangeWaves];
   int tmp[kRangeWaves];
 };
@@ -33,20 +34,21 @@ __device__ __forceinline__ int lane_scan(int x) {
 
 // Calls segment(b, t0, t1, ctx, nsplit) for every piece of range r, with a barrier after each, and
 // owner(b, first_range, nsplit) on one thread for every sequence whose first tile lies in r (the empty
-// ones: r = 0).  All kRangeThreads threads take part.  ctx is the length, at most max_tokens.
+// ones: r = 0).  All threads of the workgroup take part, those past kRangeThreads in the barriers.  ctx is the length, at most max_tokens.
 // The weights' sum stays below 2^31 (checked on the host).
 template <int kTokens, int kCost, typename SegmentFn, typename OwnerFn>
 __device__ __forceinline__ void for_each_segment(const int32_t* seqlens, int B, int max_tokens, int n_ranges, int min_width,
                                                  int r, RangeLds& lds, SegmentFn segment, OwnerFn owner) {
   const int tid = threadIdx.x;
   const int lane = tid & 63, wave = uniform(tid >> 6);
-  auto length_of = [&](int b) { return b < B ? min(max(seqlens[b], 0), max_tokens) : 0; };
+  const bool in = tid < kRangeThreads;
+  auto length_of = [&](int b) { return in && b < B ? min(max(seqlens[b], 0), max_tokens) : 0; };
   auto tiles_of = [&](int len) { return (len + kTokens - 1) / kTokens; };
   auto weight_of = [&](int nt) { return nt > 0 ? nt + kCost : 0; };
   // Sum of the threads' w up to this one; sum: over all.  The first use of lds.tmp, or after a barrier.
   auto scan = [&](int w, int& sum) {
     int x = lane_scan(w);
-    if (lane == 63) lds.tmp[wave] = x;
+    if (in && lane == 63) lds.tmp[wave] = x;
     __syncthreads();
     sum = 0;
 #pragma unroll
@@ -83,13 +85,15 @@ __device__ __forceinline__ void for_each_segment(const int32_t* seqlens, int B, 
     const int ns = nt > 0 ? (first_tile + nt - 1) / width - fr + 1 : 0;
     const int64_t at = (int64_t)r * width - first_tile;   // 64 bits: the last ranges may start past the total
     const int lo = (int)min(max(at, (int64_t)0), (int64_t)nt), hi = (int)min(max(at + width, (int64_t)0), (int64_t)nt);
-    lds.lo[tid] = lo;
-    lds.hi[tid] = hi;
-    lds.ctx[tid] = ctx;
-    lds.nsplit[tid] = ns;
     const unsigned long long live = __ballot(hi > lo);
-    if (lane == 0) lds.live[wave] = live;
-    if (b < B && (nt > 0 ? r == fr : r == 0)) owner(b, fr, ns);
+    if (in) {
+      lds.lo[tid] = lo;
+      lds.hi[tid] = hi;
+      lds.ctx[tid] = ctx;
+      lds.nsplit[tid] = (unsigned short)ns;
+      if (lane == 0) lds.live[wave] = live;
+    }
+    if (in && b < B && (nt > 0 ? r == fr : r == 0)) owner(b, fr, ns);
     __syncthreads();
     for (int v = 0; v < kRangeWaves; ++v) {
       const unsigned long long lv = lds.live[v];
