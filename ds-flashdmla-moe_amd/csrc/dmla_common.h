@@ -278,6 +278,17 @@ __device__ __forceinline__ int fast_div(int n, FastDiv f) {
   return f.m ? (int)(__umulhi((unsigned)n, f.m) >> f.shift) : n;
 }
 
+// Sum over the lanes up to and including this one.
+__device__ __forceinline__ int lane_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);   // the lane 1, 2, 4, 8 before, in rows of 16
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);   // a row's last lane to the row after it
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);   // lane 31 to the upper half
+  return x;
+}
+
 // Reductions over the four 16-lane groups of a wave (lanes l, l^16, l^32, l^48: the lanes that
 // share one MFMA column) with the gfx950 row-swap instructions.  Called with the same value in
 // both operands, permlane16_swap / permlane32_swap return, in some order, a lane's value and

@@ -10,10 +10,18 @@
 // Cutting 4096 + 64 tokens back to 4096 with R = 256 then moves at most 64 + 256 rows, where closing every
 // gap would move nearly all.  No reference counterpart.
 //
-// Three launches: the selection (one workgroup per sequence), the middle moves together with a copy of
-// the newest rows into the workspace where their old and new places overlap (N - K < R), and the newest
-// rows' move.  A middle move's destination is a freed place and its source lies at or past K - R, so those moves
-// depend on nothing; the newest rows overwrite such sources and therefore come last.
+// The selection is a radix select of the accounts' keys (digits of 11, 11 and 10 bits) and a pass in index
+// order that lists the freed places and the rows that fill them.
+//   * Up to kOneTokens tokens one workgroup per sequence holds the accounts in registers and does it all in one
+//     launch (64 sequences of 4096 to 8192 tokens: see the figures in evict_select_kernel).
+//   * Longer block tables: up to kMaxChunks workgroups per sequence, a launch per digit and one for the lists.  A
+//     chunk's counts go through the workspace and every workgroup adds up all chunks', so nothing is cleared
+//     beforehand and nothing depends on the order of atomics.  No chunk straddles the end of the kept low
+//     places: how many places a chunk frees, or how many rows it moves, follows from its counts alone.
+// Then come the middle moves, together with a copy of the newest rows into the workspace where their old and new
+// places overlap (N - K < R), and the newest rows' move.  A middle move's destination is a freed place and its
+// source lies at or past K - R, so those moves depend on nothing; the newest rows overwrite such sources and
+// therefore come last.
 #include <algorithm>
 
 #include "dmla_common.h"
@@ -25,8 +33,13 @@ namespace {
 constexpr int kPage = 64;
 constexpr int kSelThreads = 1024;
 constexpr int kSelWaves = kSelThreads / 64;
-constexpr int kDigitBits = 11, kBins = 1 << kDigitBits;   // radix digits of 11, 11 and 10 bits
-constexpr int kPerThread = 16;   // consecutive tokens of a thread in the ordered pass
+constexpr int kDigitBits = 11, kBins = 1 << kDigitBits;
+constexpr int kOneTokens = 16 * kSelThreads;
+constexpr int kMaxChunks = 16;
+constexpr int kPiece = 8;          // tokens of a thread at a time in a chunk
+constexpr int kMoveRows = 32;      // rows that a workgroup moves at a time
+constexpr int kMoveBatch = 5;      // 16-byte pieces of a thread in flight (32 bf16 rows are nine for each thread)
+#define Global __attribute__((address_space(1)))
 
 struct EvictArgs {
   char* pool;
@@ -46,6 +59,10 @@ struct EvictArgs {
   int32_t* free_at;      // [B][budget - recent - sink] freed places, and the rows that fill them
   int32_t* late_at;
   char* stage;           // [B][recent] rows
+  int32_t* counts;       // [2][B][kMaxChunks][kBins], long tables only, as the next two
+  int32_t* above;        // [B][kMaxChunks]: tokens of a chunk whose key lies above the digits picked so far
+  int32_t* sel;          // [2][B][2]: those digits, and how many of the tokens that share them are kept
+  FastDiv per_row;       // division by row_chunks
 };
 
 // An integer that orders like the account: larger is better, -0 equals 0, NaN above everything.
@@ -59,12 +76,7 @@ __device__ __forceinline__ unsigned rank_key(float f) {
 // Exclusive prefix of v over the workgroup; total gets the sum.  tmp: kSelWaves ints.
 __device__ __forceinline__ int scan_exclusive(int v, int* tmp, int& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int x = v;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int y = __shfl_up(x, o, 64);
-    if (lane >= o) x += y;
-  }
+  const int x = lane_scan(v);
   __syncthreads();   // tmp is free
   if (lane == 63) tmp[wave] = x;
   __syncthreads();
@@ -79,179 +91,447 @@ __device__ __forceinline__ int scan_exclusive(int v, int* tmp, int& total) {
   return before + x - v;
 }
 
-__global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictArgs a) {
-  __shared__ int hist[kBins];
-  __shared__ int tmp[kSelWaves];
-  __shared__ int pick[2];   // the digit that holds the last kept key, and how many keys lie above it
-  const int tid = threadIdx.x;
-  for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
-    const int n = min(max(a.seqlens[b], 0), a.max_pages * kPage);
-    const float* mass = a.mass + b * a.m_sb;
-    float* mass_out = a.mass_out + b * a.mo_sb;
-    int32_t* src = a.src + b * a.src_sb;
-    int bad = 0;
-    if (n > a.budget)
-      for (int i = tid; i < (n + kPage - 1) / kPage; i += kSelThreads) {
-        const int page = a.block_table[b * a.bt_sb + i];
-        bad |= page < 0 || page >= a.num_pages;
-      }
-    bad = __syncthreads_or(bad);
-    if (bad && a.bad != nullptr && tid == 0) a.bad[0] = 1;
-    const bool cut = n > a.budget && !bad;
-    const int new_len = cut ? a.budget : n;
-    if (!cut) {
-      if (tid == 0) {
-        a.new_lens[b] = n;
-        a.info[2 * b] = 0;
-        a.info[2 * b + 1] = 0;
-      }
-      for (int i = tid; i < a.width; i += kSelThreads) src[i] = i < n ? i : -1;
-      for (int i = tid; i < a.mass_len; i += kSelThreads) mass_out[i] = i < n ? mass[i] : 0.f;
-      continue;
+struct Shared {
+  int hist[kBins];
+  int tmp[kSelWaves];
+  int pick[2];                     // the digit that holds the last kept key, and how many keys lie above it
+  int rank[16 * kSelWaves + 1];    // by 64 consecutive tokens: counts, then their exclusive prefix and sum
+  int kept[kMaxChunks], equal[kMaxChunks];
+};
+
+// A sequence's cut: N tokens down to the budget.
+struct Cut {
+  int n, lo, hi, low_end, want;   // the middle tokens [lo, hi), and the places [lo, low_end) of the kept ones
+};
+__device__ __forceinline__ Cut cut_of(const EvictArgs& a, int b) {
+  Cut c;
+  c.n = min(max(a.seqlens[b], 0), a.max_pages * kPage);
+  c.lo = a.sink;
+  c.hi = c.n - a.recent;
+  c.low_end = a.budget - a.recent;
+  c.want = c.low_end - c.lo;
+  return c;
+}
+
+// Whether the sequence is cut: it is longer than the budget and its pages are all in the pool.
+__device__ __forceinline__ bool is_cut(const EvictArgs& a, int b, const Cut& c) {
+  int bad = 0;
+  if (c.n > a.budget)
+    for (int i = threadIdx.x; i < (c.n + kPage - 1) / kPage; i += kSelThreads) {
+      const int page = a.block_table[b * a.bt_sb + i];
+      bad |= page < 0 || page >= a.num_pages;
     }
-    const int lo = a.sink, hi = n - a.recent;      // the middle tokens
-    const int low_end = a.budget - a.recent;       // places of the kept ones: [lo, low_end)
-    const int want = low_end - lo;
-    // Radix select: the key of the last kept middle token, digit by digit, and how many tokens with
-    // exactly that key are kept.
-    unsigned prefix = 0, mask = 0;
-    int left = want;   // how many are still to be taken from the tokens whose key matches prefix
-    for (int d = 0; d < 3 && want > 0; ++d) {
-      const int shift = d == 0 ? 21 : d == 1 ? 10 : 0;
-      const int bins = d == 2 ? 1 << 10 : kBins;
-      for (int i = tid; i < bins; i += kSelThreads) hist[i] = 0;
-      __syncthreads();
-      for (int i = lo + tid; i < hi; i += kSelThreads) {
-        const unsigned key = rank_key(mass[i]);
-        if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & (bins - 1)], 1);
-      }
-      __syncthreads();
-      // bins from the top: thread t holds the bins - 1 - 2t and the one below
-      const int top = bins - 1 - 2 * tid;
-      const int c0 = top >= 0 ? hist[top] : 0, c1 = top >= 1 ? hist[top - 1] : 0;
-      int total;
-      const int above = scan_exclusive(c0 + c1, tmp, total);
-      if (above < left && left <= above + c0) {
-        pick[0] = top;
-        pick[1] = above;
-      } else if (above + c0 < left && left <= above + c0 + c1) {
-        pick[0] = top - 1;
-        pick[1] = above + c0;
-      }
-      __syncthreads();
-      prefix |= (unsigned)pick[0] << shift;
-      mask |= (unsigned)(bins - 1) << shift;
-      left -= pick[1];
-      __syncthreads();
+  bad = __syncthreads_or(bad);
+  if (bad && a.bad != nullptr && threadIdx.x == 0) a.bad[0] = 1;
+  return c.n > a.budget && !bad;
+}
+
+// The outputs of a sequence that stays as it is, by the threads first, first + step, ...
+__device__ __forceinline__ void leave(const EvictArgs& a, int b, const Cut& c, int first, int step) {
+  if (first == 0) {
+    a.new_lens[b] = c.n;
+    a.info[2 * b] = 0;
+    a.info[2 * b + 1] = 0;
+  }
+  for (int i = first; i < a.width; i += step) a.src[b * a.src_sb + i] = i < c.n ? i : -1;
+  for (int i = first; i < a.mass_len; i += step) a.mass_out[b * a.mo_sb + i] = i < c.n ? a.mass[b * a.m_sb + i] : 0.f;
+}
+
+// The outputs of a cut sequence outside the middle, likewise.
+__device__ __forceinline__ void put_ends(const EvictArgs& a, int b, const Cut& c, int first, int step) {
+  int32_t* src = a.src + b * a.src_sb;
+  float* out = a.mass_out + b * a.mo_sb;
+  const float* mass = a.mass + b * a.m_sb;
+  for (int i = first; i < c.lo; i += step) {
+    src[i] = i;
+    out[i] = mass[i];
+  }
+  for (int i = first; i < a.recent; i += step) {
+    src[c.low_end + i] = c.hi + i;
+    out[c.low_end + i] = mass[c.hi + i];
+  }
+  for (int i = a.budget + first; i < a.mass_len; i += step) out[i] = 0.f;
+}
+
+// Digits: bits 21.., 10.. and 0.. of the key.
+__device__ __forceinline__ int digit_shift(int d) { return d == 0 ? 21 : d == 1 ? 10 : 0; }
+__device__ __forceinline__ int digit_bins(int d) { return d == 2 ? 1 << 10 : kBins; }
+
+// Thread t brings the counts of the bins top = bins - 1 - 2 t and top - 1; the digit whose bin holds the left-th key
+// from above becomes part of prefix, and left counts within it.  Returns the digit.
+__device__ __forceinline__ int pick_digit(Shared& sh, int d, int top, int c0, int c1, unsigned& prefix, int& left) {
+  int total;
+  const int above = scan_exclusive(c0 + c1, sh.tmp, total);
+  if (above < left && left <= above + c0) {
+    sh.pick[0] = top;
+    sh.pick[1] = above;
+  } else if (above + c0 < left && left <= above + c0 + c1) {
+    sh.pick[0] = top - 1;
+    sh.pick[1] = above + c0;
+  }
+  __syncthreads();
+  const int digit = sh.pick[0];
+  prefix |= (unsigned)digit << digit_shift(d);
+  left -= sh.pick[1];
+  return digit;
+}
+
+// Exclusive prefix over the counts in sh.rank (groups of 64 tokens in index order); the sum behind them.
+template <int kGroups>
+__device__ __forceinline__ void scan_ranks(Shared& sh) {
+  __syncthreads();
+  if (threadIdx.x < 64) {
+    constexpr int kEach = kGroups / 64;
+    int v[kEach], sum = 0;
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      v[k] = sh.rank[threadIdx.x * kEach + k];
+      sum += v[k];
     }
-    // In index order: which tokens stay, which places below low_end are freed, which rows fill them.
-    int32_t* free_at = a.free_at + (int64_t)b * want;
-    int32_t* late_at = a.late_at + (int64_t)b * want;
-    int eq_seen = 0, n_free = 0, n_late = 0;
-    for (int base = 0; base < hi && want > 0; base += kSelThreads * kPerThread) {
-      const int i0 = base + tid * kPerThread;
-      unsigned above = 0, equal = 0;   // one bit per token
+    const int x = lane_scan(sum);
+    int at = x - sum;
 #pragma unroll
-      for (int j = 0; j < kPerThread; ++j) {
-        const int i = i0 + j;
-        if (i < lo || i >= hi) continue;
-        const unsigned key = rank_key(mass[i]);
-        above |= (key > prefix ? 1u : 0u) << j;
-        equal |= (key == prefix ? 1u : 0u) << j;
-      }
-      int total;
-      int rank = eq_seen + scan_exclusive(__popc(equal), tmp, total);
-      eq_seen += total;
-      unsigned kept = above;
-#pragma unroll
-      for (int j = 0; j < kPerThread; ++j)
-        if ((equal >> j) & 1) kept |= (rank++ < left ? 1u : 0u) << j;
-      unsigned below = 0, middle = 0;
-#pragma unroll
-      for (int j = 0; j < kPerThread; ++j) {
-        below |= (i0 + j < low_end ? 1u : 0u) << j;
-        middle |= (i0 + j >= lo && i0 + j < hi ? 1u : 0u) << j;
-      }
-      const unsigned freed = middle & below & ~kept, late = kept & ~below;
-      // both ranks in one scan: a batch of 16384 tokens keeps either sum below 16 bits
-      const int before = scan_exclusive(__popc(freed) | __popc(late) << 16, tmp, total);
-      int fr = n_free + (before & 0xffff), lr = n_late + (before >> 16);
-      n_free += total & 0xffff;
-      n_late += total >> 16;
-#pragma unroll
-      for (int j = 0; j < kPerThread; ++j) {
-        if ((freed >> j) & 1) free_at[fr++] = i0 + j;
-        if ((late >> j) & 1) late_at[lr++] = i0 + j;
-        if ((kept & below) >> j & 1) src[i0 + j] = i0 + j;
-      }
+    for (int k = 0; k < kEach; ++k) {
+      sh.rank[threadIdx.x * kEach + k] = at;
+      at += v[k];
     }
-    if (tid == 0) {
-      a.new_lens[b] = new_len;
-      a.info[2 * b] = n - a.budget;
-      a.info[2 * b + 1] = n_late;
+    if (threadIdx.x == 63) sh.rank[kGroups] = x;
+  }
+  __syncthreads();
+}
+
+// Where the lists and the count of equal keys stand.
+struct Seen {
+  int equal, freed, late;
+};
+
+// The middle tokens i0 + kSelThreads j + thread, j < kJ (those with their bit of in set), whose accounts are v:
+// which of them stay, which places below low_end are freed, which rows fill them.
+template <int kJ>
+__device__ __forceinline__ void place(const EvictArgs& a, int b, const Cut& c, Shared& sh, const float (&v)[kJ], unsigned in,
+                                      int i0, unsigned key, int left, Seen& seen) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const unsigned long long before = (1ull << lane) - 1;
+  unsigned kept = 0, equal = 0;   // a bit per j
+#pragma unroll
+  for (int j = 0; j < kJ; ++j) {
+    const unsigned k = rank_key(v[j]), bit = in & 1u << j;
+    kept |= k > key ? bit : 0u;
+    equal |= k == key ? bit : 0u;
+  }
+#pragma unroll
+  for (int j = 0; j < kJ; ++j) {
+    const unsigned long long m = __ballot(equal >> j & 1);
+    if (lane == 0) sh.rank[j * kSelWaves + wave] = __popcll(m);
+  }
+  scan_ranks<kJ * kSelWaves>(sh);
+#pragma unroll
+  for (int j = 0; j < kJ; ++j) {
+    const unsigned long long m = __ballot(equal >> j & 1);
+    const int rank = seen.equal + sh.rank[j * kSelWaves + wave] + __popcll(m & before);
+    kept |= (equal >> j & 1) && rank < left ? 1u << j : 0u;
+  }
+  seen.equal += sh.rank[kJ * kSelWaves];
+  __syncthreads();   // rank has been read
+  const int top = c.low_end - i0 - (int)threadIdx.x;   // tokens j < top / kSelThreads lie below low_end
+  unsigned below = 0;
+#pragma unroll
+  for (int j = 0; j < kJ; ++j) below |= kSelThreads * j < top ? 1u << j : 0u;
+  const unsigned freed = in & below & ~kept, late = kept & ~below;
+  // both ranks in one scan: kJ kSelThreads tokens keep either sum below 16 bits
+#pragma unroll
+  for (int j = 0; j < kJ; ++j) {
+    const unsigned long long f = __ballot(freed >> j & 1), l = __ballot(late >> j & 1);
+    if (lane == 0) sh.rank[j * kSelWaves + wave] = __popcll(f) | __popcll(l) << 16;
+  }
+  scan_ranks<kJ * kSelWaves>(sh);
+  int32_t* free_at = a.free_at + (int64_t)b * c.want;
+  int32_t* late_at = a.late_at + (int64_t)b * c.want;
+#pragma unroll
+  for (int j = 0; j < kJ; ++j) {
+    const unsigned long long f = __ballot(freed >> j & 1), l = __ballot(late >> j & 1);
+    const int base = sh.rank[j * kSelWaves + wave], i = i0 + kSelThreads * j + threadIdx.x;
+    if (freed >> j & 1) free_at[seen.freed + (base & 0xffff) + __popcll(f & before)] = i;
+    if (late >> j & 1) late_at[seen.late + (base >> 16) + __popcll(l & before)] = i;
+    if ((kept & below) >> j & 1) {
+      a.src[b * a.src_sb + i] = i;
+      a.mass_out[b * a.mo_sb + i] = v[j];
     }
-    __threadfence_block();
-    __syncthreads();   // the lists are complete
-    for (int i = tid; i < n_late; i += kSelThreads) src[free_at[i]] = late_at[i];
-    for (int i = tid; i < a.sink; i += kSelThreads) src[i] = i;
-    for (int i = tid; i < a.recent; i += kSelThreads) src[low_end + i] = hi + i;
-    __threadfence_block();
-    __syncthreads();   // src is complete
-    for (int i = tid; i < a.mass_len; i += kSelThreads) mass_out[i] = i < new_len ? mass[src[i]] : 0.f;
+  }
+  const int sum = sh.rank[kJ * kSelWaves];
+  seen.freed += sum & 0xffff;
+  seen.late += sum >> 16;
+  __syncthreads();   // rank has been read
+}
+
+// The accounts of the tokens i0 + kSelThreads j + thread that lie in [from, to), and their bits.
+template <int kJ>
+__device__ __forceinline__ unsigned load_accounts(const float* mass, int i0, int from, int to, float (&v)[kJ]) {
+  unsigned in = 0;
+#pragma unroll
+  for (int j = 0; j < kJ; ++j) {
+    const int i = i0 + kSelThreads * j + threadIdx.x;
+    const bool is = i >= from && i < to;
+    v[j] = is ? mass[i] : 0.f;
+    in |= is ? 1u << j : 0u;
+  }
+  return in;
+}
+template <int kJ>
+__device__ __forceinline__ void count_digit(int* hist, int d, unsigned prefix, const float (&v)[kJ], unsigned in) {
+  const unsigned mask = d == 0 ? 0u : ~0u << digit_shift(d - 1);
+#pragma unroll
+  for (int j = 0; j < kJ; ++j) {
+    const unsigned key = rank_key(v[j]);
+    if ((in >> j & 1) && (key & mask) == prefix) atomicAdd(&hist[(key >> digit_shift(d)) & (digit_bins(d) - 1)], 1);
   }
 }
 
-__device__ __forceinline__ char* row_at(const EvictArgs& a, int b, int pos) {
-  return a.pool + a.block_table[b * a.bt_sb + pos / kPage] * a.kv_sp + (int64_t)(pos % kPage) * a.kv_ss;
+// One workgroup per sequence, tables of up to kOneTokens tokens.
+__global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictArgs a) {
+  constexpr int kJ = kOneTokens / kSelThreads;
+  __shared__ Shared sh;
+  const int tid = threadIdx.x;
+  for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
+    const Cut c = cut_of(a, b);
+    float v[kJ];   // read beside the check of the pages
+    const unsigned in = load_accounts(a.mass + b * a.m_sb, 0, c.lo, c.hi, v);
+    if (!is_cut(a, b, c)) {
+      leave(a, b, c, tid, kSelThreads);
+      continue;
+    }
+    put_ends(a, b, c, tid, kSelThreads);
+    unsigned prefix = 0;
+    int left = c.want;   // how many are still to be taken from the tokens whose key matches prefix
+    Seen seen = {0, 0, 0};
+    if (c.want > 0) {
+      for (int d = 0; d < 3; ++d) {
+        const int bins = digit_bins(d);
+        for (int i = tid; i < bins; i += kSelThreads) sh.hist[i] = 0;
+        __syncthreads();
+        count_digit(sh.hist, d, prefix, v, in);
+        __syncthreads();
+        const int top = bins - 1 - 2 * tid;
+        pick_digit(sh, d, top, top >= 0 ? sh.hist[top] : 0, top >= 1 ? sh.hist[top - 1] : 0, prefix, left);
+      }
+      place(a, b, c, sh, v, in, 0, prefix, left, seen);
+    }
+    if (tid == 0) {
+      a.new_lens[b] = a.budget;
+      a.info[2 * b] = c.n - a.budget;
+      a.info[2 * b + 1] = seen.late;
+    }
+  }
 }
 
-// Phase 0: the middle moves, and the newest rows into the workspace where they overlap their new places.
-// Phase 1: the newest rows to their places.  Grid: x over the 16-byte pieces of a sequence, y over sequences.
+// ---- long tables ----
+// Chunks of a cut sequence: first those of [lo, low_end), then those of [low_end, hi).
+struct Chunks {
+  int span, n_low, n;
+  __device__ __forceinline__ Chunks(const Cut& c) {
+    const int each = (c.hi - c.lo + kMaxChunks - 3) / (kMaxChunks - 2);   // the two parts' last chunks may be short
+    span = max(1, (each + kSelThreads - 1) / kSelThreads) * kSelThreads;
+    n_low = (c.want + span - 1) / span;
+    n = n_low + (c.hi - c.low_end + span - 1) / span;
+  }
+  __device__ __forceinline__ int from(const Cut& c, int k) const { return k < n_low ? c.lo + k * span : c.low_end + (k - n_low) * span; }
+  __device__ __forceinline__ int to(const Cut& c, int k) const { return min(from(c, k) + span, k < n_low ? c.low_end : c.hi); }
+};
+
+// Launch d = 0 .. 2 counts digit d of every chunk, d = 3 writes the lists; each first picks digit d - 1.  Grid: x
+// over the chunks, y over sequences.
+template <int kD>
+__global__ void __launch_bounds__(kSelThreads) evict_chunk_kernel(EvictArgs a) {
+  __shared__ Shared sh;
+  const int tid = threadIdx.x, k = blockIdx.x;
+  const int lane = tid & 63, wave = tid >> 6;
+  for (int b = blockIdx.y; b < a.B; b += gridDim.y) {
+    const Cut c = cut_of(a, b);
+    if constexpr (kD == 0) {
+      const bool cut = is_cut(a, b, c);
+      if (!cut) {
+        leave(a, b, c, k * kSelThreads + tid, kMaxChunks * kSelThreads);
+        continue;
+      }
+      if (k == 0 && tid == 0) a.info[2 * b] = c.n - a.budget;
+    } else {
+      if (a.info[2 * b] == 0) continue;
+    }
+    const Chunks ch(c);
+    auto counts_of = [&](int d, int chunk) { return a.counts + (((int64_t)(d & 1) * a.B + b) * kMaxChunks + chunk) * kBins; };
+    auto sel_of = [&](int d) { return a.sel + ((int64_t)(d & 1) * a.B + b) * 2; };   // of launch d
+    unsigned prefix = kD > 1 ? (unsigned)sel_of(kD - 1)[0] : 0u;
+    int left = kD > 1 ? sel_of(kD - 1)[1] : c.want;
+    if (kD > 0 && c.want > 0) {
+      constexpr int d = kD - 1;
+      const int top = digit_bins(d) - 1 - 2 * tid;
+      int c0 = 0, c1 = 0, own = 0, own0 = 0, own1 = 0;
+      if (top > 0) {
+        for (int i = 0; i < ch.n; ++i) {
+          const int2 v = *reinterpret_cast<const int2*>(counts_of(d, i) + top - 1);
+          c1 += v.x;
+          c0 += v.y;
+          if (i == k) {
+            own1 = v.x;
+            own0 = v.y;
+          }
+        }
+      }
+      const int digit = pick_digit(sh, d, top, c0, c1, prefix, left);
+      if constexpr (kD < 3) {   // of this chunk, the tokens above the digit
+        scan_exclusive((top > digit ? own0 : 0) + (top - 1 > digit ? own1 : 0), sh.tmp, own);
+        if (tid == 0 && k < ch.n) a.above[b * kMaxChunks + k] = own + (kD > 1 ? a.above[b * kMaxChunks + k] : 0);
+        if (tid == 0 && k == 0) {
+          sel_of(kD)[0] = (int)prefix;
+          sel_of(kD)[1] = left;
+        }
+      } else if (wave < ch.n) {   // wave w: chunk w's tokens above the key, and those equal to it
+        const int32_t* counts = counts_of(d, wave);
+        int sum = 0;
+        for (int i = lane; i < digit_bins(d); i += 64) sum += i > digit ? counts[i] : 0;
+        sum = lane_scan(sum);
+        if (lane == 63) {
+          sh.kept[wave] = a.above[b * kMaxChunks + wave] + sum;
+          sh.equal[wave] = counts[digit];
+        }
+      }
+    }
+    const float* mass = a.mass + b * a.m_sb;
+    if constexpr (kD < 3) {
+      if (k < ch.n && c.want > 0) {
+        for (int i = tid; i < digit_bins(kD); i += kSelThreads) sh.hist[i] = 0;
+        __syncthreads();
+        const int from = ch.from(c, k), to = ch.to(c, k);
+        for (int i0 = from; i0 < to; i0 += kPiece * kSelThreads) {
+          float v[kPiece];
+          const unsigned in = load_accounts(mass, i0, from, to, v);
+          count_digit(sh.hist, kD, prefix, v, in);
+        }
+        __syncthreads();
+        for (int i = tid; i < digit_bins(kD); i += kSelThreads) counts_of(kD, k)[i] = sh.hist[i];
+      }
+      __syncthreads();   // hist is free for the next sequence
+    } else {
+      __syncthreads();
+      Seen seen = {0, 0, 0};
+      int late = 0;
+      if (c.want > 0) {
+        for (int i = 0, equal = 0; i < ch.n; ++i) {
+          const int kept = sh.kept[i] + min(max(left - equal, 0), sh.equal[i]);
+          if (i < k) {
+            seen.equal = equal + sh.equal[i];
+            seen.freed += i < ch.n_low ? ch.to(c, i) - ch.from(c, i) - kept : 0;
+            seen.late = late + (i >= ch.n_low ? kept : 0);
+          }
+          equal += sh.equal[i];
+          late += i >= ch.n_low ? kept : 0;
+        }
+        if (k < ch.n) {
+          const int from = ch.from(c, k), to = ch.to(c, k);
+          for (int i0 = from; i0 < to; i0 += kPiece * kSelThreads) {
+            float v[kPiece];
+            const unsigned in = load_accounts(mass, i0, from, to, v);
+            place(a, b, c, sh, v, in, i0, prefix, left, seen);
+          }
+        }
+      }
+      put_ends(a, b, c, k * kSelThreads + tid, kMaxChunks * kSelThreads);
+      if (k == 0 && tid == 0) {
+        a.new_lens[b] = a.budget;
+        a.info[2 * b + 1] = late;
+      }
+      __syncthreads();   // kept and equal are free for the next sequence
+    }
+  }
+}
+
+// Phase 0: the middle moves, with the outputs of the places they fill, and the newest rows into the workspace where
+// they overlap their new places.  Phase 1: the newest rows to their places.  A workgroup takes kMoveRows rows at a
+// time: their addresses first, then their 16-byte pieces.  Grid: x over the rows of a sequence, y over sequences.
 template <int kPhase>
 __global__ void __launch_bounds__(256) evict_move_kernel(EvictArgs a) {
+  __shared__ const Global char* from[kMoveRows];
+  __shared__ Global char* to[kMoveRows];
   const int want = a.budget - a.recent - a.sink;
-  const int step = gridDim.x * 256;
+  auto row_at = [&](int b, int pos) {
+    return a.pool + a.block_table[b * a.bt_sb + pos / kPage] * a.kv_sp + (int64_t)(pos % kPage) * a.kv_ss;
+  };
   for (int b = blockIdx.y; b < a.B; b += gridDim.y) {
     const int cut = a.info[2 * b], moves = a.info[2 * b + 1];
     if (cut == 0) continue;
     const int low_end = a.budget - a.recent;
     const bool staged = cut < a.recent;
-    char* stage = a.stage + (int64_t)b * a.recent * a.row_chunks * 16;
+    const int64_t row_bytes = (int64_t)a.row_chunks * 16;
+    char* stage = a.stage + (int64_t)b * a.recent * row_bytes;
     const int rows = kPhase == 0 ? moves + (staged ? a.recent : 0) : a.recent;
-    for (int64_t p = blockIdx.x * 256 + threadIdx.x; p < (int64_t)rows * a.row_chunks; p += step) {
-      const int r = (int)(p / a.row_chunks), c = (int)(p - (int64_t)r * a.row_chunks);
-      const char* from;
-      char* to;
-      if constexpr (kPhase == 0) {
-        if (r < moves) {
-          from = row_at(a, b, a.late_at[(int64_t)b * want + r]);
-          to = row_at(a, b, a.free_at[(int64_t)b * want + r]);
+    for (int r0 = blockIdx.x * kMoveRows; r0 < rows; r0 += gridDim.x * kMoveRows) {
+      const int n = min(kMoveRows, rows - r0);
+      __syncthreads();   // the addresses before have been read
+      if ((int)threadIdx.x < n) {
+        const int r = r0 + threadIdx.x;
+        const char* f;
+        char* t;
+        if (kPhase == 0 && r < moves) {
+          const int late = a.late_at[(int64_t)b * want + r], freed = a.free_at[(int64_t)b * want + r];
+          f = row_at(b, late);
+          t = row_at(b, freed);
+          a.src[b * a.src_sb + freed] = late;
+          a.mass_out[b * a.mo_sb + freed] = a.mass[b * a.m_sb + late];
+        } else if (kPhase == 0) {
+          f = row_at(b, low_end + cut + (r - moves));
+          t = stage + (r - moves) * row_bytes;
         } else {
-          from = row_at(a, b, low_end + cut + (r - moves));
-          to = stage + (int64_t)(r - moves) * a.row_chunks * 16;
+          f = staged ? stage + r * row_bytes : row_at(b, low_end + cut + r);
+          t = row_at(b, low_end + r);
         }
-      } else {
-        from = staged ? stage + (int64_t)r * a.row_chunks * 16 : row_at(a, b, low_end + cut + r);
-        to = row_at(a, b, low_end + r);
+        from[threadIdx.x] = (const Global char*)f;
+        to[threadIdx.x] = (Global char*)t;
       }
-      *reinterpret_cast<i32x4*>(to + 16 * c) = *reinterpret_cast<const i32x4*>(from + 16 * c);
+      __syncthreads();
+      const int pieces = n * a.row_chunks;
+      for (int q0 = threadIdx.x; q0 < pieces; q0 += 256 * kMoveBatch) {
+        i32x4 v[kMoveBatch];
+        Global i32x4* at[kMoveBatch];
+#pragma unroll
+        for (int u = 0; u < kMoveBatch; ++u) {
+          const int q = min(q0 + 256 * u, pieces - 1), r = fast_div(q, a.per_row), c = 16 * (q - r * a.row_chunks);
+          at[u] = (Global i32x4*)(to[r] + c);
+          v[u] = *(const Global i32x4*)(from[r] + c);
+        }
+#pragma unroll
+        for (int u = 0; u < kMoveBatch; ++u)
+          if (q0 + 256 * u < pieces) *at[u] = v[u];
+      }
     }
   }
 }
 
 struct EvictLayout {
-  int64_t info, lists, stage, total;   // byte offsets
+  int64_t info, free_at, late_at, stage, counts, above, sel, total;   // byte offsets, multiples of 16
 };
-// free_at and late_at hold the same number of entries; every part starts at a multiple of 16 bytes.
-EvictLayout evict_layout(int64_t B, int64_t budget, int64_t recent, int64_t sink, int64_t row_bytes) {
-  auto up = [](int64_t x) { return (x + 15) / 16 * 16; };
-  const int64_t list = up(B * (budget - recent - sink) * 4);
+EvictLayout evict_layout(int64_t B, int64_t cap, int64_t budget, int64_t recent, int64_t sink, int64_t row_bytes) {
+  int64_t at = 0;
+  auto part = [&](int64_t bytes) {
+    const int64_t from = at;
+    at += (bytes + 15) / 16 * 16;
+    return from;
+  };
+  const int64_t want = budget - recent - sink, chunked = cap > kOneTokens ? B : 0;
   EvictLayout l;
-  l.info = 0;
-  l.lists = up(B * 8);
-  l.stage = l.lists + 2 * list;
-  l.total = l.stage + B * recent * row_bytes;
+  l.info = part(B * 8);
+  l.free_at = part(B * want * 4);
+  l.late_at = part(B * want * 4);
+  l.stage = part(B * recent * row_bytes);
+  l.counts = part(chunked * 2 * kMaxChunks * kBins * 4);
+  l.above = part(chunked * kMaxChunks * 4);
+  l.sel = part(chunked * 16);
+  l.total = at;
   return l;
+}
+// The layout of a call; a budget that covers the block table cuts nothing and keeps no lists.
+EvictLayout evict_layout_of(int64_t B, int64_t row_bytes, int64_t max_pages, int64_t budget, int64_t recent, int64_t sink) {
+  const int64_t cap = max_pages * kPage;
+  return budget >= cap ? evict_layout(B, cap, 0, 0, 0, row_bytes) : evict_layout(B, cap, budget, recent, sink, row_bytes);
 }
 
 }  // namespace
@@ -267,8 +547,7 @@ static bool evict_sizes_ok(int64_t B, int64_t row_bytes, int64_t max_pages, int6
 extern "C" int64_t dmla_kv_evict_workspace_bytes(int64_t B, int64_t row_bytes, int64_t max_pages_per_seq, int64_t budget,
                                                  int64_t recent, int64_t sink) {
   if (!evict_sizes_ok(B, row_bytes, max_pages_per_seq, budget, recent, sink)) return 0;
-  if (budget >= max_pages_per_seq * kPage) return evict_layout(B, 0, 0, 0, row_bytes).total;   // nothing is ever cut
-  return evict_layout(B, budget, recent, sink, row_bytes).total;
+  return evict_layout_of(B, row_bytes, max_pages_per_seq, budget, recent, sink).total;
 }
 
 extern "C" int dmla_kv_evict(void* kv_pool, const int32_t* block_table, const int32_t* cache_seqlens, const float* mass,
@@ -308,7 +587,7 @@ extern "C" int dmla_kv_evict(void* kv_pool, const int32_t* block_table, const in
                 (long long)workspace_bytes);
   if (!aligned16(workspace)) return fail(DMLA_ERR_INVALID_ARG, "dmla_kv_evict: workspace must be 16-byte aligned");
   const bool can_cut = budget < cap;
-  const EvictLayout l = can_cut ? evict_layout(B, budget, recent, sink, row_bytes) : evict_layout(B, 0, 0, 0, row_bytes);
+  const EvictLayout l = evict_layout_of(B, row_bytes, max_pages_per_seq, budget, recent, sink);
   char* ws = static_cast<char*>(workspace);
   EvictArgs a = {};
   a.pool = static_cast<char*>(kv_pool);
@@ -322,19 +601,32 @@ extern "C" int dmla_kv_evict(void* kv_pool, const int32_t* block_table, const in
   a.budget = (int)std::min<int64_t>(budget, 0x7fffffff); a.recent = can_cut ? (int)recent : 0; a.sink = can_cut ? (int)sink : 0;
   a.row_chunks = (int)(row_bytes / 16);
   a.info = reinterpret_cast<int32_t*>(ws + l.info);
-  a.free_at = reinterpret_cast<int32_t*>(ws + l.lists);
-  a.late_at = reinterpret_cast<int32_t*>(ws + l.lists + (l.stage - l.lists) / 2);
+  a.free_at = reinterpret_cast<int32_t*>(ws + l.free_at);
+  a.late_at = reinterpret_cast<int32_t*>(ws + l.late_at);
   a.stage = ws + l.stage;
-  hipLaunchKernelGGL(evict_select_kernel, dim3((unsigned)std::min<int64_t>(B, 65535)), dim3(kSelThreads), 0,
-                     (hipStream_t)stream, a);
+  a.counts = reinterpret_cast<int32_t*>(ws + l.counts);
+  a.above = reinterpret_cast<int32_t*>(ws + l.above);
+  a.sel = reinterpret_cast<int32_t*>(ws + l.sel);
+  a.per_row = make_fastdiv((unsigned)a.row_chunks);
+  const int64_t gy = std::min<int64_t>(B, 65535);
+  if (cap <= kOneTokens) {
+    hipLaunchKernelGGL(evict_select_kernel, dim3((unsigned)gy), dim3(kSelThreads), 0, (hipStream_t)stream, a);
+  } else {
+    const dim3 grid(kMaxChunks, (unsigned)gy);
+    hipLaunchKernelGGL(evict_chunk_kernel<0>, grid, dim3(kSelThreads), 0, (hipStream_t)stream, a);
+    if (can_cut) {
+      hipLaunchKernelGGL(evict_chunk_kernel<1>, grid, dim3(kSelThreads), 0, (hipStream_t)stream, a);
+      hipLaunchKernelGGL(evict_chunk_kernel<2>, grid, dim3(kSelThreads), 0, (hipStream_t)stream, a);
+      hipLaunchKernelGGL(evict_chunk_kernel<3>, grid, dim3(kSelThreads), 0, (hipStream_t)stream, a);
+    }
+  }
   int rc = check_launch("dmla_kv_evict");
   if (rc != DMLA_OK || !can_cut) return rc;
-  // About eight workgroups per CU over all sequences, no more than a sequence has pieces to move.
-  const int64_t gy = std::min<int64_t>(B, 65535);
+  // About eight workgroups per CU over all sequences, no more than a sequence has groups of rows.
   const int64_t share = std::max<int64_t>(1, (int64_t)device_cu_count() * 8 / gy);
   auto launch = [&](auto kernel, int64_t rows) {
     if (rows == 0) return;
-    const int64_t gx = std::min(share, (rows * a.row_chunks + 255) / 256);
+    const int64_t gx = std::min(share, (rows + kMoveRows - 1) / kMoveRows);
     hipLaunchKernelGGL(kernel, dim3((unsigned)gx, (unsigned)gy), dim3(256), 0, (hipStream_t)stream, a);
   };
   launch(evict_move_kernel<0>, std::min(budget - recent - sink, cap - budget) + recent);

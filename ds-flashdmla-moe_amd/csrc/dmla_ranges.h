@@ -21,17 +21,6 @@ struct RangeLds {   // the segments of one chunk of kRangeThreads sequences
   int tmp[kRangeWaves];
 };
 
-// Sum over the lanes up to and including this one.
-__device__ __forceinline__ int lane_scan(int x) {
-  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);   // the lane 1, 2, 4, 8 before, in rows of 16
-  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);   // a row's last lane to the row after it
-  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);   // lane 31 to the upper half
-  return x;
-}
-
 // Calls segment(b, t0, t1, ctx, nsplit) for every piece of range r, with a barrier after each, and
 // owner(b, first_range, nsplit) on one thread for every sequence whose first tile lies in r (the empty
 // ones: r = 0).  All threads of the workgroup take part, those past kRangeThreads in the barriers.  ctx is the length, at most max_tokens.
