@@ -34,9 +34,9 @@ constexpr int kPage = 64;
 constexpr int kSelThreads = 1024;
 constexpr int kSelWaves = kSelThreads / 64;
 constexpr int kDigitBits = 11, kBins = 1 << kDigitBits;
-constexpr int kOneTokens = 16 * kSelThreads;
-constexpr int kMaxChunks = 16;
-constexpr int kPiece = 8;          // tokens of a thread at a time in a chunk
+constexpr int kOneTokens = 16 * kSelThreads;   // tokens that a workgroup holds in registers
+constexpr int kMaxChunks = 32;
+constexpr int kPiece = 8;          // tokens of a thread at a time
 constexpr int kMoveRows = 32;      // rows that a workgroup moves at a time
 constexpr int kMoveBatch = 5;      // 16-byte pieces of a thread in flight (32 bf16 rows are nine for each thread)
 #define Global __attribute__((address_space(1)))
@@ -95,7 +95,6 @@ struct Shared {
   int hist[kBins];
   int tmp[kSelWaves];
   int pick[2];                     // the digit that holds the last kept key, and how many keys lie above it
-  int rank[16 * kSelWaves + 1];    // by 64 consecutive tokens: counts, then their exclusive prefix and sum
   int kept[kMaxChunks], equal[kMaxChunks];
 };
 
@@ -137,22 +136,6 @@ __device__ __forceinline__ void leave(const EvictArgs& a, int b, const Cut& c, i
   for (int i = first; i < a.mass_len; i += step) a.mass_out[b * a.mo_sb + i] = i < c.n ? a.mass[b * a.m_sb + i] : 0.f;
 }
 
-// The outputs of a cut sequence outside the middle, likewise.
-__device__ __forceinline__ void put_ends(const EvictArgs& a, int b, const Cut& c, int first, int step) {
-  int32_t* src = a.src + b * a.src_sb;
-  float* out = a.mass_out + b * a.mo_sb;
-  const float* mass = a.mass + b * a.m_sb;
-  for (int i = first; i < c.lo; i += step) {
-    src[i] = i;
-    out[i] = mass[i];
-  }
-  for (int i = first; i < a.recent; i += step) {
-    src[c.low_end + i] = c.hi + i;
-    out[c.low_end + i] = mass[c.hi + i];
-  }
-  for (int i = a.budget + first; i < a.mass_len; i += step) out[i] = 0.f;
-}
-
 // Digits: bits 21.., 10.. and 0.. of the key.
 __device__ __forceinline__ int digit_shift(int d) { return d == 0 ? 21 : d == 1 ? 10 : 0; }
 __device__ __forceinline__ int digit_bins(int d) { return d == 2 ? 1 << 10 : kBins; }
@@ -176,28 +159,21 @@ __device__ __forceinline__ int pick_digit(Shared& sh, int d, int top, int c0, in
   return digit;
 }
 
-// Exclusive prefix over the counts in sh.rank (groups of 64 tokens in index order); the sum behind them.
-template <int kGroups>
-__device__ __forceinline__ void scan_ranks(Shared& sh) {
+// Exclusive prefix, over the waves, of a count that is the same in all lanes of a wave; total gets the sum.
+__device__ __forceinline__ int scan_waves(int v, int* tmp, int& total) {
+  const int wave = uniform(threadIdx.x >> 6);
+  __syncthreads();   // tmp is free
+  if ((threadIdx.x & 63) == 0) tmp[wave] = v;
   __syncthreads();
-  if (threadIdx.x < 64) {
-    constexpr int kEach = kGroups / 64;
-    int v[kEach], sum = 0;
+  int before = 0, sum = 0;
 #pragma unroll
-    for (int k = 0; k < kEach; ++k) {
-      v[k] = sh.rank[threadIdx.x * kEach + k];
-      sum += v[k];
-    }
-    const int x = lane_scan(sum);
-    int at = x - sum;
-#pragma unroll
-    for (int k = 0; k < kEach; ++k) {
-      sh.rank[threadIdx.x * kEach + k] = at;
-      at += v[k];
-    }
-    if (threadIdx.x == 63) sh.rank[kGroups] = x;
+  for (int w = 0; w < kSelWaves; ++w) {
+    const int t = uniform(tmp[w]);
+    before += w < wave ? t : 0;
+    sum += t;
   }
-  __syncthreads();
+  total = sum;
+  return before;
 }
 
 // Where the lists and the count of equal keys stand.
@@ -205,78 +181,79 @@ struct Seen {
   int equal, freed, late;
 };
 
-// The middle tokens i0 + kSelThreads j + thread, j < kJ (those with their bit of in set), whose accounts are v:
-// which of them stay, which places below low_end are freed, which rows fill them.
+// A thread's kJ tokens: a wave holds 64 kJ consecutive ones, 64 at a time, so that ranks within it are bit counts.
 template <int kJ>
-__device__ __forceinline__ void place(const EvictArgs& a, int b, const Cut& c, Shared& sh, const float (&v)[kJ], unsigned in,
-                                      int i0, unsigned key, int left, Seen& seen) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const unsigned long long before = (1ull << lane) - 1;
-  unsigned kept = 0, equal = 0;   // a bit per j
-#pragma unroll
-  for (int j = 0; j < kJ; ++j) {
-    const unsigned k = rank_key(v[j]), bit = in & 1u << j;
-    kept |= k > key ? bit : 0u;
-    equal |= k == key ? bit : 0u;
-  }
-#pragma unroll
-  for (int j = 0; j < kJ; ++j) {
-    const unsigned long long m = __ballot(equal >> j & 1);
-    if (lane == 0) sh.rank[j * kSelWaves + wave] = __popcll(m);
-  }
-  scan_ranks<kJ * kSelWaves>(sh);
-#pragma unroll
-  for (int j = 0; j < kJ; ++j) {
-    const unsigned long long m = __ballot(equal >> j & 1);
-    const int rank = seen.equal + sh.rank[j * kSelWaves + wave] + __popcll(m & before);
-    kept |= (equal >> j & 1) && rank < left ? 1u << j : 0u;
-  }
-  seen.equal += sh.rank[kJ * kSelWaves];
-  __syncthreads();   // rank has been read
-  const int top = c.low_end - i0 - (int)threadIdx.x;   // tokens j < top / kSelThreads lie below low_end
-  unsigned below = 0;
-#pragma unroll
-  for (int j = 0; j < kJ; ++j) below |= kSelThreads * j < top ? 1u << j : 0u;
-  const unsigned freed = in & below & ~kept, late = kept & ~below;
-  // both ranks in one scan: kJ kSelThreads tokens keep either sum below 16 bits
-#pragma unroll
-  for (int j = 0; j < kJ; ++j) {
-    const unsigned long long f = __ballot(freed >> j & 1), l = __ballot(late >> j & 1);
-    if (lane == 0) sh.rank[j * kSelWaves + wave] = __popcll(f) | __popcll(l) << 16;
-  }
-  scan_ranks<kJ * kSelWaves>(sh);
-  int32_t* free_at = a.free_at + (int64_t)b * c.want;
-  int32_t* late_at = a.late_at + (int64_t)b * c.want;
-#pragma unroll
-  for (int j = 0; j < kJ; ++j) {
-    const unsigned long long f = __ballot(freed >> j & 1), l = __ballot(late >> j & 1);
-    const int base = sh.rank[j * kSelWaves + wave], i = i0 + kSelThreads * j + threadIdx.x;
-    if (freed >> j & 1) free_at[seen.freed + (base & 0xffff) + __popcll(f & before)] = i;
-    if (late >> j & 1) late_at[seen.late + (base >> 16) + __popcll(l & before)] = i;
-    if ((kept & below) >> j & 1) {
-      a.src[b * a.src_sb + i] = i;
-      a.mass_out[b * a.mo_sb + i] = v[j];
-    }
-  }
-  const int sum = sh.rank[kJ * kSelWaves];
-  seen.freed += sum & 0xffff;
-  seen.late += sum >> 16;
-  __syncthreads();   // rank has been read
+__device__ __forceinline__ int token_of(int i0, int j) {
+  return i0 + (int)(threadIdx.x >> 6) * 64 * kJ + 64 * j + (int)(threadIdx.x & 63);
 }
 
-// The accounts of the tokens i0 + kSelThreads j + thread that lie in [from, to), and their bits.
+// The accounts of a thread's tokens that lie in [from, to), and their bits.
 template <int kJ>
 __device__ __forceinline__ unsigned load_accounts(const float* mass, int i0, int from, int to, float (&v)[kJ]) {
   unsigned in = 0;
 #pragma unroll
   for (int j = 0; j < kJ; ++j) {
-    const int i = i0 + kSelThreads * j + threadIdx.x;
+    const int i = token_of<kJ>(i0, j);
     const bool is = i >= from && i < to;
     v[j] = is ? mass[i] : 0.f;
     in |= is ? 1u << j : 0u;
   }
   return in;
 }
+
+// The middle tokens from i0 on (those with their bit of in set), whose accounts are v: which of them stay, which
+// places below low_end are freed, which rows fill them.
+template <int kJ>
+__device__ __forceinline__ void place(const EvictArgs& a, int b, const Cut& c, Shared& sh, const float (&v)[kJ], unsigned in,
+                                      int i0, unsigned key, int left, Seen& seen) {
+  auto rank_in = [](unsigned long long m) { return (int)__builtin_amdgcn_mbcnt_hi((unsigned)(m >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)m, 0)); };
+  unsigned kept = 0, equal = 0;   // a bit per j
+  int n_equal = 0;                // of the wave
+#pragma unroll
+  for (int j = 0; j < kJ; ++j) {
+    const unsigned k = rank_key(v[j]), bit = in & 1u << j;
+    kept |= k > key ? bit : 0u;
+    equal |= k == key ? bit : 0u;
+    n_equal += __popcll(__ballot(equal >> j & 1));
+  }
+  int sum;
+  int rank0 = seen.equal + scan_waves(n_equal, sh.tmp, sum);
+  seen.equal += sum;
+  const int top = c.low_end - token_of<kJ>(i0, 0);   // tokens with 64 j < top lie below low_end
+  unsigned below = 0;
+  int counts = 0;   // of the wave: freed places, and rows to move in the upper half; 64 kJ kSelWaves fit 16 bits
+#pragma unroll
+  for (int j = 0; j < kJ; ++j) {
+    const unsigned bit = 1u << j;
+    const unsigned long long m = __ballot(equal >> j & 1);
+    kept |= rank0 + rank_in(m) < left ? equal & bit : 0u;
+    rank0 += __popcll(m);
+    below |= 64 * j < top ? bit : 0u;
+    counts += __popcll(__ballot((in & below & ~kept) >> j & 1)) | __popcll(__ballot((kept & ~below) >> j & 1)) << 16;
+  }
+  const unsigned freed = in & below & ~kept, late = kept & ~below, stay = kept & below;
+  const int before = scan_waves(counts, sh.tmp, sum);
+  int32_t* free_at = a.free_at + (int64_t)b * c.want + seen.freed + (before & 0xffff);
+  int32_t* late_at = a.late_at + (int64_t)b * c.want + seen.late + (before >> 16);
+  int32_t* src = a.src + b * a.src_sb;
+  float* out = a.mass_out + b * a.mo_sb;
+#pragma unroll
+  for (int j = 0; j < kJ; ++j) {
+    const int i = token_of<kJ>(i0, j);
+    const unsigned long long f = __ballot(freed >> j & 1), l = __ballot(late >> j & 1);
+    if (freed >> j & 1) free_at[rank_in(f)] = i;
+    if (late >> j & 1) late_at[rank_in(l)] = i;
+    if (stay >> j & 1) {
+      src[i] = i;
+      out[i] = v[j];
+    }
+    free_at += __popcll(f);
+    late_at += __popcll(l);
+  }
+  seen.freed += sum & 0xffff;
+  seen.late += sum >> 16;
+}
+
 template <int kJ>
 __device__ __forceinline__ void count_digit(int* hist, int d, unsigned prefix, const float (&v)[kJ], unsigned in) {
   const unsigned mask = d == 0 ? 0u : ~0u << digit_shift(d - 1);
@@ -287,9 +264,9 @@ __device__ __forceinline__ void count_digit(int* hist, int d, unsigned prefix, c
   }
 }
 
-// One workgroup per sequence, tables of up to kOneTokens tokens.
+// One workgroup per sequence, tables of up to kJ tokens a thread.
+template <int kJ>
 __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictArgs a) {
-  constexpr int kJ = kOneTokens / kSelThreads;
   __shared__ Shared sh;
   const int tid = threadIdx.x;
   for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
@@ -300,7 +277,6 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictArgs a) 
       leave(a, b, c, tid, kSelThreads);
       continue;
     }
-    put_ends(a, b, c, tid, kSelThreads);
     unsigned prefix = 0;
     int left = c.want;   // how many are still to be taken from the tokens whose key matches prefix
     Seen seen = {0, 0, 0};
@@ -367,13 +343,19 @@ __global__ void __launch_bounds__(kSelThreads) evict_chunk_kernel(EvictArgs a) {
       const int top = digit_bins(d) - 1 - 2 * tid;
       int c0 = 0, c1 = 0, own = 0, own0 = 0, own1 = 0;
       if (top > 0) {
-        for (int i = 0; i < ch.n; ++i) {
-          const int2 v = *reinterpret_cast<const int2*>(counts_of(d, i) + top - 1);
-          c1 += v.x;
-          c0 += v.y;
+        int2 v[kMaxChunks];   // all on their way at once
+#pragma unroll
+        for (int i = 0; i < kMaxChunks; ++i)
+          v[i] = *reinterpret_cast<const int2*>(counts_of(d, min(i, ch.n - 1)) + top - 1);
+#pragma unroll
+        for (int i = 0; i < kMaxChunks; ++i) {
+          if (i < ch.n) {
+            c1 += v[i].x;
+            c0 += v[i].y;
+          }
           if (i == k) {
-            own1 = v.x;
-            own0 = v.y;
+            own1 = v[i].x;
+            own0 = v[i].y;
           }
         }
       }
@@ -385,14 +367,17 @@ __global__ void __launch_bounds__(kSelThreads) evict_chunk_kernel(EvictArgs a) {
           sel_of(kD)[0] = (int)prefix;
           sel_of(kD)[1] = left;
         }
-      } else if (wave < ch.n) {   // wave w: chunk w's tokens above the key, and those equal to it
-        const int32_t* counts = counts_of(d, wave);
-        int sum = 0;
-        for (int i = lane; i < digit_bins(d); i += 64) sum += i > digit ? counts[i] : 0;
-        sum = lane_scan(sum);
-        if (lane == 63) {
-          sh.kept[wave] = a.above[b * kMaxChunks + wave] + sum;
-          sh.equal[wave] = counts[digit];
+      } else {   // wave w: the tokens of chunks w, w + 16 above the key, and those equal to it
+        for (int i = wave; i < ch.n; i += kSelWaves) {
+          const int32_t* counts = counts_of(d, i);
+          int sum = 0;
+#pragma unroll
+          for (int x = lane; x < 1 << 10; x += 64) sum += x > digit ? counts[x] : 0;
+          sum = lane_scan(sum);
+          if (lane == 63) {
+            sh.kept[i] = a.above[b * kMaxChunks + i] + sum;
+            sh.equal[i] = counts[digit];
+          }
         }
       }
     }
@@ -416,16 +401,18 @@ __global__ void __launch_bounds__(kSelThreads) evict_chunk_kernel(EvictArgs a) {
       Seen seen = {0, 0, 0};
       int late = 0;
       if (c.want > 0) {
-        for (int i = 0, equal = 0; i < ch.n; ++i) {
-          const int kept = sh.kept[i] + min(max(left - equal, 0), sh.equal[i]);
-          if (i < k) {
-            seen.equal = equal + sh.equal[i];
-            seen.freed += i < ch.n_low ? ch.to(c, i) - ch.from(c, i) - kept : 0;
-            seen.late = late + (i >= ch.n_low ? kept : 0);
-          }
-          equal += sh.equal[i];
-          late += i >= ch.n_low ? kept : 0;
-        }
+        // lane i: chunk i's kept tokens, the places it frees and the rows it moves, and their sums over the chunks before
+        static_assert(kMaxChunks <= 64, "a lane per chunk");
+        const bool is = lane < ch.n;
+        const int equal = is ? sh.equal[lane] : 0, equal_to = lane_scan(equal);
+        const int kept = (is ? sh.kept[lane] : 0) + min(max(left - (equal_to - equal), 0), equal);
+        const int freed = is && lane < ch.n_low ? ch.to(c, lane) - ch.from(c, lane) - kept : 0;
+        const int moved = is && lane >= ch.n_low ? kept : 0;
+        const int freed_to = lane_scan(freed), moved_to = lane_scan(moved);
+        late = __builtin_amdgcn_readlane(moved_to, 63);
+        seen.equal = __builtin_amdgcn_readlane(equal_to - equal, k);
+        seen.freed = __builtin_amdgcn_readlane(freed_to - freed, k);
+        seen.late = __builtin_amdgcn_readlane(moved_to - moved, k);
         if (k < ch.n) {
           const int from = ch.from(c, k), to = ch.to(c, k);
           for (int i0 = from; i0 < to; i0 += kPiece * kSelThreads) {
@@ -435,7 +422,6 @@ __global__ void __launch_bounds__(kSelThreads) evict_chunk_kernel(EvictArgs a) {
           }
         }
       }
-      put_ends(a, b, c, k * kSelThreads + tid, kMaxChunks * kSelThreads);
       if (k == 0 && tid == 0) {
         a.new_lens[b] = a.budget;
         a.info[2 * b + 1] = late;
@@ -445,7 +431,24 @@ __global__ void __launch_bounds__(kSelThreads) evict_chunk_kernel(EvictArgs a) {
   }
 }
 
-// Phase 0: the middle moves, with the outputs of the places they fill, and the newest rows into the workspace where
+// The outputs of a cut sequence of n tokens outside the middle, by the threads first, first + step, ...
+__device__ __forceinline__ void put_ends(const EvictArgs& a, int b, int n, int first, int step) {
+  const int lo = a.sink, hi = n - a.recent, low_end = a.budget - a.recent;
+  int32_t* src = a.src + b * a.src_sb;
+  float* out = a.mass_out + b * a.mo_sb;
+  const float* mass = a.mass + b * a.m_sb;
+  for (int i = first; i < lo; i += step) {
+    src[i] = i;
+    out[i] = mass[i];
+  }
+  for (int i = first; i < a.recent; i += step) {
+    src[low_end + i] = hi + i;
+    out[low_end + i] = mass[hi + i];
+  }
+  for (int i = a.budget + first; i < a.mass_len; i += step) out[i] = 0.f;
+}
+
+// Phase 0: the outputs outside the middle; the middle moves, with the outputs of the places they fill, and the newest rows into the workspace where
 // they overlap their new places.  Phase 1: the newest rows to their places.  A workgroup takes kMoveRows rows at a
 // time: their addresses first, then their 16-byte pieces.  Grid: x over the rows of a sequence, y over sequences.
 template <int kPhase>
@@ -464,6 +467,7 @@ __global__ void __launch_bounds__(256) evict_move_kernel(EvictArgs a) {
     const int64_t row_bytes = (int64_t)a.row_chunks * 16;
     char* stage = a.stage + (int64_t)b * a.recent * row_bytes;
     const int rows = kPhase == 0 ? moves + (staged ? a.recent : 0) : a.recent;
+    if constexpr (kPhase == 0) put_ends(a, b, a.budget + cut, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
     for (int r0 = blockIdx.x * kMoveRows; r0 < rows; r0 += gridDim.x * kMoveRows) {
       const int n = min(kMoveRows, rows - r0);
       __syncthreads();   // the addresses before have been read
@@ -610,7 +614,9 @@ extern "C" int dmla_kv_evict(void* kv_pool, const int32_t* block_table, const in
   a.per_row = make_fastdiv((unsigned)a.row_chunks);
   const int64_t gy = std::min<int64_t>(B, 65535);
   if (cap <= kOneTokens) {
-    hipLaunchKernelGGL(evict_select_kernel, dim3((unsigned)gy), dim3(kSelThreads), 0, (hipStream_t)stream, a);
+    auto select = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)gy), dim3(kSelThreads), 0, (hipStream_t)stream, a); };
+    if (cap <= kOneTokens / 2) select(evict_select_kernel<kOneTokens / kSelThreads / 2>);
+    else select(evict_select_kernel<kOneTokens / kSelThreads>);
   } else {
     const dim3 grid(kMaxChunks, (unsigned)gy);
     hipLaunchKernelGGL(evict_chunk_kernel<0>, grid, dim3(kSelThreads), 0, (hipStream_t)stream, a);
@@ -625,11 +631,10 @@ extern "C" int dmla_kv_evict(void* kv_pool, const int32_t* block_table, const in
   // About eight workgroups per CU over all sequences, no more than a sequence has groups of rows.
   const int64_t share = std::max<int64_t>(1, (int64_t)device_cu_count() * 8 / gy);
   auto launch = [&](auto kernel, int64_t rows) {
-    if (rows == 0) return;
-    const int64_t gx = std::min(share, (rows + kMoveRows - 1) / kMoveRows);
+    const int64_t gx = std::min(share, std::max<int64_t>(1, (rows + kMoveRows - 1) / kMoveRows));
     hipLaunchKernelGGL(kernel, dim3((unsigned)gx, (unsigned)gy), dim3(256), 0, (hipStream_t)stream, a);
   };
   launch(evict_move_kernel<0>, std::min(budget - recent - sink, cap - budget) + recent);
-  launch(evict_move_kernel<1>, recent);
+  if (recent > 0) launch(evict_move_kernel<1>, recent);
   return check_launch("dmla_kv_evict(move)");
 }

@@ -77,7 +77,7 @@ def test_mass_of_long_contexts_and_many_sequences(gpu, lens, H, q4):
 @pytest.mark.gpu
 @pytest.mark.parametrize("q4", [False, True])
 def test_mass_of_more_pages_than_a_register_holds(gpu, q4):
-    """300 sequences that share 150 pages: about 170 pages and nine chunks of 1024 tokens per workgroup."""
+    """300 sequences that share 150 pages: about 170 pages per workgroup, and sums of many chunks of tokens."""
     n = 150 * 64 - 7
     pool, table, _ = _pool([n], 9, q4)
     q = seeded((1, 16, 576), 10, 0.5, torch.bfloat16)
@@ -169,6 +169,40 @@ def test_evict_long_contexts(gpu, n, budget, recent, q4):
     lens = [n, n // 2, 100]
     mass = torch.exp(2.0 * seeded((3, (n + 63) // 64 * 64), 6))
     _check_evict(gpu, lens, budget, recent, 4, q4, mass)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("budget,recent,sink", [(9000, 1000, 4), (1, 0, 0), (1, 0, 1), (16385, 0, 0), (5000, 4996, 4), (19999, 12000, 3),
+                                                (8192 + 64, 64, 0)])
+@pytest.mark.parametrize("kind", ["few", "equal", "specials"])
+def test_evict_equal_accounts_in_long_tables(gpu, kind, budget, recent, sink):
+    """Tables of more than 16384 tokens, whose accounts share a few values, or one, over all the table."""
+    lens = [20000, 16400, 16385, 5, 0]
+    shape = (5, (20000 + 63) // 64 * 64)
+    mass = torch.floor(seeded(shape, 23).abs() * 3) if kind == "few" else torch.full(shape, 0.25)
+    if kind == "specials":
+        mass[:, ::7] = float("inf")
+        mass[:, 1::7] = float("-inf")
+        mass[:, 2::7] = float("nan")
+        mass[:, 3::7] = 0.0
+        mass[:, 4::7] = -0.0
+    _check_evict(gpu, lens, budget, recent, sink, True, mass)
+
+
+@pytest.mark.gpu
+def test_evict_a_bad_page_in_a_long_table(gpu):
+    lens = [20000, 17000]
+    pool, table, sl = _pool(lens, 25, True)
+    mass = seeded((2, table.shape[1] * 64), 26).abs()
+    bad = table.clone()
+    bad[0, 300] = -1
+    pg = pool.to(gpu)
+    new_lens, src, new_mass = ops.flash_dmla_kv_evict(pg, bad.to(gpu), sl.to(gpu), mass.to(gpu), 3000, 100, 4)
+    ref_pool, ref_lens, ref_src, ref_mass = R.kv_evict(pool, table, torch.tensor([0, 17000], dtype=torch.int32), mass, 3000, 100, 4)
+    assert new_lens.tolist() == [20000, 3000]
+    assert torch.equal(pg.cpu(), ref_pool)
+    assert src[0].tolist() == list(range(3000)) and torch.equal(new_mass[0, :20000].cpu(), mass[0, :20000])
+    assert torch.equal(src[1].cpu(), ref_src[1]) and torch.equal(new_mass[1].cpu(), ref_mass[1])
 
 
 @pytest.mark.gpu
