@@ -194,8 +194,7 @@ __device__ __forceinline__ void run_segment(const Q4DecodeParams& p, const Q4Seg
     return x;
   };
   auto mask = [&](f32x16& x, int s) {
-    const int t = sg.t0 + s;
-    const int left = t < sg.t1 ? sg.ctx - t * kTile : 0;   // keys of the tile
+    const int left = sg.ctx - (sg.t0 + s) * kTile;   // keys of the tile
     if (left < kTile) {
       asm volatile("" : "+v"(x));   // rare: a branch
 #pragma unroll
@@ -310,9 +309,8 @@ __device__ __forceinline__ void run_segment(const Q4DecodeParams& p, const Q4Seg
     // with the softmax of tile s; barrier B; the start of both conversion and scores of the next step.  A
     // stands where tile s + 1 is written and P of step s - 1 posted, B where tile s - 1 has been read.  Both
     // stand among MFMAs whose operands are there, and what they guard is read a few MFMAs ahead of its use.
-    // One step more than there are tiles, whose scores are all masked: no branch in the loop.
 #pragma nounroll
-    for (int s = 1; s <= n_steps; ++s) {
+    for (int s = 1; s < n_steps; ++s) {
       f32x16 x = scores([&](auto m_tag) {
         constexpr int m = decltype(m_tag)::value;
         if constexpr (m < 16 && m % 2 == 0) convert_octet(m / 2);
@@ -358,6 +356,15 @@ __device__ __forceinline__ void run_segment(const Q4DecodeParams& p, const Q4Seg
       cur = next;
       next = t;
     }
+    // The values of the last tile.
+    wait_lds();
+    __syncthreads();   // its P is posted
+    values_begin(prev);
+#pragma unroll
+    for (int n = 0; n < kHeadBlocks; ++n) read_prob(0, n);
+    read_values(0);
+    read_values(1);
+    values([](auto) {});
     const bool over = __any(mtrue > mref + kQ4Headroom);
     if (lane == 0) lds.flag[wave] = over ? 1 : 0;
     wait_vm<0>();
