@@ -69,9 +69,6 @@ constexpr int kQ4LatentSteps = 32;
 __host__ __device__ constexpr int q4_operand_unit(int h, int c) {
   return c < kQ4LatentSteps ? 8 * (c / 4) + 4 * h + c % 4 : 2 * c + h;
 }
-__device__ __forceinline__ bf16x8 q4_query_operand(const bf16* q, int h, int c) {
-  return *reinterpret_cast<const bf16x8*>(q + 8 * q4_operand_unit(h, c));
-}
 // Codes of MFMAs 4 a .. 4 a + 3, all scales of the half (byte 2 (a % 2) of word a / 2), and rope operand c of
 // this lane's row.
 __device__ __forceinline__ u32x4 q4_key_codes(const DMLA_LDS char* row, int h, int a) {

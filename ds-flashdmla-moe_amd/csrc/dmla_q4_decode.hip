@@ -86,11 +86,27 @@ __device__ __forceinline__ void run_segment(const Q4DecodeParams& p, const Q4Seg
   };
   start_copies();
 
+  // Queries through the slot that no copy has reached yet, 8 rows x 128 bytes a copy: as operands they would be
+  // 32 rows x 32 bytes a load, four times over.
+  static_assert(kSlots - 1 >= kAhead && 36 * 1024 <= kSlotBytes, "the last slot is free");
   bf16x8 q[kQ4Steps];
   {
-    const bf16* src = p.q + sg.b * p.q_sb + min(head0 + l32, p.H - 1) * p.q_sh;
+    const unsigned stage = lds_addr(lds.ring) + (kSlots - 1) * kSlotBytes;
+    const int ln = fresh_lane_id();
+    const int head = min(head0 + 8 * wave + (ln >> 3), p.H - 1);
+    const bf16* src = p.q + sg.b * p.q_sb + head * p.q_sh + 8 * ((ln & 7) ^ (ln >> 3));
 #pragma unroll
-    for (int c = 0; c < kQ4Steps; ++c) q[c] = q4_query_operand(src, hl, c);
+    for (int d = 0; d < 9; ++d) dma16_addr(src + 64 * d, stage + (9 * wave + d) * 1024);
+    wait_vm<0>();
+    __syncthreads();
+    const unsigned row = stage + 9 * 1024 * (l32 >> 3) + 128 * (l32 & 7);
+#pragma unroll
+    for (int c = 0; c < kQ4Steps; ++c) {
+      const int u = q4_operand_unit(hl, c);
+      q[c] = *lds_ptr<const bf16x8>(row + (c / 4) * 1024 + 16 * ((u & 7) ^ (l32 & 7)));
+    }
+    wait_lds();
+    __syncthreads();
   }
 
   f32x16 acc[16];           // O^T of 32 heads and 32 columns: row m is column 16 m + j
