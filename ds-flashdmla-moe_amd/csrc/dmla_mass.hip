@@ -231,7 +231,9 @@ __device__ __forceinline__ void mass_segment(const MassParams& p, int b, int t0,
         if (hl == 0) lds.sums[hw * kChunk + (t - chunk0) * T::kTokens + 32 * kp + l32] = bad ? 0.f : sum;
       }
       const bool last = t + 1 == t1 || (t + 1 - chunk0) * T::kTokens == kChunk;
-      if (last) wait_vm<0>();   // the account's values, which later copies may follow
+      // The account's values: they are older than the copies of step chunk0 + kSlots, which landed above if that is
+      // step t or before it.
+      if (last && t - chunk0 < kSlots) wait_vm<0>();
       __syncthreads();          // the slot has been read, the sums are written
       if (last) {
         const int i = threadIdx.x, at = chunk0 * T::kTokens + i;
