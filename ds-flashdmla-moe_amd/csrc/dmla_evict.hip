@@ -59,8 +59,9 @@ struct EvictArgs {
   int32_t* free_at;      // [B][budget - recent - sink] freed places, and the rows that fill them
   int32_t* late_at;
   char* stage;           // [B][recent] rows
-  int32_t* counts;       // [2][B][kMaxChunks][kBins], long tables only, as the next two
-  int32_t* above;        // [B][kMaxChunks]: tokens of a chunk whose key lies above the digits picked so far
+  int chunks;            // workgroups of a sequence, long tables only, as the next three
+  int32_t* counts;       // [2][B][chunks][kBins]
+  int32_t* above;        // [B][chunks]: tokens of a chunk whose key lies above the digits picked so far
   int32_t* sel;          // [2][B][2]: those digits, and how many of the tokens that share them are kept
   FastDiv per_row;       // division by row_chunks
 };
@@ -304,8 +305,8 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictArgs a) 
 // Chunks of a cut sequence: first those of [lo, low_end), then those of [low_end, hi).
 struct Chunks {
   int span, n_low, n;
-  __device__ __forceinline__ Chunks(const Cut& c) {
-    const int each = (c.hi - c.lo + kMaxChunks - 3) / (kMaxChunks - 2);   // the two parts' last chunks may be short
+  __device__ __forceinline__ Chunks(const Cut& c, int most) {
+    const int each = (c.hi - c.lo + most - 3) / (most - 2);   // the two parts' last chunks may be short
     span = max(1, (each + kSelThreads - 1) / kSelThreads) * kSelThreads;
     n_low = (c.want + span - 1) / span;
     n = n_low + (c.hi - c.low_end + span - 1) / span;
@@ -321,20 +322,21 @@ __global__ void __launch_bounds__(kSelThreads) evict_chunk_kernel(EvictArgs a) {
   __shared__ Shared sh;
   const int tid = threadIdx.x, k = blockIdx.x;
   const int lane = tid & 63, wave = tid >> 6;
+  constexpr int kBatch = 8;
   for (int b = blockIdx.y; b < a.B; b += gridDim.y) {
     const Cut c = cut_of(a, b);
     if constexpr (kD == 0) {
       const bool cut = is_cut(a, b, c);
       if (!cut) {
-        leave(a, b, c, k * kSelThreads + tid, kMaxChunks * kSelThreads);
+        leave(a, b, c, k * kSelThreads + tid, a.chunks * kSelThreads);
         continue;
       }
       if (k == 0 && tid == 0) a.info[2 * b] = c.n - a.budget;
     } else {
       if (a.info[2 * b] == 0) continue;
     }
-    const Chunks ch(c);
-    auto counts_of = [&](int d, int chunk) { return a.counts + (((int64_t)(d & 1) * a.B + b) * kMaxChunks + chunk) * kBins; };
+    const Chunks ch(c, a.chunks);
+    auto counts_of = [&](int d, int chunk) { return a.counts + (((int64_t)(d & 1) * a.B + b) * a.chunks + chunk) * kBins; };
     auto sel_of = [&](int d) { return a.sel + ((int64_t)(d & 1) * a.B + b) * 2; };   // of launch d
     unsigned prefix = kD > 1 ? (unsigned)sel_of(kD - 1)[0] : 0u;
     int left = kD > 1 ? sel_of(kD - 1)[1] : c.want;
@@ -343,26 +345,25 @@ __global__ void __launch_bounds__(kSelThreads) evict_chunk_kernel(EvictArgs a) {
       const int top = digit_bins(d) - 1 - 2 * tid;
       int c0 = 0, c1 = 0, own = 0, own0 = 0, own1 = 0;
       if (top > 0) {
-        int2 v[kMaxChunks];   // all on their way at once
+        for (int i0 = 0; i0 < ch.n; i0 += kBatch) {
+          int2 v[kBatch];   // on their way together
 #pragma unroll
-        for (int i = 0; i < kMaxChunks; ++i)
-          v[i] = *reinterpret_cast<const int2*>(counts_of(d, min(i, ch.n - 1)) + top - 1);
+          for (int i = 0; i < kBatch; ++i)
+            v[i] = *reinterpret_cast<const int2*>(counts_of(d, min(i0 + i, ch.n - 1)) + top - 1);
 #pragma unroll
-        for (int i = 0; i < kMaxChunks; ++i) {
-          if (i < ch.n) {
-            c1 += v[i].x;
-            c0 += v[i].y;
-          }
-          if (i == k) {
-            own1 = v[i].x;
-            own0 = v[i].y;
+          for (int i = 0; i < kBatch; ++i) {
+            const bool is = i0 + i < ch.n, mine = i0 + i == k;
+            c1 += is ? v[i].x : 0;
+            c0 += is ? v[i].y : 0;
+            own1 = mine ? v[i].x : own1;
+            own0 = mine ? v[i].y : own0;
           }
         }
       }
       const int digit = pick_digit(sh, d, top, c0, c1, prefix, left);
       if constexpr (kD < 3) {   // of this chunk, the tokens above the digit
         scan_exclusive((top > digit ? own0 : 0) + (top - 1 > digit ? own1 : 0), sh.tmp, own);
-        if (tid == 0 && k < ch.n) a.above[b * kMaxChunks + k] = own + (kD > 1 ? a.above[b * kMaxChunks + k] : 0);
+        if (tid == 0 && k < ch.n) a.above[b * a.chunks + k] = own + (kD > 1 ? a.above[b * a.chunks + k] : 0);
         if (tid == 0 && k == 0) {
           sel_of(kD)[0] = (int)prefix;
           sel_of(kD)[1] = left;
@@ -375,7 +376,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_chunk_kernel(EvictArgs a) {
           for (int x = lane; x < 1 << 10; x += 64) sum += x > digit ? counts[x] : 0;
           sum = lane_scan(sum);
           if (lane == 63) {
-            sh.kept[i] = a.above[b * kMaxChunks + i] + sum;
+            sh.kept[i] = a.above[b * a.chunks + i] + sum;
             sh.equal[i] = counts[digit];
           }
         }
@@ -513,6 +514,9 @@ __global__ void __launch_bounds__(256) evict_move_kernel(EvictArgs a) {
 struct EvictLayout {
   int64_t info, free_at, late_at, stage, counts, above, sel, total;   // byte offsets, multiples of 16
 };
+// Workgroups of a sequence: every one adds up the counts of all, so together no more than twice the chip's
+// (64 sequences x 32 took 280 us where one workgroup each took 37), and 4 at least, two for either part.
+int64_t evict_chunks(int64_t B) { return std::min<int64_t>(kMaxChunks, std::max<int64_t>(4, 2 * device_cu_count() / B)); }
 EvictLayout evict_layout(int64_t B, int64_t cap, int64_t budget, int64_t recent, int64_t sink, int64_t row_bytes) {
   int64_t at = 0;
   auto part = [&](int64_t bytes) {
@@ -520,15 +524,15 @@ EvictLayout evict_layout(int64_t B, int64_t cap, int64_t budget, int64_t recent,
     at += (bytes + 15) / 16 * 16;
     return from;
   };
-  const int64_t want = budget - recent - sink, chunked = cap > kOneTokens ? B : 0;
+  const int64_t want = budget - recent - sink, chunked = cap > kOneTokens ? B * evict_chunks(B) : 0;
   EvictLayout l;
   l.info = part(B * 8);
   l.free_at = part(B * want * 4);
   l.late_at = part(B * want * 4);
   l.stage = part(B * recent * row_bytes);
-  l.counts = part(chunked * 2 * kMaxChunks * kBins * 4);
-  l.above = part(chunked * kMaxChunks * 4);
-  l.sel = part(chunked * 16);
+  l.counts = part(chunked * 2 * kBins * 4);
+  l.above = part(chunked * 4);
+  l.sel = part(chunked > 0 ? B * 16 : 0);
   l.total = at;
   return l;
 }
@@ -618,7 +622,8 @@ extern "C" int dmla_kv_evict(void* kv_pool, const int32_t* block_table, const in
     if (cap <= kOneTokens / 2) select(evict_select_kernel<kOneTokens / kSelThreads / 2>);
     else select(evict_select_kernel<kOneTokens / kSelThreads>);
   } else {
-    const dim3 grid(kMaxChunks, (unsigned)gy);
+    a.chunks = (int)evict_chunks(B);
+    const dim3 grid((unsigned)a.chunks, (unsigned)gy);
     hipLaunchKernelGGL(evict_chunk_kernel<0>, grid, dim3(kSelThreads), 0, (hipStream_t)stream, a);
     if (can_cut) {
       hipLaunchKernelGGL(evict_chunk_kernel<1>, grid, dim3(kSelThreads), 0, (hipStream_t)stream, a);

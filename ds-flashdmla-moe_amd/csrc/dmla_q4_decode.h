@@ -1,5 +1,4 @@
-// What the two kernels of the 4-bit decode share (dmla_q4_decode.hip up to 32 heads a workgroup,
-// dmla_q4_wide.hip up to 128).
+// What the two kernels of the 4-bit decode share (dmla_q4_decode.hip: 32 heads a workgroup, dmla_q4_wide.hip: 128).
 #pragma once
 #include "dmla_q4.h"
 #include "dmla_ranges.h"

@@ -1,5 +1,5 @@
 // Paged decode over the 4-bit latent cache (row format: dmla_q4.h): one query token per sequence.  This
-// kernel takes up to 32 heads, dmla_q4_wide.hip more.
+// kernel takes up to 64 heads, dmla_q4_wide.hip more.
 //
 //   s_ht = scale q_h . k_t,  o_h = sum_t softmax(s_h)_t k_t[:512],  k_t = code x scale (exact)
 //
@@ -368,7 +368,11 @@ __global__ __launch_bounds__(kThreads, 1) void q4_decode_kernel(Q4DecodeParams p
       });
 }
 
-int wg_heads(int64_t H) { return H <= kHeads ? kHeads : 128; }
+// Up to 64 heads, workgroups of 32 (two groups of them read a tile twice, the second time from the L2); above, of 128.
+// 64 sequences of 8192 tokens, this kernel against the wide one: 68 : 137 us with 16 heads, 71 : 140 with 32,
+// 106 : 133 with 64; 4 sequences 22 : 27, 25 : 29 and 30 : 31 us.  Three groups would cost what the wide kernel does.
+bool narrow(int64_t H) { return H <= 2 * kHeads; }
+int wg_heads(int64_t H) { return narrow(H) ? kHeads : 128; }
 int64_t q4_ranges(int64_t H) {
   const int64_t hg = (H + wg_heads(H) - 1) / wg_heads(H);
   return std::max<int64_t>(1, device_cu_count() / hg);
@@ -439,8 +443,11 @@ extern "C" int dmla_decode_paged_q4(const void* q, const void* kv_pool, const in
   p.n_ranges = (int)R;
   p.scale_log2 = softmax_scale * kLog2e;
   const int grid = (int)((R + 7) / 8 * 8 * p.head_groups);
-  if (H <= kHeads) {
-    p.min_width = 32;
+  // The least work of a workgroup, in tiles: two for each wave; 16 tiles took 25.6 us at 4 sequences of 8192 tokens
+  // x 16 heads and 25.3 at one of 5000, 8 tiles 22.2 and 21.8, 4 tiles 24.4 and 20.8.  The wide kernel: 3 and 4
+  // tiles are as good at one sequence (25.3, 25.5 us), 8 take 30.0.
+  if (narrow(H)) {
+    p.min_width = 8;
     hipLaunchKernelGGL(q4_decode_kernel, dim3((unsigned)grid), dim3(kThreads), 0, (hipStream_t)stream, p);
   } else {
     p.min_width = 4;

@@ -1,4 +1,4 @@
-// Paged decode over the 4-bit latent cache for more than 32 heads (up to 32: dmla_q4_decode.hip, which
+// Paged decode over the 4-bit latent cache for more than 64 heads (up to 64: dmla_q4_decode.hip, which
 // states what is computed).
 //
 // MI355X design:
