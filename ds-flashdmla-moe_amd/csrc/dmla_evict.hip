@@ -505,7 +505,7 @@ __global__ void __launch_bounds__(256) evict_move_kernel(EvictArgs a) {
         }
 #pragma unroll
         for (int u = 0; u < kMoveBatch; ++u)
-          if (q0 + 256 * u < pieces) *at[u] = v[u];
+          if (q0 + 256 * u < pieces) __builtin_nontemporal_store(v[u], at[u]);   // 64 sequences 66 us, plain stores 73
       }
     }
   }

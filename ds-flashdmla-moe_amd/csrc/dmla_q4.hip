@@ -92,23 +92,30 @@ __global__ void __launch_bounds__(64 * kWavesPerWG) q4_append_kernel(Q4RowArgs a
   }
 }
 
-// One wave per row: lane l turns the codes of values 8l .. 8l+7 into 16 bytes of bf16; lanes 0..7 move
-// the rope.  Rows at or past the sequence's length are zeros, rows on an invalid page are NaN.
-// Bound: HBM (400 bytes in, 1152 out per row).
+// One wave per row, kBatch neighbouring rows at a time: lane l turns the codes of values 8l .. 8l+7 into 16 bytes of
+// bf16; lanes 0..7 move the rope.  Rows at or past the sequence's length are zeros, rows on an invalid page are NaN.
+// Bound: HBM (400 bytes in, 1152 out per row): 32 x 5000 rows, half of them cached, in 36 us, 6.0 TB/s.
+// kStream: stores that do not stay in the caches, for outputs of kStreamBytes and more.  The 256 MiB of the last
+// cache hold a smaller output until it is read, and a larger one only gets in the way there: 144 MiB of rows took
+// 34 us (31.9 streamed) and 64 with a reader right behind (78), 162 MiB 40 (34) and 68 (85), 180 MiB 58 (39) and
+// 77 (94), 198 MiB 80 (41) and 117 (103), 252 MiB 105 (53) and 173 (144).  What reads it is mostly attention,
+// which the matrix units bound, so the gather's own time decides.
+constexpr int64_t kStreamBytes = (int64_t)160 << 20;
+template <bool kStream>
 __global__ void __launch_bounds__(64 * kWavesPerWG) q4_gather_kernel(Q4RowArgs a) {
   const int lane = lane_id();
   const int wave = uniform(threadIdx.x >> 6);
   const int64_t total = (int64_t)a.B * a.n;
   const int step = gridDim.x * kWavesPerWG;
   const u32x4 nan4 = {0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};
-  for (int64_t r0 = blockIdx.x * kWavesPerWG + wave; r0 < total; r0 += (int64_t)kBatch * step) {
+  for (int64_t r0 = (int64_t)(blockIdx.x * kWavesPerWG + wave) * kBatch; r0 < total; r0 += (int64_t)kBatch * step) {
     unsigned codes[kBatch];
     int sb[kBatch], kind[kBatch];   // kind: 0 nothing to do, 1 a row, 2 zeros, 3 an invalid page
     u32x4 rope[kBatch];
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
       kind[i] = 0;
-      const int64_t r = r0 + (int64_t)i * step;
+      const int64_t r = r0 + i;
       if (r >= total) continue;
       const int b = fast_div((int)r, a.ndiv), t = (int)r - b * a.n;
       const int64_t pos = (int64_t)(a.lens != nullptr ? max(a.lens[b], 0) : 0) + t;
@@ -126,7 +133,7 @@ __global__ void __launch_bounds__(64 * kWavesPerWG) q4_gather_kernel(Q4RowArgs a
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
       if (kind[i] == 0) continue;
-      const int64_t r = r0 + (int64_t)i * step;
+      const int64_t r = r0 + i;
       const int b = fast_div((int)r, a.ndiv), t = (int)r - b * a.n;
       bf16* out = a.rows + b * a.r_sb + t * a.r_ss;
       u32x4 v = {0u, 0u, 0u, 0u}, p = v;
@@ -140,8 +147,14 @@ __global__ void __launch_bounds__(64 * kWavesPerWG) q4_gather_kernel(Q4RowArgs a
       } else if (kind[i] == 3) {
         v = p = nan4;
       }
-      *reinterpret_cast<u32x4*>(out + 8 * lane) = v;
-      if (lane < 8) *reinterpret_cast<u32x4*>(out + kLat + 8 * lane) = p;
+      u32x4* to = reinterpret_cast<u32x4*>(out + 8 * lane);
+      if constexpr (kStream) {
+        __builtin_nontemporal_store(v, to);
+        if (lane < 8) __builtin_nontemporal_store(p, to + kLat / 8);
+      } else {
+        *to = v;
+        if (lane < 8) to[kLat / 8] = p;
+      }
     }
   }
 }
@@ -221,6 +234,10 @@ extern "C" int dmla_kv_gather_q4(const void* kv_pool, const int32_t* block_table
   a.B = (int)B; a.n = (int)n_out;
   a.num_pages = (int)num_pages; a.max_pages = (int)max_pages_per_seq;
   a.ndiv = make_fastdiv((unsigned)n_out);
-  hipLaunchKernelGGL(q4_gather_kernel, q4_rows_grid(B * n_out), dim3(64 * kWavesPerWG), 0, (hipStream_t)stream, a);
+  auto launch = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, q4_rows_grid(B * n_out), dim3(64 * kWavesPerWG), 0, (hipStream_t)stream, a);
+  };
+  if (B * n_out * kD * 2 >= kStreamBytes) launch(q4_gather_kernel<true>);
+  else launch(q4_gather_kernel<false>);
   return check_launch("dmla_kv_gather_q4");
 }
