@@ -25,6 +25,7 @@ struct Q4RowArgs {
   int64_t kv_sp, bt_sb, r_sb, r_ss;
   int B, n;                // rows per sequence in `rows`
   int num_pages, max_pages;
+  int each;                // rows of a wave at a time, at most kBatch
   FastDiv ndiv;            // division by n
 };
 
@@ -38,22 +39,24 @@ __device__ __forceinline__ int page_of(const Q4RowArgs& a, int b, int64_t pos) {
 // (By value: a bit cast of a vector's element takes the vector's first.)
 __device__ __forceinline__ bf16x2 as_bf16x2(unsigned w) { return __builtin_bit_cast(bf16x2, w); }
 
-// One wave per row: lane l holds values 8l .. 8l+7 (one 16-byte load, one 4-byte store of codes), four
+// A row at a time of a wave's kBatch: lane l holds values 8l .. 8l+7 (one 16-byte load, one 4-byte store of codes), four
 // lanes share a block of 32, whose largest value meets in two quad swaps; lanes 0..7 move the rope.
-// Bound: HBM (1152 bytes in, 400 out per row); kBatch rows per wave keep enough loads in flight.
+// Bound: HBM (1152 bytes in, 400 out per row), and below some 20000 rows launch and latency: 8 x 2048 rows in 6.6 us,
+// 64 x 8192 rows in 192 us, 4.2 TB/s.  kBatch rows per wave keep enough loads in flight (eight measured 13 % slower).
+// Rows built in LDS and stored in 16-byte pieces instead of 256 + 16 x 1 + 128 bytes a row took the same time.
 __global__ void __launch_bounds__(64 * kWavesPerWG) q4_append_kernel(Q4RowArgs a) {
   const int lane = lane_id();
   const int wave = uniform(threadIdx.x >> 6);
   const int64_t total = (int64_t)a.B * a.n;
   const int step = gridDim.x * kWavesPerWG;
-  for (int64_t r0 = blockIdx.x * kWavesPerWG + wave; r0 < total; r0 += (int64_t)kBatch * step) {
+  for (int64_t r0 = (int64_t)(blockIdx.x * kWavesPerWG + wave) * a.each; r0 < total; r0 += (int64_t)a.each * step) {
     bf16x8 x[kBatch], rope[kBatch];
     int64_t dst[kBatch];
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
       dst[i] = -1;
-      const int64_t r = r0 + (int64_t)i * step;
-      if (r >= total) continue;
+      const int64_t r = r0 + i;
+      if (i >= a.each || r >= total) continue;
       const int b = fast_div((int)r, a.ndiv), t = (int)r - b * a.n;
       if (a.lens != nullptr && t >= a.lens[b]) continue;
       const int64_t pos = (int64_t)max(a.seqlens[b], 0) + t;
@@ -94,7 +97,7 @@ __global__ void __launch_bounds__(64 * kWavesPerWG) q4_append_kernel(Q4RowArgs a
 
 // One wave per row, kBatch neighbouring rows at a time: lane l turns the codes of values 8l .. 8l+7 into 16 bytes of
 // bf16; lanes 0..7 move the rope.  Rows at or past the sequence's length are zeros, rows on an invalid page are NaN.
-// Bound: HBM (400 bytes in, 1152 out per row): 32 x 5000 rows, half of them cached, in 36 us, 6.0 TB/s.
+// Bound: HBM (400 bytes in, 1152 out per row): 32 x 5000 rows, half of them cached, in 32 us, 6.8 TB/s.
 // kStream: stores that do not stay in the caches, for outputs of kStreamBytes and more.  The 256 MiB of the last
 // cache hold a smaller output until it is read, and a larger one only gets in the way there: 144 MiB of rows took
 // 34 us (31.9 streamed) and 64 with a reader right behind (78), 162 MiB 40 (34) and 68 (85), 180 MiB 58 (39) and
@@ -108,7 +111,7 @@ __global__ void __launch_bounds__(64 * kWavesPerWG) q4_gather_kernel(Q4RowArgs a
   const int64_t total = (int64_t)a.B * a.n;
   const int step = gridDim.x * kWavesPerWG;
   const u32x4 nan4 = {0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};
-  for (int64_t r0 = (int64_t)(blockIdx.x * kWavesPerWG + wave) * kBatch; r0 < total; r0 += (int64_t)kBatch * step) {
+  for (int64_t r0 = (int64_t)(blockIdx.x * kWavesPerWG + wave) * a.each; r0 < total; r0 += (int64_t)a.each * step) {
     unsigned codes[kBatch];
     int sb[kBatch], kind[kBatch];   // kind: 0 nothing to do, 1 a row, 2 zeros, 3 an invalid page
     u32x4 rope[kBatch];
@@ -116,7 +119,7 @@ __global__ void __launch_bounds__(64 * kWavesPerWG) q4_gather_kernel(Q4RowArgs a
     for (int i = 0; i < kBatch; ++i) {
       kind[i] = 0;
       const int64_t r = r0 + i;
-      if (r >= total) continue;
+      if (i >= a.each || r >= total) continue;
       const int b = fast_div((int)r, a.ndiv), t = (int)r - b * a.n;
       const int64_t pos = (int64_t)(a.lens != nullptr ? max(a.lens[b], 0) : 0) + t;
       kind[i] = 2;
@@ -182,10 +185,14 @@ int q4_rows_validate(const char* what, const void* kv_pool, const int32_t* block
   return DMLA_OK;
 }
 
-dim3 q4_rows_grid(int64_t rows) {
-  const int64_t per_wg = kWavesPerWG;
-  const int64_t wgs = (rows + per_wg - 1) / per_wg;
-  return dim3((unsigned)std::min<int64_t>(wgs, (int64_t)device_cu_count() * 8));
+// A wave takes neighbouring rows, as many as leave every SIMD eight waves, up to kBatch; a CU gets up to 64 workgroups,
+// eight times what fits (64 x 8192 rows appended in 193 us, 248 with the eight that fit; a gather of 32 x 5000 rows
+// 31.7 and 35.7 us).
+dim3 q4_rows_grid(int64_t rows, int& each) {
+  const int64_t cus = device_cu_count();
+  each = (int)std::min<int64_t>(kBatch, (rows + 32 * cus - 1) / (32 * cus));
+  const int64_t per_wg = (int64_t)kWavesPerWG * each;
+  return dim3((unsigned)std::min<int64_t>((rows + per_wg - 1) / per_wg, cus * 64));
 }
 
 }  // namespace
@@ -212,7 +219,8 @@ extern "C" int dmla_kv_append_q4(void* kv_pool, const int32_t* block_table, cons
   a.B = (int)B; a.n = (int)n_new;
   a.num_pages = (int)num_pages; a.max_pages = (int)max_pages_per_seq;
   a.ndiv = make_fastdiv((unsigned)n_new);
-  hipLaunchKernelGGL(q4_append_kernel, q4_rows_grid(B * n_new), dim3(64 * kWavesPerWG), 0, (hipStream_t)stream, a);
+  const dim3 grid = q4_rows_grid(B * n_new, a.each);
+  hipLaunchKernelGGL(q4_append_kernel, grid, dim3(64 * kWavesPerWG), 0, (hipStream_t)stream, a);
   return check_launch("dmla_kv_append_q4");
 }
 
@@ -234,8 +242,9 @@ extern "C" int dmla_kv_gather_q4(const void* kv_pool, const int32_t* block_table
   a.B = (int)B; a.n = (int)n_out;
   a.num_pages = (int)num_pages; a.max_pages = (int)max_pages_per_seq;
   a.ndiv = make_fastdiv((unsigned)n_out);
+  const dim3 grid = q4_rows_grid(B * n_out, a.each);
   auto launch = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, q4_rows_grid(B * n_out), dim3(64 * kWavesPerWG), 0, (hipStream_t)stream, a);
+    hipLaunchKernelGGL(kernel, grid, dim3(64 * kWavesPerWG), 0, (hipStream_t)stream, a);
   };
   if (B * n_out * kD * 2 >= kStreamBytes) launch(q4_gather_kernel<true>);
   else launch(q4_gather_kernel<false>);

@@ -6,7 +6,7 @@
 //    every wave issues one instruction in 4 to 5 cycles whatever its kind, and a step of 68 MFMAs (32 cycles
 //    each) has room for some 480.  Converting the codes in the operands' registers takes 800: 32 heads' scores
 //    need every code of the tile in every wave.  Here a tile becomes bf16 once, in LDS, a quarter by each
-//    wave (32 conversions and 8 writes a lane), and both products read plain operands.
+//    wave (32 conversions and 8 writes a lane), and both products read plain operands: 440 instructions.
 //  * Keys lie in LDS as rows of 1024 bytes (latent dims) whose 16-byte units are permuted by key: unit u of
 //    row r at u ^ key_swz(r).  The score product reads a unit of 32 rows (ds_read_b128), the value product
 //    32 columns of 8 rows transposed (ds_read_b64_tr_b16), the conversion writes one unit of 8 rows: none
@@ -15,11 +15,19 @@
 //    values straight to where the score product reads them: they are bf16 in the cache.
 //  * A wave computes the scores and the softmax of 32 heads (their queries: 144 registers) and the outputs
 //    of all 128 heads for 128 columns; probabilities go through LDS.
-//  * Step s multiplies scores of tile s and values of tile s - 1 and converts tile s + 1: one barrier a step,
-//    and the two products are independent.
+//  * Step s multiplies scores of tile s and values of tile s - 1 and converts tiles s + 1 and s + 2, with two barriers
+//    that stand among MFMAs whose operands are there.
+//    (Barriers that also wait for what follows them, and the copies of a whole tile in one place between the two
+//    products, had cost 500 of a step's 4000 cycles.)
 //  * The softmax reference of a head is its largest score in the segment's first tile; P may grow to 2^32
 //    past it (bf16 keeps its relative precision whatever the size, sums stay in fp32), and a segment
 //    whose scores climb further starts over from their exact maximum.
+//
+// Bound: the matrix units at the clock that they leave.  A tile takes 1.9 us with all CUs at work: 128 heads x 32 keys
+// x 1088 x 2 flops, 1.18 PFLOP/s over the chip, what an 8192^3 bf16 library product reaches here (1.2 PFLOP/s); it
+// took 2.1 us converted in registers.  Measured: 64 sequences of 1024 to 8192 tokens x 128 heads 94 us, the combine's
+// 10 in it (880 TFLOP/s); one sequence of 5000 tokens 25.5 us, where a segment's start (queries, first pages, first
+// tiles: 9 us) and end (4 us) are most of it.
 #include "dmla_host.h"
 #include "dmla_q4_decode.h"
 
