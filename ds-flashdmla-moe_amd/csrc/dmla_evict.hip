@@ -13,7 +13,8 @@
 // The selection is a radix select of the accounts' keys (digits of 11, 11 and 10 bits) and a pass in index
 // order that lists the freed places and the rows that fill them.
 //   * Up to kOneTokens tokens one workgroup per sequence holds the accounts in registers and does it all in one
-//     launch: 64 sequences of 4096 to 8192 tokens in 12.4 us (chunked as below 56), one of 16384 in 13 (27).
+//     launch.  Whole calls on 4-bit pages, cut to 4096 tokens: 64 sequences of 8192 tokens 36 us (chunked as below
+//     80), one of 16384 25 us (38).
 //   * Longer block tables: up to kMaxChunks workgroups per sequence, a launch per digit and one for the lists.  A
 //     chunk's counts go through the workspace and every workgroup adds up all chunks', so nothing is cleared
 //     beforehand and nothing depends on the order of atomics.  No chunk straddles the end of the kept low
@@ -622,6 +623,7 @@ extern "C" int dmla_kv_evict(void* kv_pool, const int32_t* block_table, const in
   const int64_t gy = std::min<int64_t>(B, 65535);
   if (cap <= kOneTokens) {
     auto select = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)gy), dim3(kSelThreads), 0, (hipStream_t)stream, a); };
+    // half the tokens a thread where they are enough: 64 sequences of 8192 tokens 36.8 us, 41.5 with all
     if (cap <= kOneTokens / 2) select(evict_select_kernel<kOneTokens / kSelThreads / 2>);
     else select(evict_select_kernel<kOneTokens / kSelThreads>);
   } else {
