@@ -31,6 +31,7 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 #define DMLA_LDS __attribute__((address_space(3)))
+#define DMLA_GLOBAL __attribute__((address_space(1)))
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;

@@ -43,7 +43,6 @@ constexpr int kMaxChunks = 32;
 constexpr int kPiece = 8;          // tokens of a thread at a time
 constexpr int kMoveRows = 32;      // rows that a workgroup moves at a time
 constexpr int kMoveBatch = 5;      // 16-byte pieces of a thread in flight (32 bf16 rows are nine for each thread)
-#define Global __attribute__((address_space(1)))
 
 struct EvictArgs {
   char* pool;
@@ -458,8 +457,8 @@ __device__ __forceinline__ void put_ends(const EvictArgs& a, int b, int n, int f
 // time: their addresses first, then their 16-byte pieces.  Grid: x over the rows of a sequence, y over sequences.
 template <int kPhase>
 __global__ void __launch_bounds__(256) evict_move_kernel(EvictArgs a) {
-  __shared__ const Global char* from[kMoveRows];
-  __shared__ Global char* to[kMoveRows];
+  __shared__ const DMLA_GLOBAL char* from[kMoveRows];
+  __shared__ DMLA_GLOBAL char* to[kMoveRows];
   const int want = a.budget - a.recent - a.sink;
   auto row_at = [&](int b, int pos) {
     return a.pool + a.block_table[b * a.bt_sb + pos / kPage] * a.kv_sp + (int64_t)(pos % kPage) * a.kv_ss;
@@ -493,19 +492,19 @@ __global__ void __launch_bounds__(256) evict_move_kernel(EvictArgs a) {
           f = staged ? stage + r * row_bytes : row_at(b, low_end + cut + r);
           t = row_at(b, low_end + r);
         }
-        from[threadIdx.x] = (const Global char*)f;
-        to[threadIdx.x] = (Global char*)t;
+        from[threadIdx.x] = (const DMLA_GLOBAL char*)f;
+        to[threadIdx.x] = (DMLA_GLOBAL char*)t;
       }
       __syncthreads();
       const int pieces = n * a.row_chunks;
       for (int q0 = threadIdx.x; q0 < pieces; q0 += 256 * kMoveBatch) {
         i32x4 v[kMoveBatch];
-        Global i32x4* at[kMoveBatch];
+        DMLA_GLOBAL i32x4* at[kMoveBatch];
 #pragma unroll
         for (int u = 0; u < kMoveBatch; ++u) {
           const int q = min(q0 + 256 * u, pieces - 1), r = fast_div(q, a.per_row), c = 16 * (q - r * a.row_chunks);
-          at[u] = (Global i32x4*)(to[r] + c);
-          v[u] = *(const Global i32x4*)(from[r] + c);
+          at[u] = (DMLA_GLOBAL i32x4*)(to[r] + c);
+          v[u] = *(const DMLA_GLOBAL i32x4*)(from[r] + c);
         }
 #pragma unroll
         for (int u = 0; u < kMoveBatch; ++u)

@@ -20,7 +20,7 @@ struct Q4DecodeParams {
   const int32_t* seqlens;
   bf16* o;
   float* lse;            // nullable
-  bf16* part_o;          // [slots, H, 512]
+  float* part_o;         // [slots, H, 512]
   float* part_lse;       // [slots, H]
   int32_t* num_splits;   // [B], with split_base what the combine reads
   int32_t* split_base;

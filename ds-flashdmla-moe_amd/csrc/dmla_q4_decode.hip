@@ -21,12 +21,14 @@
 //    past it (bf16 keeps its relative precision whatever the size, sums stay in fp32), and a segment
 //    whose scores climb further starts over from their exact maximum.
 //  * Sequences are cut over the chip's workgroups by weight (dmla_ranges.h); sequences in several parts
-//    are merged by the split-KV combine.
+//    are merged by the split-KV combine, from fp32.  Parts in bf16 saved 10 of 104 us at 64 sequences x 128 heads and 4
+//    of 74 at 16 heads, and cost precision: outputs 1.5 times as far from 64 bits as the rounding of an exact result
+//    (with P's rounding beside it), where fp32 parts leave 1.2 times.
 //
 // Bound: the cache's bytes, read at some 4.3 TB/s from scattered pages of 25.6 KB (a plain reduction over such a
 // pool reads 3.9), beside them one wave's instruction issue: an instruction takes it 4 to 5 cycles whatever its
-// kind, and a tile 750 of them.  Measured: 64 sequences of 2048 to 16384 tokens (236 MB) x 16 heads 71.5 us with the
-// combine, 3.3 TB/s; 256 workgroups take 0.61 us a tile and 15 us besides while the pages lie in the last cache.
+// kind, and a tile 750 of them.  Measured: 64 sequences of 2048 to 16384 tokens (229 MB) x 16 heads 74 us with the
+// combine, 3.1 TB/s; 256 workgroups take 0.61 us a tile and 15 us besides while the pages lie in the last cache.
 #include <algorithm>
 
 #include "dmla_host.h"
@@ -294,9 +296,6 @@ __device__ __forceinline__ void run_segment(const Q4DecodeParams& p, const Q4Seg
     }
     if (poison) sum = nanv;
   };
-  auto out_row = [&](int head) {
-    return sg.nsplit == 1 ? p.o + sg.b * p.o_sb + head * p.o_sh : p.part_o + ((int64_t)sg.slot * p.H + head) * kDv;
-  };
   auto put_lse = [&](int head, float top, float sum) {
     const float lse = sum == 0.f ? kNegInf : (top + __log2f(sum)) * kLn2;
     if (sg.nsplit > 1) p.part_lse[(int64_t)sg.slot * p.H + head] = lse;
@@ -335,13 +334,19 @@ __device__ __forceinline__ void run_segment(const Q4DecodeParams& p, const Q4Seg
         v1 += *reinterpret_cast<const DMLA_LDS f32x4*>(from + 4);
       }
       if (head < p.H) {
-        bf16x8 v;
+        if (sg.nsplit > 1) {   // parts stay in fp32
+          float* to = p.part_o + ((int64_t)sg.slot * p.H + head) * kDv + 128 * q4 + cc;
+          *reinterpret_cast<f32x4*>(to) = v0 * inv;
+          *reinterpret_cast<f32x4*>(to + 4) = v1 * inv;
+        } else {
+          bf16x8 v;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          v[j] = (bf16)(v0[j] * inv);
-          v[4 + j] = (bf16)(v1[j] * inv);
+          for (int j = 0; j < 4; ++j) {
+            v[j] = (bf16)(v0[j] * inv);
+            v[4 + j] = (bf16)(v1[j] * inv);
+          }
+          *reinterpret_cast<bf16x8*>(p.o + sg.b * p.o_sb + head * p.o_sh + 128 * q4 + cc) = v;
         }
-        *reinterpret_cast<bf16x8*>(out_row(head) + 128 * q4 + cc) = v;
         if (q4 == 0 && cc == 0) put_lse(head, top, sum);
       }
     }
@@ -374,8 +379,8 @@ __global__ __launch_bounds__(kThreads, 1) void q4_decode_kernel(Q4DecodeParams p
 }
 
 // Up to 64 heads, workgroups of 32 (two groups of them read a tile twice, the second time from the L2); above, of 128.
-// 64 sequences of 8192 tokens, this kernel against the wide one: 68 : 137 us with 16 heads, 71 : 140 with 32,
-// 106 : 133 with 64; 4 sequences 22 : 27, 25 : 29 and 30 : 31 us.  Three groups would cost what the wide kernel does.
+// 64 sequences of 8192 tokens, this kernel against the wide one: 71 : 149 us with 16 heads, 76 : 143 with 32, 114 : 143
+// with 64, 268 : 147 with 96; 4 sequences 26 : 36, 30 : 37, 35 : 36 and 37 : 37 us.
 bool narrow(int64_t H) { return H <= 2 * kHeads; }
 int wg_heads(int64_t H) { return narrow(H) ? kHeads : 128; }
 int64_t q4_ranges(int64_t H) {
@@ -392,7 +397,7 @@ static int64_t q4_plan_bytes(int64_t B) { return (B * 8 + 255) / 256 * 256; }
 
 extern "C" int64_t dmla_decode_q4_workspace_bytes(int64_t B, int64_t H) {
   if (B <= 0 || H <= 0 || B > ((int64_t)1 << 20) || H > ((int64_t)1 << 16)) return 0;
-  return q4_plan_bytes(B) + (q4_ranges(H) + B) * H * (int64_t)(kDv * 2 + 4);
+  return q4_plan_bytes(B) + (q4_ranges(H) + B) * H * (int64_t)(kDv * 4 + 4);
 }
 
 extern "C" int dmla_decode_paged_q4(const void* q, const void* kv_pool, const int32_t* block_table,
@@ -440,17 +445,17 @@ extern "C" int dmla_decode_paged_q4(const void* q, const void* kv_pool, const in
   p.lse = lse;
   p.num_splits = reinterpret_cast<int32_t*>(ws);
   p.split_base = p.num_splits + B;
-  p.part_o = reinterpret_cast<bf16*>(ws + q4_plan_bytes(B));
-  p.part_lse = reinterpret_cast<float*>(p.part_o + slots * H * kDv);
+  p.part_o = reinterpret_cast<float*>(ws + q4_plan_bytes(B));
+  p.part_lse = p.part_o + slots * H * kDv;
   p.q_sb = q_sb; p.q_sh = q_sh; p.kv_sp = kv_sp; p.bt_sb = bt_sb; p.o_sb = o_sb; p.o_sh = o_sh;
   p.B = (int)B; p.H = (int)H; p.num_pages = (int)num_pages; p.max_pages = (int)max_pages_per_seq;
   p.head_groups = (int)((H + wg_heads(H) - 1) / wg_heads(H));
   p.n_ranges = (int)R;
   p.scale_log2 = softmax_scale * kLog2e;
   const int grid = (int)((R + 7) / 8 * 8 * p.head_groups);
-  // The least work of a workgroup, in tiles: two for each wave; 16 tiles took 25.6 us at 4 sequences of 8192 tokens
-  // x 16 heads and 25.3 at one of 5000, 8 tiles 22.2 and 21.8, 4 tiles 24.4 and 20.8.  The wide kernel: 3 and 4
-  // tiles are as good at one sequence (25.3, 25.5 us), 8 take 30.0.
+  // The least work of a workgroup, in tiles: two for each wave.  4 sequences of 8192 tokens x 16 heads, and one of 5000:
+  // 6 tiles 27.7 and 23.3 us, 8 tiles 25.8 and 23.5, 10 tiles 26.5 and 25.9, 16 tiles 27.9 and 27.8.  The wide kernel at
+  // one of 5000: 3 to 6 tiles 29.6 to 30.2, 8 tiles 41.8.
   if (narrow(H)) {
     p.min_width = 8;
     hipLaunchKernelGGL(q4_decode_kernel, dim3((unsigned)grid), dim3(kThreads), 0, (hipStream_t)stream, p);
@@ -462,7 +467,7 @@ extern "C" int dmla_decode_paged_q4(const void* q, const void* kv_pool, const in
   if (rc != DMLA_OK) return rc;
   // Sequences in one part were written above; the others, and the empty ones, come from the combine.
   CombineArgs c = {};
-  c.part_o16 = p.part_o;
+  c.part_o = p.part_o;
   c.part_lse = p.part_lse;
   c.split_base = p.split_base;
   c.num_splits = p.num_splits;

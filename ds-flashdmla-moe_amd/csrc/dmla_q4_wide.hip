@@ -25,9 +25,9 @@
 //
 // Bound: the matrix units at the clock that they leave.  A tile takes 1.9 us with all CUs at work: 128 heads x 32 keys
 // x 1088 x 2 flops, 1.18 PFLOP/s over the chip, what an 8192^3 bf16 library product reaches here (1.2 PFLOP/s); it
-// took 2.1 us converted in registers.  Measured: 64 sequences of 1024 to 8192 tokens x 128 heads 94 us, the combine's
-// 10 in it (880 TFLOP/s); one sequence of 5000 tokens 25.5 us, where a segment's start (queries, first pages, first
-// tiles: 9 us) and end (4 us) are most of it.
+// took 2.1 us converted in registers.  Measured: 64 sequences of 1024 to 8192 tokens x 128 heads 104 us, the combine's
+// 15 in it (800 TFLOP/s); one sequence of 5000 tokens 30 us, where a segment's start (queries, first pages, first
+// tiles: 9 us), its end (5 us) and the combine (7 us) are most of it.
 #include "dmla_host.h"
 #include "dmla_q4_decode.h"
 
@@ -398,13 +398,27 @@ __device__ __forceinline__ void run_segment(const Q4DecodeParams& p, const Q4Seg
     if (sg.nsplit > 1) p.part_lse[(int64_t)sg.slot * p.H + head] = lse;
     else if (p.lse != nullptr) p.lse[sg.b * p.H + head] = lse;
   }
-  // Through LDS, so that a store covers 256 bytes of each of 4 heads.
-  const unsigned unit = lds_sum(256 * l32, mine);   // 16-byte unit u of row r at u ^ r % 16
-  const unsigned from = lds_sum(256 * (lane >> 4) + 16 * ((lane & 15) ^ (lane >> 4)), mine);
-  const int64_t stride = sg.nsplit == 1 ? p.o_sh : kQ4Dv;
-  bf16* out = (sg.nsplit == 1 ? p.o + sg.b * p.o_sb : p.part_o + (int64_t)sg.slot * p.H * kQ4Dv) +
-              (head0 + (lane >> 4)) * stride + 128 * wave + 8 * (lane & 15);
-  const int heads = p.H - head0 - (lane >> 4);
+  // Through LDS, 32 heads at a time, so that a store covers whole lines: 256 bytes of each of 4 heads, or of a part 512
+  // bytes of each of 2.  16-byte unit u of row r lies at u ^ r.
+  const int g = lane >> 4, c = lane & 15;
+  const unsigned put = lds_sum(512 * l32 + 16 * ((4 * hl) ^ l32), mine);
+  const unsigned get16 = lds_sum(512 * g + 16 * ((2 * c) ^ g), mine);   // 8 columns of row g: this unit and the one beside it
+  const unsigned get32 = lds_sum(512 * hl + 16 * (l32 ^ hl), mine);     // 4 columns of row hl
+  bf16* out = p.o + sg.b * p.o_sb + (head0 + g) * p.o_sh + 128 * wave + 8 * c;
+  float* part = p.part_o + ((int64_t)sg.slot * p.H + head0 + hl) * kQ4Dv + 128 * wave + 4 * l32;
+  auto put16 = [&](int r, bf16* to) {   // row 4 r + g
+    const f32x4 a = *lds_ptr<const f32x4>((get16 ^ (64 * r)) + 2048 * r), b = *lds_ptr<const f32x4>((get16 ^ (64 * r) ^ 16) + 2048 * r);
+    bf16x8 v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[i] = (bf16)a[i];
+      v[4 + i] = (bf16)b[i];
+    }
+    *reinterpret_cast<bf16x8*>(to) = v;
+  };
+  auto put32 = [&](int r, float* to) {   // row 2 r + hl
+    *reinterpret_cast<f32x4*>(to) = *lds_ptr<const f32x4>((get32 ^ (32 * r)) + 1024 * r);
+  };
 #pragma unroll
   for (int n = 0; n < kHeadBlocks; ++n) {
     const float sum = poison ? __builtin_nanf("") : lds.stat[32 * n + l32];
@@ -412,17 +426,27 @@ __device__ __forceinline__ void run_segment(const Q4DecodeParams& p, const Q4Seg
 #pragma unroll
     for (int j = 0; j < kColBlocks; ++j)
 #pragma unroll
-      for (int d = 0; d < 2; ++d) {
-        bf16x8 v;
+      for (int d = 0; d < 4; ++d) {
+        f32x4 v;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = (bf16)(agpr_read(acc[n][j][8 * d + i]) * inv);
-        *lds_ptr<bf16x8>(unit + 16 * ((4 * j + 2 * hl + d) ^ (l32 & 15))) = v;
+        for (int i = 0; i < 4; ++i) v[i] = agpr_read(acc[n][j][4 * d + i]) * inv;
+        *lds_ptr<f32x4>(put ^ (16 * (8 * j + d))) = v;
       }
+    const int heads = p.H - head0 - 32 * n;
+    if (heads >= 32) {
+      if (sg.nsplit == 1) {
 #pragma unroll
-    for (int r = 0; r < 8; ++r) {   // row 4 r + lane / 16
-      const bf16x8 v = *lds_ptr<const bf16x8>((from ^ (64 * (r & 3))) + 1024 * r);
-      if (32 * n + 4 * r < heads) *reinterpret_cast<bf16x8*>(out) = v;
-      out += 4 * stride;
+        for (int r = 0; r < 8; ++r) put16(r, out + (32 * n + 4 * r) * p.o_sh);
+      } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) put32(r, part + (32 * n + 2 * r) * kQ4Dv);
+      }
+    } else {   // the last heads
+#pragma nounroll
+      for (int r = 0; r < 16; ++r) {
+        if (sg.nsplit > 1 && 2 * r + hl < heads) put32(r, part + (32 * n + 2 * r) * kQ4Dv);
+        if (sg.nsplit == 1 && r < 8 && 4 * r + g < heads) put16(r, out + (32 * n + 4 * r) * p.o_sh);
+      }
     }
   }
 }
