@@ -9,9 +9,9 @@
 //    wave (32 conversions and 8 writes a lane), and both products read plain operands: 440 instructions.
 //  * Keys lie in LDS as rows of 1024 bytes (latent dims) whose 16-byte units are permuted by key: unit u of
 //    row r at u ^ key_swz(r).  The score product reads a unit of 32 rows (ds_read_b128), the value product
-//    32 columns of 8 rows transposed (ds_read_b64_tr_b16), the conversion writes one unit of 8 rows: none
-//    meets a bank twice.
-//  * Codes and scales are copied global -> LDS by the wave that converts them, three tiles ahead, the rope
+//    32 columns of 8 rows transposed (ds_read_b64_tr_b16), the conversion writes two units of 8 rows.  Bank
+//    conflicts are a fifth of the LDS cycles, most of them the writes'; without those the time stayed.
+//  * Codes and scales are copied global -> LDS by the wave that converts them, four tiles ahead, the rope
 //    values straight to where the score product reads them: they are bf16 in the cache.
 //  * A wave computes the scores and the softmax of 32 heads (their queries: 144 registers) and the outputs
 //    of all 128 heads for 128 columns; probabilities go through LDS.
@@ -65,7 +65,7 @@ __device__ __forceinline__ void run_segment(const Q4DecodeParams& p, const Q4Seg
 
   // ---- copies ----
   // Lane l copies 16 bytes of row 8 wave + l / 8 into place l of each kilobyte.  Which of the row's eight
-  // pieces is permuted by row, so that the readers below meet no bank twice.
+  // pieces is permuted by row, against bank conflicts of the readers below.
   Q4Pages pages;
   const char* copy_src = nullptr;
   int copy_last = 0;   // last row of the tile that the sequence holds
