@@ -187,6 +187,17 @@ __device__ __forceinline__ void dma16_after_v(const void* sbase, unsigned voff, 
                : "s"(sl), "v"(voff), "s"(reinterpret_cast<const void*>(sb)), "v"(d0), "v"(d1), "v"(d2), "v"(d3)
                : "m0");
 }
+// The copy by lanes 0..7 only, 128 bytes.  All 64 lanes are active around it.
+__device__ __forceinline__ void dma16_first8(const void* sbase, unsigned voff, unsigned lds_addr) {
+  const uint64_t base = reinterpret_cast<uint64_t>(sbase);
+  const uint64_t sb = ((uint64_t)__builtin_amdgcn_readfirstlane((unsigned)(base >> 32)) << 32) |
+                      (unsigned)__builtin_amdgcn_readfirstlane((unsigned)base);
+  const unsigned sl = __builtin_amdgcn_readfirstlane(lds_addr);
+  asm volatile("s_mov_b32 m0, %0\n\ts_mov_b64 exec, 0xff\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b64 exec, -1"
+               :
+               : "s"(sl), "v"(voff), "s"(reinterpret_cast<const void*>(sb))
+               : "memory", "m0");
+}
 // 4-byte direct global->LDS copy of one wave: lane l reads sbase + voff and lands at
 // lds_addr + 4*l (per-row scalars staged beside a tile).
 __device__ __forceinline__ void dma4(const void* sbase, unsigned voff, unsigned lds_addr) {

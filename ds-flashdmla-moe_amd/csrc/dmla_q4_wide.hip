@@ -87,12 +87,7 @@ __device__ __forceinline__ void run_segment(const Q4DecodeParams& p, const Q4Seg
     const unsigned off = min(8 * wave + (ln >> 3), copy_last) * kQ4RowBytes + 16 * ((ln & 7) ^ (ln >> 3));
     dma16(copy_src + kQ4RopeOff, off, lds.rope + (s % kRopeSlots) * kRopeBytes + wave * 1024);
     const unsigned soff = min(8 * wave + (ln & 7), copy_last) * kQ4RowBytes;
-    const unsigned sdst = uniform((int)(lds.codes + (s % kCodeSlots) * kCodeBytes + wave * kCodeWave + 2048));
-    // the scales: 8 lanes, 16 bytes each
-    asm volatile("s_mov_b32 m0, %0\n\ts_mov_b64 exec, 0xff\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b64 exec, -1"
-                 :
-                 : "s"(sdst), "v"(soff), "s"(copy_src + kQ4ScaleOff)
-                 : "memory");
+    dma16_first8(copy_src + kQ4ScaleOff, soff, lds.codes + (s % kCodeSlots) * kCodeBytes + wave * kCodeWave + 2048);
   };
   auto copy_step = [&](int s) {
     copy_begin(s);
