@@ -24,8 +24,8 @@
 // source lies at or past K - R, so those moves depend on nothing; the newest rows overwrite such sources and
 // therefore come last.
 // Bound: the moved rows' bytes, twice, and where few rows move the launches' latency.  64 sequences of 4096 to 8192
-// bf16 tokens cut to 4096: 66 us (selection 12, moves 38 and 9 with plain stores; 229 MB, 3.5 TB/s); one of 131072 cut
-// to 32768: 55 us, of which the four selection launches take 41.
+// bf16 tokens cut to 4096: 66 us (selection 12, moves 41 and 9; 229 MB, 3.5 TB/s); one of 131072 cut
+// to 32768: 53 us, of which the four selection launches take 38.
 #include <algorithm>
 
 #include "dmla_common.h"
@@ -343,23 +343,40 @@ __global__ void __launch_bounds__(kSelThreads) evict_chunk_kernel(EvictArgs a) {
     auto sel_of = [&](int d) { return a.sel + ((int64_t)(d & 1) * a.B + b) * 2; };   // of launch d
     unsigned prefix = kD > 1 ? (unsigned)sel_of(kD - 1)[0] : 0u;
     int left = kD > 1 ? sel_of(kD - 1)[1] : c.want;
+    // What does not depend on the pick is on its way beside it: the chunk's first accounts, and in the last launch
+    // the counts of the chunks w and w + 16 by wave w, and in lane i the tokens of chunk i above the earlier digits.
+    const float* mass = a.mass + b * a.m_sb;
+    const bool work = k < ch.n && c.want > 0;
+    const int from = work ? ch.from(c, k) : 0, to = work ? ch.to(c, k) : 0;
+    float v[kPiece];
+    unsigned in = load_accounts(mass, from, from, to, v);
+    constexpr int kEach = kMaxChunks / kSelWaves, kCounts = (1 << 10) / 64;
+    int counts[kD == 3 ? kEach : 1][kCounts];
+    int above = 0;
+    if constexpr (kD == 3) {
+#pragma unroll
+      for (int i = 0; i < kEach; ++i)
+#pragma unroll
+        for (int x = 0; x < kCounts; ++x) counts[i][x] = counts_of(2, min(wave + kSelWaves * i, ch.n - 1))[64 * x + lane];
+      above = a.above[b * a.chunks + min(lane, ch.n - 1)];
+    }
     if (kD > 0 && c.want > 0) {
       constexpr int d = kD - 1;
       const int top = digit_bins(d) - 1 - 2 * tid;
       int c0 = 0, c1 = 0, own = 0, own0 = 0, own1 = 0;
       if (top > 0) {
         for (int i0 = 0; i0 < ch.n; i0 += kBatch) {
-          int2 v[kBatch];   // on their way together
+          int2 x[kBatch];   // on their way together
 #pragma unroll
           for (int i = 0; i < kBatch; ++i)
-            v[i] = *reinterpret_cast<const int2*>(counts_of(d, min(i0 + i, ch.n - 1)) + top - 1);
+            x[i] = *reinterpret_cast<const int2*>(counts_of(d, min(i0 + i, ch.n - 1)) + top - 1);
 #pragma unroll
           for (int i = 0; i < kBatch; ++i) {
             const bool is = i0 + i < ch.n, mine = i0 + i == k;
-            c1 += is ? v[i].x : 0;
-            c0 += is ? v[i].y : 0;
-            own1 = mine ? v[i].x : own1;
-            own0 = mine ? v[i].y : own0;
+            c1 += is ? x[i].x : 0;
+            c0 += is ? x[i].y : 0;
+            own1 = mine ? x[i].x : own1;
+            own0 = mine ? x[i].y : own0;
           }
         }
       }
@@ -371,29 +388,31 @@ __global__ void __launch_bounds__(kSelThreads) evict_chunk_kernel(EvictArgs a) {
           sel_of(kD)[0] = (int)prefix;
           sel_of(kD)[1] = left;
         }
-      } else {   // wave w: the tokens of chunks w, w + 16 above the key, and those equal to it
-        for (int i = wave; i < ch.n; i += kSelWaves) {
-          const int32_t* counts = counts_of(d, i);
-          int sum = 0;
+      } else {   // the tokens of a chunk above the digit, and those equal to it
 #pragma unroll
-          for (int x = lane; x < 1 << 10; x += 64) sum += x > digit ? counts[x] : 0;
+        for (int i = 0; i < kEach; ++i) {
+          int sum = 0, equal = 0;
+#pragma unroll
+          for (int x = 0; x < kCounts; ++x) {
+            sum += 64 * x + lane > digit ? counts[i][x] : 0;
+            equal += 64 * x + lane == digit ? counts[i][x] : 0;
+          }
           sum = lane_scan(sum);
+          equal = lane_scan(equal);
           if (lane == 63) {
-            sh.kept[i] = a.above[b * a.chunks + i] + sum;
-            sh.equal[i] = counts[digit];
+            sh.kept[wave + kSelWaves * i] = sum;
+            sh.equal[wave + kSelWaves * i] = equal;
           }
         }
       }
     }
-    const float* mass = a.mass + b * a.m_sb;
     if constexpr (kD < 3) {
-      if (k < ch.n && c.want > 0) {
+      if (work) {
         for (int i = tid; i < digit_bins(kD); i += kSelThreads) sh.hist[i] = 0;
         __syncthreads();
-        const int from = ch.from(c, k), to = ch.to(c, k);
-        for (int i0 = from; i0 < to; i0 += kPiece * kSelThreads) {
-          float v[kPiece];
-          const unsigned in = load_accounts(mass, i0, from, to, v);
+        count_digit(sh.hist, kD, prefix, v, in);
+        for (int i0 = from + kPiece * kSelThreads; i0 < to; i0 += kPiece * kSelThreads) {
+          in = load_accounts(mass, i0, from, to, v);
           count_digit(sh.hist, kD, prefix, v, in);
         }
         __syncthreads();
@@ -409,7 +428,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_chunk_kernel(EvictArgs a) {
         static_assert(kMaxChunks <= 64, "a lane per chunk");
         const bool is = lane < ch.n;
         const int equal = is ? sh.equal[lane] : 0, equal_to = lane_scan(equal);
-        const int kept = (is ? sh.kept[lane] : 0) + min(max(left - (equal_to - equal), 0), equal);
+        const int kept = (is ? above + sh.kept[lane] : 0) + min(max(left - (equal_to - equal), 0), equal);
         const int freed = is && lane < ch.n_low ? ch.to(c, lane) - ch.from(c, lane) - kept : 0;
         const int moved = is && lane >= ch.n_low ? kept : 0;
         const int freed_to = lane_scan(freed), moved_to = lane_scan(moved);
@@ -417,11 +436,10 @@ __global__ void __launch_bounds__(kSelThreads) evict_chunk_kernel(EvictArgs a) {
         seen.equal = __builtin_amdgcn_readlane(equal_to - equal, k);
         seen.freed = __builtin_amdgcn_readlane(freed_to - freed, k);
         seen.late = __builtin_amdgcn_readlane(moved_to - moved, k);
-        if (k < ch.n) {
-          const int from = ch.from(c, k), to = ch.to(c, k);
-          for (int i0 = from; i0 < to; i0 += kPiece * kSelThreads) {
-            float v[kPiece];
-            const unsigned in = load_accounts(mass, i0, from, to, v);
+        if (work) {
+          place(a, b, c, sh, v, in, from, prefix, left, seen);
+          for (int i0 = from + kPiece * kSelThreads; i0 < to; i0 += kPiece * kSelThreads) {
+            in = load_accounts(mass, i0, from, to, v);
             place(a, b, c, sh, v, in, i0, prefix, left, seen);
           }
         }
