@@ -56,7 +56,8 @@ struct Tile {
   static constexpr int kCopies = kQ4 ? kBytes / 1024 : 9 * kWaves;       // of a step, all waves
   static constexpr int kMost = (kCopies + kWaves - 1) / kWaves, kLeast = kCopies / kWaves;   // of a wave
   static constexpr int kCost = kQ4 ? 4 / kPages : 4;                     // a segment's start and end, in steps
-  static constexpr int kQBytes = 24 * 1024;                              // queries of a head block, two rounds
+  static constexpr bool kOneRound = kHW * 36 * 1024 <= kSlots * kBytes;   // all queries fit the ring at once
+  static constexpr int kQBytes = (kOneRound ? 36 : 24) * 1024;           // queries of a head block in a round
   static_assert(kHW * kQBytes <= kSlots * kBytes, "the queries pass through the ring");
 };
 
@@ -109,7 +110,7 @@ __device__ __forceinline__ void mass_segment(const MassParams& p, int b, int t0,
   const int lane = fresh_lane_id();
   const int l32 = lane & 31, hl = lane >> 5;
   const int wave = uniform(threadIdx.x >> 6);
-  const int hw = wave % kHW, kp = wave / kHW;
+  const int hw = wave / kKP, kp = wave % kKP;   // with few heads, the waves at work sit on different SIMDs
   int page0 = 0, pages = 0;   // lane i: page page0 + i of the sequence
   auto fetch_pages = [&](int from) {
     page0 = uniform(from);
@@ -175,7 +176,7 @@ __device__ __forceinline__ void mass_segment(const MassParams& p, int b, int t0,
     const int hb = h0 + 32 * hw;
     const bool idle = hb >= p.H;   // no heads for this wave: it copies
     // Queries through the ring, 8 rows x 128 bytes a copy (as operands they would be 32 rows x 32 bytes a load),
-    // in two rounds of 64-dim blocks; the waves of a head block share the copies.
+    // in one round or two of 64-dim blocks; the waves of a head block share the copies.
     bf16x8 q[kQ4Steps];
     const unsigned stage = lds.ring + hw * T::kQBytes;
     auto queries = [&](auto first_tag, auto n_tag) {
@@ -200,8 +201,12 @@ __device__ __forceinline__ void mass_segment(const MassParams& p, int b, int t0,
       wait_lds();
       __syncthreads();
     };
-    queries(std::integral_constant<int, 0>{}, std::integral_constant<int, 6>{});
-    queries(std::integral_constant<int, 6>{}, std::integral_constant<int, 3>{});
+    if constexpr (T::kOneRound) {
+      queries(std::integral_constant<int, 0>{}, std::integral_constant<int, 9>{});
+    } else {
+      queries(std::integral_constant<int, 0>{}, std::integral_constant<int, 6>{});
+      queries(std::integral_constant<int, 6>{}, std::integral_constant<int, 3>{});
+    }
     fetch_pages(t0 * kPages);
     for (int t = t0; t < t0 + kSlots && t < t1; ++t) copy_step(t);
     float lse2[16];   // of the lane's rows, in log2 units; a head with no keys, or none at all, has weight 0

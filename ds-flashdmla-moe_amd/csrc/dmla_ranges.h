@@ -23,7 +23,8 @@ struct RangeLds {   // the segments of one chunk of kRangeThreads sequences
 
 // Calls segment(b, t0, t1, ctx, nsplit) for every piece of range r, with a barrier after each, and
 // owner(b, first_range, nsplit) on one thread for every sequence whose first tile lies in r (the empty
-// ones: r = 0).  All threads of the workgroup take part, those past kRangeThreads in the barriers.  ctx is the length, at most max_tokens.
+// ones: r = 0).  All threads of the workgroup take part, those past kRangeThreads in the barriers.  ctx is
+// the length, at most max_tokens.
 // The weights' sum stays below 2^31 (checked on the host).
 template <int kTokens, int kCost, typename SegmentFn, typename OwnerFn>
 __device__ __forceinline__ void for_each_segment(const int32_t* seqlens, int B, int max_tokens, int n_ranges, int min_width,
