@@ -328,7 +328,8 @@ int dmla_attn_mass(const void* q, const void* kv_pool, const int32_t* block_tabl
  *   mass_out  [B, mass_len] fp32 row stride mo_sb: mass moved like the rows, 0 from new_lens[b] on;
  *             must not overlap mass
  *   bad_index_flag  int32 device word; may be NULL; the caller clears it
- *   workspace dmla_kv_evict_workspace_bytes bytes, 16-byte aligned, contents ignored
+ *   workspace dmla_kv_evict_workspace_bytes bytes (of the same sizes on the current device), 16-byte aligned,
+ *             contents ignored
  */
 int64_t dmla_kv_evict_workspace_bytes(int64_t B, int64_t row_bytes, int64_t max_pages_per_seq,
                                       int64_t budget, int64_t recent, int64_t sink);
