@@ -1,5 +1,5 @@
 // Paged decode over the 4-bit latent cache (row format: dmla_q4.h): one query token per sequence.  This
-// kernel takes up to 64 heads, dmla_q4_wide.hip more.
+// kernel takes up to 64 heads, and small batches of any; dmla_q4_wide.hip the others.
 //
 //   s_ht = scale q_h . k_t,  o_h = sum_t softmax(s_h)_t k_t[:512],  k_t = code x scale (exact)
 //
@@ -28,8 +28,9 @@
 // Bound: the cache's bytes, read at some 4.3 TB/s from scattered pages of 25.6 KB (a plain reduction over such a
 // pool reads 3.9), and close to them one wave's instruction issue at the clock that power leaves: an instruction takes
 // it 4 to 5 cycles whatever its kind, and a tile 750 of them.  With all pages scattered over 420 MB a tile of four
-// waves' takes 0.79 us, with all-zero data 0.65 (5.0 TB/s).  Measured: 64 sequences of 2048 to 16384 tokens (229 MB) x 16 heads 74 us with the
-// combine, 3.1 TB/s; 256 workgroups take 0.61 us a tile and 15 us besides while the pages lie in the last cache.
+// waves' takes 0.79 us, with all-zero data 0.65 (5.0 TB/s).  Measured: 64 sequences of 2048 to 16384 tokens (229 MB) x
+// 16 heads 74 us with the combine, 3.1 TB/s; one of 5000 x 128 heads 26 us, latency; 256 workgroups take 0.61 us a tile
+// and 15 us besides while the pages lie in the last cache.
 #include <algorithm>
 
 #include "dmla_host.h"
@@ -256,6 +257,8 @@ __device__ __forceinline__ void run_segment(const Q4DecodeParams& p, const Q4Seg
 #pragma unroll
     for (int j = 0; j < 16; ++j) acc[j] = mfma32_bf16(bf16x8{}, bf16x8{}, f32x16{});
     wait_vm<0>();   // whatever the compiler has in flight, so that it does not wait for it in the loop
+    // The first tile's scores are computed again: kept across the loop's start, they cost spills in the loop
+    // (64 sequences x 16 heads 79 us).
 #pragma nounroll
     for (int s = 0; s < n_steps; ++s) {
       arrive(s, s > 0);
@@ -382,10 +385,13 @@ __global__ __launch_bounds__(kThreads, 1) void q4_decode_kernel(Q4DecodeParams p
 // Up to 64 heads, workgroups of 32 (two groups of them read a tile twice, the second time from the L2); above, of 128.
 // 64 sequences of 8192 tokens, this kernel against the wide one: 71 : 149 us with 16 heads, 76 : 143 with 32, 114 : 143
 // with 64, 268 : 147 with 96; 4 sequences 26 : 36, 30 : 37, 35 : 36 and 37 : 37 us.
-bool narrow(int64_t H) { return H <= 2 * kHeads; }
-int wg_heads(int64_t H) { return narrow(H) ? kHeads : 128; }
-int64_t q4_ranges(int64_t H) {
-  const int64_t hg = (H + wg_heads(H) - 1) / wg_heads(H);
+// Where the block tables hold up to four tiles a CU, latency counts, and more and smaller workgroups win for any
+// number of heads: one sequence of 5000 tokens x 128 heads 27 : 31 us, of 16384 36 : 40, 4 of 8192 38.5 : 39.7; one of
+// 65536 x 96 heads (eight tiles a CU) 71 : 55.
+int wg_heads(int64_t H, int64_t tiles) { return H <= 2 * kHeads || tiles <= 4 * (int64_t)device_cu_count() ? kHeads : 128; }
+// Ranges of a call, given the heads of a workgroup.
+int64_t q4_ranges(int64_t H, int64_t heads) {
+  const int64_t hg = (H + heads - 1) / heads;
   return std::max<int64_t>(1, device_cu_count() / hg);
 }
 
@@ -398,7 +404,8 @@ static int64_t q4_plan_bytes(int64_t B) { return (B * 8 + 255) / 256 * 256; }
 
 extern "C" int64_t dmla_decode_q4_workspace_bytes(int64_t B, int64_t H) {
   if (B <= 0 || H <= 0 || B > ((int64_t)1 << 20) || H > ((int64_t)1 << 16)) return 0;
-  return q4_plan_bytes(B) + (q4_ranges(H) + B) * H * (int64_t)(kDv * 4 + 4);
+  const int64_t most = std::max(q4_ranges(H, wg_heads(H, 0)), q4_ranges(H, wg_heads(H, INT64_MAX)));
+  return q4_plan_bytes(B) + (most + B) * H * (int64_t)(kDv * 4 + 4);
 }
 
 extern "C" int dmla_decode_paged_q4(const void* q, const void* kv_pool, const int32_t* block_table,
@@ -435,7 +442,8 @@ extern "C" int dmla_decode_paged_q4(const void* q, const void* kv_pool, const in
     return fail(DMLA_ERR_WORKSPACE, "dmla_decode_paged_q4: workspace of %lld bytes needed (got %lld)", (long long)need,
                 (long long)workspace_bytes);
   if (!aligned16(workspace)) return fail(DMLA_ERR_INVALID_ARG, "dmla_decode_paged_q4: workspace must be 16-byte aligned");
-  const int64_t R = q4_ranges(H), slots = R + B;
+  const int heads = wg_heads(H, B * max_pages_per_seq * (kPage / kTile));
+  const int64_t R = q4_ranges(H, heads), slots = R + B;
   char* ws = static_cast<char*>(workspace);
   Q4DecodeParams p = {};
   p.q = static_cast<const bf16*>(q);
@@ -450,14 +458,14 @@ extern "C" int dmla_decode_paged_q4(const void* q, const void* kv_pool, const in
   p.part_lse = p.part_o + slots * H * kDv;
   p.q_sb = q_sb; p.q_sh = q_sh; p.kv_sp = kv_sp; p.bt_sb = bt_sb; p.o_sb = o_sb; p.o_sh = o_sh;
   p.B = (int)B; p.H = (int)H; p.num_pages = (int)num_pages; p.max_pages = (int)max_pages_per_seq;
-  p.head_groups = (int)((H + wg_heads(H) - 1) / wg_heads(H));
+  p.head_groups = (int)((H + heads - 1) / heads);
   p.n_ranges = (int)R;
   p.scale_log2 = softmax_scale * kLog2e;
   const int grid = (int)((R + 7) / 8 * 8 * p.head_groups);
   // The least work of a workgroup, in tiles: two for each wave.  4 sequences of 8192 tokens x 16 heads, and one of 5000:
   // 6 tiles 27.7 and 23.3 us, 8 tiles 25.8 and 23.5, 10 tiles 26.5 and 25.9, 16 tiles 27.9 and 27.8.  The wide kernel at
   // one of 5000: 3 to 6 tiles 29.6 to 30.2, 8 tiles 41.8.
-  if (narrow(H)) {
+  if (heads == kHeads) {
     p.min_width = 8;
     hipLaunchKernelGGL(q4_decode_kernel, dim3((unsigned)grid), dim3(kThreads), 0, (hipStream_t)stream, p);
   } else {

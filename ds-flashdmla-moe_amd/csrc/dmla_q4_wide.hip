@@ -1,5 +1,5 @@
-// Paged decode over the 4-bit latent cache for more than 64 heads (up to 64: dmla_q4_decode.hip, which
-// states what is computed).
+// Paged decode over the 4-bit latent cache for more than 64 heads (up to 64, and small batches: dmla_q4_decode.hip,
+// which states what is computed).
 //
 // MI355X design:
 //  * One wave per SIMD: the fp32 outputs of 128 heads x 512 columns fill the AGPRs of the four waves, so
@@ -26,8 +26,7 @@
 // Bound: the matrix units at the clock that they leave.  A tile takes 1.9 us with all CUs at work: 128 heads x 32 keys
 // x 1088 x 2 flops, 1.18 PFLOP/s over the chip, what an 8192^3 bf16 library product reaches here (1.2 PFLOP/s); it
 // took 2.1 us converted in registers.  Measured: 64 sequences of 1024 to 8192 tokens x 128 heads 104 us, the combine's
-// 15 in it (800 TFLOP/s); one sequence of 5000 tokens 30 us, where a segment's start (queries, first pages, first
-// tiles: 9 us), its end (5 us) and the combine (7 us) are most of it.
+// 15 in it (800 TFLOP/s); a segment's start (queries, first pages, first tiles) takes 9 us and its end 5.
 #include "dmla_host.h"
 #include "dmla_q4_decode.h"
 

@@ -63,7 +63,15 @@ def _reference(q, pool, table, lens, scale):
     return o, lse, tol_o, tol_l
 
 
+def _spacious(table, tiles=1200):
+    """The same table in a wider one of at least that many 32-token tiles, with pages that must not be touched."""
+    B, n = table.shape
+    return torch.cat((table, torch.full((B, max(0, tiles // (2 * B) + 1 - n)), -1, dtype=torch.int32)), 1)
+
+
 def _check(gpu, q, pool, table, lens, scale=SCALE):
+    if q.shape[1] > 64 and 2 * table.numel() < 1200:   # small and large batches run in different kernels
+        _check(gpu, q, pool, _spacious(table), lens, scale)
     o, lse = ops.flash_dmla_decode_paged_q4(q.to(gpu), pool.to(gpu), table.to(gpu), lens.to(gpu), 512, scale, return_lse=True)
     torch.cuda.synchronize()
     o_ref, lse_ref, tol_o, tol_l = _reference(q, pool, table, lens, scale)
@@ -231,19 +239,21 @@ def test_decode_wide_query_ranges(gpu):
 
 
 @pytest.mark.gpu
-def test_decode_strided_tensors_large_offsets_and_lengths_past_the_table(gpu):
+@pytest.mark.parametrize("H,spacious", [(24, False), (24, True), (128, False), (128, True)])
+def test_decode_strided_tensors_and_large_offsets(gpu, H, spacious):
     lens = [130, 64, 77]
     pool, table, sl = _cache(lens, 71)
-    q = seeded((3, 24, 576), 72, 0.5, torch.bfloat16)
+    table = _spacious(table) if spacious else table
+    q = seeded((3, H, 576), 72, 0.5, torch.bfloat16)
     o_ref = ops.flash_dmla_decode_paged_q4(q.to(gpu), pool.to(gpu), table.to(gpu), sl.to(gpu), 512, SCALE)
     # query and table as parts of larger tensors, pages with a gap between them
-    qw = torch.zeros(3, 30, 640, dtype=torch.bfloat16, device=gpu)
-    qw[:, 3:27, 32:608] = q.to(gpu)
-    tw = torch.full((3, 9), 1 << 30, dtype=torch.int32, device=gpu)
+    qw = torch.zeros(3, H + 6, 640, dtype=torch.bfloat16, device=gpu)
+    qw[:, 3:3 + H, 32:608] = q.to(gpu)
+    tw = torch.full((3, table.shape[1] + 6), 1 << 30, dtype=torch.int32, device=gpu)
     tw[:, 2:2 + table.shape[1]] = table.to(gpu)
     pw = torch.zeros(pool.shape[0], 70, 400, dtype=torch.uint8, device=gpu)
     pw[:, :64] = pool.to(gpu)
-    o = ops.flash_dmla_decode_paged_q4(qw[:, 3:27, 32:608], pw[:, :64], tw[:, 2:2 + table.shape[1]], sl.to(gpu), 512, SCALE)
+    o = ops.flash_dmla_decode_paged_q4(qw[:, 3:3 + H, 32:608], pw[:, :64], tw[:, 2:2 + table.shape[1]], sl.to(gpu), 512, SCALE)
     assert torch.equal(o, o_ref)
     # pages past 4 GiB of the pool
     far = torch.empty(200000, 64, 400, dtype=torch.uint8, device=gpu)
@@ -253,8 +263,26 @@ def test_decode_strided_tensors_large_offsets_and_lengths_past_the_table(gpu):
     assert torch.equal(o, o_ref)
     rows = ops.flash_dmla_kv_gather_q4(far, tf.to(gpu), sl.to(gpu), 130)
     assert torch.equal(rows, ops.flash_dmla_kv_gather_q4(pool.to(gpu), table.to(gpu), sl.to(gpu), 130))
-    del far
-    # a length past the table ends at the table, a negative one is empty
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,spacious", [(24, False), (128, False), (128, True)])
+def test_decode_lengths_past_the_table_and_negative_ones(gpu, H, spacious):
+    """A length past the table ends at the table, a negative one is empty."""
+    lens = [130, 64, 77]
+    pool, table, sl = _cache(lens, 71)
+    q = seeded((3, H, 576), 72, 0.5, torch.bfloat16)
+    if spacious:   # 400 columns of one good page: the first sequence fills the table
+        table = torch.cat((table, table[:, :1].expand(3, 397)), 1).contiguous()
+        over, full = torch.tensor([10 ** 9, 64, -3], dtype=torch.int32), torch.tensor([25600, 64, 0], dtype=torch.int32)
+        pool2 = pool.clone()
+        pool2[int(table[0, 2]), 2:] = pool[int(table[0, 0]), 2:]
+        args = (q.to(gpu), pool2.to(gpu), table.to(gpu))
+        a, la = ops.flash_dmla_decode_paged_q4(*args, over.to(gpu), 512, SCALE, return_lse=True)
+        b, lb = ops.flash_dmla_decode_paged_q4(*args, full.to(gpu), 512, SCALE, return_lse=True)
+        assert a.isfinite().all() and torch.equal(a, b) and torch.equal(la, lb)
+        assert torch.isneginf(la[2]).all() and (a[2] == 0).all()
+        return
     over = torch.tensor([10 ** 9, 64, -3], dtype=torch.int32)
     full = torch.tensor([192, 64, 0], dtype=torch.int32)
     pool2 = pool.clone()
@@ -266,10 +294,11 @@ def test_decode_strided_tensors_large_offsets_and_lengths_past_the_table(gpu):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("H", [16, 64, 128])
-def test_decode_poison_stays_with_its_sequence_or_head(gpu, H):
+@pytest.mark.parametrize("H,spacious", [(16, False), (64, False), (128, False), (128, True)])
+def test_decode_poison_stays_with_its_sequence_or_head(gpu, H, spacious):
     lens = [200, 3000, 90, 64]
     pool, table, sl = _cache(lens, 81)
+    table = _spacious(table) if spacious else table
     q = seeded((4, H, 576), 82, 0.5, torch.bfloat16)
     good = ops.flash_dmla_decode_paged_q4(q.to(gpu), pool.to(gpu), table.to(gpu), sl.to(gpu), 512, SCALE)
     for bad_page in (pool.shape[0], -1, 1 << 30):
