@@ -10,6 +10,8 @@ constexpr int kQ4Tile = 32;                                // tokens of a key ti
 constexpr int kQ4TileBytes = kQ4Tile * kQ4RowBytes;        // 12800
 constexpr int kQ4Waves = 4, kQ4Threads = 64 * kQ4Waves;    // a wave per SIMD: 512 registers each
 static_assert(kQ4Threads == kRangeThreads, "one workgroup cuts the ranges");
+// What starting and ending a segment costs, in tiles (dmla_ranges.h), with 32 and with 128 heads a workgroup.
+constexpr int kQ4Cost = 24, kQ4WideCost = 8;
 // log2 headroom of P over a head's reference
 constexpr float kQ4Headroom = 32.0f;
 

@@ -47,7 +47,6 @@ constexpr int kSlotBytes = kWaves * kTileBytes, kSlots = 3;
 constexpr int kRingBytes = kSlots * kSlotBytes;
 constexpr int kMergeRow = 128 + 4;             // floats, padded against bank conflicts
 static_assert(kWaves * kHeads * kMergeRow * 4 <= kRingBytes, "the merge reuses the ring");
-constexpr int kSegCost = 24;
 
 struct Lds {
   DMLA_LDS char* ring;
@@ -370,7 +369,7 @@ __global__ __launch_bounds__(kThreads, 1) void q4_decode_kernel(Q4DecodeParams p
   const int hg = (id / 8) % p.head_groups;
   const int r = (id / (8 * p.head_groups)) * 8 + id % 8;
   if (r >= p.n_ranges) return;
-  for_each_segment<kTile, kSegCost>(
+  for_each_segment<kTile, kQ4Cost>(
       p.seqlens, p.B, p.max_pages * kPage, p.n_ranges, p.min_width, r, ranges,
       [&](int b, int t0, int t1, int ctx, int nsplit) {
         run_segment(p, Q4Segment{b, t0, t1, ctx, nsplit, r + b}, lds, hg * kHeads);
@@ -431,19 +430,21 @@ extern "C" int dmla_decode_paged_q4(const void* q, const void* kv_pool, const in
     return fail(DMLA_ERR_INVALID_ARG, "dmla_decode_paged_q4: page stride must be a multiple of 16 bytes and cover a page");
   if (bt_sb < max_pages_per_seq)
     return fail(DMLA_ERR_INVALID_ARG, "dmla_decode_paged_q4: block_table row stride < max_pages_per_seq");
-  if (H > ((int64_t)1 << 16) || B > ((int64_t)1 << 20) || max_pages_per_seq > ((int64_t)1 << 24) || num_pages > 0x7fffffff ||
-      B * (max_pages_per_seq * 2 + 16) >= ((int64_t)1 << 31))
+  if (H > ((int64_t)1 << 16) || B > ((int64_t)1 << 20) || max_pages_per_seq > ((int64_t)1 << 24) || num_pages > 0x7fffffff)
     return fail(DMLA_ERR_UNSUPPORTED, "dmla_decode_paged_q4: size too large");
   if (B == 0 || H == 0) return DMLA_OK;
   if (num_pages == 0 || max_pages_per_seq == 0)
     return fail(DMLA_ERR_INVALID_ARG, "dmla_decode_paged_q4: empty page pool or block table");
+  const int64_t tiles = max_pages_per_seq * (kPage / kTile);   // of a sequence, at most
+  const int heads = wg_heads(H, B * tiles);
+  const int64_t R = q4_ranges(H, heads), slots = R + B;
+  if (!ranges_fit(B, tiles, heads == kHeads ? kQ4Cost : kQ4WideCost, R))
+    return fail(DMLA_ERR_UNSUPPORTED, "dmla_decode_paged_q4: size too large");
   const int64_t need = dmla_decode_q4_workspace_bytes(B, H);
   if (workspace == nullptr || workspace_bytes < need)
     return fail(DMLA_ERR_WORKSPACE, "dmla_decode_paged_q4: workspace of %lld bytes needed (got %lld)", (long long)need,
                 (long long)workspace_bytes);
   if (!aligned16(workspace)) return fail(DMLA_ERR_INVALID_ARG, "dmla_decode_paged_q4: workspace must be 16-byte aligned");
-  const int heads = wg_heads(H, B * max_pages_per_seq * (kPage / kTile));
-  const int64_t R = q4_ranges(H, heads), slots = R + B;
   char* ws = static_cast<char*>(workspace);
   Q4DecodeParams p = {};
   p.q = static_cast<const bf16*>(q);

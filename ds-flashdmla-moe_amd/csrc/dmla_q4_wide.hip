@@ -45,7 +45,6 @@ constexpr int kRopeBytes = kTile * 128, kRopeSlots = 4;
 constexpr int kProbBytes = kWaves * 2048;      // P of a step
 constexpr int kAhead = 4;                      // tiles between a copy's start and its step
 constexpr int kCopies = 4;                     // copies of a wave and step
-constexpr int kSegCost = 8;
 
 // Unit permutation of row r: 16 consecutive rows differ, and rows r .. r + 3 differ in the upper two bits.
 __device__ __forceinline__ int key_swz(int r) { return (r & 3) << 2 | (r >> 2 & 3); }
@@ -461,7 +460,7 @@ __global__ __launch_bounds__(kThreads, 1) void q4_wide_kernel(Q4DecodeParams p) 
   const int hg = (id / 8) % p.head_groups;
   const int r = (id / (8 * p.head_groups)) * 8 + id % 8;
   if (r >= p.n_ranges) return;
-  for_each_segment<kTile, kSegCost>(
+  for_each_segment<kTile, kQ4WideCost>(
       p.seqlens, p.B, p.max_pages * kQ4Page, p.n_ranges, p.min_width, r, ranges,
       [&](int b, int t0, int t1, int ctx, int nsplit) {
         run_segment(p, Q4Segment{b, t0, t1, ctx, nsplit, r + b}, lds, hg * kHeads);

@@ -21,11 +21,17 @@ struct RangeLds {   // the segments of one chunk of kRangeThreads sequences
   int tmp[kRangeWaves];
 };
 
+// Whether the cut of B sequences of at most `tiles` tiles stays within 32-bit integers: their weights' sum, the
+// rounding up of its division by the ranges, and the cost that stands before an empty sequence at the end.
+inline bool ranges_fit(int64_t B, int64_t tiles, int64_t cost, int64_t n_ranges) {
+  return B * (tiles + cost) + n_ranges + cost <= 0x7fffffff;
+}
+
 // Calls segment(b, t0, t1, ctx, nsplit) for every piece of range r, with a barrier after each, and
 // owner(b, first_range, nsplit) on one thread for every sequence whose first tile lies in r (the empty
 // ones: r = 0).  All threads of the workgroup take part, those past kRangeThreads in the barriers.  ctx is
 // the length, at most max_tokens.
-// The weights' sum stays below 2^31 (checked on the host).
+// The sums are 32-bit integers: the host has checked ranges_fit.
 template <int kTokens, int kCost, typename SegmentFn, typename OwnerFn>
 __device__ __forceinline__ void for_each_segment(const int32_t* seqlens, int B, int max_tokens, int n_ranges, int min_width,
                                                  int r, RangeLds& lds, SegmentFn segment, OwnerFn owner) {
