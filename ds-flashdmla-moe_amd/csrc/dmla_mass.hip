@@ -209,12 +209,14 @@ __device__ __forceinline__ void mass_segment(const MassParams& p, int b, int t0,
     }
     fetch_pages(t0 * kPages);
     for (int t = t0; t < t0 + kSlots && t < t1; ++t) copy_step(t);
-    float lse2[16];   // of the lane's rows, in log2 units; a head with no keys, or none at all, has weight 0
+    float lse2[16];   // of the lane's rows, in log2 units
+    bool on[16];      // a head with lse = -inf, or none at all, adds nothing, whatever its score (a lane mask in SGPRs)
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       const int head = hb + 8 * (i >> 2) + 4 * hl + (i & 3);
       const float v = head < p.H ? p.lse[(int64_t)b * p.H + head] : kNegInf;
-      lse2[i] = v == kNegInf ? -kNegInf : v * kLog2e;
+      lse2[i] = v * kLog2e;
+      on[i] = v != kNegInf;
     }
     const int n_hw = min(kHW, (p.H - h0 + 31) / 32);
     float* mass = p.mass + b * p.m_sb;
@@ -232,7 +234,10 @@ __device__ __forceinline__ void mass_segment(const MassParams& p, int b, int t0,
         const f32x16 s = scores<kQ4>(q, tile, lane);
         float sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) sum += fast_exp2(__builtin_fmaf(s[i], p.scale_log2, -lse2[i]));
+        for (int i = 0; i < 16; ++i) {
+          const float w = fast_exp2(__builtin_fmaf(s[i], p.scale_log2, -lse2[i]));
+          sum += on[i] ? w : 0.f;
+        }
         sum = half_sum(sum);
         const bool bad = (bad_bits >> (kPages * slot + kp / 2) & 1) != 0;
         if (hl == 0) lds.sums[hw * kChunk + (t - chunk0) * T::kTokens + 32 * kp + l32] = bad ? 0.f : sum;

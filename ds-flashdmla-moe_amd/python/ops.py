@@ -557,7 +557,7 @@ def flash_dmla_attn_mass(
 
     q, block_table, cache_seqlens and softmax_scale as the step's decode took them; lse [B, H] as it
     returned it; kv_pool its bf16 [num_pages, 64, 576] or 4-bit [num_pages, 64, 400] pages; mass
-    [B, >= 64 * max_pages] fp32.  Heads with lse = -inf add nothing, and tokens on a page outside the pool get
+    [B, >= 64 * max_pages] fp32.  Heads with lse = -inf add nothing, whatever their queries hold, and tokens on a page outside the pool get
     nothing.  Deterministic.
     """
     _check_bf16("q", q, 3)

@@ -295,7 +295,8 @@ int dmla_decode_paged_q4(const void* q, const void* kv_pool, const int32_t* bloc
  *   q        [B, H, 576] bf16   strides (q_sb, q_sh)
  *   kv_pool  pages of 64 tokens, bf16 rows of 576 (q4 = 0) or 4-bit rows of 400 bytes (q4 != 0, rows
  *            following each other); strides (kv_sp, kv_ss) in BYTES, multiples of 16
- *   lse      [B, H] fp32 contiguous, as dmla_decode_paged[_q4] wrote it; a head with lse = -inf adds 0
+ *   lse      [B, H] fp32 contiguous, as dmla_decode_paged[_q4] wrote it; a head with lse = -inf adds 0,
+ *            whatever its query and the keys hold
  *   mass     [B, mass_len] fp32 row stride m_sb, mass_len >= 64 max_pages_per_seq; added to in place,
  *            untouched from the sequence's length on and for tokens whose page index is outside
  *            [0, num_pages)
