@@ -586,7 +586,8 @@ extern "C" int dmla_kv_evict(void* kv_pool, const int32_t* block_table, const in
                              int64_t budget, int64_t recent, int64_t sink, void* workspace, int64_t workspace_bytes,
                              dmla_stream_t stream) {
   clear_error();
-  if (!kv_pool || !block_table || !cache_seqlens || !mass || !new_lens || !src || !mass_out)
+  // (Of an empty call any address does: empty tensors have none.)
+  if (B != 0 && (!kv_pool || !block_table || !cache_seqlens || !mass || !new_lens || !src || !mass_out))
     return fail(DMLA_ERR_INVALID_ARG, "dmla_kv_evict: null pointer argument");
   if (B < 0 || num_pages < 0 || max_pages_per_seq < 0 || mass_len < 0)
     return fail(DMLA_ERR_INVALID_ARG, "dmla_kv_evict: negative size");

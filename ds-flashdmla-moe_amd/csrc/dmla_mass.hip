@@ -287,7 +287,8 @@ extern "C" int dmla_attn_mass(const void* q, const void* kv_pool, const int32_t*
                               int64_t kv_ss, int64_t bt_sb, int64_t m_sb, int q4, float softmax_scale,
                               dmla_stream_t stream) {
   clear_error();
-  if (!q || !kv_pool || !block_table || !cache_seqlens || !lse || !mass)
+  // (Of an empty call any address does: empty tensors have none.)
+  if (B != 0 && H != 0 && (!q || !kv_pool || !block_table || !cache_seqlens || !lse || !mass))
     return fail(DMLA_ERR_INVALID_ARG, "dmla_attn_mass: null pointer argument");
   if (B < 0 || H < 0 || num_pages < 0 || max_pages_per_seq < 0 || mass_len < 0)
     return fail(DMLA_ERR_INVALID_ARG, "dmla_attn_mass: negative size");

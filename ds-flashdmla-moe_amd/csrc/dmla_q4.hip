@@ -166,7 +166,8 @@ __global__ void __launch_bounds__(64 * kWavesPerWG) q4_gather_kernel(Q4RowArgs a
 int q4_rows_validate(const char* what, const void* kv_pool, const int32_t* block_table, const int32_t* cache_seqlens,
                      const void* rows, int64_t B, int64_t n, int64_t num_pages, int64_t max_pages_per_seq,
                      int64_t kv_sp, int64_t bt_sb, int64_t r_sb, int64_t r_ss) {
-  if (!kv_pool || !block_table || !cache_seqlens || !rows)
+  // (Of an empty call any address does: empty tensors have none.)
+  if (B != 0 && n != 0 && (!kv_pool || !block_table || !cache_seqlens || !rows))
     return fail(DMLA_ERR_INVALID_ARG, "%s: null pointer argument", what);
   if (B < 0 || n < 0 || num_pages < 0 || max_pages_per_seq < 0)
     return fail(DMLA_ERR_INVALID_ARG, "%s: negative size", what);

@@ -413,7 +413,8 @@ extern "C" int dmla_decode_paged_q4(const void* q, const void* kv_pool, const in
                                     int64_t q_sb, int64_t q_sh, int64_t kv_sp, int64_t bt_sb, int64_t o_sb, int64_t o_sh,
                                     float softmax_scale, void* workspace, int64_t workspace_bytes, dmla_stream_t stream) {
   clear_error();
-  if (!q || !kv_pool || !block_table || !cache_seqlens || !o)
+  // (Of an empty call any address does: empty tensors have none.)
+  if (B != 0 && H != 0 && (!q || !kv_pool || !block_table || !cache_seqlens || !o))
     return fail(DMLA_ERR_INVALID_ARG, "dmla_decode_paged_q4: null pointer argument");
   if (B < 0 || H < 0 || num_pages < 0 || max_pages_per_seq < 0)
     return fail(DMLA_ERR_INVALID_ARG, "dmla_decode_paged_q4: negative size");
