@@ -1,7 +1,7 @@
 // The writer and the reader of the 4-bit paged latent cache (row format: dmla_q4.h):
 //   * the append quantises new bf16 rows into pages through the block table;
 //   * the gather reads a window of each sequence back as dense bf16 rows (what a chunked prefill over
-//     cached context takes as k_lat).
+//     cached context takes as k_lat, one length a call).
 // No reference counterpart: the reference has no paged cache.
 #include <algorithm>
 

@@ -461,10 +461,12 @@ def flash_dmla_kv_gather_q4(
     max_len: int,
     starts: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
-    """Reads 4-bit pages back as dense rows: [B, max_len, 576] bf16, what flash_dmla_fwd takes as k_lat.
+    """Reads 4-bit pages back as dense rows: [B, max_len, 576] bf16.
 
     Row i of sequence b is the token at starts[b] + i (starts [B] int32, zeros when None); rows at or
-    past cache_seqlens[b] are zeros, rows on a page outside the pool are NaN.
+    past cache_seqlens[b] are zeros, rows on a page outside the pool are NaN.  flash_dmla_fwd takes them
+    as k_lat where all sequences have max_len rows; it knows no lengths, and a zero row is a key to it,
+    so a shorter sequence goes in a call of its own, with rows[b:b + 1, :n].
     """
     _check_q4_pool(kv_pool)
     B = cache_seqlens.shape[0]
@@ -557,8 +559,8 @@ def flash_dmla_attn_mass(
 
     q, block_table, cache_seqlens and softmax_scale as the step's decode took them; lse [B, H] as it
     returned it; kv_pool its bf16 [num_pages, 64, 576] or 4-bit [num_pages, 64, 400] pages; mass
-    [B, >= 64 * max_pages] fp32.  Heads with lse = -inf add nothing, whatever their queries hold, and tokens on a page outside the pool get
-    nothing.  Deterministic.
+    [B, >= 64 * max_pages] fp32.  Heads with lse = -inf add nothing, whatever their queries hold, and
+    tokens on a page outside the pool get nothing.  Deterministic.
     """
     _check_bf16("q", q, 3)
     row_bytes, kv_sp, kv_ss = _check_pool(kv_pool)

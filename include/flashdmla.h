@@ -260,7 +260,8 @@ int dmla_lse_combine(const float* part_o, const float* part_lse, const int32_t* 
  *
  * Gather: out [B, n_out, 576] bf16, strides (o_sb, o_ss).  Row i of sequence b is the value of the
  * token at starts[b] + i (starts NULL: i; negative: 0), zeros at or past cache_seqlens[b] (at most
- * 64 max_pages_per_seq), NaN where the token's page index is outside [0, num_pages).
+ * 64 max_pages_per_seq), NaN where the token's page index is outside [0, num_pages).  The prefill takes
+ * no lengths and sees such zeros as keys: give it a shorter sequence's rows only, in a call of its own.
  */
 int dmla_kv_append_q4(void* kv_pool, const int32_t* block_table, const int32_t* cache_seqlens,
                       const int32_t* new_lens, const void* new_kv, int32_t* bad_index_flag, int64_t B,
