@@ -22,6 +22,7 @@ constexpr int kQ4Chunks = kQ4RowBytes / 16;   // 16-byte pieces of a row
 constexpr int kQ4MinExp = -125, kQ4MaxExp = 125;
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 

@@ -14,6 +14,9 @@ static_assert(kQ4Threads == kRangeThreads, "one workgroup cuts the ranges");
 constexpr int kQ4Cost = 24, kQ4WideCost = 8;
 // log2 headroom of P over a head's reference
 constexpr float kQ4Headroom = 32.0f;
+// A block scale from which values (up to 6 scales) may overflow the sums together with the headroom: below it
+// 6 x 2^60 x 2^32 leaves room for 2^33 tokens.
+constexpr int kQ4BigScale = 60;   // log2
 
 struct Q4DecodeParams {
   const bf16* q;
@@ -82,6 +85,16 @@ struct Q4Pages {
     return p.kv + page * p.kv_sp + (t & 1) * kQ4TileBytes;
   }
 };
+
+// What a wave posts at the end of a segment.  It starts over from the largest scores seen if one of them is past the
+// headroom, or past its reference at all where big values are in it.
+constexpr int kQ4Over = 1, kQ4Climbed = 2, kQ4Big = 4;
+__device__ __forceinline__ int q4_climb(float mtrue, float mref, bool big) {
+  return (__any(mtrue > mref + kQ4Headroom) ? kQ4Over : 0) | (__any(mtrue > mref) ? kQ4Climbed : 0) | (__any(big) ? kQ4Big : 0);
+}
+__device__ __forceinline__ bool q4_repeat(int posted) {
+  return (posted & kQ4Over) != 0 || (posted & (kQ4Climbed | kQ4Big)) == (kQ4Climbed | kQ4Big);
+}
 
 void launch_q4_wide(const Q4DecodeParams& p, int grid, hipStream_t stream);
 

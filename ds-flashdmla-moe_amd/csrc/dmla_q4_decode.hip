@@ -19,7 +19,8 @@
 //    at the end of a segment.
 //  * The softmax reference of a head is its largest score in the wave's first tile; P may grow to 2^32
 //    past it (bf16 keeps its relative precision whatever the size, sums stay in fp32), and a segment
-//    whose scores climb further starts over from their exact maximum.
+//    whose scores climb further starts over from their exact maximum.  So does one whose scores climb at all
+//    where the latents reach 2^60, since 2^32 times those might leave fp32.
 //  * Sequences are cut over the chip's workgroups by weight (dmla_ranges.h); sequences in several parts
 //    are merged by the split-KV combine, from fp32.  Parts in bf16 saved 10 of 104 us at 64 sequences x 128 heads and 4
 //    of 74 at 16 heads, and cost precision: outputs 1.5 times as far from 64 bits as the rounding of an exact result
@@ -120,6 +121,7 @@ __device__ __forceinline__ void run_segment(const Q4DecodeParams& p, const Q4Seg
   f32x16 acc[16];           // O^T of 32 heads and 32 columns: row m is column 16 m + j
   float mref = kNegInf, mtrue = kNegInf, lsum = 0.f;   // reference, largest score seen, sum
   bf16x8 pv[2];             // P, 16 keys each
+  u16x2 vtop = {0, 0};      // largest scales seen, in the upper bytes
 
   // S^T[key 8 (i / 4) + 4 hl + i % 4][head l32] of a tile.
   auto scores = [&](int s, int t) -> f32x16 {
@@ -145,6 +147,7 @@ __device__ __forceinline__ void run_segment(const Q4DecodeParams& p, const Q4Seg
     auto block = [&](auto a_tag) {
       constexpr int a = decltype(a_tag)::value;
       if constexpr (a + 2 < kBlocks) w[(a + 2) % 3] = codes_of(a + 2);
+      if constexpr (a < 4) vtop = __builtin_elementwise_max(vtop, __builtin_bit_cast(u16x2, scales[a] << 8));   // bytes 0 and 2
       float sc = 0.f;
       if constexpr (a + 1 < kBlocks) {
         sc = q4_key_scale<a + 1>(scales);
@@ -264,12 +267,12 @@ __device__ __forceinline__ void run_segment(const Q4DecodeParams& p, const Q4Seg
       softmax(scores(s, sg.t0 + s * kWaves + wave));
       values(s);
     }
-    const bool over = __any(mtrue > mref + kQ4Headroom);
-    if (lane == 0) lds.flag[wave] = over ? 1 : 0;
+    const int climb = q4_climb(mtrue, mref, max(vtop[0], vtop[1]) >> 8 >= kQ4BigScale + 127);
+    if (lane == 0) lds.flag[wave] = climb;
     wait_vm<0>();
     wait_lds();
     __syncthreads();   // flags posted; the ring is free
-    const bool repeat = (lds.flag[0] | lds.flag[1] | lds.flag[2] | lds.flag[3]) != 0;
+    const bool repeat = q4_repeat(lds.flag[0] | lds.flag[1] | lds.flag[2] | lds.flag[3]);
     __syncthreads();   // flags read
     if (again || !repeat) break;
     start_copies();

@@ -21,7 +21,7 @@
 //    products, had cost 500 of a step's 4000 cycles.)
 //  * The softmax reference of a head is its largest score in the segment's first tile; P may grow to 2^32
 //    past it (bf16 keeps its relative precision whatever the size, sums stay in fp32), and a segment
-//    whose scores climb further starts over from their exact maximum.
+//    whose scores climb further, or at all over latents of 2^60 and more, starts over from their exact maximum.
 //
 // Bound: the matrix units at the clock that they leave.  A tile takes 1.9 us with all CUs at work: 128 heads x 32 keys
 // x 1088 x 2 flops, 1.18 PFLOP/s over the chip, what an 8192^3 bf16 library product reaches here (1.2 PFLOP/s); it
@@ -154,6 +154,7 @@ __device__ __forceinline__ void run_segment(const Q4DecodeParams& p, const Q4Seg
     float sc[2];
     unsigned to;
   } cv;
+  float vtop = 0.f;   // largest scale of the converted rows
   auto convert_begin = [&](int s, unsigned tile) {
     const int r = lane & 7, c = lane >> 3, row = 8 * wave + r;
     const unsigned from = opaque(lds.codes + (unsigned)(s % kCodeSlots) * kCodeBytes + wave * kCodeWave);
@@ -276,6 +277,7 @@ __device__ __forceinline__ void run_segment(const Q4DecodeParams& p, const Q4Seg
       convert_begin(s, tile);
 #pragma unroll
       for (int i = 0; i < 8; ++i) convert_octet(i);
+      vtop = fmaxf(vtop, fmaxf(cv.sc[0], cv.sc[1]));
     };
     convert(0, prev);
     convert(1, cur);
@@ -315,6 +317,7 @@ __device__ __forceinline__ void run_segment(const Q4DecodeParams& p, const Q4Seg
       f32x16 x = scores([&](auto m_tag) {
         constexpr int m = decltype(m_tag)::value;
         if constexpr (m < 16 && m % 2 == 0) convert_octet(m / 2);
+        if constexpr (m == 16) vtop = fmaxf(vtop, fmaxf(cv.sc[0], cv.sc[1]));
         if constexpr (m == 22) {
           wait_lds<5>();   // the octets are written; reads of later keys may be on their way
           barrier();           // A
@@ -366,12 +369,12 @@ __device__ __forceinline__ void run_segment(const Q4DecodeParams& p, const Q4Seg
     read_values(0);
     read_values(1);
     values([](auto) {});
-    const bool over = __any(mtrue > mref + kQ4Headroom);
-    if (lane == 0) lds.flag[wave] = over ? 1 : 0;
+    const int climb = q4_climb(mtrue, mref, vtop >= q4_scale(kQ4BigScale + 127));
+    if (lane == 0) lds.flag[wave] = climb;
     wait_vm<0>();
     wait_lds();
     __syncthreads();   // flags posted; all of the memory is free
-    const bool repeat = (lds.flag[0] | lds.flag[1] | lds.flag[2] | lds.flag[3]) != 0;
+    const bool repeat = q4_repeat(lds.flag[0] | lds.flag[1] | lds.flag[2] | lds.flag[3]);
     __syncthreads();   // flags read
     if (again || !repeat) break;
     start_copies();

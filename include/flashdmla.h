@@ -276,7 +276,8 @@ int dmla_kv_gather_q4(const void* kv_pool, const int32_t* block_table, const int
  * dmla_decode_paged over 4-bit pages: same arguments, results and treatment of lengths and page
  * indices, without the page and row sizes (64 tokens of 400 bytes).
  *   Codes become bf16 values exactly; scores are bf16 products summed in fp32, the probabilities enter
- *   the value product as bf16, sums and the parts of a sequence that is split stay in fp32.
+ *   the value product as bf16, sums and the parts of a sequence that is split stay in fp32: outputs are
+ *   finite while the largest |value| times the number of tokens stays below 2^127.
  * The workspace (16-byte aligned, contents ignored) holds the partial outputs; its size depends on
  * the current device.  Supported: d_qk = 576, d_v = 512.
  */
