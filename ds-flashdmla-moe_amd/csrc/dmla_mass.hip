@@ -13,8 +13,8 @@
 //  * A wave holds its heads' queries in registers (144) as the MFMA's row operand, keys are its columns, so a
 //    lane ends with one key's scores of 16 heads and the sum over heads is in-lane adds and a lane swap.
 //  * Every token belongs to one workgroup and its sum to one thread: no atomics, the same bits every time.
-//    Measured: 64 sequences of 1024 to 8192 tokens x 128 heads on bf16 pages 74 us, 4.8 TB/s (four waves, each with
-//    half the registers idle, 115); one of 5000 tokens 9.9 us; 16 sequences x 16 heads on 4-bit pages 13.1 us.
+//    Measured: 64 sequences of 1024 to 8192 tokens x 128 heads on bf16 pages 76 us, 4.7 TB/s (four waves, each with
+//    half the registers idle, 115); one of 5000 tokens 10.1 us; 16 sequences x 16 heads on 4-bit pages 13.2 us.
 //    The sums of kChunk tokens wait in LDS, beside the account's old values, which are copied there like keys:
 //    a load into registers would wait for every copy before it.
 #include <algorithm>
@@ -328,8 +328,8 @@ extern "C" int dmla_attn_mass(const void* q, const void* kv_pool, const int32_t*
   const dim3 grid((unsigned)p.n_ranges);
   auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, (hipStream_t)stream, p); };
   // bf16 rows bound the pass whatever the heads.  Of 4-bit rows, up to 64 heads, four blocks of keys at once keep
-  // more waves busy: 64 sequences of 8192 tokens 44 us with 16 heads, 56 with 64 (two blocks: 60 and 65); 128 heads
-  // take 104 (89).
+  // more waves busy: 64 sequences of 8192 tokens 44 us with 16 heads, 56 with 64 (two blocks: 60 and 63); 128 heads
+  // take 102 (86).
   if (!q4) launch(mass_kernel<false, 1>);
   else if (H > 64) launch(mass_kernel<true, 1>);
   else launch(mass_kernel<true, 2>);
