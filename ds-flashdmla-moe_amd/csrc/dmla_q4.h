@@ -9,9 +9,7 @@
 // held as that), so code x scale is exact in bf16 and reading a row back rounds nothing.  The rope
 // values carry the position and stay in bf16.  A block that holds an infinity or a NaN is all NaN.
 #pragma once
-#include <type_traits>
-
-#include "dmla_common.h"
+#include "dmla_pipe.h"
 
 namespace dmla {
 
@@ -84,47 +82,6 @@ __device__ __forceinline__ bf16x8 q4_key_rope(const DMLA_LDS char* row, int h, i
 template <int kA>
 __device__ __forceinline__ float q4_key_scale(const u32x4& scales) {
   return q4_scale_of<2 * (kA % 2)>(scales[kA / 2]);
-}
-
-// f(0), f(1), .., f(kN - 1) with compile-time arguments.
-template <int kN, typename F, int kI = 0>
-__device__ __forceinline__ void static_for(F f) {
-  if constexpr (kI < kN) {
-    f(std::integral_constant<int, kI>{});
-    static_for<kN, F, kI + 1>(f);
-  }
-}
-
-// Nothing moves across: the order of a pipelined loop body is the source's.
-__device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); }
-
-// Address lane_off + add as one register that the compiler does not see into: it would keep an address per
-// read up to date in a loop otherwise.
-__device__ __forceinline__ unsigned lds_sum(int lane_off, unsigned add) {
-  unsigned a;
-  asm("v_add_u32 %0, %1, %2" : "=v"(a) : "v"(lane_off), "s"(add));
-  return a;
-}
-template <typename T>
-__device__ __forceinline__ DMLA_LDS T* lds_ptr(unsigned addr) {
-  return reinterpret_cast<DMLA_LDS T*>(static_cast<uintptr_t>(addr));
-}
-
-// Wait until at most N vector-memory (LDS) operations of this wave are outstanding; they end in order, and no
-// memory access moves across.
-template <int N>
-__device__ __forceinline__ void wait_vm() {
-  static_assert(N >= 0 && N < 64, "vmcnt field");
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | 0x0f70);
-  asm volatile("" ::: "memory");
-}
-template <int N = 0>
-__device__ __forceinline__ void wait_lds() {
-  static_assert(N >= 0 && N < 16, "lgkmcnt field");
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_waitcnt(0xc07f | (N << 8));
-  asm volatile("" ::: "memory");
 }
 
 }  // namespace dmla

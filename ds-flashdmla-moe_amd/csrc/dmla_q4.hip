@@ -20,6 +20,7 @@ struct Q4RowArgs {
   const int32_t* block_table;
   const int32_t* seqlens;
   const int32_t* lens;     // append: new_lens; gather: starts (both nullable)
+  const int32_t* slots;    // append by slot: page * 64 + row of each row; below 0: not written
   bf16* rows;              // append: new_kv (read); gather: out
   int32_t* bad;            // append only; nullable
   int64_t kv_sp, bt_sb, r_sb, r_ss;
@@ -44,6 +45,8 @@ __device__ __forceinline__ bf16x2 as_bf16x2(unsigned w) { return __builtin_bit_c
 // Bound: HBM (1152 bytes in, 400 out per row), and below some 20000 rows launch and latency: 8 x 2048 rows in 6.6 us,
 // 64 x 8192 rows in 192 us, 4.2 TB/s.  kBatch rows per wave keep enough loads in flight (eight measured 13 % slower).
 // Rows built in LDS and stored in 16-byte pieces instead of 256 + 16 x 1 + 128 bytes a row took the same time.
+// kSlots: packed rows (B = 1) that go where their slots say.
+template <bool kSlots>
 __global__ void __launch_bounds__(64 * kWavesPerWG) q4_append_kernel(Q4RowArgs a) {
   const int lane = lane_id();
   const int wave = uniform(threadIdx.x >> 6);
@@ -57,16 +60,28 @@ __global__ void __launch_bounds__(64 * kWavesPerWG) q4_append_kernel(Q4RowArgs a
       dst[i] = -1;
       const int64_t r = r0 + i;
       if (i >= a.each || r >= total) continue;
-      const int b = fast_div((int)r, a.ndiv), t = (int)r - b * a.n;
-      if (a.lens != nullptr && t >= a.lens[b]) continue;
-      const int64_t pos = (int64_t)max(a.seqlens[b], 0) + t;
-      const int page = page_of(a, b, pos);
-      if (page < 0) {
-        if (a.bad != nullptr && lane == 0) a.bad[0] = 1;
-        continue;
+      const bf16* src;
+      if constexpr (kSlots) {
+        const int slot = a.slots[r];
+        if (slot < 0) continue;
+        if (slot / kPage >= a.num_pages) {
+          if (a.bad != nullptr && lane == 0) a.bad[0] = 1;
+          continue;
+        }
+        dst[i] = slot / kPage * a.kv_sp + slot % kPage * kQ4RowBytes;
+        src = a.rows + r * a.r_ss;
+      } else {
+        const int b = fast_div((int)r, a.ndiv), t = (int)r - b * a.n;
+        if (a.lens != nullptr && t >= a.lens[b]) continue;
+        const int64_t pos = (int64_t)max(a.seqlens[b], 0) + t;
+        const int page = page_of(a, b, pos);
+        if (page < 0) {
+          if (a.bad != nullptr && lane == 0) a.bad[0] = 1;
+          continue;
+        }
+        dst[i] = page * a.kv_sp + (pos % kPage) * kQ4RowBytes;
+        src = a.rows + b * a.r_sb + t * a.r_ss;
       }
-      dst[i] = page * a.kv_sp + (pos % kPage) * kQ4RowBytes;
-      const bf16* src = a.rows + b * a.r_sb + t * a.r_ss;
       x[i] = *reinterpret_cast<const bf16x8*>(src + 8 * lane);
       if (lane < 8) rope[i] = *reinterpret_cast<const bf16x8*>(src + kLat + 8 * lane);
     }
@@ -221,8 +236,37 @@ extern "C" int dmla_kv_append_q4(void* kv_pool, const int32_t* block_table, cons
   a.num_pages = (int)num_pages; a.max_pages = (int)max_pages_per_seq;
   a.ndiv = make_fastdiv((unsigned)n_new);
   const dim3 grid = q4_rows_grid(B * n_new, a.each);
-  hipLaunchKernelGGL(q4_append_kernel, grid, dim3(64 * kWavesPerWG), 0, (hipStream_t)stream, a);
+  hipLaunchKernelGGL(q4_append_kernel<false>, grid, dim3(64 * kWavesPerWG), 0, (hipStream_t)stream, a);
   return check_launch("dmla_kv_append_q4");
+}
+
+extern "C" int dmla_kv_append_rows_q4(void* kv_pool, const int32_t* slots, const void* rows, int32_t* bad_index_flag,
+                                      int64_t T, int64_t num_pages, int64_t kv_sp, int64_t r_ss, dmla_stream_t stream) {
+  clear_error();
+  if (T > 0 && (!slots || !rows || (num_pages > 0 && !kv_pool)))
+    return fail(DMLA_ERR_INVALID_ARG, "dmla_kv_append_rows_q4: null pointer argument");
+  if (T < 0 || num_pages < 0) return fail(DMLA_ERR_INVALID_ARG, "dmla_kv_append_rows_q4: negative size");
+  if (!aligned16(kv_pool) || !aligned16(rows))
+    return fail(DMLA_ERR_INVALID_ARG, "dmla_kv_append_rows_q4: the pool and the rows must be 16-byte aligned");
+  if (kv_sp % 16 != 0 || kv_sp < kPage * kQ4RowBytes)
+    return fail(DMLA_ERR_INVALID_ARG, "dmla_kv_append_rows_q4: page stride must be a multiple of 16 bytes and cover a page (got %lld)",
+                (long long)kv_sp);
+  if (!mult8(r_ss) || r_ss < kD)
+    return fail(DMLA_ERR_INVALID_ARG, "dmla_kv_append_rows_q4: row strides must be multiples of 8 and cover a row");
+  if (T >= ((int64_t)1 << 31) || num_pages > ((int64_t)1 << 25))
+    return fail(DMLA_ERR_UNSUPPORTED, "dmla_kv_append_rows_q4: size too large");
+  if (T == 0) return DMLA_OK;
+  Q4RowArgs a = {};
+  a.pool = static_cast<uint8_t*>(kv_pool);
+  a.slots = slots;
+  a.rows = static_cast<bf16*>(const_cast<void*>(rows));
+  a.bad = bad_index_flag;
+  a.kv_sp = kv_sp; a.r_ss = r_ss;
+  a.B = 1; a.n = (int)T;
+  a.num_pages = (int)num_pages;
+  const dim3 grid = q4_rows_grid(T, a.each);
+  hipLaunchKernelGGL(q4_append_kernel<true>, grid, dim3(64 * kWavesPerWG), 0, (hipStream_t)stream, a);
+  return check_launch("dmla_kv_append_rows_q4");
 }
 
 extern "C" int dmla_kv_gather_q4(const void* kv_pool, const int32_t* block_table, const int32_t* cache_seqlens,

@@ -40,30 +40,6 @@ struct Q4Segment {
   int b, t0, t1, ctx, nsplit, slot;
 };
 
-// The output accumulators fill the AGPR file.  Where ordinary code touches them, the compiler gives them a
-// home among the VGPRs as well and spills the queries; these accesses leave them where they are.  The
-// compiler does not see into the assembly, so agpr_settle() keeps them clear of MFMAs on the same register.
-__device__ __forceinline__ float agpr_read(float x) {
-  float v;
-  asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(v) : "a"(x));
-  return v;
-}
-// Longer than any MFMA takes to write its result, or a write to reach one.
-__device__ __forceinline__ void agpr_settle() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
-
-// One step of the score product, x += k q (x = k q for the first of a tile).  In assembly because the
-// AGPRs have no room for x beside the accumulators and the compiler gives every MFMA of a kernel the same
-// register file.  It does not see the waits that such an operand needs.  An operand written by the vector ALU
-// has to be two instructions old.  (An s_nop in every step would cost half an MFMA: 24.0 against 18.4 ns for
-// an MFMA with four conversions beside it, 15.4 alone.)  Steps on the same x follow each other without a
-// wait.  score_done() stands between the last and the first read.
-template <bool kFirst>
-__device__ __forceinline__ void score_step(f32x16& x, const bf16x8& k, const bf16x8& q) {
-  if constexpr (kFirst) asm("v_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(x) : "v"(k), "v"(q));
-  else asm("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(x) : "v"(k), "v"(q));
-}
-__device__ __forceinline__ void score_done(f32x16& x) { asm("s_nop 15\n\ts_nop 7" : "+v"(x)); }
-
 // The pages of a segment, 64 at a time in a register (lane i: page first + i).
 struct Q4Pages {
   int first = 0, pages = 0;

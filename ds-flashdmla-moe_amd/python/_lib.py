@@ -144,6 +144,59 @@ SIGNATURES = {
         + [_i64] * 3  # budget, recent, sink
         + [_ptr, _i64, _ptr],  # workspace, workspace_bytes, stream
     ),
+    "dmla_kv_release": (
+        _int,
+        [_ptr] * 7  # block_table, old_lens, new_lens, free_pages, free_count, new_count, bad_index_flag
+        + [_i64] * 5  # B, num_pages, max_pages_per_seq, capacity, bt_sb
+        + [_ptr],  # stream
+    ),
+    "dmla_kv_reserve": (
+        _int,
+        # block_table, cache_seqlens, new_lens, free_pages, free_count, total_lens, cu_seqlens, slots, new_count, flag
+        [_ptr] * 10
+        + [_i64] * 6  # B, num_rows, num_pages, max_pages_per_seq, capacity, bt_sb
+        + [_ptr],  # stream
+    ),
+    "dmla_kv_append_rows": (
+        _int,
+        [_ptr] * 4  # kv_pool, slots, rows, bad_index_flag
+        + [_i64] * 6  # T, d, num_pages, kv_sp, kv_ss, r_ss
+        + [_ptr],  # stream
+    ),
+    "dmla_kv_append_rows_q4": (
+        _int,
+        [_ptr] * 4  # kv_pool, slots, rows, bad_index_flag
+        + [_i64] * 4  # T, num_pages, kv_sp, r_ss
+        + [_ptr],  # stream
+    ),
+    "dmla_chunk_paged_workspace_bytes": (_i64, [_i64] * 4),  # T B H max_pages
+    "dmla_chunk_paged": (
+        _int,
+        [_ptr] * 7  # q, kv_pool, block_table, cache_seqlens, cu_seqlens_q, o, lse
+        + [_i64] * 7  # T, B, H, d_qk, d_v, num_pages, max_pages_per_seq
+        + [_i64] * 7  # q_st q_sh kv_sp kv_ss bt_sb o_st o_sh
+        + [_f32, _int, _ptr, _i64, _ptr],  # scale, causal, workspace, workspace_bytes, stream
+    ),
+    "dmla_page_means": (
+        _int,
+        [_ptr] * 5  # kv_pool, block_table, cache_seqlens, starts, means
+        + [_i64] * 7  # B, num_pages, max_pages_per_seq, kv_sp, kv_ss, bt_sb, m_sp
+        + [_int, _ptr],  # q4, stream
+    ),
+    "dmla_page_scores_workspace_bytes": (_i64, [_i64] * 3 + [_int]),  # T H max_pages packed
+    "dmla_page_scores": (
+        _int,
+        [_ptr] * 6  # q, means, block_table, cache_seqlens, cu_seqlens_q, scores
+        + [_i64] * 6  # T, B, H, d_qk, num_pages, max_pages_per_seq
+        + [_i64] * 5  # q_st q_sh m_sp bt_sb s_st
+        + [_f32, _ptr, _i64, _ptr],  # scale, workspace, workspace_bytes, stream
+    ),
+    "dmla_page_select": (
+        _int,
+        [_ptr] * 7  # scores, block_table, cache_seqlens, cu_seqlens_q, sel_table, sel_lens, sel_index
+        + [_i64] * 10  # T, B, max_pages_per_seq, s_st, bt_sb, st_st, si_st, top_pages, recent, sink
+        + [_ptr],  # stream
+    ),
     "dmla_bwd_workspace_bytes": (_i64, [_i64] * 6 + [_int]),  # B H Sq Sk d_qk d_v causal
     "dmla_bwd_cache_latent": (
         _int,

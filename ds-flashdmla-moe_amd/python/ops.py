@@ -400,6 +400,11 @@ def _check_q4_pool(t: torch.Tensor) -> None:
                      "follow each other")
 
 
+def _row_stride(t: torch.Tensor) -> int:
+    """Stride of a matrix's rows, at least their width: of at most one row it is free."""
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
 def _check_tables(block_table: torch.Tensor, cache_seqlens: torch.Tensor, B: int) -> None:
     _check_index("block_table", block_table, 2)
     _check_index("cache_seqlens", cache_seqlens, 1)
@@ -632,6 +637,351 @@ def flash_dmla_kv_evict(
     if check_indices:
         _require(int(flag.item()) == 0, "kv evict: a sequence has a page index outside the pool (left as it was)")
     return new_lens, src, new_mass
+
+
+def _check_lens(name: str, t: torch.Tensor, B: int) -> None:
+    _check_index(name, t, 1)
+    if t.shape[0] != B:
+        raise ValueError(f"{name} must hold {B} entries, got {t.shape[0]}")
+
+
+def _check_free(block_table: torch.Tensor, free_pages: torch.Tensor, free_count: torch.Tensor, num_pages: int) -> None:
+    _check_index("block_table", block_table, 2)
+    _check_index("free_pages", free_pages, 1)
+    _check_lens("free_count", free_count, 1)
+    _require(num_pages >= 0, "num_pages must be >= 0")
+
+
+@_on_tensor_device
+def flash_dmla_kv_release(
+    block_table: torch.Tensor,
+    old_lens: torch.Tensor,
+    new_lens: torch.Tensor,
+    free_pages: torch.Tensor,
+    free_count: torch.Tensor,
+    num_pages: int,
+    check_indices: bool = False,
+) -> torch.Tensor:
+    """Gives back the pages that shorter or finished sequences no longer need: returns the new free count [1] int32.
+
+    block_table [B, max_pages] int32 (its entries stay as they are); old_lens, new_lens [B] int32, the lengths
+    before and after (0: finished; what flash_dmla_kv_evict returned as new_lens: evicted).  free_pages [capacity]
+    int32 is a stack whose first free_count[0] (free_count [1] int32, not changed) entries are the pages that nobody
+    has: the pages go on its top, in place.  Entries outside [0, num_pages), and pages past the capacity, are left
+    out; check_indices=True raises afterwards (one device sync).
+    """
+    _check_free(block_table, free_pages, free_count, num_pages)
+    B, max_pages = block_table.shape
+    _check_lens("old_lens", old_lens, B)
+    _check_lens("new_lens", new_lens, B)
+    _same_device(block_table=block_table, old_lens=old_lens, new_lens=new_lens, free_pages=free_pages,
+                 free_count=free_count)
+    new_count = torch.empty((1,), dtype=torch.int32, device=block_table.device)
+    flag = torch.zeros(1, dtype=torch.int32, device=block_table.device) if check_indices else None
+    _lib.call(
+        "dmla_kv_release",
+        _ptr(block_table), _ptr(old_lens), _ptr(new_lens), _ptr(free_pages), _ptr(free_count), _ptr(new_count), _ptr(flag),
+        B, num_pages, max_pages, free_pages.shape[0], _row_stride(block_table), _stream(block_table),
+    )
+    if check_indices:
+        _require(int(flag.item()) == 0, "kv release: a page index outside the pool, or more pages than free_pages holds")
+    return new_count
+
+
+@_on_tensor_device
+def flash_dmla_kv_reserve(
+    block_table: torch.Tensor,
+    cache_seqlens: torch.Tensor,
+    new_lens: torch.Tensor,
+    free_pages: torch.Tensor,
+    free_count: torch.Tensor,
+    num_rows: int,
+    num_pages: int,
+    check_indices: bool = False,
+) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Pages for the tokens that sequences are about to get, and the slot of each of their rows.
+
+    block_table [B, max_pages] int32, in place: sequence b of cache_seqlens[b] tokens gets the pages that new_lens[b]
+    more need, from the top of the stack free_pages (flash_dmla_kv_release).  Returns
+      total_lens [B] int32 -- cache_seqlens + new_lens;
+      cu_seqlens [B + 1] int32 -- where each sequence's rows start in a packed array of num_rows;
+      slots [num_rows] int32 -- page * 64 + row of each packed row, -1 behind the last sequence;
+      new_count [1] int32 -- the free pages left (free_count is not changed).
+    A sequence whose pages are not there, whose tokens do not fit its row of the table or whose rows pass num_rows gets
+    none: its total stays cache_seqlens[b] and its slots are -1; check_indices=True raises afterwards (one device sync).
+    """
+    _check_free(block_table, free_pages, free_count, num_pages)
+    B, max_pages = block_table.shape
+    _check_lens("cache_seqlens", cache_seqlens, B)
+    _check_lens("new_lens", new_lens, B)
+    _require(num_rows >= 0, "num_rows must be >= 0")
+    _same_device(block_table=block_table, cache_seqlens=cache_seqlens, new_lens=new_lens, free_pages=free_pages,
+                 free_count=free_count)
+    dev = block_table.device
+    total = torch.empty((B,), dtype=torch.int32, device=dev)
+    cu = torch.empty((B + 1,), dtype=torch.int32, device=dev)
+    slots = torch.empty((num_rows,), dtype=torch.int32, device=dev)
+    new_count = torch.empty((1,), dtype=torch.int32, device=dev)
+    flag = torch.zeros(1, dtype=torch.int32, device=dev) if check_indices else None
+    _lib.call(
+        "dmla_kv_reserve",
+        _ptr(block_table), _ptr(cache_seqlens), _ptr(new_lens), _ptr(free_pages), _ptr(free_count), _ptr(total), _ptr(cu),
+        _ptr(slots), _ptr(new_count), _ptr(flag), B, num_rows, num_pages, max_pages, free_pages.shape[0],
+        _row_stride(block_table), _stream(block_table),
+    )
+    if check_indices:
+        _require(int(flag.item()) == 0, "kv reserve: a sequence got no pages, or has a page index outside the pool")
+    return total, cu, slots, new_count
+
+
+@_on_tensor_device
+def flash_dmla_kv_append_rows(
+    kv_pool: torch.Tensor,
+    slots: torch.Tensor,
+    rows: torch.Tensor,
+    check_indices: bool = False,
+) -> None:
+    """Writes packed latent rows into the paged cache in place, each to its slot (flash_dmla_kv_reserve).
+
+    kv_pool bf16 [num_pages, 64, d] or 4-bit [num_pages, 64, 400]; rows [T, d] bf16 (d = 576 for 4-bit pages);
+    slots [T] int32: page * 64 + row of the page.  Rows with a negative slot are skipped, and those past the pool too;
+    check_indices=True raises afterwards for the latter (one device sync).
+    """
+    row_bytes, kv_sp, kv_ss = _check_pool(kv_pool)
+    _check_bf16("rows", rows, 2)
+    q4 = kv_pool.dtype is torch.uint8
+    T, d = rows.shape
+    if d != (D_QK if q4 else kv_pool.shape[2]):
+        raise ValueError(f"rows of {d} values do not fit the pool")
+    _check_lens("slots", slots, T)
+    _same_device(kv_pool=kv_pool, slots=slots, rows=rows)
+    flag = torch.zeros(1, dtype=torch.int32, device=rows.device) if check_indices else None
+    r_ss = max(rows.stride(0), d) if T <= 1 else rows.stride(0)
+    if q4:
+        _lib.call("dmla_kv_append_rows_q4", _ptr(kv_pool), _ptr(slots), _ptr(rows), _ptr(flag), T, kv_pool.shape[0], kv_sp,
+                  r_ss, _stream(rows))
+    else:
+        _lib.call("dmla_kv_append_rows", _ptr(kv_pool), _ptr(slots), _ptr(rows), _ptr(flag), T, d, kv_pool.shape[0],
+                  kv_pool.stride(0), kv_pool.stride(1), r_ss, _stream(rows))
+    if check_indices:
+        _require(int(flag.item()) == 0, "kv append: a slot is past the pool (row skipped)")
+
+
+def _check_queries(T: int, block_table: torch.Tensor, cache_seqlens: torch.Tensor,
+                   cu_seqlens_q: Optional[torch.Tensor]) -> int:
+    """The number of sequences, of T queries packed by cu_seqlens_q or, without it, one of each."""
+    _check_index("cache_seqlens", cache_seqlens, 1)
+    B = cache_seqlens.shape[0]
+    _check_tables(block_table, cache_seqlens, B)
+    if cu_seqlens_q is None:
+        if T != B:
+            raise ValueError(f"without cu_seqlens_q there is one query per sequence, got {T} of {B}")
+    else:
+        _check_lens("cu_seqlens_q", cu_seqlens_q, B + 1)
+    return B
+
+
+def _check_packed(cu_seqlens_q: Optional[torch.Tensor], T: int) -> None:
+    """Raises unless the queries' starts ascend from 0 to at most T (one device sync)."""
+    if cu_seqlens_q is None:
+        return
+    cu = cu_seqlens_q.cpu().long()
+    _require(int(cu[0]) == 0 and bool((cu[1:] >= cu[:-1]).all()) and int(cu[-1]) <= T,
+             f"cu_seqlens_q must ascend from 0 to at most {T}")
+
+
+@_on_tensor_device
+def flash_dmla_chunk_paged(
+    q: torch.Tensor,
+    kv_pool: torch.Tensor,
+    block_table: torch.Tensor,
+    cache_seqlens: torch.Tensor,
+    cu_seqlens_q: Optional[torch.Tensor] = None,
+    d_v: int = D_V,
+    softmax_scale: Optional[float] = None,
+    causal: bool = True,
+    return_lse: bool = False,
+    check_indices: bool = False,
+):
+    """Attention of each sequence's newest tokens, one or many, over its pages, which hold them already.
+
+    q [T, H, 576] bf16: the queries of all sequences packed one sequence after another, sequence b's at
+    cu_seqlens_q[b] .. cu_seqlens_q[b + 1] - 1 ([B + 1] int32, ascending from 0; None: one query per sequence); kv_pool
+    [num_pages, 64, 576] bf16; block_table [B, max_pages] int32; cache_seqlens [B] int32, the new tokens among them.
+    Returns o [T, H, d_v] bf16 (and lse [T, H] fp32 natural log with return_lse).  With causal, query i of n attends the
+    tokens j <= cache_seqlens[b] - n + i, else all.  Queries without a token, and those behind the last sequence, give
+    o = 0 and lse = -inf, queries that attend a page outside the pool NaN (check_indices=True raises instead, one
+    device sync).
+    """
+    _check_bf16("q", q, 3)
+    _check_bf16("kv_pool", kv_pool, 3)
+    T, H, Dqk = q.shape
+    num_pages, page, Dk = kv_pool.shape
+    if Dk != Dqk:
+        raise ValueError(f"kv_pool last dim {Dk} != q last dim {Dqk}")
+    if page != PAGE_SIZE:
+        raise ValueError(f"page size must be {PAGE_SIZE}, got {page}")
+    B = _check_queries(T, block_table, cache_seqlens, cu_seqlens_q)
+    _same_device(q=q, kv_pool=kv_pool, block_table=block_table, cache_seqlens=cache_seqlens, cu_seqlens_q=cu_seqlens_q)
+    if check_indices:
+        _check_packed(cu_seqlens_q, T)
+        _check_page_indices(block_table, cache_seqlens, num_pages)
+    o = torch.empty((T, H, d_v), dtype=torch.bfloat16, device=q.device)
+    lse = torch.empty((T, H), dtype=torch.float32, device=q.device) if return_lse else None
+    max_pages = block_table.shape[1]
+    ws_bytes = int(_lib.lib().dmla_chunk_paged_workspace_bytes(T, B, H, max_pages))
+    ws = torch.empty((max(ws_bytes, 1),), dtype=torch.uint8, device=q.device)
+    _lib.call(
+        "dmla_chunk_paged",
+        _ptr(q), _ptr(kv_pool), _ptr(block_table), _ptr(cache_seqlens), _ptr(cu_seqlens_q), _ptr(o), _ptr(lse),
+        T, B, H, Dqk, d_v, num_pages, max_pages,
+        q.stride(0), q.stride(1), kv_pool.stride(0), kv_pool.stride(1), _row_stride(block_table), o.stride(0), o.stride(1),
+        _scale(softmax_scale, Dqk), 1 if causal else 0, _ptr(ws), ws_bytes, _stream(q),
+    )
+    return (o, lse) if return_lse else o
+
+
+def _check_means(means: torch.Tensor, num_pages: Optional[int]) -> None:
+    _check_bf16("means", means, 2)
+    if means.shape[1] != D_QK or (num_pages is not None and means.shape[0] != num_pages):
+        raise ValueError(f"means must be [num_pages, {D_QK}], got {tuple(means.shape)}")
+
+
+@_on_tensor_device
+def flash_dmla_page_means(
+    kv_pool: torch.Tensor,
+    block_table: torch.Tensor,
+    cache_seqlens: torch.Tensor,
+    means: torch.Tensor,
+    starts: Optional[torch.Tensor] = None,
+) -> None:
+    """Writes the mean row of full pages into means [num_pages, 576] bf16, in place.
+
+    kv_pool bf16 [num_pages, 64, 576] or 4-bit [num_pages, 64, 400]; block_table, cache_seqlens as for a decode.  The
+    pages are starts[b] // 64 .. cache_seqlens[b] // 64 - 1 of each sequence (starts [B] int32, the lengths at the
+    last call; None: 0): those that have become full since.  The last page, where it is not full, has no mean.
+    """
+    row_bytes, kv_sp, kv_ss = _check_pool(kv_pool)
+    q4 = kv_pool.dtype is torch.uint8
+    if not q4 and kv_pool.shape[2] != D_QK:
+        raise ValueError(f"kv_pool rows must hold {D_QK} values, got {kv_pool.shape[2]}")
+    _check_index("cache_seqlens", cache_seqlens, 1)
+    B = cache_seqlens.shape[0]
+    _check_tables(block_table, cache_seqlens, B)
+    if starts is not None:
+        _check_lens("starts", starts, B)
+    _check_means(means, kv_pool.shape[0])
+    _same_device(kv_pool=kv_pool, block_table=block_table, cache_seqlens=cache_seqlens, means=means, starts=starts)
+    _lib.call(
+        "dmla_page_means",
+        _ptr(kv_pool), _ptr(block_table), _ptr(cache_seqlens), _ptr(starts), _ptr(means),
+        B, kv_pool.shape[0], block_table.shape[1], kv_sp, kv_ss, _row_stride(block_table), _row_stride(means),
+        1 if q4 else 0, _stream(kv_pool),
+    )
+
+
+@_on_tensor_device
+def flash_dmla_page_scores(
+    q: torch.Tensor,
+    means: torch.Tensor,
+    block_table: torch.Tensor,
+    cache_seqlens: torch.Tensor,
+    cu_seqlens_q: Optional[torch.Tensor] = None,
+    softmax_scale: Optional[float] = None,
+) -> torch.Tensor:
+    """How much each page matters to each query: scores [T, max_pages] fp32.
+
+    scores[t, p] is the weight that the attention of query t over the mean rows (flash_dmla_page_means) of the pages
+    before its own gives page p, summed over the heads; 0 from its own page on.  q [T, H, 576] bf16, cu_seqlens_q,
+    block_table, cache_seqlens and softmax_scale as for flash_dmla_chunk_paged.  Deterministic.
+    """
+    _check_bf16("q", q, 3)
+    T, H, Dqk = q.shape
+    _check_means(means, None)
+    if Dqk != D_QK:
+        raise ValueError(f"q rows must hold {D_QK} values, got {Dqk}")
+    B = _check_queries(T, block_table, cache_seqlens, cu_seqlens_q)
+    _same_device(q=q, means=means, block_table=block_table, cache_seqlens=cache_seqlens, cu_seqlens_q=cu_seqlens_q)
+    max_pages = block_table.shape[1]
+    scores = torch.empty((T, max_pages), dtype=torch.float32, device=q.device)
+    ws_bytes = int(_lib.lib().dmla_page_scores_workspace_bytes(T, H, max_pages, 0 if cu_seqlens_q is None else 1))
+    ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=q.device) if ws_bytes else None
+    _lib.call(
+        "dmla_page_scores",
+        _ptr(q), _ptr(means), _ptr(block_table), _ptr(cache_seqlens), _ptr(cu_seqlens_q), _ptr(scores),
+        T, B, H, Dqk, means.shape[0], max_pages, q.stride(0), q.stride(1), _row_stride(means), _row_stride(block_table),
+        max_pages, _scale(softmax_scale, Dqk), _ptr(ws), ws_bytes, _stream(q),
+    )
+    return scores
+
+
+@_on_tensor_device
+def flash_dmla_page_select(
+    scores: torch.Tensor,
+    block_table: torch.Tensor,
+    cache_seqlens: torch.Tensor,
+    cu_seqlens_q: Optional[torch.Tensor],
+    top_pages: int,
+    recent: int = 1,
+    sink: int = 0,
+) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Selects the pages that each query attends, a block table of its own for each.
+
+    scores [T, max_pages] fp32 (flash_dmla_page_scores); cu_seqlens_q, block_table and cache_seqlens as there.  The
+    first `sink` pages and the newest `recent` (the query's own among them) stay, and of the others those with the
+    largest scores (the lower page first among equals), top_pages in all.  Returns
+      sel_table [T, top_pages] int32 -- their entries of block_table in order, -1 behind the last;
+      sel_lens [T] int32 -- their tokens up to the query's own;
+      sel_index [T, top_pages] int32 -- their places in the sequence, -1 behind the last.
+    flash_dmla_chunk_paged (without cu_seqlens_q) and the decodes take sel_table and sel_lens as block_table and
+    cache_seqlens of T sequences.
+    """
+    if not (isinstance(scores, torch.Tensor) and scores.is_cuda and scores.dtype is torch.float32 and scores.dim() == 2
+            and (scores.stride(1) == 1 or scores.shape[1] <= 1)):
+        raise ValueError("scores must be a 2-D float32 GPU tensor, contiguous in its last dim")
+    T = scores.shape[0]
+    B = _check_queries(T, block_table, cache_seqlens, cu_seqlens_q)
+    max_pages = block_table.shape[1]
+    _require(scores.shape[1] >= max_pages, "scores must hold an entry per page of block_table")
+    _require(recent >= 1 and sink >= 0 and recent + sink <= top_pages,
+             "recent must be at least 1, sink at least 0, and top_pages cover both")
+    _same_device(scores=scores, block_table=block_table, cache_seqlens=cache_seqlens, cu_seqlens_q=cu_seqlens_q)
+    table = torch.empty((T, top_pages), dtype=torch.int32, device=scores.device)
+    lens = torch.empty((T,), dtype=torch.int32, device=scores.device)
+    index = torch.empty((T, top_pages), dtype=torch.int32, device=scores.device)
+    _lib.call(
+        "dmla_page_select",
+        _ptr(scores), _ptr(block_table), _ptr(cache_seqlens), _ptr(cu_seqlens_q), _ptr(table), _ptr(lens), _ptr(index),
+        T, B, max_pages, _row_stride(scores), _row_stride(block_table), top_pages, top_pages, top_pages, recent, sink,
+        _stream(scores),
+    )
+    return table, lens, index
+
+
+def flash_dmla_sparse_paged(
+    q: torch.Tensor,
+    kv_pool: torch.Tensor,
+    means: torch.Tensor,
+    block_table: torch.Tensor,
+    cache_seqlens: torch.Tensor,
+    cu_seqlens_q: Optional[torch.Tensor],
+    top_pages: int,
+    recent: int = 1,
+    sink: int = 0,
+    softmax_scale: Optional[float] = None,
+    return_lse: bool = False,
+):
+    """Attention of each query over the top_pages pages of its sequence that matter to it (causal).
+
+    flash_dmla_page_scores, flash_dmla_page_select and the attention over the selection: flash_dmla_chunk_paged for bf16
+    pages, flash_dmla_decode_paged_q4 for 4-bit ones.  Returns o [T, H, 512] bf16 (and lse [T, H] with return_lse);
+    where a query sees no more than top_pages pages, this is its attention over all of them.
+    """
+    scores = flash_dmla_page_scores(q, means, block_table, cache_seqlens, cu_seqlens_q, softmax_scale)
+    table, lens, _ = flash_dmla_page_select(scores, block_table, cache_seqlens, cu_seqlens_q, top_pages, recent, sink)
+    if kv_pool.dtype is torch.uint8:
+        return flash_dmla_decode_paged_q4(q, kv_pool, table, lens, D_V, softmax_scale, return_lse)
+    return flash_dmla_chunk_paged(q, kv_pool, table, lens, None, D_V, softmax_scale, True, return_lse)
 
 
 class FlashDMLACacheLatent(torch.autograd.Function):

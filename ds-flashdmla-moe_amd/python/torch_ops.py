@@ -23,6 +23,17 @@ matching backward op.  Only GPU tensors have a kernel: CPU tensors raise, as eve
     torch.ops.flashdmla.attn_mass(q, kv_pool, block_table, cache_seqlens, lse, mass, softmax_scale) -> ()   (mass in place)
     torch.ops.flashdmla.kv_evict(kv_pool, block_table, cache_seqlens, mass, budget, recent, sink)
         -> (new_lens, src, new_mass)   (kv_pool in place)
+    torch.ops.flashdmla.kv_release(block_table, old_lens, new_lens, free_pages, free_count, num_pages)
+        -> new_count   (free_pages in place)
+    torch.ops.flashdmla.kv_reserve(block_table, cache_seqlens, new_lens, free_pages, free_count, num_rows, num_pages)
+        -> (total_lens, cu_seqlens, slots, new_count)   (block_table in place)
+    torch.ops.flashdmla.kv_append_rows(kv_pool, slots, rows) -> ()   (kv_pool in place)
+    torch.ops.flashdmla.chunk_paged(q, kv_pool, block_table, cache_seqlens, cu_seqlens_q, d_v, softmax_scale, causal)
+        -> (o, lse)
+    torch.ops.flashdmla.page_means(kv_pool, block_table, cache_seqlens, means, starts) -> ()   (means in place)
+    torch.ops.flashdmla.page_scores(q, means, block_table, cache_seqlens, cu_seqlens_q, softmax_scale) -> scores
+    torch.ops.flashdmla.page_select(scores, block_table, cache_seqlens, cu_seqlens_q, top_pages, recent, sink)
+        -> (sel_table, sel_lens, sel_index)
 
 Shapes and conventions are those of python/ops.py.  m and l are outputs without a gradient;
 the backwards return dk_lat and dwk / dwv in float32 (the autograd formulas cast them to the
@@ -241,3 +252,87 @@ def _(kv_pool, block_table, cache_seqlens, mass, budget, recent, sink):
     B, width = mass.shape[0], min(budget, block_table.shape[1] * ops.PAGE_SIZE)
     return (cache_seqlens.new_empty((B,), dtype=torch.int32), cache_seqlens.new_empty((B, width), dtype=torch.int32),
             mass.new_empty((B, mass.shape[1])))
+
+
+# ---- pages by request lengths, chunk attention, page scores and selection ----------------------
+@custom_op("flashdmla::kv_release", mutates_args=("free_pages",), device_types="cuda")
+def kv_release(block_table: Tensor, old_lens: Tensor, new_lens: Tensor, free_pages: Tensor, free_count: Tensor,
+               num_pages: int) -> Tensor:
+    return ops.flash_dmla_kv_release(block_table, old_lens, new_lens, free_pages, free_count, num_pages)
+
+
+@kv_release.register_fake
+def _(block_table, old_lens, new_lens, free_pages, free_count, num_pages):
+    return free_count.new_empty((1,))
+
+
+@custom_op("flashdmla::kv_reserve", mutates_args=("block_table",), device_types="cuda")
+def kv_reserve(block_table: Tensor, cache_seqlens: Tensor, new_lens: Tensor, free_pages: Tensor, free_count: Tensor,
+               num_rows: int, num_pages: int) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
+    return ops.flash_dmla_kv_reserve(block_table, cache_seqlens, new_lens, free_pages, free_count, num_rows, num_pages)
+
+
+@kv_reserve.register_fake
+def _(block_table, cache_seqlens, new_lens, free_pages, free_count, num_rows, num_pages):
+    B = block_table.shape[0]
+    return (cache_seqlens.new_empty((B,)), cache_seqlens.new_empty((B + 1,)), cache_seqlens.new_empty((num_rows,)),
+            free_count.new_empty((1,)))
+
+
+@custom_op("flashdmla::kv_append_rows", mutates_args=("kv_pool",), device_types="cuda")
+def kv_append_rows(kv_pool: Tensor, slots: Tensor, rows: Tensor) -> None:
+    ops.flash_dmla_kv_append_rows(kv_pool, slots, rows)
+
+
+@kv_append_rows.register_fake
+def _(kv_pool, slots, rows):
+    return None
+
+
+@custom_op("flashdmla::chunk_paged", mutates_args=(), device_types="cuda")
+def chunk_paged(q: Tensor, kv_pool: Tensor, block_table: Tensor, cache_seqlens: Tensor, cu_seqlens_q: Optional[Tensor],
+                d_v: int, softmax_scale: Optional[float], causal: bool) -> Tuple[Tensor, Tensor]:
+    o, lse = ops.flash_dmla_chunk_paged(q, kv_pool, block_table, cache_seqlens, cu_seqlens_q, d_v, softmax_scale, causal,
+                                        return_lse=True)
+    return o, lse
+
+
+@chunk_paged.register_fake
+def _(q, kv_pool, block_table, cache_seqlens, cu_seqlens_q, d_v, softmax_scale, causal):
+    T, H, _ = q.shape
+    return q.new_empty((T, H, d_v), dtype=_BF16), q.new_empty((T, H), dtype=_F32)
+
+
+@custom_op("flashdmla::page_means", mutates_args=("means",), device_types="cuda")
+def page_means(kv_pool: Tensor, block_table: Tensor, cache_seqlens: Tensor, means: Tensor,
+               starts: Optional[Tensor]) -> None:
+    ops.flash_dmla_page_means(kv_pool, block_table, cache_seqlens, means, starts)
+
+
+@page_means.register_fake
+def _(kv_pool, block_table, cache_seqlens, means, starts):
+    return None
+
+
+@custom_op("flashdmla::page_scores", mutates_args=(), device_types="cuda")
+def page_scores(q: Tensor, means: Tensor, block_table: Tensor, cache_seqlens: Tensor, cu_seqlens_q: Optional[Tensor],
+                softmax_scale: Optional[float]) -> Tensor:
+    return ops.flash_dmla_page_scores(q, means, block_table, cache_seqlens, cu_seqlens_q, softmax_scale)
+
+
+@page_scores.register_fake
+def _(q, means, block_table, cache_seqlens, cu_seqlens_q, softmax_scale):
+    return q.new_empty((q.shape[0], block_table.shape[1]), dtype=_F32)
+
+
+@custom_op("flashdmla::page_select", mutates_args=(), device_types="cuda")
+def page_select(scores: Tensor, block_table: Tensor, cache_seqlens: Tensor, cu_seqlens_q: Optional[Tensor], top_pages: int,
+                recent: int, sink: int) -> Tuple[Tensor, Tensor, Tensor]:
+    return ops.flash_dmla_page_select(scores, block_table, cache_seqlens, cu_seqlens_q, top_pages, recent, sink)
+
+
+@page_select.register_fake
+def _(scores, block_table, cache_seqlens, cu_seqlens_q, top_pages, recent, sink):
+    T = scores.shape[0]
+    new = lambda *shape: scores.new_empty(shape, dtype=torch.int32)
+    return new(T, top_pages), new(T), new(T, top_pages)

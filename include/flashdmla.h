@@ -345,6 +345,107 @@ int dmla_kv_evict(void* kv_pool, const int32_t* block_table, const int32_t* cach
                   dmla_stream_t stream);
 
 /*
+ * Pages by request lengths, on the device.  No reference counterpart.
+ *
+ * free_pages[0 .. free_count[0]) are the pages that nobody has, a stack whose top is taken first; block_table,
+ * pages of 64 tokens and lengths are those of dmla_decode_paged.  new_count may not be free_count: the calls read the
+ * one and write the other.
+ *
+ * dmla_kv_release: the pages that a sequence of old_lens[b] tokens has and one of new_lens[b] does not need
+ *   (entries ceil(new_lens[b] / 64) .. ceil(old_lens[b] / 64) - 1 of its row; new_lens[b] = 0: it has ended) go on
+ *   the stack in order.  block_table keeps the entries.  An entry outside [0, num_pages), and pages past `capacity`
+ *   (entries of free_pages), are left out and set *bad_index_flag to 1.
+ * dmla_kv_reserve: sequence b of cache_seqlens[b] tokens gets the pages that new_lens[b] more need, in order, into its
+ *   row of block_table.  Its new rows are rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 of a packed array of num_rows.
+ *   cu_seqlens [B + 1]  row starts: running sums of new_lens (at most num_rows)
+ *   total_lens [B]      cache_seqlens[b] + new_lens[b]
+ *   slots [num_rows]    place of each row in the pool, page * 64 + row of the page; -1 from cu_seqlens[B] on
+ *   A sequence whose pages are not there (as long as the ones before it got theirs), whose tokens do not fit its row
+ *   of block_table or whose rows pass num_rows gets none: total_lens[b] = cache_seqlens[b], slots -1, and
+ *   *bad_index_flag is set to 1.  So it is, with slot -1, where a page is outside [0, num_pages).
+ * dmla_kv_append_rows, dmla_kv_append_rows_q4: row t of rows [T, d] (strides r_ss; d = 576 for 4-bit pages) goes to slot
+ *   slots[t] of the pool (rows and pages of dmla_kv_append and dmla_kv_append_q4); a negative slot: nowhere, one past
+ *   the pool as well, with *bad_index_flag set to 1.  Of rows with one slot, any byte may be any of theirs.
+ *
+ * bad_index_flag is a device word that the caller clears, or NULL.  num_pages <= 2^25.
+ */
+int dmla_kv_release(const int32_t* block_table, const int32_t* old_lens, const int32_t* new_lens,
+                    int32_t* free_pages, const int32_t* free_count, int32_t* new_count, int32_t* bad_index_flag,
+                    int64_t B, int64_t num_pages, int64_t max_pages_per_seq, int64_t capacity, int64_t bt_sb,
+                    dmla_stream_t stream);
+int dmla_kv_reserve(int32_t* block_table, const int32_t* cache_seqlens, const int32_t* new_lens,
+                    const int32_t* free_pages, const int32_t* free_count, int32_t* total_lens,
+                    int32_t* cu_seqlens, int32_t* slots, int32_t* new_count, int32_t* bad_index_flag, int64_t B,
+                    int64_t num_rows, int64_t num_pages, int64_t max_pages_per_seq, int64_t capacity, int64_t bt_sb,
+                    dmla_stream_t stream);
+int dmla_kv_append_rows(void* kv_pool, const int32_t* slots, const void* rows, int32_t* bad_index_flag, int64_t T,
+                        int64_t d, int64_t num_pages, int64_t kv_sp, int64_t kv_ss, int64_t r_ss,
+                        dmla_stream_t stream);
+int dmla_kv_append_rows_q4(void* kv_pool, const int32_t* slots, const void* rows, int32_t* bad_index_flag,
+                           int64_t T, int64_t num_pages, int64_t kv_sp, int64_t r_ss, dmla_stream_t stream);
+
+/*
+ * Attention of new tokens over a paged bf16 cache that holds them already.  No reference counterpart.
+ *
+ *   q             [T, H, d_qk] bf16  strides (q_st, q_sh): the queries of all sequences, one sequence after another
+ *   cu_seqlens_q  [B + 1] int32: sequence b has the queries cu_seqlens_q[b] .. cu_seqlens_q[b + 1] - 1, its newest
+ *                 tokens; ascending from 0.  NULL: one query per sequence (T = B)
+ *   kv_pool, block_table, cache_seqlens   as for dmla_decode_paged; the lengths count the new tokens
+ *   o             [T, H, d_v] bf16   strides (o_st, o_sh)
+ *   lse           [T, H] fp32        contiguous, natural log; may be NULL
+ *
+ * Of a sequence of N tokens (at most 64 max_pages_per_seq) and n queries, query i attends, with causal, the tokens
+ * j <= N - n + i, else all N.  A query without a token, and one from cu_seqlens_q[B] on, gets o = 0, lse = -inf; one that
+ * attends a page outside [0, num_pages) NaN.  What a query does not attend does not reach it, whatever it holds.
+ * Probabilities enter the value product as bf16, sums stay in fp32.
+ * The workspace (16-byte aligned, contents ignored) is of dmla_chunk_paged_workspace_bytes of the same sizes on the
+ * current device.  Supported: d_qk = 576, d_v = 512, T * H <= 2^30.
+ */
+int64_t dmla_chunk_paged_workspace_bytes(int64_t T, int64_t B, int64_t H, int64_t max_pages_per_seq);
+int dmla_chunk_paged(const void* q, const void* kv_pool, const int32_t* block_table, const int32_t* cache_seqlens,
+                     const int32_t* cu_seqlens_q, void* o, float* lse, int64_t T, int64_t B, int64_t H,
+                     int64_t d_qk, int64_t d_v, int64_t num_pages, int64_t max_pages_per_seq, int64_t q_st,
+                     int64_t q_sh, int64_t kv_sp, int64_t kv_ss, int64_t bt_sb, int64_t o_st, int64_t o_sh,
+                     float softmax_scale, int causal, void* workspace, int64_t workspace_bytes,
+                     dmla_stream_t stream);
+
+/*
+ * Attention over some pages of a long context, chosen for each query by a score.  No reference counterpart.
+ *
+ * dmla_page_means: the mean of the 64 rows of every full page of sequence b from token starts[b] on (NULL: 0) goes to
+ *   its row of means [num_pages, 576] bf16 (row stride m_sp): pages starts[b] / 64 .. cache_seqlens[b] / 64 - 1 of the
+ *   sequence.  kv_pool holds bf16 rows of 576 or (q4 != 0) 4-bit rows; strides in BYTES, multiples of 16.  Pages outside
+ *   [0, num_pages) are left out.  Sums in fp32, one rounding.
+ * dmla_page_scores: scores [T, max_pages_per_seq] fp32 (row stride s_st):
+ *     scores[t, p] = sum_h exp(s_hp) / sum_p' exp(s_hp'),  s_hp = softmax_scale q[t, h] . means[block_table[b, p]]
+ *   over the pages p, p' of t's sequence b that lie before the page of token t itself, 0 for the other entries.  Pages
+ *   outside [0, num_pages) count as not there.  Queries and cu_seqlens_q as for dmla_chunk_paged (causal).
+ *   The workspace is of dmla_page_scores_workspace_bytes(T, H, max_pages_per_seq, cu_seqlens_q != NULL) bytes on
+ *   the current device (0: none), 16-byte aligned, contents ignored.
+ * dmla_page_select: for each query the first `sink` pages of its sequence, the newest `recent` (from the page of its own
+ *   token back) and of those between the ones with the largest scores, top_pages in all, or every page where they are
+ *   no more.  The lower page goes first among equals, -0 is equal to 0, NaN above everything.
+ *   sel_index [T, top_pages]  the selected pages' places in block_table's row, ascending, -1 behind the last
+ *   sel_table [T, top_pages]  their entries of block_table, -1 behind the last
+ *   sel_lens  [T]             tokens of them up to the query's own
+ *   dmla_chunk_paged (without cu_seqlens_q) and dmla_decode_paged[_q4] take sel_table and sel_lens as block_table
+ *   and cache_seqlens of T sequences: the last selected page is the query's own, so its tokens are the first sel_lens.
+ */
+int dmla_page_means(const void* kv_pool, const int32_t* block_table, const int32_t* cache_seqlens,
+                    const int32_t* starts, void* means, int64_t B, int64_t num_pages, int64_t max_pages_per_seq,
+                    int64_t kv_sp, int64_t kv_ss, int64_t bt_sb, int64_t m_sp, int q4, dmla_stream_t stream);
+int64_t dmla_page_scores_workspace_bytes(int64_t T, int64_t H, int64_t max_pages_per_seq, int packed);
+int dmla_page_scores(const void* q, const void* means, const int32_t* block_table, const int32_t* cache_seqlens,
+                     const int32_t* cu_seqlens_q, float* scores, int64_t T, int64_t B, int64_t H, int64_t d_qk,
+                     int64_t num_pages, int64_t max_pages_per_seq, int64_t q_st, int64_t q_sh, int64_t m_sp,
+                     int64_t bt_sb, int64_t s_st, float softmax_scale, void* workspace, int64_t workspace_bytes,
+                     dmla_stream_t stream);
+int dmla_page_select(const float* scores, const int32_t* block_table, const int32_t* cache_seqlens,
+                     const int32_t* cu_seqlens_q, int32_t* sel_table, int32_t* sel_lens, int32_t* sel_index,
+                     int64_t T, int64_t B, int64_t max_pages_per_seq, int64_t s_st, int64_t bt_sb, int64_t st_st,
+                     int64_t si_st, int64_t top_pages, int64_t recent, int64_t sink, dmla_stream_t stream);
+
+/*
  * Cache-latent DMLA backward from the forward's saved statistics.
  * Replaces: fa2_backward (csrc/attention/fa2_bwd.cu:319-356, math of :198-310) specialised
  * to the cache-latent mode of README.md:12,15 -- the role of the absent
