@@ -12,7 +12,7 @@
 //    row r at u ^ key_swz(r), copied there directly, a row per copy.  The score product reads a unit of 32 rows
 //    (ds_read_b128), the value product 32 columns of 8 rows transposed (ds_read_b64_tr_b16).  The rope dims have
 //    rows of 128 bytes of their own, eight of them a copy.
-//  * The softmax reference of a row is its largest score in the first tile; P may grow to 2^32 past it.
+//  * Step s multiplies scores of tile s and values of tile s - 1; copies run two tiles ahead, four tiles fit.
 #include <algorithm>
 
 #include "dmla_host.h"
@@ -29,7 +29,8 @@ constexpr int kColBlocks = 4;                              // 32 columns each, o
 constexpr int kSteps = kDqk / 16, kLatSteps = kDv / 16;    // MFMAs of a tile's scores
 constexpr int kKeyRow = 1024, kKeyBytes = kTile * kKeyRow, kSlots = 4;
 constexpr int kRopeBytes = kTile * 128;
-constexpr int kProbBytes = kWaves * 2048;
+constexpr int kProbBytes = kWaves * 2048;                   // P of a step
+constexpr int kCopies = 9;                                 // of a wave and tile
 constexpr int kQueryBytes = 32 * 2 * kDqk;                 // of a wave, in the keys' and the ropes' memory
 static_assert(kWaves * kQueryBytes == kSlots * (kKeyBytes + kRopeBytes), "the queries fill it");
 constexpr float kHeadroom = 32.0f;                         // log2 headroom of P over a row's reference
@@ -44,13 +45,16 @@ struct ChunkParams {
   const int32_t* cu;     // nullable: one query per sequence
   bf16* o;
   float* lse;            // nullable
+  float* part_o;         // [2 ranges, 128 rows, 512] normalised partial outputs
+  float* part_lse;       // [2 ranges, 128 rows], log2 units
+  int4* links;           // [ranges] (RangeLink)
   int64_t q_st, q_sh, kv_sp, kv_ss, bt_sb, o_st, o_sh;   // kv strides in bytes
-  int T, B, H, num_pages, max_pages, causal;
+  int T, B, H, num_pages, max_pages, causal, n_ranges;
   FastDiv hdiv;          // division by H
   float scale_log2;
 };
 
-// A sequence's queries: q0 .. q0 + n - 1, the first of them at token `base` of its len tokens.
+// A sequence's queries: q0 .. q0 + n - 1, the newest of its len tokens.
 struct Sequence {
   int q0, n, len;
 };
@@ -67,14 +71,27 @@ __device__ __forceinline__ Sequence sequence(const ChunkParams& p, int b) {
   return s;
 }
 
-// 128 rows of a sequence from row0 on, and the key tiles [t0, t1) of them.
+// 128 rows of a sequence from row0 on, the key tiles [t0, t1) of them, and where their output goes: slot < 0 to o, else
+// a part.
 struct Piece {
-  int b, q0, n, len, row0, t0, t1;
+  Sequence s;
+  int b, row0, t0, t1, slot;
+};
+
+// A piece runs once, against each row's largest score in the first tile.  Where scores have climbed more than kHeadroom
+// above it, or an output is not a number or infinite, it runs the careful way: a row's reference is the largest score
+// that was seen, and a row sees nothing of later tokens, as a probability of 0 times a latent that is not a number is
+// none either.  So the rows are cut where a later row's token holds such a latent, and the rows before it run
+// without it.  Both are rare, and the loop holds neither rescaling nor tests.
+struct Pass {
+  bool careful;
+  int from, to;   // rows with a limit in [from, to) are written
 };
 
 struct Lds {
   unsigned keys, rope, prob;   // addresses
   DMLA_LDS float* stat;        // [kRows]: sums
+  DMLA_LDS float* top;         // [kRows]: largest scores, log2 units
   DMLA_LDS int* flag;          // [kWaves]
 };
 
@@ -93,42 +110,60 @@ struct Pages {
   __device__ __forceinline__ const char* tile(const ChunkParams& p, const Piece& pc, int t) {
     if (t / 2 - first >= 64) fetch(p, pc, first + 64);
     int page = __builtin_amdgcn_readlane(pages, uniform((t / 2 - first) & 63));
-    if (page < 0 || page >= p.num_pages) {
-      bad = min(bad, t / 2);
-      page = 0;
-    }
+    const bool off = page < 0 || page >= p.num_pages;
+    bad = off ? min(bad, t / 2) : bad;
+    page = off ? 0 : page;
     return p.kv + page * p.kv_sp + (t & 1) * kTile * p.kv_ss;
   }
 };
 
-__device__ __forceinline__ void run_piece(const ChunkParams& p, const Piece& pc, const Lds& lds) {
+// Whether another pass has to follow.
+__device__ __forceinline__ bool run_piece(const ChunkParams& p, const Piece& pc, const Lds& lds, const Pass& pass) {
   const int lane = fresh_lane_id();
   const int l32 = lane & 31, hl = lane >> 5;
   const int wave = uniform(threadIdx.x >> 6);
-  const int rows = min(pc.n * p.H - pc.row0, kRows);
+  const int rows = min(pc.s.n * p.H - pc.row0, kRows);
   // Rows past the last one are the last one again, and not written.
-  auto token_of = [&](int r) { return fast_div(pc.row0 + min(r, rows - 1), p.hdiv); };
-  auto limit_of = [&](int r) { return p.causal ? pc.len - pc.n + token_of(r) : pc.len - 1; };   // last key
+  auto limit_of = [&](int r) {   // last key of row r
+    return p.causal ? pc.s.len - pc.s.n + fast_div(pc.row0 + min(r, rows - 1), p.hdiv) : pc.s.len - 1;
+  };
   const int lim = limit_of(32 * wave + l32);
   const int lim0 = uniform(limit_of(32 * wave));   // the wave's smallest
 
-  // ---- copies: lane l copies 16 bytes into place l of each kilobyte ----
+  // ---- copies: lane l copies 16 bytes into place l of each kilobyte, nine of a wave and tile ----
   Pages pages;
-  auto copy_tile = [&](int s) {
-    const int t = pc.t0 + s;
-    const char* src = pages.tile(p, pc, t);
-    // Rows past the sequence's end are its last row again.
-    const int last = uniform(min(pc.len - t * kTile, kTile) - 1);
-    const unsigned dst = lds.keys + (s % kSlots) * kKeyBytes + wave * 8 * kKeyRow;
+  // Rows of a tile from key_end on are its last row before, again.
+  const int key_end = uniform(min(limit_of(rows - 1) + 1, pass.to));
+  const int t1 = max(pc.t0, min(pc.t1, (max(key_end, 0) + kTile - 1) / kTile));
+  const char* copy_src = nullptr;
+  int copy_last = 0;
+  unsigned copy_dst = 0;
+  auto copy_begin = [&](int s) {
+    const int t = min(pc.t0 + s, t1 - 1);   // past the end: the last tile, which nobody counts
+    copy_src = pages.tile(p, pc, t);
+    copy_last = uniform(min(key_end - t * kTile, kTile) - 1);
+    copy_dst = (unsigned)(s % kSlots);
+  };
+  auto copy = [&](int i) {
     const int ln = fresh_lane_id();
+    if (i < 8) {
+      const int r = 8 * wave + i;
+      const unsigned off = (16 * (ln ^ key_swz(8 * wave))) ^ (16 * key_swz(i));   // key_swz(8 w + i) is the two's xor
+      dma16(copy_src + min(r, copy_last) * p.kv_ss, off, lds.keys + copy_dst * kKeyBytes + r * kKeyRow);
+    } else {
+      const unsigned off = min(8 * wave + (ln >> 3), copy_last) * (unsigned)p.kv_ss + 2 * kDv + 16 * ((ln & 7) ^ (ln >> 3));
+      dma16(copy_src, off, lds.rope + copy_dst * kRopeBytes + wave * 1024);
+    }
+  };
+  auto copy_tile = [&](int s) {
+    copy_begin(s);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      dma16(src + min(8 * wave + i, last) * p.kv_ss, 16 * (ln ^ key_swz(8 * wave + i)), dst + i * kKeyRow);
-    const unsigned off = min(8 * wave + (ln >> 3), last) * (unsigned)p.kv_ss + 2 * kDv + 16 * ((ln & 7) ^ (ln >> 3));
-    dma16(src, off, lds.rope + (s % kSlots) * kRopeBytes + wave * 1024);
+    for (int i = 0; i < kCopies; ++i) copy(i);
   };
 
   // ---- queries: 36 operands of 16 dims; operand c holds dims 16 c + 8 hl .. of row l32 ----
+  // Through the keys' memory, eight rows x 128 bytes a copy: read straight into the operands, a load would touch 32 rows
+  // for 32 bytes each.
   bf16x8 q[kSteps];
   {
     const unsigned mine = lds.keys + wave * kQueryBytes;   // the ropes' memory follows the keys'
@@ -137,10 +172,11 @@ __device__ __forceinline__ void run_piece(const ChunkParams& p, const Piece& pc,
     for (int g = 0; g < 4; ++g) {
       const int r = pc.row0 + min(32 * wave + 8 * g + (ln >> 3), rows - 1);
       const int token = fast_div(r, p.hdiv), head = r - token * p.H;
-      const bf16* src = p.q + (pc.q0 + token) * p.q_st + head * p.q_sh + 8 * ((ln & 7) ^ (ln >> 3));
+      const bf16* src = p.q + (pc.s.q0 + token) * p.q_st + head * p.q_sh + 8 * ((ln & 7) ^ (ln >> 3));
 #pragma unroll
       for (int i = 0; i < 9; ++i) dma16_addr(src + 64 * i, mine + (9 * g + i) * 1024);
     }
+    pages.fetch(p, pc, pc.t0 / 2);
     wait_vm<0>();
     const unsigned a = lds_sum(9 * 1024 * (l32 >> 3) + 128 * (l32 & 7) + 16 * (hl ^ (l32 & 7)), mine);
 #pragma unroll
@@ -151,191 +187,607 @@ __device__ __forceinline__ void run_piece(const ChunkParams& p, const Piece& pc,
 
   f32x16 acc[kRowBlocks][kColBlocks];   // O^T: register i is column 128 wave + 32 j + 16 hl + i of row l32
   float mref = kNegInf, mtrue = kNegInf, lsum = 0.f;   // reference, largest score seen, sum
+  bf16x8 pv[2];             // P of the wave's own rows, 16 keys each
 
-  for (bool again = false;; again = true) {
+  // A barrier that waits for nothing else: what it orders has been waited for.
+  auto barrier = [] {
+    in_order();
+    asm volatile("s_barrier" ::: "memory");
+    in_order();
+  };
+  auto opaque = [](unsigned a) {
+    asm("" : "+s"(a));
+    return a;
+  };
+
+  // ---- scores: S^T[key 8 (i / 4) + 4 hl + i % 4][row l32] of step s's tile ----
+  bf16x8 rope[4];
+  constexpr int kDepth = 6;   // operands in flight
+  unsigned key_addr = 0;
+  bf16x8 k[kDepth];
+  auto read_rope = [&](int s) {
+    const unsigned a = lds_sum(128 * l32 + 16 * (hl ^ (l32 & 7)), opaque(lds.rope + (unsigned)(s % kSlots) * kRopeBytes));
+#pragma unroll
+    for (int c = 0; c < 4; ++c) rope[c] = *lds_ptr<const bf16x8>(a ^ (32 * c));
+  };
+  auto read_key = [&](int c) { k[c % kDepth] = *lds_ptr<const bf16x8>((key_addr ^ (32 * (c & 7))) + 256 * (c >> 3)); };
+  auto scores_begin = [&](int s) {
+    key_addr = lds_sum(kKeyRow * l32 + 16 * (hl ^ key_swz(l32)), opaque(lds.keys + (unsigned)(s % kSlots) * kKeyBytes));
+  };
+  // After read_rope(s), scores_begin(s) and the first kDepth reads; beside(m) runs after MFMA m = 0 .. 35.
+  // The result may be read after score_done or two more MFMAs.
+  auto scores = [&](auto beside) -> f32x16 {
+    f32x16 x;
+    static_for<kSteps>([&](auto m_tag) {
+      constexpr int m = decltype(m_tag)::value, c = m - 4;
+      if constexpr (m < 4) score_step<m == 0>(x, rope[m], q[kLatSteps + m]);
+      else score_step<false>(x, k[c % kDepth], q[c]);
+      if constexpr (m >= 4 && c + kDepth < kLatSteps) read_key(c + kDepth);
+      beside(m_tag);
+      in_order();
+    });
+    return x;
+  };
+  auto mask = [&](f32x16& x, int s) {
+    const int key = (pc.t0 + s) * kTile;
+    if (key + kTile - 1 > lim0) {
+      asm volatile("" : "+v"(x));   // the last tiles only: a branch
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] = key + 8 * (i >> 2) + 4 * hl + (i & 3) <= lim ? x[i] : kNegInf;
+    }
+  };
+  auto tile_max = [&](const f32x16& x) {
+    float mx = x[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, x[i]);
+    return half_max(mx) * p.scale_log2;   // scale > 0
+  };
+  // The softmax of a tile in kPieces pieces, which the value product of another tile takes between its
+  // MFMAs: the maximum, then an element at a time.
+  constexpr int kPieces = 21;
+  float mx_part[4];
+  float ms = 0.f;
+  auto softmax_piece = [&](const f32x16& x, auto i_tag) {
+    constexpr int i = decltype(i_tag)::value;
+    if constexpr (i < 4) {
+      mx_part[i] = fmaxf(fmaxf(x[4 * i], x[4 * i + 1]), fmaxf(x[4 * i + 2], x[4 * i + 3]));
+    } else if constexpr (i == 4) {
+      const float mx = half_max(fmaxf(fmaxf(mx_part[0], mx_part[1]), fmaxf(mx_part[2], mx_part[3])));
+      mtrue = fmaxf(mtrue, mx * p.scale_log2);   // scale > 0
+      ms = mref == kNegInf ? 0.f : mref;
+    } else if constexpr (i < kPieces) {
+      constexpr int e = i - 5;
+      const float v = fast_exp2(__builtin_fmaf(x[e], p.scale_log2, -ms));
+      lsum += v;
+      pv[e >> 3][e & 7] = (bf16)v;   // what the value product takes; the sum keeps fp32
+    }
+  };
+  // P through LDS, between the waves.
+  auto post = [&] {
+    const unsigned at = lds_sum(16 * lane, opaque(lds.prob + wave * 2048));
+#pragma unroll
+    for (int u = 0; u < 2; ++u) *lds_ptr<bf16x8>(at + 1024 * u) = pv[u];
+  };
+
+  // ---- values: O^T += V^T P of a tile, in groups g of 16 keys (u = g / 4) and 32 columns (j = g % 4) ----
+  // Row m of the operand is column 4 (m / 8) + 16 (m / 4 % 2) + m % 4 of the block: a lane then ends with 16
+  // neighbouring columns.
+  bf16x8 prob[2][kRowBlocks], val[3];
+  unsigned val_addr = 0, prob_addr = 0;
+  auto values_begin = [&](int s) {
+    const int r = (lane & 15) >> 2, g = lane >> 4 & 1;
+    val_addr = lds_sum(kKeyRow * (4 * hl + r) + 256 * wave + 16 * (4 * r | ((g + 2 * (lane & 1)) ^ hl)) + 8 * ((lane & 3) >> 1),
+                       opaque(lds.keys + (unsigned)(s % kSlots) * kKeyBytes));
+    prob_addr = lds_sum(16 * lane, lds.prob);
+  };
+  auto read_prob = [&](int u, int n) { prob[u][n] = *lds_ptr<const bf16x8>(prob_addr + 2048 * n + 1024 * u); };
+  auto read_values = [&](int g) {
+    const unsigned a = val_addr ^ (64 * (g % 4));
+    const int at = 16 * kKeyRow * (g / 4);
+    val[g % 3] = concat(lds_read_tr16(lds_ptr<const bf16x4>(a + at)),
+                        lds_read_tr16(lds_ptr<const bf16x4>((a ^ 32) + at + 8 * kKeyRow)));
+  };
+  // After values_begin(s), the probabilities of the first 16 keys and the values of groups 0 and 1;
+  // beside(i) runs after MFMA i = 0 .. 31.
+  auto values = [&](auto beside) {
+    static_for<32>([&](auto i_tag) {
+      constexpr int i = decltype(i_tag)::value, g = i / 4, n = i % 4, u = g / 4;
+      acc[n][g % 4] = mfma32_bf16(val[g % 3], prob[u][n], acc[n][g % 4]);
+      if constexpr (n == 0 && g + 2 < 8) read_values(g + 2);
+      if constexpr (n == 2 && g < 4) read_prob(1, g);
+      beside(i_tag);
+      in_order();
+    });
+  };
+  auto any_of = [&](int mine) {   // over the waves; everything before it is done for all of them
+    wait_vm<0>();
+    wait_lds();
+    __syncthreads();
+    if (lane == 0) lds.flag[wave] = mine;
+    __syncthreads();
+    const int all = lds.flag[0] | lds.flag[1] | lds.flag[2] | lds.flag[3];
+    __syncthreads();
+    return all != 0;
+  };
+
+  {
+    lsum = 0.f;
+    const int n_steps = t1 - pc.t0;
+    // Zeros by the matrix core, a whole accumulator at a time: element by element the compiler would
+    // assemble them elsewhere and move them.
 #pragma unroll
     for (int n = 0; n < kRowBlocks; ++n)
 #pragma unroll
       for (int j = 0; j < kColBlocks; ++j) acc[n][j] = mfma32_bf16(bf16x8{}, bf16x8{}, f32x16{});
-    lsum = 0.f;
-    if (pc.t0 < pc.t1) pages.fetch(p, pc, pc.t0 / 2);
+    if (n_steps > 0) {
+      copy_tile(0);
+      copy_tile(1);
+      copy_tile(2);
+      wait_vm<2 * kCopies>();
+      __syncthreads();   // tile 0 landed
+      read_rope(0);
+      scores_begin(0);
+#pragma unroll
+      for (int c = 0; c < kDepth; ++c) read_key(c);
+      f32x16 x0 = scores([](auto) {});
+      score_done(x0);
+      mask(x0, 0);
+      const float top = tile_max(x0);
+      mref = pass.careful ? lds.top[32 * wave + l32] : top;
+      mtrue = top;
+      static_for<kPieces>([&](auto i) { softmax_piece(x0, i); });
+      post();
+      wait_vm<kCopies>();
+      wait_lds();
+      __syncthreads();   // tile 1 landed
+      read_rope(1);
+      scores_begin(1);
+#pragma unroll
+      for (int c = 0; c < kDepth; ++c) read_key(c);
+      // Step s: scores of tile s; barrier A; values of tile s - 1, with the softmax of tile s; barrier B; the start of
+      // the next step's scores.  A stands where P of step s - 1 is posted, B where tile s - 1 has been read and tile
+      // s + 1 has landed.  Both stand among MFMAs whose operands are there, and what they guard is read a few MFMAs
+      // ahead of its use.  Copies start two tiles ahead.
 #pragma nounroll
-    for (int s = 0; s < pc.t1 - pc.t0; ++s) {
-      const int t = pc.t0 + s;
-      copy_tile(s);
-      wait_vm<0>();
-      __syncthreads();
-      // scores: S^T[key 8 (i / 4) + 4 hl + i % 4][row l32]
-      f32x16 x;
-      const unsigned rope = lds_sum(128 * l32 + 16 * (hl ^ (l32 & 7)), lds.rope + (s % kSlots) * kRopeBytes);
-      const unsigned key = lds_sum(kKeyRow * l32 + 16 * (hl ^ key_swz(l32)), lds.keys + (s % kSlots) * kKeyBytes);
-      static_for<kSteps>([&](auto m_tag) {
-        constexpr int m = decltype(m_tag)::value, c = m - 4;
-        const bf16x8 k = *lds_ptr<const bf16x8>(m < 4 ? rope ^ (32 * m) : (key ^ (32 * (c & 7))) + 256 * (c >> 3));
-        score_step<m == 0>(x, k, q[m < 4 ? kLatSteps + m : c]);
-      });
-      score_done(x);
-      if (t * kTile + kTile - 1 > lim0) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = t * kTile + 8 * (i >> 2) + 4 * hl + (i & 3) <= lim ? x[i] : kNegInf;
+      for (int s = 1; s < n_steps; ++s) {
+        f32x16 x = scores([&](auto m_tag) {
+          constexpr int m = decltype(m_tag)::value;
+          if constexpr (m == 1) copy_begin(s + 2);
+          if constexpr (m >= 2 && m < 2 + 2 * kCopies && m % 2 == 0) copy(m / 2 - 1);
+          if constexpr (m == 22) {
+            wait_lds<5>();   // P is posted; reads of later keys may be on their way
+            barrier();       // A
+          }
+          if constexpr (m == 23) values_begin(s - 1);
+          if constexpr (m >= 24 && m < 28) read_prob(0, m - 24);
+          if constexpr (m >= 30 && m % 2 == 0 && m < 34) read_values((m - 30) / 2);
+        });
+        values([&](auto i_tag) {
+          constexpr int i = decltype(i_tag)::value;
+          if constexpr (i == 2) {
+            asm("s_nop 7" : "+v"(x));
+            mask(x, s);
+          } else if constexpr (i > 2 && i - 3 < kPieces) {
+            softmax_piece(x, std::integral_constant<int, i - 3>{});
+          } else if constexpr (i == 24) {
+            wait_vm<kCopies>();   // this wave's copies of tile s + 1; those of one tile more may be on their way
+            wait_lds();           // the values of tile s - 1
+            barrier();            // B
+          } else if constexpr (i == 25) {
+            post();
+          } else if constexpr (i == 26) {
+            read_rope(s + 1);
+          } else if constexpr (i == 27) {
+            scores_begin(s + 1);
+          } else if constexpr (i > 28) {
+            read_key(2 * (i - 29));
+            read_key(2 * (i - 29) + 1);
+          }
+        });
       }
-      float mx = x[0];
+      // The values of the last tile.
+      wait_lds();
+      __syncthreads();   // its P is posted
+      values_begin(n_steps - 1);
 #pragma unroll
-      for (int i = 1; i < 16; ++i) mx = fmaxf(mx, x[i]);
-      mx = half_max(mx) * p.scale_log2;   // scale > 0
-      if (s == 0) mref = again ? mtrue : mx;
-      mtrue = fmaxf(mtrue, mx);
-      const float ms = mref == kNegInf ? 0.f : mref;
-      bf16x8 pv[2];
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const float v = fast_exp2(__builtin_fmaf(x[e], p.scale_log2, -ms));
-        lsum += v;
-        pv[e >> 3][e & 7] = (bf16)v;
-      }
-      const unsigned at = lds_sum(16 * lane, lds.prob + wave * 2048);
-#pragma unroll
-      for (int u = 0; u < 2; ++u) *lds_ptr<bf16x8>(at + 1024 * u) = pv[u];
-      __syncthreads();
-      // values: groups of 16 keys (u) and 32 columns (j).  Row m of the operand is column
-      // 4 (m / 8) + 16 (m / 4 % 2) + m % 4 of the block: a lane then ends with 16 neighbouring columns.
-      const int r = (lane & 15) >> 2, g = lane >> 4 & 1;
-      const unsigned val = lds_sum(kKeyRow * (4 * hl + r) + 256 * wave + 16 * (4 * r | ((g + 2 * (lane & 1)) ^ hl)) + 8 * ((lane & 3) >> 1),
-                                   lds.keys + (s % kSlots) * kKeyBytes);
-      const unsigned prob = lds_sum(16 * lane, lds.prob);
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        bf16x8 pr[kRowBlocks];
-#pragma unroll
-        for (int n = 0; n < kRowBlocks; ++n) pr[n] = *lds_ptr<const bf16x8>(prob + 2048 * n + 1024 * u);
-#pragma unroll
-        for (int j = 0; j < kColBlocks; ++j) {
-          const unsigned a = (val ^ (64 * j)) ;
-          const bf16x8 v = concat(lds_read_tr16(lds_ptr<const bf16x4>(a + 16 * kKeyRow * u)),
-                                  lds_read_tr16(lds_ptr<const bf16x4>((a ^ 32) + 16 * kKeyRow * u + 8 * kKeyRow)));
-#pragma unroll
-          for (int n = 0; n < kRowBlocks; ++n) acc[n][j] = mfma32_bf16(v, pr[n], acc[n][j]);
-        }
-      }
-      __syncthreads();   // keys and probabilities are read
+      for (int n = 0; n < kRowBlocks; ++n) read_prob(0, n);
+      read_values(0);
+      read_values(1);
+      values([](auto) {});
     }
-    const bool over = __any(mtrue > mref + kHeadroom);
-    if (lane == 0) lds.flag[wave] = over ? 1 : 0;
-    __syncthreads();
-    const bool repeat = (lds.flag[0] | lds.flag[1] | lds.flag[2] | lds.flag[3]) != 0;
-    __syncthreads();
-    if (again || !repeat) break;
   }
 
   // ---- output ----
-  lsum = half_sum(lsum);
-  agpr_settle();
-  if (hl == 0) lds.stat[wave * 32 + l32] = lim >= pages.bad * (int64_t)kPage ? __builtin_nanf("") : lsum;
-  __syncthreads();
-  if (hl == 0 && 32 * wave + l32 < rows && p.lse != nullptr) {
-    const int r = pc.row0 + 32 * wave + l32;
-    const int token = fast_div(r, p.hdiv), head = r - token * p.H;
-    const float sum = lds.stat[32 * wave + l32];
-    p.lse[(int64_t)(pc.q0 + token) * p.H + head] = sum == 0.f ? kNegInf : (mref + __log2f(sum)) * kLn2;
-  }
-  // Through LDS, 32 rows at a time, so that a store covers whole lines: 256 bytes of each of 4 rows.  16-byte unit u
-  // of row r lies at u ^ r.
-  const unsigned mine = lds.keys + wave * 16 * 1024;
-  const int g = lane >> 4, c = lane & 15;
-  const unsigned put = lds_sum(512 * l32 + 16 * ((4 * hl) ^ l32), mine);
-  const unsigned get = lds_sum(512 * g + 16 * ((2 * c) ^ g), mine);   // 8 columns of row g: this unit and the one beside it
-#pragma unroll
-  for (int n = 0; n < kRowBlocks; ++n) {
-    const float sum = lds.stat[32 * n + l32];
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll
-    for (int j = 0; j < kColBlocks; ++j)
-#pragma unroll
-      for (int d = 0; d < 4; ++d) {
-        f32x4 v;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = agpr_read(acc[n][j][4 * d + i]) * inv;
-        *lds_ptr<f32x4>(put ^ (16 * (8 * j + d))) = v;
-      }
-#pragma unroll
-    for (int r = 0; r < 8; ++r) {
-      const int row = 32 * n + 4 * r + g;
-      const f32x4 a = *lds_ptr<const f32x4>((get ^ (64 * r)) + 2048 * r), b = *lds_ptr<const f32x4>((get ^ (64 * r) ^ 16) + 2048 * r);
-      if (row < rows) {
-        const int token = fast_div(pc.row0 + row, p.hdiv), head = pc.row0 + row - token * p.H;
-        bf16x8 v;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          v[i] = (bf16)a[i];
-          v[4 + i] = (bf16)b[i];
+  if (hl == 0 && !pass.careful) lds.top[32 * wave + l32] = mtrue;
+  if (any_of(!pass.careful && __any(mtrue > mref + kHeadroom))) return true;
+  {
+    {
+      lsum = half_sum(lsum);
+      agpr_settle();
+      if (hl == 0) lds.stat[wave * 32 + l32] = (int64_t)lim >= pages.bad * (int64_t)kPage ? __builtin_nanf("") : lsum;
+      __syncthreads();
+      const bool mine_too = 32 * wave + l32 < rows && lim >= pass.from && lim < pass.to;
+      if (hl == 0 && mine_too) {
+        const float sum = lds.stat[32 * wave + l32];
+        const float lse2 = sum == 0.f ? kNegInf : mref + __log2f(sum);
+        if (pc.slot >= 0) {
+          p.part_lse[(int64_t)pc.slot * kRows + 32 * wave + l32] = lse2;
+        } else if (p.lse != nullptr) {
+          const int r = pc.row0 + 32 * wave + l32;
+          const int token = fast_div(r, p.hdiv), head = r - token * p.H;
+          p.lse[(int64_t)(pc.s.q0 + token) * p.H + head] = lse2 * kLn2;
         }
-        *reinterpret_cast<bf16x8*>(p.o + (pc.q0 + token) * p.o_st + head * p.o_sh + 128 * wave + 8 * c) = v;
       }
+      // Through LDS, 32 rows at a time, so that a store covers whole lines: 256 bytes of each of 4 rows, or of a part
+      // 512 bytes of each of 2.  16-byte unit u of row r lies at u ^ r.
+      const unsigned mine = lds.keys + wave * 16 * 1024;
+      const int g = lane >> 4, c = lane & 15;
+      const unsigned put = lds_sum(512 * l32 + 16 * ((4 * hl) ^ l32), mine);
+      const unsigned get16 = lds_sum(512 * g + 16 * ((2 * c) ^ g), mine);   // 8 columns of row g: this unit and the one beside it
+      const unsigned get32 = lds_sum(512 * hl + 16 * (l32 ^ hl), mine);     // 4 columns of row hl
+      float check = 0.f;   // not a number where an output is none, or infinite
+      auto written = [&](int row) {
+        const int l = limit_of(row);
+        return row < rows && l >= pass.from && l < pass.to;
+      };
+#pragma unroll
+      for (int n = 0; n < kRowBlocks; ++n) {
+        if (32 * n >= rows) break;
+        const float sum = lds.stat[32 * n + l32];
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+        for (int j = 0; j < kColBlocks; ++j)
+#pragma unroll
+          for (int d = 0; d < 4; ++d) {
+            f32x4 v;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = agpr_read(acc[n][j][4 * d + i]) * inv;
+            *lds_ptr<f32x4>(put ^ (16 * (8 * j + d))) = v;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) check = __builtin_fmaf(v[i], 0.f, check);
+          }
+        if (pc.slot < 0) {
+#pragma unroll
+          for (int r = 0; r < 8; ++r) {   // row 4 r + g
+            const f32x4 a = *lds_ptr<const f32x4>((get16 ^ (64 * r)) + 2048 * r), b = *lds_ptr<const f32x4>((get16 ^ (64 * r) ^ 16) + 2048 * r);
+            const int row = 32 * n + 4 * r + g;
+            if (!written(row)) continue;
+            const int token = fast_div(pc.row0 + row, p.hdiv), head = pc.row0 + row - token * p.H;
+            bf16x8 v;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              v[i] = (bf16)a[i];
+              v[4 + i] = (bf16)b[i];
+            }
+            *reinterpret_cast<bf16x8*>(p.o + (pc.s.q0 + token) * p.o_st + head * p.o_sh + 128 * wave + 8 * c) = v;
+          }
+        } else {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {   // row 2 r + hl
+            const f32x4 a = *lds_ptr<const f32x4>((get32 ^ (32 * r)) + 1024 * r);
+            const int row = 32 * n + 2 * r + hl;
+            if (written(row))
+              *reinterpret_cast<f32x4*>(p.part_o + ((int64_t)pc.slot * kRows + row) * kDv + 128 * wave + 4 * l32) = a;
+          }
+        }
+      }
+      return any_of(__any(check != check));
     }
   }
 }
 
-// One workgroup per 128 rows; those past the last clear the queries that no sequence has.
+// The next rows to run the careful way, from the limit `from` on: up to a later token whose latents are not all finite.
+__device__ __forceinline__ Pass careful_pass(const ChunkParams& p, const Piece& pc, const Lds& lds, int from, int lim_last) {
+  const int wave = uniform(threadIdx.x >> 6);
+  int to = 0x7fffffff;
+  for (int j = max(from + 1, 0) + wave; j <= min(lim_last, pc.t1 * kTile - 1); j += kWaves) {
+    const int page = uniform(p.block_table[pc.b * p.bt_sb + j / kPage]);
+    if (page < 0 || page >= p.num_pages) continue;
+    const u32x4 v = *reinterpret_cast<const u32x4*>(p.kv + page * p.kv_sp + j % kPage * p.kv_ss + 16 * fresh_lane_id());
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) odd = odd || (v[i] & 0x7f80u) == 0x7f80u || (v[i] & 0x7f800000u) == 0x7f800000u;
+    if (__any(odd)) {
+      to = j;
+      break;
+    }
+  }
+  if (fresh_lane_id() == 0) lds.flag[wave] = to;
+  __syncthreads();
+  to = uniform(min(min(lds.flag[0], lds.flag[1]), min(lds.flag[2], lds.flag[3])));
+  __syncthreads();
+  return Pass{true, from, to};
+}
+
+// ---- cutting the work ---------------------------------------------------------------------------------
+// The row tiles (128 rows) of all sequences, in order, each with its key tiles behind kCost virtual ones (what starting
+// and ending a piece costs), are cut into ranges of equal weight, one per workgroup: no list, no plan kernel, no order
+// of workgroups.  Every workgroup works the cut out from the lengths.  A row tile that spans ranges leaves a part in
+// each, merged by chunk_combine_kernel: range r writes the part that it begins with to slot 2 r (a row tile that an
+// earlier range began) and the one that it ends with to slot 2 r + 1.
+//
+// Weights are estimates, in closed form: A(n) = n (kCost + (base + 31) / 32) + 2 n (n + 1) / H for the first n row
+// tiles of a sequence whose first query is token `base` (row tile i ends at token base + 128 (i + 1) / H, causal).
+// A range's end is the next one's start by the same arithmetic, so nothing is lost or done twice where they are off.
+constexpr int kCost = 8;
+constexpr int kMinWidth = 16;   // of a range
+constexpr int kSnap = 3;        // a cut this near to a row tile's end moves there
+
+struct Window {   // the sequences of 256 at a time, and what the threads share
+  int q0[kThreads], n[kThreads], len[kThreads];
+  int64_t tmp[kWaves];
+  int at[4];
+  int64_t rest[2];
+};
+
+__device__ __forceinline__ int row_tiles(const ChunkParams& p, const Sequence& s) { return (s.n * p.H + kRows - 1) / kRows; }
+__device__ __forceinline__ int key_tiles(const ChunkParams& p, const Sequence& s, int rt) {
+  const int last = fast_div(min((rt + 1) * kRows, s.n * p.H) - 1, p.hdiv);
+  const int end = p.causal ? s.len - s.n + last + 1 : s.len;
+  return (max(end, 0) + kTile - 1) / kTile;
+}
+// Weight of a row tile before its growth along the sequence.
+__device__ __forceinline__ int64_t base_weight(const ChunkParams& p, const Sequence& s) {
+  return kCost + (p.causal ? max(s.len - s.n, 0) + kTile - 1 : s.len + kTile - 1) / kTile;
+}
+__device__ __forceinline__ int64_t weight(const ChunkParams& p, const Sequence& s, int64_t n) {
+  return n * base_weight(p, s) + (p.causal ? 2 * n * (n + 1) / p.H : 0);
+}
+
+struct Place {   // in the row tiles and key tiles of all sequences
+  int b, rt, t;
+};
+
+// The place at weight y of sequence b.
+__device__ __forceinline__ Place place_of(const ChunkParams& p, int b, const Sequence& s, int64_t y) {
+  int lo = 0, hi = row_tiles(p, s) - 1;   // the last row tile that begins at or before y
+  const int64_t w = base_weight(p, s) * p.H, x = (y + 1) * p.H;
+  while (lo < hi) {
+    const int64_t mid = (lo + hi + 1) / 2;
+    if (mid * w + (p.causal ? 2 * mid * (mid + 1) : 0) < x) lo = (int)mid; else hi = (int)mid - 1;
+  }
+  const int nt = key_tiles(p, s, lo);
+  int t = (int)min((int64_t)nt, max((int64_t)0, y - weight(p, s, lo) - kCost));
+  if (t < kSnap) t = 0;
+  if (t > 0 && nt - t < kSnap) return Place{b, lo + 1, 0};
+  return Place{b, lo, t};
+}
+
+// What the combine reads of a range: x the rows of a row tile that begins in it and goes on in the next (0: none), their
+// packed query q0 and first row, w how its first part goes on: 1 it ends here, 2 it does not.
+typedef int4 RangeLink;
+
 __global__ __launch_bounds__(kThreads, 1) void chunk_kernel(ChunkParams p) {
   __shared__ __attribute__((aligned(1024))) char mem[kSlots * (kKeyBytes + kRopeBytes) + kProbBytes];
-  __shared__ __attribute__((aligned(16))) float stat[kRows];
+  __shared__ __attribute__((aligned(16))) float stat[kRows], top[kRows];
   __shared__ __attribute__((aligned(16))) int flag[kWaves];
-  __shared__ int found[4];
+  __shared__ __attribute__((aligned(16))) Window win;
   const unsigned base = lds_addr((DMLA_LDS char*)mem);
-  const Lds lds = {base, base + kSlots * kKeyBytes, base + kSlots * (kKeyBytes + kRopeBytes), (DMLA_LDS float*)stat,
+  const Lds lds = {base, base + kSlots * kKeyBytes, base + kSlots * (kKeyBytes + kRopeBytes), (DMLA_LDS float*)stat, (DMLA_LDS float*)top,
                    (DMLA_LDS int*)flag};
-  // The piece's sequence, by one wave.
-  if (threadIdx.x < 64) {
-    const int lane = threadIdx.x;
-    int64_t before = 0;
-    int b = -1, row0 = 0;
-    for (int b0 = 0; b0 < p.B && b < 0; b0 += 64) {
-      const int64_t mine = b0 + lane < p.B ? ((int64_t)sequence(p, b0 + lane).n * p.H + kRows - 1) / kRows : 0;
-      int64_t x = mine;
-      for (int o = 1; o < 64; o <<= 1) {
-        const int64_t y = __shfl_up(x, o, 64);
-        if (lane >= o) x += y;
-      }
-      const unsigned long long past = __ballot(before + x > (int64_t)blockIdx.x);
-      if (past != 0) {
-        const int i = __builtin_ctzll(past);
-        b = b0 + i;
-        row0 = (int)((int64_t)blockIdx.x - before - __shfl(x - mine, i, 64)) * kRows;
-      }
-      before += __shfl(x, 63, 64);
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+  // Ranges that follow each other run on one XCD: they read the same keys.
+  const int per_xcd = (p.n_ranges + 7) / 8;
+  const int range = (int)(blockIdx.x % 8) * per_xcd + (int)(blockIdx.x / 8);
+  if (range >= p.n_ranges) return;
+
+  int window = 0;   // first sequence of the window
+  auto load_window = [&](int b0) {
+    __syncthreads();   // the window is read
+    Sequence s = {0, 0, 0};
+    if (b0 + tid < p.B) s = sequence(p, b0 + tid);
+    win.q0[tid] = s.q0;
+    win.n[tid] = s.n;
+    win.len[tid] = s.len;
+    window = b0;
+    return s;
+  };
+  auto known = [&](int b) {   // of the window
+    const int i = b - window;
+    return Sequence{uniform(win.q0[i]), uniform(win.n[i]), uniform(win.len[i])};
+  };
+  // Inclusive sum over the threads and their total.
+  auto scan = [&](int64_t v, int64_t& sum) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int64_t y = __shfl_up(v, o, 64);
+      if (lane >= o) v += y;
     }
-    if (lane == 0) {
-      found[0] = b;
-      found[1] = row0;
+    __syncthreads();   // tmp is read
+    if (lane == 63) win.tmp[wave] = v;
+    __syncthreads();
+    sum = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      if (w < wave) v += win.tmp[w];
+      sum += win.tmp[w];
     }
+    return v;
+  };
+  int64_t total = 0, upto = 0, mine = 0, sum;
+  for (int b0 = 0; b0 < p.B; b0 += kThreads) {
+    const Sequence s = load_window(b0);
+    mine = weight(p, s, row_tiles(p, s));
+    upto = scan(mine, sum);
+    total += sum;
+  }
+  const int64_t width = max((int64_t)kMinWidth, (total + p.n_ranges - 1) / p.n_ranges);
+  const int64_t x0 = range * width, x1 = min(x0 + width, total);
+  if (x0 >= total) {
+    if (tid == 0) p.links[range] = make_int4(0, 0, 0, 0);
+    return;
+  }
+  // The sequences at x0 and at x1 - 1, and the weights in them.
+  if (tid == 0) win.at[0] = win.at[1] = -1;
+  int64_t before = 0;
+  for (int b0 = 0; b0 < p.B; b0 += kThreads) {
+    if (p.B > kThreads) {
+      const Sequence s = load_window(b0);
+      mine = weight(p, s, row_tiles(p, s));
+      upto = scan(mine, sum);
+    } else {
+      __syncthreads();
+    }
+    const int64_t lo = before + upto - mine, hi = before + upto;
+    if (lo <= x0 && x0 < hi) {
+      win.at[0] = b0 + tid;
+      win.rest[0] = x0 - lo;
+    }
+    if (lo < x1 && x1 <= hi) {
+      win.at[1] = b0 + tid;
+      win.rest[1] = x1 - lo;
+    }
+    before += sum;
+    if (before >= x1) break;   // (the same for all threads)
   }
   __syncthreads();
-  Piece pc;
-  pc.b = uniform(found[0]);
-  if (pc.b < 0) return;
-  const Sequence s = sequence(p, pc.b);
-  pc.q0 = uniform(s.q0);
-  pc.n = uniform(s.n);
-  pc.len = uniform(s.len);
-  pc.row0 = uniform(found[1]);
-  const int last = fast_div(min(pc.row0 + kRows, pc.n * p.H) - 1, p.hdiv);
-  const int end = p.causal ? pc.len - pc.n + last + 1 : pc.len;   // keys of the last row
-  pc.t0 = 0;
-  pc.t1 = uniform((max(end, 0) + kTile - 1) / kTile);
-  run_piece(p, pc, lds);
+  const int b_first = uniform(win.at[0]), b_last = uniform(win.at[1]);
+  const int64_t y0 = win.rest[0], y1 = win.rest[1];
+  auto sequence_at = [&](int b) {
+    if (b < window || b >= window + kThreads) {
+      load_window(b);
+      __syncthreads();
+    }
+    return known(b);
+  };
+  Sequence s = sequence_at(b_last);
+  // The end of the last sequence's work is its last row tile's.
+  Place end = place_of(p, b_last, s, y1);
+  if (y1 >= weight(p, s, row_tiles(p, s))) end = Place{b_last, row_tiles(p, s), 0};
+  s = sequence_at(b_first);
+  Place at = place_of(p, b_first, s, y0);
+  end.rt = uniform(end.rt); end.t = uniform(end.t);
+  at.rt = uniform(at.rt); at.t = uniform(at.t);
+  RangeLink link = make_int4(0, 0, 0, 0);
+  while (at.b < end.b || (at.b == end.b && (at.rt < end.rt || (at.rt == end.rt && at.t < end.t)))) {
+    if (at.rt >= row_tiles(p, s)) {   // the next sequence with queries: 256 looked at together
+      int b = at.b + 1;
+      for (;; b = window + kThreads) {
+        if (b >= window + kThreads) {
+          load_window(b);
+          __syncthreads();
+        }
+        // (b - window < 256) the first sequence from b on in the window that has queries
+        int found = kThreads;
+        for (int i0 = (b - window) & ~63; i0 < kThreads; i0 += 64) {
+          const unsigned long long m = __ballot(i0 + lane >= b - window && win.n[i0 + lane] > 0);
+          if (m != 0) {
+            found = i0 + __builtin_ctzll(m);
+            break;
+          }
+        }
+        if (found < kThreads) {
+          b = window + found;
+          break;
+        }
+      }
+      at = Place{uniform(b), 0, 0};
+      s = known(at.b);
+      continue;
+    }
+    const int nt = key_tiles(p, s, at.rt);
+    Piece pc;
+    pc.s = s;
+    pc.b = at.b;
+    pc.row0 = at.rt * kRows;
+    pc.t0 = at.t;
+    const bool whole = !(at.b == end.b && at.rt == end.rt);   // to its end
+    pc.t1 = whole ? nt : min(end.t, nt);
+    pc.slot = at.t > 0 ? 2 * range : whole ? -1 : 2 * range + 1;
+    if (at.t > 0) link.w = whole ? 1 : 2;
+    else if (!whole) link = make_int4(min(s.n * p.H - pc.row0, kRows), s.q0, pc.row0, link.w);
+    Pass pass = {false, (int)0x80000000, 0x7fffffff};
+    while (run_piece(p, pc, lds, pass) || (pass.careful && pass.to != 0x7fffffff)) {
+      if (pass.careful && pass.to == 0x7fffffff) break;
+      const int base = pc.s.len - pc.s.n, last = min(pc.row0 + kRows, pc.s.n * p.H) - 1;
+      const int first_lim = p.causal ? base + fast_div(pc.row0, p.hdiv) : pc.s.len - 1;
+      const int last_lim = p.causal ? base + fast_div(last, p.hdiv) : pc.s.len - 1;
+      pass = careful_pass(p, pc, lds, pass.careful ? pass.to : first_lim, last_lim);
+    }
+    if (!whole) break;
+    ++at.rt;
+    at.t = 0;
+  }
+  if (tid == 0) p.links[range] = link;
 }
 
-// Queries behind the last sequence: zeros, and -inf.
-__global__ __launch_bounds__(256) void chunk_tail_kernel(ChunkParams p) {
-  const int first = p.cu == nullptr ? p.B : min(max(p.cu[p.B], 0), p.T);
-  const int64_t total = (int64_t)(p.T - first) * p.H * (kDv / 8);
-  for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < total; u += (int64_t)gridDim.x * 256) {
-    const int64_t row = u / (kDv / 8);
-    const int c = (int)(u % (kDv / 8)), token = first + (int)(row / p.H), head = (int)(row % p.H);
-    *reinterpret_cast<bf16x8*>(p.o + token * p.o_st + head * p.o_sh + 8 * c) = bf16x8{};
-    if (c == 0 && p.lse != nullptr) p.lse[(int64_t)token * p.H + head] = kNegInf;
+// Row tiles that span ranges: o = sum_j w_j o_j / sum_j w_j with w_j = 2^(lse_j - max); and the queries behind the last
+// sequence.  Four rows per workgroup, one a wave.
+__global__ __launch_bounds__(256) void chunk_combine_kernel(ChunkParams p) {
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int range = (int)blockIdx.x / (kRows / 4), row = 4 * ((int)blockIdx.x % (kRows / 4)) + wave;
+  const RangeLink link = range < p.n_ranges ? p.links[range] : make_int4(0, 0, 0, 0);
+  if (row < link.x) {
+    // Its parts: the range's last, then those that the next ranges begin with, up to one that ends there.
+    int parts = 1;
+    for (int r0 = range + 1;; r0 += 64) {
+      const int w = r0 + lane < p.n_ranges ? p.links[r0 + lane].w : 1;
+      const unsigned long long ends = __ballot(w != 2);
+      parts += ends != 0 ? __builtin_ctzll(ends) + 1 : 64;
+      if (ends != 0) break;
+    }
+    auto slot = [&](int j) { return (int64_t)(j == 0 ? 2 * range + 1 : 2 * (range + j)); };
+    float top = kNegInf;
+    bool none = true;   // no number among them
+    for (int j0 = 0; j0 < parts; j0 += 64) {
+      const float l = j0 + lane < parts ? p.part_lse[slot(j0 + lane) * kRows + row] : kNegInf;
+      top = fmaxf(top, l);
+      none = none && l == l;
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+    const bool number = __all(none);
+    float sum = 0.f;
+    f32x4 a0 = {0.f, 0.f, 0.f, 0.f}, a1 = a0;
+    for (int j0 = 0; j0 < parts; j0 += 4) {
+      f32x4 v0[4], v1[4];
+      float l[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int64_t at = slot(min(j0 + i, parts - 1)) * kRows + row;
+        l[i] = p.part_lse[at];
+        v0[i] = *reinterpret_cast<const f32x4*>(p.part_o + at * kDv + 8 * lane);
+        v1[i] = *reinterpret_cast<const f32x4*>(p.part_o + at * kDv + 8 * lane + 4);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (j0 + i >= parts) break;
+        const float w = top == kNegInf ? 0.f : fast_exp2(l[i] - top);
+        if (w == 0.f) continue;   // a part without a weight adds nothing, whatever it holds
+        sum += w;
+        a0 += w * v0[i];
+        a1 += w * v1[i];
+      }
+    }
+    const float inv = !number ? __builtin_nanf("") : sum > 0.f ? 1.f / sum : 0.f;
+    bf16x8 v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[i] = (bf16)(a0[i] * inv);
+      v[4 + i] = (bf16)(a1[i] * inv);
+    }
+    const int r = link.z + row;
+    const int token = link.y + fast_div(r, p.hdiv), head = r - (token - link.y) * p.H;
+    *reinterpret_cast<bf16x8*>(p.o + token * p.o_st + head * p.o_sh + 8 * lane) = v;
+    if (lane == 0 && p.lse != nullptr)
+      p.lse[(int64_t)token * p.H + head] = !number ? __builtin_nanf("") : sum > 0.f ? (top + __log2f(sum)) * kLn2 : kNegInf;
+  }
+  const int behind = p.cu == nullptr ? p.T : p.B == 0 ? 0 : min(max(p.cu[p.B], 0), p.T);
+  const int64_t total = (int64_t)(p.T - behind) * p.H;
+  for (int64_t u = (int64_t)blockIdx.x * 4 + wave; u < total; u += (int64_t)gridDim.x * 4) {
+    const int token = behind + (int)(u / p.H), head = (int)(u % p.H);
+    *reinterpret_cast<bf16x8*>(p.o + token * p.o_st + head * p.o_sh + 8 * lane) = bf16x8{};
+    if (lane == 0 && p.lse != nullptr) p.lse[(int64_t)token * p.H + head] = kNegInf;
   }
 }
+
+// Ranges of a call: one per CU, as many as its work can fill at most.
+int64_t chunk_ranges(int64_t T, int64_t B, int64_t H, int64_t max_pages) {
+  const int64_t tiles = T * H / kRows + std::min(B, T);
+  const int64_t most = tiles * (kCost + 1 + max_pages * (kPage / kTile)) + 2 * T;   // at least what the kernel adds up
+  return std::max<int64_t>(1, std::min<int64_t>(device_cu_count(), (most + kMinWidth - 1) / kMinWidth));
+}
+int64_t chunk_bytes(int64_t ranges) { return ranges * (2 * kRows * (int64_t)(kDv + 1) * 4 + (int64_t)sizeof(RangeLink)); }
 
 }  // namespace
 }  // namespace dmla
@@ -343,8 +795,10 @@ __global__ __launch_bounds__(256) void chunk_tail_kernel(ChunkParams p) {
 using namespace dmla;
 
 extern "C" int64_t dmla_chunk_paged_workspace_bytes(int64_t T, int64_t B, int64_t H, int64_t max_pages_per_seq) {
-  (void)T; (void)B; (void)H; (void)max_pages_per_seq;
-  return 0;
+  if (T <= 0 || B <= 0 || H <= 0 || max_pages_per_seq <= 0 || T > ((int64_t)1 << 30) || H > ((int64_t)1 << 16) ||
+      B > ((int64_t)1 << 20) || T * H > ((int64_t)1 << 30) || max_pages_per_seq > ((int64_t)1 << 20))
+    return 0;
+  return chunk_bytes(chunk_ranges(T, B, H, max_pages_per_seq));
 }
 
 extern "C" int dmla_chunk_paged(const void* q, const void* kv_pool, const int32_t* block_table, const int32_t* cache_seqlens,
@@ -355,7 +809,6 @@ extern "C" int dmla_chunk_paged(const void* q, const void* kv_pool, const int32_
                                 dmla_stream_t stream) {
   clear_error();
   const char* what = "dmla_chunk_paged";
-  (void)workspace; (void)workspace_bytes;
   if (T < 0 || B < 0 || H < 0 || num_pages < 0 || max_pages_per_seq < 0)
     return fail(DMLA_ERR_INVALID_ARG, "%s: negative size", what);
   if (cu_seqlens_q == nullptr && T != B)
@@ -373,7 +826,7 @@ extern "C" int dmla_chunk_paged(const void* q, const void* kv_pool, const int32_
     return fail(DMLA_ERR_INVALID_ARG, "%s: kv_pool strides out of range", what);
   if (bt_sb < max_pages_per_seq) return fail(DMLA_ERR_INVALID_ARG, "%s: block_table row stride < max_pages_per_seq", what);
   if (H > ((int64_t)1 << 16) || B > ((int64_t)1 << 20) || T > ((int64_t)1 << 30) || T * H > ((int64_t)1 << 30) ||
-      max_pages_per_seq > ((int64_t)1 << 24) || num_pages > 0x7fffffff)
+      max_pages_per_seq > ((int64_t)1 << 20) || num_pages > 0x7fffffff)
     return fail(DMLA_ERR_UNSUPPORTED, "%s: size too large", what);
   if (T == 0 || H == 0) return DMLA_OK;
   if (!q || !o || (B > 0 && !cache_seqlens) || (B > 0 && max_pages_per_seq > 0 && !block_table) || (num_pages > 0 && !kv_pool))
@@ -393,10 +846,21 @@ extern "C" int dmla_chunk_paged(const void* q, const void* kv_pool, const int32_
   p.causal = causal ? 1 : 0;
   p.hdiv = make_fastdiv((unsigned)H);
   p.scale_log2 = softmax_scale * kLog2e;
-  const int64_t tiles = cu_seqlens_q == nullptr ? T * ((H + kRows - 1) / kRows) : T * H / kRows + std::min(B, T);
-  if (tiles > 0)
-    hipLaunchKernelGGL(chunk_kernel, dim3((unsigned)tiles), dim3(kThreads), 0, (hipStream_t)stream, p);
-  if (cu_seqlens_q != nullptr)
-    hipLaunchKernelGGL(chunk_tail_kernel, dim3(256), dim3(256), 0, (hipStream_t)stream, p);
+  p.n_ranges = (int)chunk_ranges(T, B, H, max_pages_per_seq);
+  if (B == 0) {   // nothing but queries behind the last sequence
+    p.n_ranges = 0;
+    hipLaunchKernelGGL(chunk_combine_kernel, dim3(256), dim3(256), 0, (hipStream_t)stream, p);
+    return check_launch(what);
+  }
+  const int64_t need = chunk_bytes(p.n_ranges);
+  if (workspace == nullptr || workspace_bytes < need)
+    return fail(DMLA_ERR_WORKSPACE, "%s: workspace of %lld bytes needed (got %lld)", what, (long long)need,
+                (long long)workspace_bytes);
+  if (!aligned16(workspace)) return fail(DMLA_ERR_INVALID_ARG, "%s: workspace must be 16-byte aligned", what);
+  p.part_o = static_cast<float*>(workspace);
+  p.part_lse = p.part_o + (int64_t)p.n_ranges * 2 * kRows * kDv;
+  p.links = reinterpret_cast<int4*>(p.part_lse + (int64_t)p.n_ranges * 2 * kRows);
+  hipLaunchKernelGGL(chunk_kernel, dim3((unsigned)((p.n_ranges + 7) / 8 * 8)), dim3(kThreads), 0, (hipStream_t)stream, p);
+  hipLaunchKernelGGL(chunk_combine_kernel, dim3((unsigned)(p.n_ranges * (kRows / 4))), dim3(256), 0, (hipStream_t)stream, p);
   return check_launch(what);
 }

@@ -6,6 +6,8 @@
 
 namespace dmla {
 
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
 // f(0), f(1), .., f(kN - 1) with compile-time arguments.
 template <int kN, typename F, int kI = 0>
 __device__ __forceinline__ void static_for(F f) {

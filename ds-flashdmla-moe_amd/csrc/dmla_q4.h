@@ -22,7 +22,6 @@ constexpr int kQ4MinExp = -125, kQ4MaxExp = 125;
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
-typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 // The scale byte of a block whose largest |value| has the fp32 bits `top` (a bf16 value).  With
 // top = m 2^k, 1 <= m < 2: top <= 6 2^e = 1.5 2^(e + 2) needs e = k - 2 for m <= 1.5, else k - 1.

@@ -110,19 +110,20 @@ def test_what_a_query_does_not_attend_does_not_reach_it(gpu, H, value):
         assert not torch.isfinite(o[clean:, :, 5]).any(), "a query that attends it"
 
 
-def test_huge_latents_and_climbing_scores_stay_finite(gpu):
-    """Values of 2^100 under scores that climb by hundreds: sums and outputs stay finite."""
+@pytest.mark.parametrize("steepest", [4.0, 60.0])
+def test_huge_latents_and_climbing_scores_stay_finite(gpu, steepest):
+    """Values of 2^110 under scores that climb by tens and by hundreds: sums and outputs stay finite."""
     from python import ops
     N = 400
     rows = torch.zeros(N, D_QK)
-    rows[:, :D_V] = 2.0 ** 100
+    rows[:, :D_V] = 2.0 ** 110
     rows[:, D_V] = torch.linspace(0, 60, N)
     rows = rows.to(torch.bfloat16)
     pool = torch.zeros(7, PAGE, D_QK, dtype=torch.bfloat16)
     pool[:6] = rows[:384].view(6, PAGE, D_QK)
     pool[6, :16] = rows[384:]
     q = torch.zeros(3, 16, D_QK)
-    q[:, :, D_V] = torch.linspace(0.1, 60, 16)
+    q[:, :, D_V] = torch.linspace(0.1, steepest, 16)
     q = q.to(torch.bfloat16)
     o, lse = ops.flash_dmla_chunk_paged(q.to(gpu), pool.to(gpu), ints([list(range(7))], gpu), ints([N], gpu), ints([0, 3], gpu),
                                         softmax_scale=SCALE, return_lse=True)
