@@ -31,8 +31,12 @@ constexpr int kKeyRow = 1024, kKeyBytes = kTile * kKeyRow, kSlots = 4;
 constexpr int kRopeBytes = kTile * 128;
 constexpr int kProbBytes = kWaves * 2048;                   // P of a step
 constexpr int kCopies = 9;                                 // of a wave and tile
-constexpr int kQueryBytes = 32 * 2 * kDqk;                 // of a wave, in the keys' and the ropes' memory
-static_assert(kWaves * kQueryBytes == kSlots * (kKeyBytes + kRopeBytes), "the queries fill it");
+// Queries come through that memory, in blocks of 64 dims (4 KB of a wave): the first six in the first three slots
+// of keys, where they may land while the piece before puts out through the fourth, two in the fourth, and one
+// in the third and fourth of the ropes and P.
+constexpr int kQueryEarly = 6, kQueryBlock = 4096;
+static_assert(kWaves * kQueryEarly * kQueryBlock == 3 * kKeyBytes && kWaves * 2 * kQueryBlock == kKeyBytes &&
+              kWaves * kQueryBlock == 2 * kRopeBytes + kProbBytes, "where the queries lie");
 constexpr float kHeadroom = 32.0f;                         // log2 headroom of P over a row's reference
 
 __device__ __forceinline__ int key_swz(int r) { return (r & 3) << 2 | (r >> 2 & 3); }
@@ -117,8 +121,30 @@ struct Pages {
   }
 };
 
+// The queries of 128 rows of a sequence from row0 on, this wave's 32: blocks [kFirst, kFirst + kN) of 64 dims.  Read
+// straight into the operands, a load would touch 32 rows for 32 bytes each; a copy moves eight rows x 128 bytes.
+__device__ __forceinline__ unsigned query_block(const Lds& lds, int wave, int i) {
+  if (i < kQueryEarly) return lds.keys + (wave * kQueryEarly + i) * kQueryBlock;
+  if (i < kQueryEarly + 2) return lds.keys + 3 * kKeyBytes + (wave * 2 + i - kQueryEarly) * kQueryBlock;
+  return lds.rope + 2 * kRopeBytes + wave * kQueryBlock;
+}
+template <int kFirst, int kN>
+__device__ __forceinline__ void copy_queries(const ChunkParams& p, const Lds& lds, int wave, int q0, int row0, int rows) {
+  const int ln = fresh_lane_id();
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const int r = row0 + min(32 * wave + 8 * g + (ln >> 3), rows - 1);
+    const int token = fast_div(r, p.hdiv), head = r - token * p.H;
+    const bf16* src = p.q + (q0 + token) * p.q_st + head * p.q_sh + 8 * ((ln & 7) ^ (ln >> 3));
+#pragma unroll
+    for (int i = kFirst; i < kFirst + kN; ++i) dma16_addr(src + 64 * i, query_block(lds, wave, i) + g * 1024);
+  }
+}
+
 // Whether another pass has to follow.
-__device__ __forceinline__ bool run_piece(const ChunkParams& p, const Piece& pc, const Lds& lds, const Pass& pass) {
+// have: the first queries are on their way.  After it, those of the next piece's rows are (next_rows > 0).
+__device__ __forceinline__ bool run_piece(const ChunkParams& p, const Piece& pc, const Lds& lds, const Pass& pass, bool have,
+                                          const DMLA_LDS int* next) {
   const int lane = fresh_lane_id();
   const int l32 = lane & 31, hl = lane >> 5;
   const int wave = uniform(threadIdx.x >> 6);
@@ -137,21 +163,23 @@ __device__ __forceinline__ bool run_piece(const ChunkParams& p, const Piece& pc,
   const int t1 = max(pc.t0, min(pc.t1, (max(key_end, 0) + kTile - 1) / kTile));
   const char* copy_src = nullptr;
   int copy_last = 0;
-  unsigned copy_dst = 0;
+  unsigned copy_dst = 0, copy_lane = 0;
+  const int row_step = uniform((int)p.kv_ss);
   auto copy_begin = [&](int s) {
+    copy_lane = 16 * (fresh_lane_id() ^ key_swz(8 * wave));
     const int t = min(pc.t0 + s, t1 - 1);   // past the end: the last tile, which nobody counts
     copy_src = pages.tile(p, pc, t);
     copy_last = uniform(min(key_end - t * kTile, kTile) - 1);
     copy_dst = (unsigned)(s % kSlots);
   };
   auto copy = [&](int i) {
-    const int ln = fresh_lane_id();
     if (i < 8) {
       const int r = 8 * wave + i;
-      const unsigned off = (16 * (ln ^ key_swz(8 * wave))) ^ (16 * key_swz(i));   // key_swz(8 w + i) is the two's xor
-      dma16(copy_src + min(r, copy_last) * p.kv_ss, off, lds.keys + copy_dst * kKeyBytes + r * kKeyRow);
+      // key_swz(8 wave + i) is key_swz(8 wave) ^ key_swz(i)
+      dma16(copy_src, (copy_lane ^ (16 * key_swz(i))) + min(r, copy_last) * row_step, lds.keys + copy_dst * kKeyBytes + r * kKeyRow);
     } else {
-      const unsigned off = min(8 * wave + (ln >> 3), copy_last) * (unsigned)p.kv_ss + 2 * kDv + 16 * ((ln & 7) ^ (ln >> 3));
+      const int ln = fresh_lane_id();
+      const unsigned off = min(8 * wave + (ln >> 3), copy_last) * row_step + 2 * kDv + 16 * ((ln & 7) ^ (ln >> 3));
       dma16(copy_src, off, lds.rope + copy_dst * kRopeBytes + wave * 1024);
     }
   };
@@ -162,28 +190,26 @@ __device__ __forceinline__ bool run_piece(const ChunkParams& p, const Piece& pc,
   };
 
   // ---- queries: 36 operands of 16 dims; operand c holds dims 16 c + 8 hl .. of row l32 ----
-  // Through the keys' memory, eight rows x 128 bytes a copy: read straight into the operands, a load would touch 32 rows
-  // for 32 bytes each.
+  const int n_steps = t1 - pc.t0;
   bf16x8 q[kSteps];
-  {
-    const unsigned mine = lds.keys + wave * kQueryBytes;   // the ropes' memory follows the keys'
-    const int ln = fresh_lane_id();
+  auto take_queries = [&](auto first_tag, auto n_tag) {
+    constexpr int kFirst = decltype(first_tag)::value, kN = decltype(n_tag)::value;
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int r = pc.row0 + min(32 * wave + 8 * g + (ln >> 3), rows - 1);
-      const int token = fast_div(r, p.hdiv), head = r - token * p.H;
-      const bf16* src = p.q + (pc.s.q0 + token) * p.q_st + head * p.q_sh + 8 * ((ln & 7) ^ (ln >> 3));
+    for (int i = kFirst; i < kFirst + kN; ++i) {
+      const unsigned a = lds_sum(1024 * (l32 >> 3) + 128 * (l32 & 7) + 16 * (hl ^ (l32 & 7)), query_block(lds, wave, i));
 #pragma unroll
-      for (int i = 0; i < 9; ++i) dma16_addr(src + 64 * i, mine + (9 * g + i) * 1024);
+      for (int c = 0; c < 4; ++c) q[4 * i + c] = *lds_ptr<const bf16x8>(a ^ (32 * c));
     }
-    pages.fetch(p, pc, pc.t0 / 2);
-    wait_vm<0>();
-    const unsigned a = lds_sum(9 * 1024 * (l32 >> 3) + 128 * (l32 & 7) + 16 * (hl ^ (l32 & 7)), mine);
-#pragma unroll
-    for (int c = 0; c < kSteps; ++c) q[c] = *lds_ptr<const bf16x8>((a ^ (32 * (c & 3))) + 1024 * (c >> 2));
-    wait_lds();
-    __syncthreads();   // the keys' memory is free
-  }
+  };
+  if (!have) copy_queries<0, kQueryEarly>(p, lds, wave, pc.s.q0, pc.row0, rows);
+  copy_queries<kQueryEarly, 3>(p, lds, wave, pc.s.q0, pc.row0, rows);
+  pages.fetch(p, pc, pc.t0 / 2);
+  wait_vm<0>();
+  using std::integral_constant;
+  take_queries(integral_constant<int, 0>{}, integral_constant<int, 9>{});
+  wait_lds();
+  __syncthreads();   // the keys' memory is free
+  if (n_steps > 0) copy_tile(0);
 
   f32x16 acc[kRowBlocks][kColBlocks];   // O^T: register i is column 128 wave + 32 j + 16 hl + i of row l32
   float mref = kNegInf, mtrue = kNegInf, lsum = 0.f;   // reference, largest score seen, sum
@@ -202,7 +228,7 @@ __device__ __forceinline__ bool run_piece(const ChunkParams& p, const Piece& pc,
 
   // ---- scores: S^T[key 8 (i / 4) + 4 hl + i % 4][row l32] of step s's tile ----
   bf16x8 rope[4];
-  constexpr int kDepth = 6;   // operands in flight
+  constexpr int kDepth = 8;   // operands in flight
   unsigned key_addr = 0;
   bf16x8 k[kDepth];
   auto read_rope = [&](int s) {
@@ -272,7 +298,7 @@ __device__ __forceinline__ bool run_piece(const ChunkParams& p, const Piece& pc,
   // ---- values: O^T += V^T P of a tile, in groups g of 16 keys (u = g / 4) and 32 columns (j = g % 4) ----
   // Row m of the operand is column 4 (m / 8) + 16 (m / 4 % 2) + m % 4 of the block: a lane then ends with 16
   // neighbouring columns.
-  bf16x8 prob[2][kRowBlocks], val[3];
+  bf16x8 prob[kRowBlocks], val[3];
   unsigned val_addr = 0, prob_addr = 0;
   auto values_begin = [&](int s) {
     const int r = (lane & 15) >> 2, g = lane >> 4 & 1;
@@ -280,7 +306,7 @@ __device__ __forceinline__ bool run_piece(const ChunkParams& p, const Piece& pc,
                        opaque(lds.keys + (unsigned)(s % kSlots) * kKeyBytes));
     prob_addr = lds_sum(16 * lane, lds.prob);
   };
-  auto read_prob = [&](int u, int n) { prob[u][n] = *lds_ptr<const bf16x8>(prob_addr + 2048 * n + 1024 * u); };
+  auto read_prob = [&](int u, int n) { prob[n] = *lds_ptr<const bf16x8>(prob_addr + 2048 * n + 1024 * u); };
   auto read_values = [&](int g) {
     const unsigned a = val_addr ^ (64 * (g % 4));
     const int at = 16 * kKeyRow * (g / 4);
@@ -291,28 +317,16 @@ __device__ __forceinline__ bool run_piece(const ChunkParams& p, const Piece& pc,
   // beside(i) runs after MFMA i = 0 .. 31.
   auto values = [&](auto beside) {
     static_for<32>([&](auto i_tag) {
-      constexpr int i = decltype(i_tag)::value, g = i / 4, n = i % 4, u = g / 4;
-      acc[n][g % 4] = mfma32_bf16(val[g % 3], prob[u][n], acc[n][g % 4]);
+      constexpr int i = decltype(i_tag)::value, g = i / 4, n = i % 4;
+      acc[n][g % 4] = mfma32_bf16(val[g % 3], prob[n], acc[n][g % 4]);
       if constexpr (n == 0 && g + 2 < 8) read_values(g + 2);
-      if constexpr (n == 2 && g < 4) read_prob(1, g);
+      if constexpr (g == 3) read_prob(1, n);
       beside(i_tag);
       in_order();
     });
   };
-  auto any_of = [&](int mine) {   // over the waves; everything before it is done for all of them
-    wait_vm<0>();
-    wait_lds();
-    __syncthreads();
-    if (lane == 0) lds.flag[wave] = mine;
-    __syncthreads();
-    const int all = lds.flag[0] | lds.flag[1] | lds.flag[2] | lds.flag[3];
-    __syncthreads();
-    return all != 0;
-  };
-
   {
     lsum = 0.f;
-    const int n_steps = t1 - pc.t0;
     // Zeros by the matrix core, a whole accumulator at a time: element by element the compiler would
     // assemble them elsewhere and move them.
 #pragma unroll
@@ -320,16 +334,17 @@ __device__ __forceinline__ bool run_piece(const ChunkParams& p, const Piece& pc,
 #pragma unroll
       for (int j = 0; j < kColBlocks; ++j) acc[n][j] = mfma32_bf16(bf16x8{}, bf16x8{}, f32x16{});
     if (n_steps > 0) {
-      copy_tile(0);
-      copy_tile(1);
-      copy_tile(2);
-      wait_vm<2 * kCopies>();
+      wait_vm<0>();
       __syncthreads();   // tile 0 landed
       read_rope(0);
       scores_begin(0);
 #pragma unroll
       for (int c = 0; c < kDepth; ++c) read_key(c);
-      f32x16 x0 = scores([](auto) {});
+      f32x16 x0 = scores([&](auto m_tag) {
+        constexpr int m = decltype(m_tag)::value;
+        if constexpr (m % 18 == 0) copy_begin(1 + m / 18);
+        if constexpr (m % 2 == 1) copy(m % 18 / 2);
+      });
       score_done(x0);
       mask(x0, 0);
       const float top = tile_max(x0);
@@ -353,9 +368,9 @@ __device__ __forceinline__ bool run_piece(const ChunkParams& p, const Piece& pc,
         f32x16 x = scores([&](auto m_tag) {
           constexpr int m = decltype(m_tag)::value;
           if constexpr (m == 1) copy_begin(s + 2);
-          if constexpr (m >= 2 && m < 2 + 2 * kCopies && m % 2 == 0) copy(m / 2 - 1);
+          if constexpr (m % 7 == 2) copy(m / 7);
           if constexpr (m == 22) {
-            wait_lds<5>();   // P is posted; reads of later keys may be on their way
+            wait_lds<7>();   // P is posted; reads of later keys may be on their way
             barrier();       // A
           }
           if constexpr (m == 23) values_begin(s - 1);
@@ -364,6 +379,7 @@ __device__ __forceinline__ bool run_piece(const ChunkParams& p, const Piece& pc,
         });
         values([&](auto i_tag) {
           constexpr int i = decltype(i_tag)::value;
+          if constexpr (i % 6 == 1 && i < 20) copy(5 + i / 6);
           if constexpr (i == 2) {
             asm("s_nop 7" : "+v"(x));
             mask(x, s);
@@ -377,11 +393,10 @@ __device__ __forceinline__ bool run_piece(const ChunkParams& p, const Piece& pc,
             post();
           } else if constexpr (i == 26) {
             read_rope(s + 1);
-          } else if constexpr (i == 27) {
             scores_begin(s + 1);
-          } else if constexpr (i > 28) {
-            read_key(2 * (i - 29));
-            read_key(2 * (i - 29) + 1);
+          } else if constexpr (i > 26 && i < 31) {
+            read_key(2 * (i - 27));
+            read_key(2 * (i - 27) + 1);
           }
         });
       }
@@ -398,82 +413,123 @@ __device__ __forceinline__ bool run_piece(const ChunkParams& p, const Piece& pc,
   }
 
   // ---- output ----
-  if (hl == 0 && !pass.careful) lds.top[32 * wave + l32] = mtrue;
-  if (any_of(!pass.careful && __any(mtrue > mref + kHeadroom))) return true;
-  {
-    {
-      lsum = half_sum(lsum);
-      agpr_settle();
-      if (hl == 0) lds.stat[wave * 32 + l32] = (int64_t)lim >= pages.bad * (int64_t)kPage ? __builtin_nanf("") : lsum;
-      __syncthreads();
-      const bool mine_too = 32 * wave + l32 < rows && lim >= pass.from && lim < pass.to;
-      if (hl == 0 && mine_too) {
-        const float sum = lds.stat[32 * wave + l32];
-        const float lse2 = sum == 0.f ? kNegInf : mref + __log2f(sum);
-        if (pc.slot >= 0) {
-          p.part_lse[(int64_t)pc.slot * kRows + 32 * wave + l32] = lse2;
-        } else if (p.lse != nullptr) {
-          const int r = pc.row0 + 32 * wave + l32;
-          const int token = fast_div(r, p.hdiv), head = r - token * p.H;
-          p.lse[(int64_t)(pc.s.q0 + token) * p.H + head] = lse2 * kLn2;
+  lsum = half_sum(lsum);
+  if (hl == 0) {
+    if (!pass.careful) lds.top[32 * wave + l32] = mtrue;
+    lds.stat[wave * 32 + l32] = (int64_t)lim >= pages.bad * (int64_t)kPage ? __builtin_nanf("") : lsum;
+  }
+  bool wrong = !pass.careful && mtrue > mref + kHeadroom;
+  agpr_settle();
+  wait_vm<0>();
+  wait_lds();
+  __syncthreads();   // the keys' memory is free, the sums are posted
+  auto written = [&](int row) {
+    bool w = row < rows;
+    if (pass.careful) {
+      const int l = limit_of(row);
+      w = w && l >= pass.from && l < pass.to;
+    }
+    return w;
+  };
+  auto place = [&](int row, int64_t st, int64_t sh) {   // of a row in o
+    const int r = pc.row0 + row, token = fast_div(r, p.hdiv);
+    return (pc.s.q0 + token) * st + (r - token * p.H) * sh;
+  };
+  if (hl == 0 && written(32 * wave + l32)) {
+    const float sum = lds.stat[32 * wave + l32];
+    const float lse2 = sum == 0.f ? kNegInf : mref + __log2f(sum);
+    if (pc.slot >= 0) p.part_lse[(int64_t)pc.slot * kRows + 32 * wave + l32] = lse2;
+    else if (p.lse != nullptr) p.lse[place(32 * wave + l32, p.H, 1)] = lse2 * kLn2;
+  }
+  // Through LDS, so that a store covers whole lines: 256 bytes of each of 4 rows, or of a part 512 bytes of each of 2.
+  // A wave has its own memory there.
+  float check = 0.f;   // the largest output
+  auto look = [&](float a, float b) { asm("v_maximum3_f32 %0, |%1|, |%2|, %0" : "+v"(check) : "v"(a), "v"(b)); };
+  auto inverse = [&](int n) {
+    const float sum = lds.stat[32 * n + l32];
+    return sum == 0.f ? 0.f : 1.f / sum;
+  };
+  if (pc.slot < 0) {
+    if (next[2] > 0) copy_queries<0, kQueryEarly>(p, lds, wave, uniform(next[0]), uniform(next[1]), uniform(next[2]));
+    // Rows of 256 bytes, 16-byte unit u of row r at u ^ (r % 16), 32 rows at a time in the last slot.
+    const unsigned mine = lds.keys + 3 * kKeyBytes + wave * 8192;
+    const unsigned put = lds_sum(256 * l32 + 16 * ((2 * hl) ^ (l32 & 15)), mine);
+    const int g = lane >> 4, c = lane & 15;
+    const unsigned get = lds_sum(256 * g + 16 * (c ^ g), mine);   // 8 columns of row g
+    // Where rows follow each other evenly (contiguous outputs), offsets from the first one need no division.
+    const bool even = p.o_st == p.H * p.o_sh && p.o_sh < (1 << 20);
+    const int out_step = (int)p.o_sh;
+    bf16* first = p.o + pc.s.q0 * p.o_st + pc.row0 * p.o_sh + 128 * wave + (g * out_step + 8 * c);
+    const bool plain = even && rows == kRows && !pass.careful;
+#pragma unroll
+    for (int n = 0; n < kRowBlocks; ++n) {
+      if (32 * n >= rows) break;
+      const float inv = inverse(n);
+#pragma unroll
+      for (int j = 0; j < kColBlocks; ++j)
+#pragma unroll
+        for (int d = 0; d < 2; ++d) {
+          bf16x8 v;
+#pragma unroll
+          for (int i = 0; i < 8; i += 2) {
+            const float a = agpr_read(acc[n][j][8 * d + i]) * inv, b = agpr_read(acc[n][j][8 * d + i + 1]) * inv;
+            look(a, b);
+            v[i] = (bf16)a;
+            v[i + 1] = (bf16)b;
+          }
+          *lds_ptr<bf16x8>(put ^ (16 * (4 * j + d))) = v;
+        }
+      bf16x8 v[8];   // row 4 r + g
+#pragma unroll
+      for (int r = 0; r < 8; ++r) v[r] = *lds_ptr<const bf16x8>((get ^ (64 * (r & 3))) + 1024 * r);
+      if (plain) {
+#pragma unroll
+        for (int r = 0; r < 8; ++r) *reinterpret_cast<bf16x8*>(first + (32 * n + 4 * r) * out_step) = v[r];
+      } else {
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          const int row = 32 * n + 4 * r + g;
+          if (!written(row)) continue;
+          if (even) *reinterpret_cast<bf16x8*>(first + (32 * n + 4 * r) * out_step) = v[r];
+          else *reinterpret_cast<bf16x8*>(p.o + place(row, p.o_st, p.o_sh) + 128 * wave + 8 * c) = v[r];
         }
       }
-      // Through LDS, 32 rows at a time, so that a store covers whole lines: 256 bytes of each of 4 rows, or of a part
-      // 512 bytes of each of 2.  16-byte unit u of row r lies at u ^ r.
-      const unsigned mine = lds.keys + wave * 16 * 1024;
-      const int g = lane >> 4, c = lane & 15;
-      const unsigned put = lds_sum(512 * l32 + 16 * ((4 * hl) ^ l32), mine);
-      const unsigned get16 = lds_sum(512 * g + 16 * ((2 * c) ^ g), mine);   // 8 columns of row g: this unit and the one beside it
-      const unsigned get32 = lds_sum(512 * hl + 16 * (l32 ^ hl), mine);     // 4 columns of row hl
-      float check = 0.f;   // not a number where an output is none, or infinite
-      auto written = [&](int row) {
-        const int l = limit_of(row);
-        return row < rows && l >= pass.from && l < pass.to;
-      };
+    }
+  } else {
+    // Rows of 512 bytes, 16-byte unit u of row r at u ^ r.
+    const unsigned mine = lds.keys + wave * kKeyBytes;
+    const unsigned put = lds_sum(512 * l32 + 16 * ((4 * hl) ^ l32), mine);
+    const unsigned get = lds_sum(512 * hl + 16 * (l32 ^ hl), mine);     // 4 columns of row hl
+    float* part = p.part_o + (int64_t)pc.slot * kRows * kDv + 128 * wave;
 #pragma unroll
-      for (int n = 0; n < kRowBlocks; ++n) {
-        if (32 * n >= rows) break;
-        const float sum = lds.stat[32 * n + l32];
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    for (int n = 0; n < kRowBlocks; ++n) {
+      if (32 * n >= rows) break;
+      const float inv = inverse(n);
 #pragma unroll
-        for (int j = 0; j < kColBlocks; ++j)
+      for (int j = 0; j < kColBlocks; ++j)
 #pragma unroll
-          for (int d = 0; d < 4; ++d) {
-            f32x4 v;
+        for (int d = 0; d < 4; ++d) {
+          f32x4 v;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = agpr_read(acc[n][j][4 * d + i]) * inv;
-            *lds_ptr<f32x4>(put ^ (16 * (8 * j + d))) = v;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) check = __builtin_fmaf(v[i], 0.f, check);
-          }
-        if (pc.slot < 0) {
-#pragma unroll
-          for (int r = 0; r < 8; ++r) {   // row 4 r + g
-            const f32x4 a = *lds_ptr<const f32x4>((get16 ^ (64 * r)) + 2048 * r), b = *lds_ptr<const f32x4>((get16 ^ (64 * r) ^ 16) + 2048 * r);
-            const int row = 32 * n + 4 * r + g;
-            if (!written(row)) continue;
-            const int token = fast_div(pc.row0 + row, p.hdiv), head = pc.row0 + row - token * p.H;
-            bf16x8 v;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              v[i] = (bf16)a[i];
-              v[4 + i] = (bf16)b[i];
-            }
-            *reinterpret_cast<bf16x8*>(p.o + (pc.s.q0 + token) * p.o_st + head * p.o_sh + 128 * wave + 8 * c) = v;
-          }
-        } else {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {   // row 2 r + hl
-            const f32x4 a = *lds_ptr<const f32x4>((get32 ^ (32 * r)) + 1024 * r);
-            const int row = 32 * n + 2 * r + hl;
-            if (written(row))
-              *reinterpret_cast<f32x4*>(p.part_o + ((int64_t)pc.slot * kRows + row) * kDv + 128 * wave + 4 * l32) = a;
-          }
+          for (int i = 0; i < 4; ++i) v[i] = agpr_read(acc[n][j][4 * d + i]) * inv;
+          look(v[0], v[1]);
+          look(v[2], v[3]);
+          *lds_ptr<f32x4>(put ^ (16 * (8 * j + d))) = v;
         }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {   // row 2 r + hl
+        const f32x4 v = *lds_ptr<const f32x4>((get ^ (32 * r)) + 1024 * r);
+        const int row = 32 * n + 2 * r + hl;
+        if (written(row)) *reinterpret_cast<f32x4*>(part + row * kDv + 4 * l32) = v;
       }
-      return any_of(__any(check != check));
     }
   }
+  wrong = wrong || !(check < __builtin_inff());
+  wait_lds();
+  if (lane == 0) lds.flag[wave] = 0;
+  if (__any(wrong)) lds.flag[wave] = 1;
+  __syncthreads();   // the keys' memory is free
+  return uniform(lds.flag[0] | lds.flag[1] | lds.flag[2] | lds.flag[3]) != 0;
 }
 
 // The next rows to run the careful way, from the limit `from` on: up to a later token whose latents are not all finite.
@@ -510,14 +566,16 @@ __device__ __forceinline__ Pass careful_pass(const ChunkParams& p, const Piece& 
 // tiles of a sequence whose first query is token `base` (row tile i ends at token base + 128 (i + 1) / H, causal).
 // A range's end is the next one's start by the same arithmetic, so nothing is lost or done twice where they are off.
 constexpr int kCost = 8;
-constexpr int kMinWidth = 16;   // of a range
-constexpr int kSnap = 3;        // a cut this near to a row tile's end moves there
+constexpr int kMinWidth = 6;    // of a range
+constexpr int kSnap = 8;        // a cut this near to a row tile's end moves there, or a quarter of a range's width
 
+constexpr int kPieceInts = 12;
 struct Window {   // the sequences of 256 at a time, and what the threads share
   int q0[kThreads], n[kThreads], len[kThreads];
   int64_t tmp[kWaves];
   int at[4];
   int64_t rest[2];
+  int piece[2 * kPieceInts];
 };
 
 __device__ __forceinline__ int row_tiles(const ChunkParams& p, const Sequence& s) { return (s.n * p.H + kRows - 1) / kRows; }
@@ -539,7 +597,7 @@ struct Place {   // in the row tiles and key tiles of all sequences
 };
 
 // The place at weight y of sequence b.
-__device__ __forceinline__ Place place_of(const ChunkParams& p, int b, const Sequence& s, int64_t y) {
+__device__ __forceinline__ Place place_of(const ChunkParams& p, int b, const Sequence& s, int64_t y, int snap) {
   int lo = 0, hi = row_tiles(p, s) - 1;   // the last row tile that begins at or before y
   const int64_t w = base_weight(p, s) * p.H, x = (y + 1) * p.H;
   while (lo < hi) {
@@ -548,8 +606,8 @@ __device__ __forceinline__ Place place_of(const ChunkParams& p, int b, const Seq
   }
   const int nt = key_tiles(p, s, lo);
   int t = (int)min((int64_t)nt, max((int64_t)0, y - weight(p, s, lo) - kCost));
-  if (t < kSnap) t = 0;
-  if (t > 0 && nt - t < kSnap) return Place{b, lo + 1, 0};
+  if (t <= snap) t = 0;
+  if (t > 0 && nt - t <= snap) return Place{b, lo + 1, 0};
   return Place{b, lo, t};
 }
 
@@ -652,22 +710,29 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_kernel(ChunkParams p) {
   };
   Sequence s = sequence_at(b_last);
   // The end of the last sequence's work is its last row tile's.
-  Place end = place_of(p, b_last, s, y1);
+  const int snap = (int)min((int64_t)kSnap, width / 4);
+  Place end = place_of(p, b_last, s, y1, snap);
   if (y1 >= weight(p, s, row_tiles(p, s))) end = Place{b_last, row_tiles(p, s), 0};
   s = sequence_at(b_first);
-  Place at = place_of(p, b_first, s, y0);
+  Place at = place_of(p, b_first, s, y0, snap);
   end.rt = uniform(end.rt); end.t = uniform(end.t);
   at.rt = uniform(at.rt); at.t = uniform(at.t);
   RangeLink link = make_int4(0, 0, 0, 0);
-  while (at.b < end.b || (at.b == end.b && (at.rt < end.rt || (at.rt == end.rt && at.t < end.t)))) {
-    if (at.rt >= row_tiles(p, s)) {   // the next sequence with queries: 256 looked at together
+  // The piece at `at`, which moves on; none: rows 0.
+  auto piece = [&](DMLA_LDS int* to) {
+    for (;;) {
+      if (!(at.b < end.b || (at.b == end.b && (at.rt < end.rt || (at.rt == end.rt && at.t < end.t))))) {
+        if (tid == 0) to[2] = 0;
+        return;
+      }
+      if (at.rt < row_tiles(p, s)) break;
+      // The next sequence with queries: 256 looked at together.
       int b = at.b + 1;
       for (;; b = window + kThreads) {
         if (b >= window + kThreads) {
           load_window(b);
           __syncthreads();
         }
-        // (b - window < 256) the first sequence from b on in the window that has queries
         int found = kThreads;
         for (int i0 = (b - window) & ~63; i0 < kThreads; i0 += 64) {
           const unsigned long long m = __ballot(i0 + lane >= b - window && win.n[i0 + lane] > 0);
@@ -683,30 +748,59 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_kernel(ChunkParams p) {
       }
       at = Place{uniform(b), 0, 0};
       s = known(at.b);
-      continue;
     }
-    const int nt = key_tiles(p, s, at.rt);
-    Piece pc;
-    pc.s = s;
-    pc.b = at.b;
-    pc.row0 = at.rt * kRows;
-    pc.t0 = at.t;
+    const int nt = key_tiles(p, s, at.rt), row0 = at.rt * kRows, rows = min(s.n * p.H - row0, kRows);
     const bool whole = !(at.b == end.b && at.rt == end.rt);   // to its end
-    pc.t1 = whole ? nt : min(end.t, nt);
-    pc.slot = at.t > 0 ? 2 * range : whole ? -1 : 2 * range + 1;
+    const int slot = at.t > 0 ? 2 * range : whole ? -1 : 2 * range + 1;
     if (at.t > 0) link.w = whole ? 1 : 2;
-    else if (!whole) link = make_int4(min(s.n * p.H - pc.row0, kRows), s.q0, pc.row0, link.w);
+    else if (!whole) link = make_int4(rows, s.q0, row0, link.w);
+    if (tid == 0) {
+      to[0] = s.q0;
+      to[1] = row0;
+      to[2] = rows;
+      to[3] = s.n;
+      to[4] = s.len;
+      to[5] = at.b;
+      to[6] = at.t;
+      to[7] = whole ? nt : min(end.t, nt);
+      to[8] = slot;
+    }
+    if (whole) {
+      ++at.rt;
+      at.t = 0;
+    } else {
+      at = end;
+    }
+  };
+  DMLA_LDS int* pieces = (DMLA_LDS int*)win.piece;
+  piece(pieces);
+  bool have = false;
+  for (int turn = 0;; turn ^= 1) {
+    DMLA_LDS int* now = pieces + turn * kPieceInts;
+    DMLA_LDS int* next = pieces + (turn ^ 1) * kPieceInts;
+    __syncthreads();   // this piece is known, the one before it is read
+    if (uniform(now[2]) == 0) break;
+    Piece pc;
+    pc.s = Sequence{uniform(now[0]), uniform(now[3]), uniform(now[4])};
+    pc.row0 = uniform(now[1]);
+    pc.b = uniform(now[5]);
+    pc.t0 = uniform(now[6]);
+    pc.t1 = uniform(now[7]);
+    pc.slot = uniform(now[8]);
+    piece(next);
     Pass pass = {false, (int)0x80000000, 0x7fffffff};
-    while (run_piece(p, pc, lds, pass) || (pass.careful && pass.to != 0x7fffffff)) {
+    bool again = run_piece(p, pc, lds, pass, have, next);
+    have = pc.slot < 0;
+    while (again || (pass.careful && pass.to != 0x7fffffff)) {
       if (pass.careful && pass.to == 0x7fffffff) break;
       const int base = pc.s.len - pc.s.n, last = min(pc.row0 + kRows, pc.s.n * p.H) - 1;
       const int first_lim = p.causal ? base + fast_div(pc.row0, p.hdiv) : pc.s.len - 1;
       const int last_lim = p.causal ? base + fast_div(last, p.hdiv) : pc.s.len - 1;
       pass = careful_pass(p, pc, lds, pass.careful ? pass.to : first_lim, last_lim);
+      wait_vm<0>();   // the next piece's queries, which are copied once more
+      __syncthreads();
+      again = run_piece(p, pc, lds, pass, false, next);
     }
-    if (!whole) break;
-    ++at.rt;
-    at.t = 0;
   }
   if (tid == 0) p.links[range] = link;
 }
