@@ -128,21 +128,25 @@ __device__ __forceinline__ unsigned query_block(const Lds& lds, int wave, int i)
   if (i < kQueryEarly + 2) return lds.keys + 3 * kKeyBytes + (wave * 2 + i - kQueryEarly) * kQueryBlock;
   return lds.rope + 2 * kRopeBytes + wave * kQueryBlock;
 }
+// This lane's place in rows 8 g .. 8 g + 7 of them.
+__device__ __forceinline__ const bf16* query_rows(const ChunkParams& p, int wave, int q0, int row0, int rows, int g) {
+  const int ln = fresh_lane_id();
+  const int r = row0 + min(32 * wave + 8 * g + (ln >> 3), rows - 1);
+  const int token = fast_div(r, p.hdiv), head = r - token * p.H;
+  return p.q + (q0 + token) * p.q_st + head * p.q_sh + 8 * ((ln & 7) ^ (ln >> 3));
+}
 template <int kFirst, int kN>
 __device__ __forceinline__ void copy_queries(const ChunkParams& p, const Lds& lds, int wave, int q0, int row0, int rows) {
-  const int ln = fresh_lane_id();
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
-    const int r = row0 + min(32 * wave + 8 * g + (ln >> 3), rows - 1);
-    const int token = fast_div(r, p.hdiv), head = r - token * p.H;
-    const bf16* src = p.q + (q0 + token) * p.q_st + head * p.q_sh + 8 * ((ln & 7) ^ (ln >> 3));
+    const bf16* src = query_rows(p, wave, q0, row0, rows, g);
 #pragma unroll
     for (int i = kFirst; i < kFirst + kN; ++i) dma16_addr(src + 64 * i, query_block(lds, wave, i) + g * 1024);
   }
 }
 
 // Whether another pass has to follow.
-// have: the first queries are on their way.  After it, those of the next piece's rows are (next_rows > 0).
+// have: the queries are on their way.  After it, those of the next piece's rows are.
 __device__ __forceinline__ bool run_piece(const ChunkParams& p, const Piece& pc, const Lds& lds, const Pass& pass, bool have,
                                           const DMLA_LDS int* next) {
   const int lane = fresh_lane_id();
@@ -201,8 +205,7 @@ __device__ __forceinline__ bool run_piece(const ChunkParams& p, const Piece& pc,
       for (int c = 0; c < 4; ++c) q[4 * i + c] = *lds_ptr<const bf16x8>(a ^ (32 * c));
     }
   };
-  if (!have) copy_queries<0, kQueryEarly>(p, lds, wave, pc.s.q0, pc.row0, rows);
-  copy_queries<kQueryEarly, 3>(p, lds, wave, pc.s.q0, pc.row0, rows);
+  if (!have) copy_queries<0, 9>(p, lds, wave, pc.s.q0, pc.row0, rows);
   pages.fetch(p, pc, pc.t0 / 2);
   wait_vm<0>();
   using std::integral_constant;
@@ -450,7 +453,9 @@ __device__ __forceinline__ bool run_piece(const ChunkParams& p, const Piece& pc,
     return sum == 0.f ? 0.f : 1.f / sum;
   };
   if (pc.slot < 0) {
-    if (next[2] > 0) copy_queries<0, kQueryEarly>(p, lds, wave, uniform(next[0]), uniform(next[1]), uniform(next[2]));
+    // The next piece's queries are asked for between the conversions, a copy every other 16 values: in one go they
+    // would wait for each other (24 of them 3600 cycles).
+    const int next_q0 = uniform(next[0]), next_row0 = uniform(next[1]), next_rows = uniform(next[2]);
     // Rows of 256 bytes, 16-byte unit u of row r at u ^ (r % 16), 32 rows at a time in the last slot.
     const unsigned mine = lds.keys + 3 * kKeyBytes + wave * 8192;
     const unsigned put = lds_sum(256 * l32 + 16 * ((2 * hl) ^ (l32 & 15)), mine);
@@ -463,12 +468,22 @@ __device__ __forceinline__ bool run_piece(const ChunkParams& p, const Piece& pc,
     const bool plain = even && rows == kRows && !pass.careful;
 #pragma unroll
     for (int n = 0; n < kRowBlocks; ++n) {
-      if (32 * n >= rows) break;
+      const bf16* src = nullptr;
+      if (next_rows > 0) src = query_rows(p, wave, next_q0, next_row0, next_rows, n);
+      auto ask = [&](int i) {
+        if (next_rows > 0 && i < kQueryEarly) dma16_addr(src + 64 * i, query_block(lds, wave, i) + n * 1024);
+      };
+      if (32 * n >= rows) {   // no rows there
+#pragma unroll
+        for (int i = 0; i < kQueryEarly; ++i) ask(i);
+        continue;
+      }
       const float inv = inverse(n);
 #pragma unroll
       for (int j = 0; j < kColBlocks; ++j)
 #pragma unroll
         for (int d = 0; d < 2; ++d) {
+          ask(2 * j + d);
           bf16x8 v;
 #pragma unroll
           for (int i = 0; i < 8; i += 2) {
@@ -529,6 +544,12 @@ __device__ __forceinline__ bool run_piece(const ChunkParams& p, const Piece& pc,
   if (lane == 0) lds.flag[wave] = 0;
   if (__any(wrong)) lds.flag[wave] = 1;
   __syncthreads();   // the keys' memory is free
+  // The rest of the next queries, while the piece after that is worked out.
+  const int next_q0 = uniform(next[0]), next_row0 = uniform(next[1]), next_rows = uniform(next[2]);
+  if (next_rows > 0) {
+    if (pc.slot >= 0) copy_queries<0, kQueryEarly>(p, lds, wave, next_q0, next_row0, next_rows);
+    copy_queries<kQueryEarly, 3>(p, lds, wave, next_q0, next_row0, next_rows);
+  }
   return uniform(lds.flag[0] | lds.flag[1] | lds.flag[2] | lds.flag[3]) != 0;
 }
 
@@ -790,7 +811,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_kernel(ChunkParams p) {
     piece(next);
     Pass pass = {false, (int)0x80000000, 0x7fffffff};
     bool again = run_piece(p, pc, lds, pass, have, next);
-    have = pc.slot < 0;
+    have = true;
     while (again || (pass.careful && pass.to != 0x7fffffff)) {
       if (pass.careful && pass.to == 0x7fffffff) break;
       const int base = pc.s.len - pc.s.n, last = min(pc.row0 + kRows, pc.s.n * p.H) - 1;
