@@ -827,12 +827,30 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_kernel(ChunkParams p) {
 }
 
 // Row tiles that span ranges: o = sum_j w_j o_j / sum_j w_j with w_j = 2^(lse_j - max); and the queries behind the last
-// sequence.  Four rows per workgroup, one a wave.
+// sequence.  32 workgroups per range.  Of a row tile with few parts those of its first range take four rows each, one a
+// wave.  With kManyParts and more, those of the ranges that it fills whole (which begin no row tile) help: a
+// workgroup takes a row, its waves every fourth part (one sequence of 100000 tokens x 16 heads, 256 parts: 52 -> 9 us).
+constexpr int kManyParts = 8;
+static_assert((kManyParts - 1) * (kRows / 4) >= kRows, "a workgroup per row");
 __global__ __launch_bounds__(256) void chunk_combine_kernel(ChunkParams p) {
+  __shared__ f32x4 sums[4][2][64];
+  __shared__ float s_sum[4];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-  const int range = (int)blockIdx.x / (kRows / 4), row = 4 * ((int)blockIdx.x % (kRows / 4)) + wave;
-  const RangeLink link = range < p.n_ranges ? p.links[range] : make_int4(0, 0, 0, 0);
-  if (row < link.x) {
+  const int mine = (int)blockIdx.x / (kRows / 4), index = (int)blockIdx.x % (kRows / 4);
+  RangeLink link = mine < p.n_ranges ? p.links[mine] : make_int4(0, 0, 0, 0);
+  int range = mine;   // where the row tile begins
+  if (link.x == 0 && link.w == 2) {
+    for (int r0 = mine - 1; r0 >= 0; r0 -= 64) {
+      const int x = r0 - lane >= 0 ? p.links[r0 - lane].x : 0;
+      const unsigned long long begins = __ballot(x > 0);
+      if (begins != 0) {
+        range = r0 - __builtin_ctzll(begins);
+        link = p.links[range];
+        break;
+      }
+    }
+  }
+  if (link.x > 0) {
     // Its parts: the range's last, then those that the next ranges begin with, up to one that ends there.
     int parts = 1;
     for (int r0 = range + 1;; r0 += 64) {
@@ -841,51 +859,69 @@ __global__ __launch_bounds__(256) void chunk_combine_kernel(ChunkParams p) {
       parts += ends != 0 ? __builtin_ctzll(ends) + 1 : 64;
       if (ends != 0) break;
     }
-    auto slot = [&](int j) { return (int64_t)(j == 0 ? 2 * range + 1 : 2 * (range + j)); };
-    float top = kNegInf;
-    bool none = true;   // no number among them
-    for (int j0 = 0; j0 < parts; j0 += 64) {
-      const float l = j0 + lane < parts ? p.part_lse[slot(j0 + lane) * kRows + row] : kNegInf;
-      top = fmaxf(top, l);
-      none = none && l == l;
-    }
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-    const bool number = __all(none);
-    float sum = 0.f;
-    f32x4 a0 = {0.f, 0.f, 0.f, 0.f}, a1 = a0;
-    for (int j0 = 0; j0 < parts; j0 += 4) {
-      f32x4 v0[4], v1[4];
-      float l[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int64_t at = slot(min(j0 + i, parts - 1)) * kRows + row;
-        l[i] = p.part_lse[at];
-        v0[i] = *reinterpret_cast<const f32x4*>(p.part_o + at * kDv + 8 * lane);
-        v1[i] = *reinterpret_cast<const f32x4*>(p.part_o + at * kDv + 8 * lane + 4);
+    const bool many = parts >= kManyParts;
+    const int row = many ? (mine - range) * (kRows / 4) + index : mine == range ? 4 * index + wave : kRows;
+    if (row < link.x) {   // (with many parts the same for all waves)
+      const int first = many ? wave : 0, step = many ? 4 : 1;
+      auto place = [&](int j) { return (int64_t)(j == 0 ? 2 * range + 1 : 2 * (range + j)) * kRows + row; };
+      float top = kNegInf;
+      bool odd = false;   // not a number among them
+      for (int j0 = 0; j0 < parts; j0 += 64) {
+        const float l = j0 + lane < parts ? p.part_lse[place(j0 + lane)] : kNegInf;
+        top = fmaxf(top, l);
+        odd = odd || l != l;
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (j0 + i >= parts) break;
-        const float w = top == kNegInf ? 0.f : fast_exp2(l[i] - top);
-        if (w == 0.f) continue;   // a part without a weight adds nothing, whatever it holds
-        sum += w;
-        a0 += w * v0[i];
-        a1 += w * v1[i];
+      for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+      odd = __any(odd);
+      float sum = 0.f;
+      f32x4 a0 = {0.f, 0.f, 0.f, 0.f}, a1 = a0;
+      constexpr int kBatch = 8;   // parts in flight
+      for (int j0 = first; j0 < parts; j0 += kBatch * step) {
+        f32x4 v0[kBatch], v1[kBatch];
+        float l[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          const int64_t at = place(min(j0 + i * step, parts - 1));
+          l[i] = p.part_lse[at];
+          v0[i] = *reinterpret_cast<const f32x4*>(p.part_o + at * kDv + 8 * lane);
+          v1[i] = *reinterpret_cast<const f32x4*>(p.part_o + at * kDv + 8 * lane + 4);
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          if (j0 + i * step >= parts) break;
+          const float w = top == kNegInf ? 0.f : fast_exp2(l[i] - top);
+          if (w == 0.f) continue;   // a part without a weight adds nothing, whatever it holds
+          sum += w;
+          a0 += w * v0[i];
+          a1 += w * v1[i];
+        }
+      }
+      if (many) {
+        sums[wave][0][lane] = a0;
+        sums[wave][1][lane] = a1;
+        if (lane == 0) s_sum[wave] = sum;
+        __syncthreads();
+        sum = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
+        a0 = sums[0][0][lane] + sums[1][0][lane] + sums[2][0][lane] + sums[3][0][lane];
+        a1 = sums[0][1][lane] + sums[1][1][lane] + sums[2][1][lane] + sums[3][1][lane];
+      }
+      if (!many || wave == 0) {
+        const float inv = odd ? __builtin_nanf("") : sum > 0.f ? 1.f / sum : 0.f;
+        bf16x8 v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          v[i] = (bf16)(a0[i] * inv);
+          v[4 + i] = (bf16)(a1[i] * inv);
+        }
+        const int r = link.z + row;
+        const int token = fast_div(r, p.hdiv), head = r - token * p.H;
+        *reinterpret_cast<bf16x8*>(p.o + (link.y + token) * p.o_st + head * p.o_sh + 8 * lane) = v;
+        if (lane == 0 && p.lse != nullptr)
+          p.lse[(int64_t)(link.y + token) * p.H + head] =
+              odd ? __builtin_nanf("") : sum > 0.f ? (top + __log2f(sum)) * kLn2 : kNegInf;
       }
     }
-    const float inv = !number ? __builtin_nanf("") : sum > 0.f ? 1.f / sum : 0.f;
-    bf16x8 v;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[i] = (bf16)(a0[i] * inv);
-      v[4 + i] = (bf16)(a1[i] * inv);
-    }
-    const int r = link.z + row;
-    const int token = link.y + fast_div(r, p.hdiv), head = r - (token - link.y) * p.H;
-    *reinterpret_cast<bf16x8*>(p.o + token * p.o_st + head * p.o_sh + 8 * lane) = v;
-    if (lane == 0 && p.lse != nullptr)
-      p.lse[(int64_t)token * p.H + head] = !number ? __builtin_nanf("") : sum > 0.f ? (top + __log2f(sum)) * kLn2 : kNegInf;
   }
   const int behind = p.cu == nullptr ? p.T : p.B == 0 ? 0 : min(max(p.cu[p.B], 0), p.T);
   const int64_t total = (int64_t)(p.T - behind) * p.H;
