@@ -110,168 +110,240 @@ struct ScoreArgs {
   int H, num_pages;
   int blocks, passes;   // 16-row blocks of a query (at most kBlocks of a pass), passes over the heads
   int group;            // queries of a workgroup
-  int chunk, chunks;    // pages of a workgroup, a multiple of 64
+  int chunk, chunks;    // pages of a workgroup, a multiple of kTile
   float scale_log2;
 };
 
-constexpr int kBlocks = 8;                      // 16-row blocks in LDS: 128 rows (query, head), heads padded to 16
-constexpr int kRowBytes = 2 * kD + 16;          // 16 rows at one place of a row lie in different banks
 constexpr int kScoreThreads = 256, kScoreWaves = 4;
+constexpr int kBlocks = 8;                                // 16-row blocks of a workgroup, heads padded to 16: two a wave
+constexpr int kTile = 32;                                 // pages of a tile
+constexpr int kSteps = kD / 16, kLatSteps = kLat / 16;    // MFMAs of a tile
+constexpr int kMeanRow = 2 * kLat, kTileBytes = kTile * kMeanRow, kRopeBytes = kTile * 2 * (kD - kLat), kRing = 4;
+constexpr int kCopies = 9;                                // of a wave and tile
+constexpr int kIdTiles = 64;                              // tiles whose table entries are in LDS
+constexpr int kQueryBytes = 32 * 2 * kD;                  // of a wave, in the tiles' memory
+static_assert(kScoreWaves * kQueryBytes == kRing * (kTileBytes + kRopeBytes), "the queries fill it");
 enum { kFused, kStats, kSum };
 
-// kFused: one workgroup has all pages of its queries, their sums first and then the scores.  Else the pages are
-// cut in chunks over workgroups, kStats leaves each chunk's maxima and sums and kSum reads all of them.
-// A wave multiplies 16 pages (in registers) with the rows in LDS, 16x16x32 MFMAs; a lane then holds four heads of
-// a page.  Scores of a page are summed in a fixed order, by one lane.
+// 16-byte unit u of row r of a tile lies at u ^ mean_swz(r): 16 rows' units at one place of a row lie in different banks.
+__device__ __forceinline__ int mean_swz(int r) { return r & 15; }
+
+// kFused: one workgroup has all pages of its queries, their sums first and then the scores.  Else the pages are cut in
+// chunks over workgroups, kStats leaves each chunk's maxima and sums and kSum reads all of them.
+//
+// A wave holds 32 rows (query, head) in registers, as chunk attention does, and tiles of 32 mean rows come through LDS,
+// three tiles ahead.  For the sums over pages the means are the MFMA's rows, so a lane has 16 pages of one head; for
+// the sums over heads they are its columns, so a lane has 16 heads of one page.  Both sums are then in-lane, in a
+// fixed order.
+// Bound: latency (a launch, queries, the first tile); the rates would allow 3 us for the means of 64 sequences of 8192 to
+// 32768 tokens and their queries.  The first version held the queries in LDS, 147 KB for each 64 pages.
 template <int kMode>
-__global__ void __launch_bounds__(kScoreThreads) page_scores_kernel(ScoreArgs a) {
-  extern __shared__ __attribute__((aligned(16))) char smem[];
+__global__ void __launch_bounds__(kScoreThreads, 1) page_scores_kernel(ScoreArgs a) {
+  __shared__ __attribute__((aligned(1024))) char mem[kRing * (kTileBytes + kRopeBytes)];
   __shared__ int s_seq[kBlocks], s_pages[kBlocks];
-  __shared__ float s_lse[16 * kBlocks];
-  __shared__ float2 s_part[kScoreWaves][16 * kBlocks];
+  __shared__ __attribute__((aligned(16))) float s_max[16 * kBlocks], s_inv[16 * kBlocks];
+  __shared__ float s_part[2][kBlocks][kTile];
+  __shared__ int s_ids[kIdTiles * kTile];
+  const unsigned tiles = lds_addr((DMLA_LDS char*)mem), ropes = tiles + kRing * kTileBytes;
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
-  const int l16 = lane & 15, g = lane >> 4;
+  const int l32 = lane & 31, hl = lane >> 5;
   const int t0 = blockIdx.x * a.group, nt = min(a.group, a.qs.T - t0);
   const int c0 = blockIdx.y * a.chunk, c1 = min(c0 + a.chunk, a.qs.max_pages);
-  for (int i = wave; i < nt; i += kScoreWaves) {
-    const int b = sequence_of(a.qs, t0 + i);
-    const int n = visible(a.qs, b, t0 + i);
-    if (lane == 0) {
-      s_seq[i] = b;
-      s_pages[i] = n > 0 ? (n - 1) / kPage : 0;   // pages before its own
-    }
-  }
-  __syncthreads();
-  const int nb = a.passes > 1 ? kBlocks : a.blocks * nt;   // blocks in use
+  const bool multi = a.passes > 1;   // the heads of one query take several passes
+  // Row r of the workgroup: query i, head `head0` + offset.
+  auto query_of = [&](int r) { return multi ? 0 : min((r >> 4) / a.blocks, nt - 1); };
+  auto head_of = [&](int r) { return multi ? r : (((r >> 4) % a.blocks) << 4) + (r & 15); };
   for (int pass = 0; pass < a.passes; ++pass) {
     const int head0 = pass * 16 * kBlocks;
-    if (pass > 0) __syncthreads();   // the rows of the pass before are read
-    for (int k = tid; k < nb * 16 * (kD / 8); k += kScoreThreads) {
-      const int r = k / (kD / 8), c = k - r * (kD / 8);
-      const int i = a.passes > 1 ? 0 : r / (16 * a.blocks);
-      const int head = min(head0 + r - i * 16 * a.blocks, a.H - 1);
-      *reinterpret_cast<bf16x8*>(smem + r * kRowBytes + 16 * c) =
-          *reinterpret_cast<const bf16x8*>(a.q + (t0 + i) * a.q_st + head * a.q_sh + 8 * c);
+    if (pass > 0) __syncthreads();
+    // ---- queries: operand c holds dims 16 c + 8 hl .. of row 32 wave + l32; eight rows x 128 bytes a copy ----
+    const unsigned mine = tiles + wave * kQueryBytes;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int r = 32 * wave + 8 * g + (lane >> 3);
+      const int head = min(head0 + head_of(r), a.H - 1);
+      const bf16* src = a.q + (t0 + query_of(r)) * a.q_st + head * a.q_sh + 8 * ((lane & 7) ^ (lane >> 3));
+#pragma unroll
+      for (int i = 0; i < 9; ++i) dma16_addr(src + 64 * i, mine + (9 * g + i) * 1024);
     }
-    if constexpr (kMode == kSum) {
-      for (int r = tid; r < nb * 16; r += kScoreThreads) {
-        const int i = a.passes > 1 ? 0 : r / (16 * a.blocks);
-        const int head = min(head0 + r - i * 16 * a.blocks, a.H - 1);
-        float m = kNegInf, l = 0.f;
-        for (int c = 0; c < a.chunks; ++c) {
-          const float2 s = a.stats[((int64_t)c * a.qs.T + t0 + i) * a.H + head];
-          const float mm = fmaxf(m, s.x);
-          if (mm != kNegInf) l = l * fast_exp2(m - mm) + s.y * fast_exp2(s.x - mm);
-          else l += s.y;   // 0, or not a number
-          m = mm;
+    if (pass == 0) {
+      for (int i = wave; i < nt; i += kScoreWaves) {
+        const int b = sequence_of(a.qs, t0 + i);
+        const int n = visible(a.qs, b, t0 + i);
+        if (lane == 0) {
+          s_seq[i] = b;
+          s_pages[i] = n > 0 ? (n - 1) / kPage : 0;   // pages before its own
         }
-        s_lse[r] = m == kNegInf ? l : m + __log2f(l);
       }
     }
-    __syncthreads();
+    if constexpr (kMode == kSum) {
+      for (int r = tid; r < 16 * kBlocks; r += kScoreThreads) {
+        const int head = head0 + head_of(r), i = query_of(r);
+        float m = kNegInf, l = 0.f;
+        for (int c = 0; c < a.chunks; ++c) {
+          const float2 s = a.stats[((int64_t)c * a.qs.T + t0 + i) * a.H + min(head, a.H - 1)];
+          const float mm = fmaxf(m, s.x);
+          l = mm == kNegInf ? l + s.y : l * fast_exp2(m - mm) + s.y * fast_exp2(s.x - mm);   // (0 or not a number)
+          m = mm;
+        }
+        // (m and 1 / l apart: their product's logarithm would lose the digits of a large m.)
+        const bool head_there = head < a.H;
+        s_max[r] = !head_there ? __builtin_inff() : m == kNegInf ? 0.f : m;
+        s_inv[r] = !head_there || l == 0.f ? 0.f : 1.f / l;
+      }
+    }
+    wait_vm<0>();
+    bf16x8 q[kSteps];
+    {
+      const unsigned at = lds_sum(9 * 1024 * (l32 >> 3) + 128 * (l32 & 7) + 16 * (hl ^ (l32 & 7)), mine);
+#pragma unroll
+      for (int c = 0; c < kSteps; ++c) q[c] = *lds_ptr<const bf16x8>((at ^ (32 * (c & 3))) + 1024 * (c >> 2));
+    }
+    wait_lds();
+    __syncthreads();   // the tiles' memory is free; the queries' pages are known
+
     for (int i0 = 0; i0 < nt;) {   // the queries of one sequence at a time
-      const int b = s_seq[i0];
+      const int b = uniform(s_seq[i0]);
       int i1 = i0 + 1, most = s_pages[i0];
       for (; i1 < nt && s_seq[i1] == b; ++i1) most = max(most, s_pages[i1]);
-      // f(rb, page of this lane, scores of heads 16 (rb % blocks) + 4 g + 0 .. 3, their query): for every row block
-      // of the sequence; -inf where there is nothing.
-      auto tile = [&](int p0, auto f) {
-        const int p = p0 + l16;
-        const int page = p < min(most, c1) ? a.block_table[b * a.bt_sb + p] : -1;
-        const bool there = page >= 0 && page < a.num_pages;
-        const bf16* row = a.means + (there ? page : 0) * a.m_sp + 8 * g;
-        bf16x8 k[kD / 32];
+      i1 = uniform(i1);
+      most = uniform(most);
+      const int n_tiles = max(0, (min(most, c1) - c0 + kTile - 1) / kTile);
+      auto rows_pages = [&](int r) {   // pages of row r's query, 0 where it is of another sequence
+        const int i = query_of(r);
+        return i >= i0 && i < i1 ? s_pages[i] : 0;
+      };
+      // Tiles in order, each through each(s, k, there): operand reader and a bit per page in the pool.
+      auto stream = [&](auto each) {
+        if (n_tiles == 0) return;
+        // Table entries of tiles [s, s + kIdTiles / 2), -1 where there is no page of the pool.
+        auto load_ids = [&](int s) {
+          for (int k = tid; k < kIdTiles / 2 * kTile; k += kScoreThreads) {
+            const int p = c0 + kTile * s + k;
+            const int id = p < min(most, c1) ? a.block_table[b * a.bt_sb + p] : -1;
+            s_ids[(kTile * s + k) % (kTile * kIdTiles)] = id < a.num_pages ? id : -1;
+          }
+        };
+        auto copy = [&](int s) {   // (past the end: the last tile once more, so that the copies count the same)
+          const int t = min(s, n_tiles - 1);
+          const unsigned slot = (unsigned)(s % kRing);
+          const int id = max(s_ids[(kTile * t) % (kTile * kIdTiles) + 8 * wave + (lane >> 3)], 0);   // not there: page 0, masked
 #pragma unroll
-        for (int c = 0; c < kD / 32; ++c) k[c] = *reinterpret_cast<const bf16x8*>(row + 32 * c);
-#pragma unroll
-        for (int rb = 0; rb < kBlocks; ++rb) {
-          const int i = a.passes > 1 ? 0 : rb / a.blocks;
-          if (rb >= nb || i < i0 || i >= i1) continue;
-          f32x4 x = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int c = 0; c < kD / 32; ++c)
-            x = mfma_bf16(*reinterpret_cast<const bf16x8*>(smem + (16 * rb + l16) * kRowBytes + 64 * c + 16 * g), k[c], x);
-          const int head = head0 + 16 * (rb - i * a.blocks) + 4 * g;
-          const bool seen = there && p < s_pages[i];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] = seen && head + e < a.H ? x[e] * a.scale_log2 : kNegInf;
-          f(rb, p, x, i);
+          for (int i = 0; i < 8; ++i) {
+            const int r = 8 * wave + i;
+            dma16(a.means + __builtin_amdgcn_readlane(id, 8 * i) * a.m_sp, 16 * (lane ^ mean_swz(r)), tiles + slot * kTileBytes + r * kMeanRow);
+          }
+          dma16_addr(a.means + id * a.m_sp + kLat + 8 * ((lane & 7) ^ (lane >> 3)), ropes + slot * kRopeBytes + wave * 1024);
+        };
+        load_ids(0);
+        if (n_tiles > kIdTiles / 2) load_ids(kIdTiles / 2);
+        __syncthreads();
+        copy(0);
+        copy(1);
+        copy(2);
+        for (int s = 0; s < n_tiles; ++s) {
+          // Half the entries ahead of their use, into the half that every wave is past.
+          if (s > 1 && s % (kIdTiles / 2) == 1 && s - 1 + kIdTiles / 2 < n_tiles) load_ids(s - 1 + kIdTiles / 2);
+          wait_vm<2 * kCopies>();   // tile s; those of two tiles more may be on their way
+          __syncthreads();          // tile s landed, tile s - 1 is read
+          copy(s + 3);
+          const unsigned key = lds_sum(kMeanRow * l32 + 16 * (hl ^ mean_swz(l32)), tiles + (unsigned)(s % kRing) * kTileBytes);
+          const unsigned rope = lds_sum(128 * l32 + 16 * (hl ^ (l32 & 7)), ropes + (unsigned)(s % kRing) * kRopeBytes);
+          each(s, [&](int c) {
+            return *lds_ptr<const bf16x8>(c < kLatSteps ? (key ^ (32 * (c & 7))) + 256 * (c >> 3) : rope ^ (32 * (c - kLatSteps)));
+          }, (unsigned)__ballot(s_ids[(kTile * s) % (kTile * kIdTiles) + l32] >= 0));
         }
+        wait_vm<0>();
+        __syncthreads();   // the last tile is read, no copy is on its way
+      };
+      // Bit k: page k of tile s is one of the first n of the sequence.
+      auto first_pages = [&](int s, int n) {
+        const int k = n - c0 - kTile * s;
+        return k >= 32 ? ~0u : k <= 0 ? 0u : (1u << k) - 1;
       };
       if constexpr (kMode != kSum) {
-        float m[kBlocks][4], l[kBlocks][4];
+        float m = kNegInf, l = 0.f;   // of row 32 wave + l32
+        const int limit = rows_pages(32 * wave + l32);
+        stream([&](int s, auto k, unsigned there) {
+          f32x16 x = {};
 #pragma unroll
-        for (int rb = 0; rb < kBlocks; ++rb)
+          for (int c = 0; c < kSteps; ++c) x = mfma32_bf16(k(c), q[c], x);
+          const unsigned seen = (there & first_pages(s, limit)) >> (4 * hl);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            m[rb][e] = kNegInf;
-            l[rb][e] = 0.f;
-          }
-        auto merge = [](float& m0, float& l0, float m1, float l1) {
-          const float mm = fmaxf(m0, m1);
-          if (mm != kNegInf) l0 = l0 * fast_exp2(m0 - mm) + l1 * fast_exp2(m1 - mm);
-          else l0 += l1;   // 0, or not a number
-          m0 = mm;
-        };
-        for (int p0 = c0 + 16 * wave; p0 < min(most, c1); p0 += 16 * kScoreWaves)
-          tile(p0, [&](auto rb, int, const f32x4& x, int) {
+          for (int i = 0; i < 16; ++i) x[i] = seen >> (8 * (i >> 2) + (i & 3)) & 1 ? x[i] * a.scale_log2 : kNegInf;
+          float top = x[0];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const bool number = x[e] == x[e];
-              merge(m[rb][e], l[rb][e], number ? x[e] : kNegInf, number ? (x[e] == kNegInf ? 0.f : 1.f) : x[e]);
-            }
-          });
+          for (int i = 1; i < 16; ++i) top = fmaxf(top, x[i]);
+          const float mm = fmaxf(m, half_max(top));
+          const float ms = mm == kNegInf ? 0.f : mm;
+          l = m == mm ? l : l * fast_exp2(m - mm);
+          m = mm;
 #pragma unroll
-        for (int rb = 0; rb < kBlocks; ++rb)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-#pragma unroll
-            for (int o = 1; o < 16; o <<= 1) {
-              const float m1 = __shfl_xor(m[rb][e], o, 64), l1 = __shfl_xor(l[rb][e], o, 64);
-              merge(m[rb][e], l[rb][e], m1, l1);
-            }
-            if (l16 == 0) s_part[wave][16 * rb + 4 * g + e] = make_float2(m[rb][e], l[rb][e]);
-          }
-        __syncthreads();
-        for (int r = tid; r < nb * 16; r += kScoreThreads) {
-          const int i = a.passes > 1 ? 0 : r / (16 * a.blocks);
-          if (i < i0 || i >= i1) continue;
-          float mm = kNegInf, ll = 0.f;
-#pragma unroll
-          for (int w = 0; w < kScoreWaves; ++w) merge(mm, ll, s_part[w][r].x, s_part[w][r].y);
+          for (int i = 0; i < 16; ++i) l += fast_exp2(x[i] - ms);   // (not a number stays)
+        });
+        l = half_sum(l);
+        const int r = 32 * wave + l32, i = query_of(r), head = head0 + head_of(r);
+        // (Rows behind the last query are its rows again.)
+        const bool own = i >= i0 && i < i1 && (multi || (r >> 4) / a.blocks < nt);
+        if (hl == 0 && own) {
           if constexpr (kMode == kStats) {
-            const int head = head0 + r - i * 16 * a.blocks;
-            if (head < a.H) a.stats[((int64_t)blockIdx.y * a.qs.T + t0 + i) * a.H + head] = make_float2(mm, ll);
+            if (head < a.H) a.stats[((int64_t)blockIdx.y * a.qs.T + t0 + i) * a.H + head] = make_float2(m, l);
           } else {
-            s_lse[r] = mm == kNegInf ? ll : mm + __log2f(ll);
+            s_max[r] = head >= a.H ? __builtin_inff() : m == kNegInf ? 0.f : m;
+            s_inv[r] = head >= a.H || l == 0.f ? 0.f : 1.f / l;
           }
         }
         __syncthreads();
       }
       if constexpr (kMode != kStats) {
-        for (int p0 = c0 + 16 * wave; p0 < c1; p0 += 16 * kScoreWaves) {
-          auto put = [&](int i, int p, float v) {
-            if (g != 0 || p >= c1) return;
-            float* to = a.scores + (t0 + i) * a.s_st + p;
-            *to = pass > 0 ? *to + v : v;
-          };
-          if (p0 >= most) {
-            for (int i = i0; i < i1; ++i) put(i, p0 + l16, 0.f);
-            continue;
-          }
-          float sum = 0.f;
-          tile(p0, [&](auto rb, int p, const f32x4& x, int i) {
-            float v = 0.f;
+        // Scores of tile s: the sums of each query's blocks, posted by the waves.
+        auto put = [&](int s) {
+          const int i = tid >> 5, p = c0 + kTile * s + (tid & 31);
+          if (i < i0 || i >= i1 || p >= c1) return;
+          float v = 0.f;
+          const int first = multi ? 0 : i * a.blocks, n = multi ? kBlocks : a.blocks;
+          for (int j = 0; j < n; ++j) v += s_part[s & 1][first + j][tid & 31];
+          float* to = a.scores + (t0 + i) * a.s_st + p;
+          *to = pass > 0 ? *to + v : v;
+        };
+        float mx[16], inv[16];   // of rows 8 (i / 4) + 4 hl + i % 4 of the wave
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (x[e] != kNegInf) v += fast_exp2(x[e] - s_lse[16 * rb + 4 * g + e]);   // (not a number stays)
-            sum += group_sum(v);
-            if (a.passes > 1 ? rb == kBlocks - 1 : (rb + 1) % a.blocks == 0) {
-              put(i, p, sum);
-              sum = 0.f;
-            }
-          });
+        for (int j = 0; j < 4; ++j) {
+          const f32x4 u = *reinterpret_cast<const DMLA_LDS f32x4*>((const DMLA_LDS float*)s_max + 32 * wave + 8 * j + 4 * hl);
+          const f32x4 v = *reinterpret_cast<const DMLA_LDS f32x4*>((const DMLA_LDS float*)s_inv + 32 * wave + 8 * j + 4 * hl);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            mx[4 * j + i] = u[i];
+            inv[4 * j + i] = v[i];
+          }
         }
+        const int limit0 = rows_pages(32 * wave), limit1 = rows_pages(32 * wave + 16);
+        stream([&](int s, auto k, unsigned there) {
+          if (s > 0) put(s - 1);
+          f32x16 x = {};
+#pragma unroll
+          for (int c = 0; c < kSteps; ++c) x = mfma32_bf16(q[c], k(c), x);
+          float v0 = 0.f, v1 = 0.f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            v0 += fast_exp2(__builtin_fmaf(x[i], a.scale_log2, -mx[i])) * inv[i];
+            v1 += fast_exp2(__builtin_fmaf(x[8 + i], a.scale_log2, -mx[8 + i])) * inv[8 + i];
+          }
+          v0 = half_sum(v0);
+          v1 = half_sum(v1);
+          if (hl == 0) {
+            s_part[s & 1][2 * wave][l32] = (there & first_pages(s, limit0)) >> l32 & 1 ? v0 : 0.f;
+            s_part[s & 1][2 * wave + 1][l32] = (there & first_pages(s, limit1)) >> l32 & 1 ? v1 : 0.f;
+          }
+        });
+        if (n_tiles > 0) put(n_tiles - 1);
+        // Behind the last page that any of them sees: zeros.
+        if (pass == 0)
+          for (int s = n_tiles; c0 + kTile * s < c1; ++s) {
+            const int i = tid >> 5, p = c0 + kTile * s + (tid & 31);
+            if (i >= i0 && i < i1 && p < c1) a.scores[(t0 + i) * a.s_st + p] = 0.f;
+          }
+        __syncthreads();   // the last tile's sums are read
       }
       i0 = i1;
     }
@@ -296,8 +368,11 @@ __device__ __forceinline__ unsigned ordered(float x) {
   return x != x ? 0xffffffffu : u >> 31 ? ~u : u | 0x80000000u;
 }
 
-// A query per wave: its candidates' scores in registers (kN of a lane; kN = 0: read again for every bit), the
-// smallest selected one found bit by bit with counts over the wave, then the selected pages in order by ballots.
+// A query per wave: its candidates' scores and table entries in registers (kN of a lane; kN = 0: read again for every bit).
+// The smallest selected score is found bit by bit, from the highest bit in which candidates differ, with counts over
+// the wave, until the candidates at or above are as many as asked for; then the selected pages go out in order, their
+// places from ballots.
+// Bound: latency; a query of 512 pages takes 5 dependent loads and some 15 counts.
 constexpr int kSelectWaves = 4;
 template <int kN>
 __global__ void __launch_bounds__(64 * kSelectWaves) page_select_kernel(SelectArgs a) {
@@ -309,43 +384,74 @@ __global__ void __launch_bounds__(64 * kSelectWaves) page_select_kernel(SelectAr
   const int n = (seen + kPage - 1) / kPage;
   const int c0 = min(a.sink, n), c1 = max(c0, n - a.recent);   // candidates
   const bool all = n <= a.k;
-  int left = a.k - a.sink - a.recent;                          // of them to select
+  const int left = a.k - a.sink - a.recent;                    // of them to select
   const float* row = a.scores + t * a.s_st;
+  const int32_t* entries = a.block_table + b * a.bt_sb;
   unsigned key[kN > 0 ? kN : 1];
-  auto load = [&](int i) {
+  int entry[kN > 0 ? kN : 1];
+  auto load = [&](int i) {   // 0: no candidate
     const int p = 64 * i + lane;
     return p >= c0 && p < c1 ? ordered(row[p]) : 0u;
   };
   const int steps = (n + 63) / 64;
   if constexpr (kN > 0) {
 #pragma unroll
-    for (int i = 0; i < kN; ++i) key[i] = all ? 0u : load(i);
+    for (int i = 0; i < kN; ++i) {
+      const int p = 64 * i + lane;
+      entry[i] = p < n ? entries[p] : 0;
+      key[i] = all ? 0u : load(i);
+    }
   }
-  auto count = [&](auto test) {   // over the candidates
-    int c = 0;
+  auto over = [&](auto f) {   // the candidates' keys of this lane
     if constexpr (kN > 0) {
 #pragma unroll
-      for (int i = 0; i < kN; ++i) c += __popcll(__ballot(test(key[i])));
+      for (int i = 0; i < kN; ++i) f(key[i]);
     } else {
-      for (int i = 0; i < steps; ++i) c += __popcll(__ballot(test(load(i))));
+      for (int i = 0; i < steps; ++i) f(load(i));
     }
-    return c;
   };
-  unsigned least = 0xffffffffu;   // of the selected
-  int ties = 0;                   // of those equal to it
+  auto wave_sum = [&](int c) { return __builtin_amdgcn_readlane(lane_scan(c), 63); };
+  auto at_least = [&](unsigned w) {
+    int c = 0;
+    over([&](unsigned x) { c += x >= w ? 1 : 0; });
+    return wave_sum(c);
+  };
+  unsigned least = 0xffffffffu;   // selected: the keys above it, and the first `ties` of those equal to it
+  int ties = 0;
   if (!all && left > 0) {
-    unsigned v = 0;
-    for (int bit = 31; bit >= 0; --bit) {
+    unsigned ones = 0, zeros = 0;   // bits set, and not set, in some candidate
+    over([&](unsigned x) {
+      ones |= x;
+      zeros |= x != 0 ? ~x : 0u;
+    });
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      ones |= __shfl_xor(ones, o, 64);
+      zeros |= __shfl_xor(zeros, o, 64);
+    }
+    const unsigned differ = ones & zeros;
+    const int top = differ != 0 ? 31 - __builtin_clz(differ) : -1;
+    unsigned v = top < 31 ? ones >> (top + 1) << (top + 1) : 0u;   // what they have in common
+    if (top < 0) v = ones;
+    int above = -1;   // candidates >= v, where counted
+    for (int bit = top; bit >= 0 && above != left; --bit) {
       const unsigned w = v | 1u << bit;
-      if (count([&](unsigned x) { return x >= w; }) >= left) v = w;
+      const int c = at_least(w);
+      if (c >= left) {
+        v = w;
+        above = c;
+      }
     }
     least = v;
-    ties = left - count([&](unsigned x) { return x > v; });
+    int c = 0;
+    over([&](unsigned x) { c += x > v ? 1 : 0; });
+    // (v need not be a candidate's key where exactly as many as asked for are at or above it)
+    ties = left - wave_sum(c);
   }
   int at = 0;
   int32_t* table = a.sel_table + t * a.st_st;
   int32_t* index = a.sel_index + t * a.si_st;
-  auto place = [&](int i, unsigned x) {
+  auto place = [&](int i, unsigned x, int e) {
     const int p = 64 * i + lane;
     const uint64_t below = (1ull << lane) - 1;
     bool take = p < n;
@@ -360,16 +466,19 @@ __global__ void __launch_bounds__(64 * kSelectWaves) page_select_kernel(SelectAr
     if (take) {
       const int to = at + __popcll(taken & below);
       index[to] = p;
-      table[to] = a.block_table[b * a.bt_sb + p];
+      table[to] = e;
     }
     at += __popcll(taken);
   };
   if constexpr (kN > 0) {
 #pragma unroll
     for (int i = 0; i < kN; ++i)
-      if (64 * i < n) place(i, key[i]);
+      if (64 * i < n) place(i, key[i], entry[i]);
   } else {
-    for (int i = 0; i < steps; ++i) place(i, all ? 0u : load(i));
+    for (int i = 0; i < steps; ++i) {
+      const int p = 64 * i + lane;
+      place(i, all ? 0u : load(i), p < n ? entries[p] : 0);
+    }
   }
   for (int i = at + lane; i < a.k; i += 64) {
     index[i] = -1;
@@ -401,10 +510,11 @@ ScoreShape score_shape(int64_t T, int64_t H, int64_t max_pages, bool packed) {
   s.blocks = (int)std::min<int64_t>(blocks, kBlocks);
   s.group = packed && s.passes == 1 ? kBlocks / s.blocks : 1;
   s.groups = (T + s.group - 1) / s.group;
-  const int64_t most = std::max<int64_t>(1, (max_pages + 63) / 64);
-  const int64_t want = std::max<int64_t>(1, 2 * device_cu_count() / std::max<int64_t>(1, s.groups));
-  const int64_t each = (most + std::min(most, want) - 1) / std::min(most, want);
-  s.chunk = (int)(64 * each);
+  // As many chunks of the pages as fill the CUs once.
+  const int64_t most = std::max<int64_t>(1, (max_pages + kTile - 1) / kTile);
+  const int64_t want = std::min(most, std::max<int64_t>(1, device_cu_count() / std::max<int64_t>(1, s.groups)));
+  const int64_t each = (most + want - 1) / want;
+  s.chunk = (int)(kTile * each);
   s.chunks = (int)((most + each - 1) / each);
   return s;
 }
@@ -501,11 +611,8 @@ extern "C" int dmla_page_scores(const void* q, const void* means, const int32_t*
   a.blocks = s.blocks; a.passes = s.passes; a.group = s.group; a.chunk = s.chunk; a.chunks = s.chunks;
   a.scale_log2 = softmax_scale * kLog2e;
   const dim3 grid((unsigned)s.groups, (unsigned)s.chunks);
-  const size_t lds = (size_t)16 * (s.passes > 1 ? kBlocks : s.blocks * s.group) * kRowBytes;
-  auto launch = [&](auto kernel) -> int {
-    hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    if (e != hipSuccess) return fail(DMLA_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
-    hipLaunchKernelGGL(kernel, grid, dim3(kScoreThreads), lds, (hipStream_t)stream, a);
+  auto launch = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, grid, dim3(kScoreThreads), 0, (hipStream_t)stream, a);
     return check_launch(what);
   };
   if (s.chunks == 1) return launch(page_scores_kernel<kFused>);

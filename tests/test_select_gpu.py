@@ -119,6 +119,20 @@ def test_scores(gpu, H, lens, counts, wide):
     assert torch.equal(got, again)
 
 
+def test_scores_of_many_queries_over_long_tables(gpu):
+    """As many queries as fill the GPU over more pages than a workgroup keeps table entries of."""
+    from python import ops
+    N, n, H = 64 * 2300 + 5, 270, 128
+    pool = 3000
+    table = torch.randint(0, pool, (1, pages(N)), generator=torch.Generator().manual_seed(0), dtype=torch.int32)
+    means = (torch.randn(pool, D_QK, generator=torch.Generator().manual_seed(1)) * 0.3).to(torch.bfloat16).to(gpu)
+    q = torch.randn(n, H, D_QK, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16).to(gpu)
+    got = ops.flash_dmla_page_scores(q, means, table.to(gpu), ints([N], gpu), ints([0, n], gpu), SCALE)
+    for i in (0, 133, n - 1):
+        s, tol = scores64(q[i:i + 1], means, table[0], [N - n + i + 1])
+        assert ((got[i:i + 1].double().cpu() - s).abs() <= tol).all()
+
+
 @pytest.mark.parametrize("lens", [[700], [40000]])
 def test_scores_leave_out_what_is_not_there(gpu, lens):
     """Pages outside the pool count as not there; means of other pages, of the query's own and of later ones do not
