@@ -587,7 +587,7 @@ __device__ __forceinline__ Pass careful_pass(const ChunkParams& p, const Piece& 
 // tiles of a sequence whose first query is token `base` (row tile i ends at token base + 128 (i + 1) / H, causal).
 // A range's end is the next one's start by the same arithmetic, so nothing is lost or done twice where they are off.
 constexpr int kCost = 8;
-constexpr int kMinWidth = 6;    // of a range
+constexpr int kMinWidth = 4;    // of a range
 constexpr int kSnap = 8;        // a cut this near to a row tile's end moves there, or a quarter of a range's width
 
 constexpr int kPieceInts = 12;

@@ -676,8 +676,8 @@ def flash_dmla_kv_release(
     _check_lens("new_lens", new_lens, B)
     _same_device(block_table=block_table, old_lens=old_lens, new_lens=new_lens, free_pages=free_pages,
                  free_count=free_count)
-    new_count = torch.empty((1,), dtype=torch.int32, device=block_table.device)
-    flag = torch.zeros(1, dtype=torch.int32, device=block_table.device) if check_indices else None
+    new_count = torch.empty_like(free_count)
+    flag = torch.zeros_like(free_count) if check_indices else None
     _lib.call(
         "dmla_kv_release",
         _ptr(block_table), _ptr(old_lens), _ptr(new_lens), _ptr(free_pages), _ptr(free_count), _ptr(new_count), _ptr(flag),
@@ -717,12 +717,11 @@ def flash_dmla_kv_reserve(
     _require(num_rows >= 0, "num_rows must be >= 0")
     _same_device(block_table=block_table, cache_seqlens=cache_seqlens, new_lens=new_lens, free_pages=free_pages,
                  free_count=free_count)
-    dev = block_table.device
-    total = torch.empty((B,), dtype=torch.int32, device=dev)
-    cu = torch.empty((B + 1,), dtype=torch.int32, device=dev)
-    slots = torch.empty((num_rows,), dtype=torch.int32, device=dev)
-    new_count = torch.empty((1,), dtype=torch.int32, device=dev)
-    flag = torch.zeros(1, dtype=torch.int32, device=dev) if check_indices else None
+    total = torch.empty_like(cache_seqlens)
+    cu = cache_seqlens.new_empty(B + 1)
+    slots = cache_seqlens.new_empty(num_rows)
+    new_count = torch.empty_like(free_count)
+    flag = torch.zeros_like(free_count) if check_indices else None
     _lib.call(
         "dmla_kv_reserve",
         _ptr(block_table), _ptr(cache_seqlens), _ptr(new_lens), _ptr(free_pages), _ptr(free_count), _ptr(total), _ptr(cu),
@@ -826,7 +825,7 @@ def flash_dmla_chunk_paged(
     if check_indices:
         _check_packed(cu_seqlens_q, T)
         _check_page_indices(block_table, cache_seqlens, num_pages)
-    o = torch.empty((T, H, d_v), dtype=torch.bfloat16, device=q.device)
+    o = q.new_empty((T, H, d_v))
     lse = torch.empty((T, H), dtype=torch.float32, device=q.device) if return_lse else None
     max_pages = block_table.shape[1]
     ws_bytes = int(_lib.lib().dmla_chunk_paged_workspace_bytes(T, B, H, max_pages))
@@ -946,9 +945,9 @@ def flash_dmla_page_select(
     _require(recent >= 1 and sink >= 0 and recent + sink <= top_pages,
              "recent must be at least 1, sink at least 0, and top_pages cover both")
     _same_device(scores=scores, block_table=block_table, cache_seqlens=cache_seqlens, cu_seqlens_q=cu_seqlens_q)
-    table = torch.empty((T, top_pages), dtype=torch.int32, device=scores.device)
-    lens = torch.empty((T,), dtype=torch.int32, device=scores.device)
-    index = torch.empty((T, top_pages), dtype=torch.int32, device=scores.device)
+    table = cache_seqlens.new_empty((T, top_pages))
+    lens = cache_seqlens.new_empty(T)
+    index = torch.empty_like(table)
     _lib.call(
         "dmla_page_select",
         _ptr(scores), _ptr(block_table), _ptr(cache_seqlens), _ptr(cu_seqlens_q), _ptr(table), _ptr(lens), _ptr(index),
