@@ -30,6 +30,9 @@ constexpr int kSteps = kDqk / 16, kLatSteps = kDv / 16;    // MFMAs of a tile's 
 constexpr int kKeyRow = 1024, kKeyBytes = kTile * kKeyRow, kSlots = 4;
 constexpr int kRopeBytes = kTile * 128;
 constexpr int kProbBytes = kWaves * 2048;                   // P of a step
+constexpr int kNarrowRows = 32;                            // up to here the waves share the rows' scores
+constexpr int kNarrowRopes = 3, kShareBytes = 3 * kWaves * 1024;   // scores that the waves exchange, behind three ropes
+constexpr int kLdsBytes = kSlots * kKeyBytes + std::max(kSlots * kRopeBytes + kProbBytes, kNarrowRopes * kRopeBytes + kShareBytes + 2048);
 constexpr int kCopies = 9;                                 // of a wave and tile
 // Queries come through that memory, in blocks of 64 dims (4 KB of a wave): the first six in the first three slots
 // of keys, where they may land while the piece before puts out through the fourth, two in the fourth, and one
@@ -128,10 +131,16 @@ __device__ __forceinline__ unsigned query_block(const Lds& lds, int wave, int i)
   if (i < kQueryEarly + 2) return lds.keys + 3 * kKeyBytes + (wave * 2 + i - kQueryEarly) * kQueryBlock;
   return lds.rope + 2 * kRopeBytes + wave * kQueryBlock;
 }
+// Of up to kNarrowRows rows every wave has all of them, but only a quarter of the dims: two latent blocks, and of
+// the rope block 16 dims.  They lie where the first three of the six would.
+__device__ __forceinline__ bool narrow(int rows) { return rows <= kNarrowRows; }
+__device__ __forceinline__ int query_dims(int wave, int rows, int i) {
+  return 64 * (!narrow(rows) ? i : i < 2 ? 2 * wave + i : 8);
+}
 // This lane's place in rows 8 g .. 8 g + 7 of them.
 __device__ __forceinline__ const bf16* query_rows(const ChunkParams& p, int wave, int q0, int row0, int rows, int g) {
   const int ln = fresh_lane_id();
-  const int r = row0 + min(32 * wave + 8 * g + (ln >> 3), rows - 1);
+  const int r = row0 + min((narrow(rows) ? 0 : 32 * wave) + 8 * g + (ln >> 3), rows - 1);
   const int token = fast_div(r, p.hdiv), head = r - token * p.H;
   return p.q + (q0 + token) * p.q_st + head * p.q_sh + 8 * ((ln & 7) ^ (ln >> 3));
 }
@@ -141,50 +150,55 @@ __device__ __forceinline__ void copy_queries(const ChunkParams& p, const Lds& ld
   for (int g = 0; g < 4; ++g) {
     const bf16* src = query_rows(p, wave, q0, row0, rows, g);
 #pragma unroll
-    for (int i = kFirst; i < kFirst + kN; ++i) dma16_addr(src + 64 * i, query_block(lds, wave, i) + g * 1024);
+    for (int i = kFirst; i < kFirst + kN; ++i)
+      if (i < 3 || !narrow(rows)) dma16_addr(src + query_dims(wave, rows, i), query_block(lds, wave, i) + g * 1024);
   }
 }
 
 // Whether another pass has to follow.
 // have: the queries are on their way.  After it, those of the next piece's rows are.
+template <bool kNarrow>
 __device__ __forceinline__ bool run_piece(const ChunkParams& p, const Piece& pc, const Lds& lds, const Pass& pass, bool have,
                                           const DMLA_LDS int* next) {
   const int lane = fresh_lane_id();
   const int l32 = lane & 31, hl = lane >> 5;
   const int wave = uniform(threadIdx.x >> 6);
   const int rows = min(pc.s.n * p.H - pc.row0, kRows);
+  constexpr int kBlocks = kNarrow ? 1 : kRowBlocks;   // of 32 rows
+  const int first_row = kNarrow ? 0 : 32 * wave;      // of the wave's 32
   // Rows past the last one are the last one again, and not written.
   auto limit_of = [&](int r) {   // last key of row r
     return p.causal ? pc.s.len - pc.s.n + fast_div(pc.row0 + min(r, rows - 1), p.hdiv) : pc.s.len - 1;
   };
-  const int lim = limit_of(32 * wave + l32);
-  const int lim0 = uniform(limit_of(32 * wave));   // the wave's smallest
+  const int lim = limit_of(first_row + l32);
+  const int lim0 = uniform(limit_of(first_row));   // the wave's smallest
 
   // ---- copies: lane l copies 16 bytes into place l of each kilobyte, nine of a wave and tile ----
   Pages pages;
   // Rows of a tile from key_end on are its last row before, again.
   const int key_end = uniform(min(limit_of(rows - 1) + 1, pass.to));
   const int t1 = max(pc.t0, min(pc.t1, (max(key_end, 0) + kTile - 1) / kTile));
-  const char* copy_src = nullptr;
-  int copy_last = 0;
-  unsigned copy_dst = 0, copy_lane = 0;
+  // (Few scalars between them: what the compiler keeps of a loop's scalars, it keeps in lanes of a register.)
+  const char* copy_src = nullptr;   // the first of the wave's rows
+  int copy_more = 0;                // rows behind it
+  unsigned copy_keys = 0, copy_rope = 0, copy_lane = 0;
   const int row_step = uniform((int)p.kv_ss);
   auto copy_begin = [&](int s) {
     copy_lane = 16 * (fresh_lane_id() ^ key_swz(8 * wave));
     const int t = min(pc.t0 + s, t1 - 1);   // past the end: the last tile, which nobody counts
-    copy_src = pages.tile(p, pc, t);
-    copy_last = uniform(min(key_end - t * kTile, kTile) - 1);
-    copy_dst = (unsigned)(s % kSlots);
+    const int last = uniform(min(key_end - t * kTile, kTile) - 1), row = min(8 * wave, last);
+    copy_src = pages.tile(p, pc, t) + row * row_step;
+    copy_more = last - row;
+    copy_keys = lds.keys + (unsigned)(s % kSlots) * kKeyBytes + wave * 8 * kKeyRow;
+    copy_rope = lds.rope + (unsigned)(s % (kNarrow ? kNarrowRopes : kSlots)) * kRopeBytes + wave * 1024;
   };
   auto copy = [&](int i) {
-    if (i < 8) {
-      const int r = 8 * wave + i;
-      // key_swz(8 wave + i) is key_swz(8 wave) ^ key_swz(i)
-      dma16(copy_src, (copy_lane ^ (16 * key_swz(i))) + min(r, copy_last) * row_step, lds.keys + copy_dst * kKeyBytes + r * kKeyRow);
+    if (i < 8) {   // key_swz(8 wave + i) is key_swz(8 wave) ^ key_swz(i)
+      dma16(copy_src, (copy_lane ^ (16 * key_swz(i))) + min(i, copy_more) * row_step, copy_keys + i * kKeyRow);
     } else {
       const int ln = fresh_lane_id();
-      const unsigned off = min(8 * wave + (ln >> 3), copy_last) * row_step + 2 * kDv + 16 * ((ln & 7) ^ (ln >> 3));
-      dma16(copy_src, off, lds.rope + copy_dst * kRopeBytes + wave * 1024);
+      const unsigned off = min(ln >> 3, copy_more) * row_step + 2 * kDv + 16 * ((ln & 7) ^ (ln >> 3));
+      dma16(copy_src, off, copy_rope);
     }
   };
   auto copy_tile = [&](int s) {
@@ -193,28 +207,31 @@ __device__ __forceinline__ bool run_piece(const ChunkParams& p, const Piece& pc,
     for (int i = 0; i < kCopies; ++i) copy(i);
   };
 
-  // ---- queries: 36 operands of 16 dims; operand c holds dims 16 c + 8 hl .. of row l32 ----
+  // ---- queries: 36 operands of 16 dims; operand c holds dims 16 c + 8 hl .. of row l32.  Narrow: those of dims
+  // 128 wave .. + 127, and of rope dims 16 wave .. + 15 ----
   const int n_steps = t1 - pc.t0;
-  bf16x8 q[kSteps];
+  constexpr int kOwnSteps = kNarrow ? kSteps / kWaves : kSteps;
+  bf16x8 q[kOwnSteps];
   auto take_queries = [&](auto first_tag, auto n_tag) {
     constexpr int kFirst = decltype(first_tag)::value, kN = decltype(n_tag)::value;
 #pragma unroll
     for (int i = kFirst; i < kFirst + kN; ++i) {
       const unsigned a = lds_sum(1024 * (l32 >> 3) + 128 * (l32 & 7) + 16 * (hl ^ (l32 & 7)), query_block(lds, wave, i));
 #pragma unroll
-      for (int c = 0; c < 4; ++c) q[4 * i + c] = *lds_ptr<const bf16x8>(a ^ (32 * c));
+      for (int c = 0; c < 4; ++c)
+        if (4 * i + c < kOwnSteps) q[4 * i + c] = *lds_ptr<const bf16x8>(kNarrow && i == 2 ? a ^ (32 * wave) : a ^ (32 * c));
     }
   };
   if (!have) copy_queries<0, 9>(p, lds, wave, pc.s.q0, pc.row0, rows);
   pages.fetch(p, pc, pc.t0 / 2);
   wait_vm<0>();
   using std::integral_constant;
-  take_queries(integral_constant<int, 0>{}, integral_constant<int, 9>{});
+  take_queries(integral_constant<int, 0>{}, integral_constant<int, kNarrow ? 3 : 9>{});
   wait_lds();
   __syncthreads();   // the keys' memory is free
   if (n_steps > 0) copy_tile(0);
 
-  f32x16 acc[kRowBlocks][kColBlocks];   // O^T: register i is column 128 wave + 32 j + 16 hl + i of row l32
+  f32x16 acc[kBlocks][kColBlocks];   // O^T: register i is column 128 wave + 32 j + 16 hl + i of row l32
   float mref = kNegInf, mtrue = kNegInf, lsum = 0.f;   // reference, largest score seen, sum
   bf16x8 pv[2];             // P of the wave's own rows, 16 keys each
 
@@ -225,6 +242,7 @@ __device__ __forceinline__ bool run_piece(const ChunkParams& p, const Piece& pc,
     in_order();
   };
   auto opaque = [](unsigned a) {
+    if constexpr (kNarrow) a = (unsigned)uniform((int)a);
     asm("" : "+s"(a));
     return a;
   };
@@ -301,7 +319,7 @@ __device__ __forceinline__ bool run_piece(const ChunkParams& p, const Piece& pc,
   // ---- values: O^T += V^T P of a tile, in groups g of 16 keys (u = g / 4) and 32 columns (j = g % 4) ----
   // Row m of the operand is column 4 (m / 8) + 16 (m / 4 % 2) + m % 4 of the block: a lane then ends with 16
   // neighbouring columns.
-  bf16x8 prob[kRowBlocks], val[3];
+  bf16x8 prob[kBlocks], val[3];
   unsigned val_addr = 0, prob_addr = 0;
   auto values_begin = [&](int s) {
     const int r = (lane & 15) >> 2, g = lane >> 4 & 1;
@@ -328,15 +346,129 @@ __device__ __forceinline__ bool run_piece(const ChunkParams& p, const Piece& pc,
       in_order();
     });
   };
+  // ---- up to 32 rows.  Scores: wave w multiplies its quarter of the dims and finishes, from the four partial
+  // products, keys 8 w .. 8 w + 7 of the tile (elements 4 w .. 4 w + 3); values: all keys for its 128 columns.  Two
+  // barriers a tile: products of scores and values between them, the softmax of 4 elements behind the second.
+  // A wave alone with 32 rows' scores takes 3400 cycles a tile.
+  const unsigned share = lds.rope + kNarrowRopes * kRopeBytes, narrow_prob = share + kShareBytes;
+  auto total_of = [&](float v, auto f) {   // of a row, over the waves
+    const auto halves = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = f(__uint_as_float(halves[0]), __uint_as_float(halves[1]));
+    __syncthreads();
+    if (hl == 0) lds.stat[32 * wave + l32] = v;
+    __syncthreads();
+    v = f(f(lds.stat[l32], lds.stat[32 + l32]), f(lds.stat[64 + l32], lds.stat[96 + l32]));
+    __syncthreads();   // read
+    return v;
+  };
+  auto narrow_steps = [&] {
+    f32x4 own;
+    auto partial = [&](int s) {   // its quarter of tile s's scores, and the others' keys of it to them
+      const unsigned kb = lds_sum(kKeyRow * l32 + 16 * (hl ^ key_swz(l32)), opaque(lds.keys + (unsigned)(s % kSlots) * kKeyBytes + 256 * wave));
+      const unsigned rb = lds_sum(128 * l32 + 16 * (hl ^ (l32 & 7)), opaque(lds.rope + (unsigned)(s % kNarrowRopes) * kRopeBytes)) ^ (32 * wave);
+      bf16x8 k[kOwnSteps];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) k[c] = *lds_ptr<const bf16x8>(kb ^ (32 * c));
+      k[8] = *lds_ptr<const bf16x8>(rb);
+      f32x16 x;
+      static_for<kOwnSteps>([&](auto c_tag) {
+        constexpr int c = decltype(c_tag)::value;
+        score_step<c == 0>(x, k[c], q[c]);
+      });
+      score_done(x);
+      static_for<kWaves>([&](auto d_tag) {
+        constexpr int d = decltype(d_tag)::value;
+        const f32x4 v = {x[4 * d], x[4 * d + 1], x[4 * d + 2], x[4 * d + 3]};
+        if (d == wave) own = v;
+        else *lds_ptr<f32x4>(lds_sum(16 * lane, opaque(share + (3 * d + wave - (wave > d ? 1 : 0)) * 1024))) = v;
+      });
+    };
+    // Scores of the wave's keys of tile s: what the others have of them (always in the waves' order), the mask.
+    auto finish = [&](int s) {
+      const unsigned at = lds_sum(16 * lane, opaque(share + 3 * wave * 1024));
+      f32x4 part[3];
+#pragma unroll
+      for (int i = 0; i < 3; ++i) part[i] = *lds_ptr<const f32x4>(at + 1024 * i);
+      f32x4 sum = wave == 0 ? own : part[0];
+      sum += wave == 1 ? own : part[wave > 1 ? 1 : 0];
+      sum += wave == 2 ? own : part[wave > 2 ? 2 : 1];
+      sum += wave == 3 ? own : part[2];
+      const int key = (pc.t0 + s) * kTile + 8 * wave + 4 * hl;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum[i] = key + i <= lim ? sum[i] * p.scale_log2 : kNegInf;
+      mtrue = fmaxf(mtrue, fmaxf(fmaxf(sum[0], sum[1]), fmaxf(sum[2], sum[3])));
+      return sum;
+    };
+    auto softmax = [&](const f32x4& x) {
+      const float ms = mref == kNegInf ? 0.f : mref;
+      bf16x4 pr;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float v = fast_exp2(x[i] - ms);
+        lsum += v;
+        pr[i] = (bf16)v;   // what the value product takes; the sum keeps fp32
+      }
+      *lds_ptr<bf16x4>(lds_sum(16 * lane, opaque(narrow_prob + 1024 * (wave >> 1) + 8 * (wave & 1)))) = pr;
+    };
+    copy_tile(1);
+    copy_tile(2);
+    wait_vm<2 * kCopies>();
+    __syncthreads();   // tile 0 landed
+    partial(0);
+    __syncthreads();   // partial products posted
+    const f32x4 x0 = finish(0);
+    if (pass.careful) {
+      mref = lds.top[l32];
+    } else {
+      mref = total_of(mtrue, [](float a, float b) { return fmaxf(a, b); });
+    }
+    softmax(x0);
+    wait_vm<kCopies>();
+    wait_lds();
+    __syncthreads();   // P posted, tile 1 landed
+#pragma nounroll
+    for (int s = 0;; ++s) {
+      copy_tile(s + 3);   // where tile s - 1 was
+      {
+        const int r = (lane & 15) >> 2, g = lane >> 4 & 1;
+        const unsigned vb = lds_sum(kKeyRow * (4 * hl + r) + 256 * wave + 16 * (4 * r | ((g + 2 * (lane & 1)) ^ hl)) + 8 * ((lane & 3) >> 1),
+                                    opaque(lds.keys + (unsigned)(s % kSlots) * kKeyBytes));
+        const unsigned pb = lds_sum(16 * lane, opaque(narrow_prob));
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const bf16x8 pr = *lds_ptr<const bf16x8>(pb + 1024 * u);
+#pragma unroll
+          for (int j = 0; j < kColBlocks; ++j) {
+            const unsigned a = (vb ^ (64 * j));
+            const bf16x8 v = concat(lds_read_tr16(lds_ptr<const bf16x4>(a + 16 * kKeyRow * u)),
+                                    lds_read_tr16(lds_ptr<const bf16x4>((a ^ 32) + 16 * kKeyRow * u + 8 * kKeyRow)));
+            acc[0][j] = mfma32_bf16(v, pr, acc[0][j]);
+          }
+        }
+      }
+      if (s + 1 == n_steps) break;
+      partial(s + 1);
+      wait_lds();
+      barrier();   // partial products posted, P and tile s read
+      softmax(finish(s + 1));
+      wait_vm<kCopies>();   // tile s + 2; one tile more may be on its way
+      wait_lds();
+      barrier();   // P posted, tile s + 2 landed
+    }
+    mtrue = total_of(mtrue, [](float a, float b) { return fmaxf(a, b); });
+  };
+
   {
     lsum = 0.f;
     // Zeros by the matrix core, a whole accumulator at a time: element by element the compiler would
     // assemble them elsewhere and move them.
 #pragma unroll
-    for (int n = 0; n < kRowBlocks; ++n)
+    for (int n = 0; n < kBlocks; ++n)
 #pragma unroll
       for (int j = 0; j < kColBlocks; ++j) acc[n][j] = mfma32_bf16(bf16x8{}, bf16x8{}, f32x16{});
-    if (n_steps > 0) {
+    if constexpr (kNarrow) {
+      if (n_steps > 0) narrow_steps();
+    } else if (n_steps > 0) {
       wait_vm<0>();
       __syncthreads();   // tile 0 landed
       read_rope(0);
@@ -351,7 +483,7 @@ __device__ __forceinline__ bool run_piece(const ChunkParams& p, const Piece& pc,
       score_done(x0);
       mask(x0, 0);
       const float top = tile_max(x0);
-      mref = pass.careful ? lds.top[32 * wave + l32] : top;
+      mref = pass.careful ? lds.top[first_row + l32] : top;
       mtrue = top;
       static_for<kPieces>([&](auto i) { softmax_piece(x0, i); });
       post();
@@ -414,12 +546,13 @@ __device__ __forceinline__ bool run_piece(const ChunkParams& p, const Piece& pc,
       values([](auto) {});
     }
   }
+  if constexpr (kNarrow) lsum = total_of(lsum, [](float a, float b) { return a + b; });
 
   // ---- output ----
-  lsum = half_sum(lsum);
-  if (hl == 0) {
-    if (!pass.careful) lds.top[32 * wave + l32] = mtrue;
-    lds.stat[wave * 32 + l32] = (int64_t)lim >= pages.bad * (int64_t)kPage ? __builtin_nanf("") : lsum;
+  if constexpr (!kNarrow) lsum = half_sum(lsum);
+  if (hl == 0 && (!kNarrow || wave == 0)) {
+    if (!pass.careful) lds.top[first_row + l32] = mtrue;
+    lds.stat[first_row + l32] = (int64_t)lim >= pages.bad * (int64_t)kPage ? __builtin_nanf("") : lsum;
   }
   bool wrong = !pass.careful && mtrue > mref + kHeadroom;
   agpr_settle();
@@ -438,11 +571,11 @@ __device__ __forceinline__ bool run_piece(const ChunkParams& p, const Piece& pc,
     const int r = pc.row0 + row, token = fast_div(r, p.hdiv);
     return (pc.s.q0 + token) * st + (r - token * p.H) * sh;
   };
-  if (hl == 0 && written(32 * wave + l32)) {
-    const float sum = lds.stat[32 * wave + l32];
+  if (hl == 0 && (!kNarrow || wave == 0) && written(first_row + l32)) {
+    const float sum = lds.stat[first_row + l32];
     const float lse2 = sum == 0.f ? kNegInf : mref + __log2f(sum);
-    if (pc.slot >= 0) p.part_lse[(int64_t)pc.slot * kRows + 32 * wave + l32] = lse2;
-    else if (p.lse != nullptr) p.lse[place(32 * wave + l32, p.H, 1)] = lse2 * kLn2;
+    if (pc.slot >= 0) p.part_lse[(int64_t)pc.slot * kRows + first_row + l32] = lse2;
+    else if (p.lse != nullptr) p.lse[place(first_row + l32, p.H, 1)] = lse2 * kLn2;
   }
   // Through LDS, so that a store covers whole lines: 256 bytes of each of 4 rows, or of a part 512 bytes of each of 2.
   // A wave has its own memory there.
@@ -471,9 +604,10 @@ __device__ __forceinline__ bool run_piece(const ChunkParams& p, const Piece& pc,
       const bf16* src = nullptr;
       if (next_rows > 0) src = query_rows(p, wave, next_q0, next_row0, next_rows, n);
       auto ask = [&](int i) {
-        if (next_rows > 0 && i < kQueryEarly) dma16_addr(src + 64 * i, query_block(lds, wave, i) + n * 1024);
+        if (next_rows > 0 && i < (narrow(next_rows) ? 3 : kQueryEarly))
+          dma16_addr(src + query_dims(wave, next_rows, i), query_block(lds, wave, i) + n * 1024);
       };
-      if (32 * n >= rows) {   // no rows there
+      if (n >= kBlocks || 32 * n >= rows) {   // no rows there
 #pragma unroll
         for (int i = 0; i < kQueryEarly; ++i) ask(i);
         continue;
@@ -487,7 +621,7 @@ __device__ __forceinline__ bool run_piece(const ChunkParams& p, const Piece& pc,
           bf16x8 v;
 #pragma unroll
           for (int i = 0; i < 8; i += 2) {
-            const float a = agpr_read(acc[n][j][8 * d + i]) * inv, b = agpr_read(acc[n][j][8 * d + i + 1]) * inv;
+            const float a = agpr_read(acc[n % kBlocks][j][8 * d + i]) * inv, b = agpr_read(acc[n % kBlocks][j][8 * d + i + 1]) * inv;
             look(a, b);
             v[i] = (bf16)a;
             v[i + 1] = (bf16)b;
@@ -517,7 +651,7 @@ __device__ __forceinline__ bool run_piece(const ChunkParams& p, const Piece& pc,
     const unsigned get = lds_sum(512 * hl + 16 * (l32 ^ hl), mine);     // 4 columns of row hl
     float* part = p.part_o + (int64_t)pc.slot * kRows * kDv + 128 * wave;
 #pragma unroll
-    for (int n = 0; n < kRowBlocks; ++n) {
+    for (int n = 0; n < kBlocks; ++n) {
       if (32 * n >= rows) break;
       const float inv = inverse(n);
 #pragma unroll
@@ -637,7 +771,7 @@ __device__ __forceinline__ Place place_of(const ChunkParams& p, int b, const Seq
 typedef int4 RangeLink;
 
 __global__ __launch_bounds__(kThreads, 1) void chunk_kernel(ChunkParams p) {
-  __shared__ __attribute__((aligned(1024))) char mem[kSlots * (kKeyBytes + kRopeBytes) + kProbBytes];
+  __shared__ __attribute__((aligned(1024))) char mem[kLdsBytes];
   __shared__ __attribute__((aligned(16))) float stat[kRows], top[kRows];
   __shared__ __attribute__((aligned(16))) int flag[kWaves];
   __shared__ __attribute__((aligned(16))) Window win;
@@ -810,17 +944,18 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_kernel(ChunkParams p) {
     pc.slot = uniform(now[8]);
     piece(next);
     Pass pass = {false, (int)0x80000000, 0x7fffffff};
-    bool again = run_piece(p, pc, lds, pass, have, next);
-    have = true;
-    while (again || (pass.careful && pass.to != 0x7fffffff)) {
-      if (pass.careful && pass.to == 0x7fffffff) break;
+    const bool few = narrow(uniform(now[2]));
+    for (;;) {
+      const bool again = few ? run_piece<true>(p, pc, lds, pass, have, next) : run_piece<false>(p, pc, lds, pass, have, next);
+      have = true;
+      if (pass.careful ? pass.to == 0x7fffffff : !again) break;
       const int base = pc.s.len - pc.s.n, last = min(pc.row0 + kRows, pc.s.n * p.H) - 1;
       const int first_lim = p.causal ? base + fast_div(pc.row0, p.hdiv) : pc.s.len - 1;
       const int last_lim = p.causal ? base + fast_div(last, p.hdiv) : pc.s.len - 1;
       pass = careful_pass(p, pc, lds, pass.careful ? pass.to : first_lim, last_lim);
       wait_vm<0>();   // the next piece's queries, which are copied once more
       __syncthreads();
-      again = run_piece(p, pc, lds, pass, false, next);
+      have = false;
     }
   }
   if (tid == 0) p.links[range] = link;
