@@ -711,18 +711,22 @@ __device__ __forceinline__ Pass careful_pass(const ChunkParams& p, const Piece& 
 }
 
 // ---- cutting the work ---------------------------------------------------------------------------------
-// The row tiles (128 rows) of all sequences, in order, each with its key tiles behind kCost virtual ones (what starting
+// The row tiles (128 rows) of all sequences, in order, each with its key tiles behind some virtual ones (what starting
 // and ending a piece costs), are cut into ranges of equal weight, one per workgroup: no list, no plan kernel, no order
 // of workgroups.  Every workgroup works the cut out from the lengths.  A row tile that spans ranges leaves a part in
 // each, merged by chunk_combine_kernel: range r writes the part that it begins with to slot 2 r (a row tile that an
 // earlier range began) and the one that it ends with to slot 2 r + 1.
 //
-// Weights are estimates, in closed form: A(n) = n (kCost + (base + 31) / 32) + 2 n (n + 1) / H for the first n row
-// tiles of a sequence whose first query is token `base` (row tile i ends at token base + 128 (i + 1) / H, causal).
-// A range's end is the next one's start by the same arithmetic, so nothing is lost or done twice where they are off.
-constexpr int kCost = 8;
-constexpr int kMinWidth = 4;    // of a range
-constexpr int kSnap = 8;        // a cut this near to a row tile's end moves there, or a quarter of a range's width
+// Weights are estimates in closed form, in halves of what a key tile of 128 rows takes: a tile weighs u = 2, of a
+// sequence with up to kNarrowRows rows u = 1, a start and end c.  The first n row tiles of a sequence whose first query is
+// token `base` weigh A(n) = n (c + u (base + 31) / 32) + 2 u n (n + 1) / H (row tile i ends at token
+// base + 128 (i + 1) / H, causal).  A range's end is the next one's start by the same arithmetic, so nothing is lost
+// or done twice where they are off.
+// (Costs from 12 / 8 to 24 / 16 were within 4 % of each other over thirteen batches, least widths of 8 and 12 cost
+// single sequences of 16 heads 3 and 10 us.)
+constexpr int kCost = 20, kNarrowCost = 20;
+constexpr int kMinWidth = 6;    // of a range
+constexpr int kSnap = 8;        // tiles: a cut this near to a row tile's end moves there, or a quarter of a range's width
 
 constexpr int kPieceInts = 12;
 struct Window {   // the sequences of 256 at a time, and what the threads share
@@ -739,12 +743,20 @@ __device__ __forceinline__ int key_tiles(const ChunkParams& p, const Sequence& s
   const int end = p.causal ? s.len - s.n + last + 1 : s.len;
   return (max(end, 0) + kTile - 1) / kTile;
 }
-// Weight of a row tile before its growth along the sequence.
-__device__ __forceinline__ int64_t base_weight(const ChunkParams& p, const Sequence& s) {
-  return kCost + (p.causal ? max(s.len - s.n, 0) + kTile - 1 : s.len + kTile - 1) / kTile;
+struct Weights {
+  int unit, cost;
+  int64_t base;   // of a row tile before its growth along the sequence
+};
+__device__ __forceinline__ Weights weights(const ChunkParams& p, const Sequence& s) {
+  const bool few = s.n * p.H <= kNarrowRows;
+  Weights w = {few ? 1 : 2, few ? kNarrowCost : kCost, 0};
+  w.base = w.cost + w.unit * (int64_t)((p.causal ? max(s.len - s.n, 0) + kTile - 1 : s.len + kTile - 1) / kTile);
+  return w;
 }
+// A(n).
 __device__ __forceinline__ int64_t weight(const ChunkParams& p, const Sequence& s, int64_t n) {
-  return n * base_weight(p, s) + (p.causal ? 2 * n * (n + 1) / p.H : 0);
+  const Weights w = weights(p, s);
+  return n * w.base + (p.causal ? 2 * w.unit * n * (n + 1) / p.H : 0);
 }
 
 struct Place {   // in the row tiles and key tiles of all sequences
@@ -752,15 +764,16 @@ struct Place {   // in the row tiles and key tiles of all sequences
 };
 
 // The place at weight y of sequence b.
-__device__ __forceinline__ Place place_of(const ChunkParams& p, int b, const Sequence& s, int64_t y, int snap) {
+__device__ __forceinline__ Place place_of(const ChunkParams& p, int b, const Sequence& s, int64_t y, int64_t width) {
+  const Weights w = weights(p, s);
   int lo = 0, hi = row_tiles(p, s) - 1;   // the last row tile that begins at or before y
-  const int64_t w = base_weight(p, s) * p.H, x = (y + 1) * p.H;
+  const int64_t wh = w.base * p.H, x = (y + 1) * p.H;
   while (lo < hi) {
     const int64_t mid = (lo + hi + 1) / 2;
-    if (mid * w + (p.causal ? 2 * mid * (mid + 1) : 0) < x) lo = (int)mid; else hi = (int)mid - 1;
+    if (mid * wh + (p.causal ? 2 * w.unit * mid * (mid + 1) : 0) < x) lo = (int)mid; else hi = (int)mid - 1;
   }
-  const int nt = key_tiles(p, s, lo);
-  int t = (int)min((int64_t)nt, max((int64_t)0, y - weight(p, s, lo) - kCost));
+  const int nt = key_tiles(p, s, lo), snap = (int)min((int64_t)kSnap, width / (4 * w.unit));
+  int t = (int)min((int64_t)nt, max((int64_t)0, y - weight(p, s, lo) - w.cost) / w.unit);
   if (t <= snap) t = 0;
   if (t > 0 && nt - t <= snap) return Place{b, lo + 1, 0};
   return Place{b, lo, t};
@@ -865,11 +878,10 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_kernel(ChunkParams p) {
   };
   Sequence s = sequence_at(b_last);
   // The end of the last sequence's work is its last row tile's.
-  const int snap = (int)min((int64_t)kSnap, width / 4);
-  Place end = place_of(p, b_last, s, y1, snap);
+  Place end = place_of(p, b_last, s, y1, width);
   if (y1 >= weight(p, s, row_tiles(p, s))) end = Place{b_last, row_tiles(p, s), 0};
   s = sequence_at(b_first);
-  Place at = place_of(p, b_first, s, y0, snap);
+  Place at = place_of(p, b_first, s, y0, width);
   end.rt = uniform(end.rt); end.t = uniform(end.t);
   at.rt = uniform(at.rt); at.t = uniform(at.t);
   RangeLink link = make_int4(0, 0, 0, 0);
@@ -1070,7 +1082,7 @@ __global__ __launch_bounds__(256) void chunk_combine_kernel(ChunkParams p) {
 // Ranges of a call: one per CU, as many as its work can fill at most.
 int64_t chunk_ranges(int64_t T, int64_t B, int64_t H, int64_t max_pages) {
   const int64_t tiles = T * H / kRows + std::min(B, T);
-  const int64_t most = tiles * (kCost + 1 + max_pages * (kPage / kTile)) + 2 * T;   // at least what the kernel adds up
+  const int64_t most = tiles * (kCost + 2 + max_pages * (2 * kPage / kTile)) + 4 * T;   // at least what the kernel adds up
   return std::max<int64_t>(1, std::min<int64_t>(device_cu_count(), (most + kMinWidth - 1) / kMinWidth));
 }
 int64_t chunk_bytes(int64_t ranges) { return ranges * (2 * kRows * (int64_t)(kDv + 1) * 4 + (int64_t)sizeof(RangeLink)); }
