@@ -14,6 +14,7 @@
 //    rows of 128 bytes of their own, eight of them a copy.
 //  * Step s multiplies scores of tile s and values of tile s - 1; copies run two tiles ahead, four tiles fit.
 #include <algorithm>
+#include <cmath>
 
 #include "dmla_host.h"
 #include "dmla_pipe.h"
@@ -59,6 +60,8 @@ struct ChunkParams {
   int T, B, H, num_pages, max_pages, causal, n_ranges;
   FastDiv hdiv;          // division by H
   float scale_log2;
+  float two_by_h, weight_scale;   // 2 / H, 2^-weight_shift
+  int weight_shift;
 };
 
 // A sequence's queries: q0 .. q0 + n - 1, the newest of its len tokens.
@@ -721,20 +724,23 @@ __device__ __forceinline__ Pass careful_pass(const ChunkParams& p, const Piece& 
 // sequence with up to kNarrowRows rows u = 1, a start and end c.  The first n row tiles of a sequence whose first query is
 // token `base` weigh A(n) = n (c + u (base + 31) / 32) + 2 u n (n + 1) / H (row tile i ends at token
 // base + 128 (i + 1) / H, causal).  A range's end is the next one's start by the same arithmetic, so nothing is lost
-// or done twice where they are off.
+// or done twice where they are off.  They are integers (of fp32 products, ascending in n whatever the rounding); where
+// the host finds that they could pass 2^30, all are taken in units of 2^weight_shift.
 // (Costs from 12 / 8 to 24 / 16 were within 4 % of each other over thirteen batches, least widths of 8 and 12 cost
 // single sequences of 16 heads 3 and 10 us.)
 constexpr int kCost = 20, kNarrowCost = 20;
 constexpr int kMinWidth = 6;    // of a range
 constexpr int kSnap = 8;        // tiles: a cut this near to a row tile's end moves there, or a quarter of a range's width
 
-constexpr int kPieceInts = 12;
+struct Place {   // in the row tiles and key tiles of all sequences
+  int b, rt, t;
+};
 struct Window {   // the sequences of 256 at a time, and what the threads share
   int q0[kThreads], n[kThreads], len[kThreads];
-  int64_t tmp[kWaves];
-  int at[4];
-  int64_t rest[2];
-  int piece[2 * kPieceInts];
+  int tmp[kWaves];
+  Place at, end;        // where the next piece begins, and the range's end
+  int first;            // sequence of the window
+  i32x4 piece[2][3];   // q0, row0, rows, n; len, b, t0, t1; slot: this one and the next
 };
 
 __device__ __forceinline__ int row_tiles(const ChunkParams& p, const Sequence& s) { return (s.n * p.H + kRows - 1) / kRows; }
@@ -745,35 +751,31 @@ __device__ __forceinline__ int key_tiles(const ChunkParams& p, const Sequence& s
 }
 struct Weights {
   int unit, cost;
-  int64_t base;   // of a row tile before its growth along the sequence
+  float base, growth;   // of a row tile, and how much more each one weighs
 };
 __device__ __forceinline__ Weights weights(const ChunkParams& p, const Sequence& s) {
   const bool few = s.n * p.H <= kNarrowRows;
-  Weights w = {few ? 1 : 2, few ? kNarrowCost : kCost, 0};
-  w.base = w.cost + w.unit * (int64_t)((p.causal ? max(s.len - s.n, 0) + kTile - 1 : s.len + kTile - 1) / kTile);
+  Weights w = {few ? 1 : 2, few ? kNarrowCost : kCost, 0.f, 0.f};
+  const int tiles = ((p.causal ? max(s.len - s.n, 0) : s.len) + kTile - 1) / kTile;
+  w.base = (float)(w.cost + w.unit * tiles);
+  w.growth = p.causal ? w.unit * p.two_by_h : 0.f;
   return w;
 }
 // A(n).
-__device__ __forceinline__ int64_t weight(const ChunkParams& p, const Sequence& s, int64_t n) {
-  const Weights w = weights(p, s);
-  return n * w.base + (p.causal ? 2 * w.unit * n * (n + 1) / p.H : 0);
+__device__ __forceinline__ int weight(const ChunkParams& p, const Weights& w, int n) {
+  return (int)((float)n * (w.base + w.growth * (float)(n + 1)) * p.weight_scale);
 }
-
-struct Place {   // in the row tiles and key tiles of all sequences
-  int b, rt, t;
-};
-
 // The place at weight y of sequence b.
-__device__ __forceinline__ Place place_of(const ChunkParams& p, int b, const Sequence& s, int64_t y, int64_t width) {
+__device__ __forceinline__ Place place_of(const ChunkParams& p, int b, const Sequence& s, int y, int width) {
   const Weights w = weights(p, s);
   int lo = 0, hi = row_tiles(p, s) - 1;   // the last row tile that begins at or before y
-  const int64_t wh = w.base * p.H, x = (y + 1) * p.H;
   while (lo < hi) {
-    const int64_t mid = (lo + hi + 1) / 2;
-    if (mid * wh + (p.causal ? 2 * w.unit * mid * (mid + 1) : 0) < x) lo = (int)mid; else hi = (int)mid - 1;
+    const int mid = (lo + hi + 1) / 2;
+    if (weight(p, w, mid) <= y) lo = mid; else hi = mid - 1;
   }
-  const int nt = key_tiles(p, s, lo), snap = (int)min((int64_t)kSnap, width / (4 * w.unit));
-  int t = (int)min((int64_t)nt, max((int64_t)0, y - weight(p, s, lo) - w.cost) / w.unit);
+  const int nt = key_tiles(p, s, lo), snap = min(kSnap, width >> (w.unit + 1) << p.weight_shift);
+  const int64_t in = (int64_t)(y - weight(p, w, lo)) << p.weight_shift;
+  int t = (int)min((int64_t)nt, max((int64_t)0, in - w.cost) >> (w.unit - 1));
   if (t <= snap) t = 0;
   if (t > 0 && nt - t <= snap) return Place{b, lo + 1, 0};
   return Place{b, lo, t};
@@ -783,180 +785,180 @@ __device__ __forceinline__ Place place_of(const ChunkParams& p, int b, const Seq
 // packed query q0 and first row, w how its first part goes on: 1 it ends here, 2 it does not.
 typedef int4 RangeLink;
 
-__global__ __launch_bounds__(kThreads, 1) void chunk_kernel(ChunkParams p) {
-  __shared__ __attribute__((aligned(1024))) char mem[kLdsBytes];
-  __shared__ __attribute__((aligned(16))) float stat[kRows], top[kRows];
-  __shared__ __attribute__((aligned(16))) int flag[kWaves];
-  __shared__ __attribute__((aligned(16))) Window win;
-  const unsigned base = lds_addr((DMLA_LDS char*)mem);
-  const Lds lds = {base, base + kSlots * kKeyBytes, base + kSlots * (kKeyBytes + kRopeBytes), (DMLA_LDS float*)stat, (DMLA_LDS float*)top,
-                   (DMLA_LDS int*)flag};
-  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
-  // Ranges that follow each other run on one XCD: they read the same keys.
-  const int per_xcd = (p.n_ranges + 7) / 8;
-  const int range = (int)(blockIdx.x % 8) * per_xcd + (int)(blockIdx.x / 8);
-  if (range >= p.n_ranges) return;
+// The window from sequence b0 on; this thread's sequence.
+__device__ __forceinline__ Sequence load_window(const ChunkParams& p, DMLA_LDS Window* win, int b0) {
+  const int tid = threadIdx.x;
+  __syncthreads();   // the window is read
+  Sequence s = {0, 0, 0};
+  if (b0 + tid < p.B) s = sequence(p, b0 + tid);
+  win->q0[tid] = s.q0;
+  win->n[tid] = s.n;
+  win->len[tid] = s.len;
+  if (tid == 0) win->first = b0;
+  return s;
+}
+__device__ __forceinline__ Sequence known(const DMLA_LDS Window* win, int i) {
+  return Sequence{uniform(win->q0[i]), uniform(win->n[i]), uniform(win->len[i])};
+}
 
-  int window = 0;   // first sequence of the window
-  auto load_window = [&](int b0) {
-    __syncthreads();   // the window is read
-    Sequence s = {0, 0, 0};
-    if (b0 + tid < p.B) s = sequence(p, b0 + tid);
-    win.q0[tid] = s.q0;
-    win.n[tid] = s.n;
-    win.len[tid] = s.len;
-    window = b0;
-    return s;
-  };
-  auto known = [&](int b) {   // of the window
-    const int i = b - window;
-    return Sequence{uniform(win.q0[i]), uniform(win.n[i]), uniform(win.len[i])};
-  };
+// The range's end and its first place; whether it has any.
+__device__ __forceinline__ bool cut(const ChunkParams& p, DMLA_LDS Window* win, int range) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   // Inclusive sum over the threads and their total.
-  auto scan = [&](int64_t v, int64_t& sum) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int64_t y = __shfl_up(v, o, 64);
-      if (lane >= o) v += y;
-    }
-    __syncthreads();   // tmp is read
-    if (lane == 63) win.tmp[wave] = v;
+  auto scan = [&](int v, int& sum) {
+    v = lane_scan(v);
+    if (lane == 63) win->tmp[wave] = v;
     __syncthreads();
     sum = 0;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
-      if (w < wave) v += win.tmp[w];
-      sum += win.tmp[w];
+      if (w < wave) v += win->tmp[w];
+      sum += win->tmp[w];
     }
     return v;
   };
-  int64_t total = 0, upto = 0, mine = 0, sum;
+  int total = 0, upto = 0, mine = 0, sum = 0;
+  Sequence s = {0, 0, 0};
   for (int b0 = 0; b0 < p.B; b0 += kThreads) {
-    const Sequence s = load_window(b0);
-    mine = weight(p, s, row_tiles(p, s));
+    s = load_window(p, win, b0);
+    mine = weight(p, weights(p, s), row_tiles(p, s));
     upto = scan(mine, sum);
     total += sum;
   }
-  const int64_t width = max((int64_t)kMinWidth, (total + p.n_ranges - 1) / p.n_ranges);
-  const int64_t x0 = range * width, x1 = min(x0 + width, total);
-  if (x0 >= total) {
-    if (tid == 0) p.links[range] = make_int4(0, 0, 0, 0);
-    return;
-  }
-  // The sequences at x0 and at x1 - 1, and the weights in them.
-  if (tid == 0) win.at[0] = win.at[1] = -1;
-  int64_t before = 0;
-  for (int b0 = 0; b0 < p.B; b0 += kThreads) {
+  const int width = max(max(1, kMinWidth >> p.weight_shift), (int)(((int64_t)total + p.n_ranges - 1) / p.n_ranges));
+  const int x0 = (int)min((int64_t)range * width, (int64_t)total), x1 = (int)min((int64_t)x0 + width, (int64_t)total);
+  if (tid == 0) p.links[range] = make_int4(0, 0, 0, 0);
+  if (x0 >= total) return false;
+  // The places of x0 and x1, by the threads whose sequences hold them; x1 at the end of one is that end.
+  for (int b0 = 0, before = 0; b0 < p.B && before < x1; b0 += kThreads, before += sum) {
     if (p.B > kThreads) {
-      const Sequence s = load_window(b0);
-      mine = weight(p, s, row_tiles(p, s));
+      s = load_window(p, win, b0);
+      mine = weight(p, weights(p, s), row_tiles(p, s));
       upto = scan(mine, sum);
-    } else {
-      __syncthreads();
     }
-    const int64_t lo = before + upto - mine, hi = before + upto;
-    if (lo <= x0 && x0 < hi) {
-      win.at[0] = b0 + tid;
-      win.rest[0] = x0 - lo;
-    }
-    if (lo < x1 && x1 <= hi) {
-      win.at[1] = b0 + tid;
-      win.rest[1] = x1 - lo;
-    }
-    before += sum;
-    if (before >= x1) break;   // (the same for all threads)
+    const int lo = before + upto - mine, hi = before + upto;
+    auto put = [](DMLA_LDS Place* to, const Place& v) {
+      to->b = v.b;
+      to->rt = v.rt;
+      to->t = v.t;
+    };
+    if (lo <= x0 && x0 < hi) put(&win->at, place_of(p, b0 + tid, s, x0 - lo, width));
+    if (lo < x1 && x1 <= hi) put(&win->end, x1 == hi ? Place{b0 + tid, row_tiles(p, s), 0} : place_of(p, b0 + tid, s, x1 - lo, width));
   }
   __syncthreads();
-  const int b_first = uniform(win.at[0]), b_last = uniform(win.at[1]);
-  const int64_t y0 = win.rest[0], y1 = win.rest[1];
-  auto sequence_at = [&](int b) {
-    if (b < window || b >= window + kThreads) {
-      load_window(b);
-      __syncthreads();
+  const int b = uniform(win->at.b), first = uniform(win->first);
+  if (b < first || b >= first + kThreads) {
+    load_window(p, win, b);
+    __syncthreads();
+  }
+  return true;
+}
+
+// The next piece of the range (rows 0: none).  What it goes by is in LDS and not in registers: run_piece has none to
+// spare, and a value reloaded from scratch memory would wait for every copy and store in flight.
+__device__ __forceinline__ void next_piece(const ChunkParams& p, DMLA_LDS Window* win, DMLA_LDS i32x4* to, int range) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  Place at = {uniform(win->at.b), uniform(win->at.rt), uniform(win->at.t)};
+  const Place end = {uniform(win->end.b), uniform(win->end.rt), uniform(win->end.t)};
+  Sequence s;
+  for (;;) {
+    if (!(at.b < end.b || (at.b == end.b && (at.rt < end.rt || (at.rt == end.rt && at.t < end.t))))) {
+      if (tid == 0) to[0] = i32x4{0, 0, 0, 0};
+      return;
     }
-    return known(b);
-  };
-  Sequence s = sequence_at(b_last);
-  // The end of the last sequence's work is its last row tile's.
-  Place end = place_of(p, b_last, s, y1, width);
-  if (y1 >= weight(p, s, row_tiles(p, s))) end = Place{b_last, row_tiles(p, s), 0};
-  s = sequence_at(b_first);
-  Place at = place_of(p, b_first, s, y0, width);
-  end.rt = uniform(end.rt); end.t = uniform(end.t);
-  at.rt = uniform(at.rt); at.t = uniform(at.t);
-  RangeLink link = make_int4(0, 0, 0, 0);
-  // The piece at `at`, which moves on; none: rows 0.
-  auto piece = [&](DMLA_LDS int* to) {
-    for (;;) {
-      if (!(at.b < end.b || (at.b == end.b && (at.rt < end.rt || (at.rt == end.rt && at.t < end.t))))) {
-        if (tid == 0) to[2] = 0;
-        return;
+    int first = uniform(win->first);
+    s = known(win, at.b - first);
+    if (at.rt < row_tiles(p, s)) break;
+    // The next sequence with queries (there is one, end.b at the latest): 256 looked at together.
+    int b = at.b + 1;
+    for (;; b = first + kThreads) {
+      if (b >= first + kThreads) {
+        load_window(p, win, b);
+        __syncthreads();
+        first = b;
       }
-      if (at.rt < row_tiles(p, s)) break;
-      // The next sequence with queries: 256 looked at together.
-      int b = at.b + 1;
-      for (;; b = window + kThreads) {
-        if (b >= window + kThreads) {
-          load_window(b);
-          __syncthreads();
-        }
-        int found = kThreads;
-        for (int i0 = (b - window) & ~63; i0 < kThreads; i0 += 64) {
-          const unsigned long long m = __ballot(i0 + lane >= b - window && win.n[i0 + lane] > 0);
-          if (m != 0) {
-            found = i0 + __builtin_ctzll(m);
-            break;
-          }
-        }
-        if (found < kThreads) {
-          b = window + found;
+      int found = kThreads;
+      for (int i0 = (b - first) & ~63; i0 < kThreads; i0 += 64) {
+        const unsigned long long m = __ballot(i0 + lane >= b - first && win->n[i0 + lane] > 0);
+        if (m != 0) {
+          found = i0 + __builtin_ctzll(m);
           break;
         }
       }
-      at = Place{uniform(b), 0, 0};
-      s = known(at.b);
+      if (found < kThreads) {
+        b = first + found;
+        break;
+      }
     }
-    const int nt = key_tiles(p, s, at.rt), row0 = at.rt * kRows, rows = min(s.n * p.H - row0, kRows);
-    const bool whole = !(at.b == end.b && at.rt == end.rt);   // to its end
-    const int slot = at.t > 0 ? 2 * range : whole ? -1 : 2 * range + 1;
-    if (at.t > 0) link.w = whole ? 1 : 2;
-    else if (!whole) link = make_int4(rows, s.q0, row0, link.w);
-    if (tid == 0) {
-      to[0] = s.q0;
-      to[1] = row0;
-      to[2] = rows;
-      to[3] = s.n;
-      to[4] = s.len;
-      to[5] = at.b;
-      to[6] = at.t;
-      to[7] = whole ? nt : min(end.t, nt);
-      to[8] = slot;
+    at = Place{uniform(b), 0, 0};
+  }
+  const int row0 = at.rt * kRows, rows = min(s.n * p.H - row0, kRows);
+  const bool whole = !(at.b == end.b && at.rt == end.rt);   // to its end
+  __syncthreads();   // the place is read
+  if (tid == 0) {
+    to[0] = i32x4{s.q0, row0, rows, s.n};
+    to[1] = i32x4{s.len, at.b, at.t, whole ? key_tiles(p, s, at.rt) : end.t};
+    to[2] = i32x4{at.t > 0 ? 2 * range : whole ? -1 : 2 * range + 1, 0, 0, 0};
+    RangeLink* link = p.links + range;
+    if (at.t > 0) {
+      link->w = whole ? 1 : 2;
+    } else if (!whole) {
+      link->x = rows;
+      link->y = s.q0;
+      link->z = row0;
     }
-    if (whole) {
-      ++at.rt;
-      at.t = 0;
-    } else {
-      at = end;
-    }
+    win->at.b = at.b;
+    win->at.rt = whole ? at.rt + 1 : at.rt;
+    win->at.t = whole ? 0 : end.t;
+  }
+}
+
+// A copy of the kernel's arguments, read again: kept in scalar registers from piece to piece they would be spilled.
+struct ArgumentWords {
+  int w[sizeof(ChunkParams) / 4];
+};
+static_assert(sizeof(ArgumentWords) == sizeof(ChunkParams), "whole words");
+__device__ __forceinline__ ChunkParams arguments() {
+  auto a = (const __attribute__((address_space(4))) int*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(a));
+  ArgumentWords words;
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(ChunkParams) / 4); ++i) words.w[i] = a[i];
+  return __builtin_bit_cast(ChunkParams, words);
+}
+
+__global__ __launch_bounds__(kThreads, 1) void chunk_kernel(ChunkParams) {
+  __shared__ __attribute__((aligned(1024))) char mem[kLdsBytes];
+  __shared__ __attribute__((aligned(16))) float stat[kRows], top[kRows];
+  __shared__ __attribute__((aligned(16))) int flag[kWaves];
+  __shared__ __attribute__((aligned(16))) Window window;
+  DMLA_LDS Window* win = (DMLA_LDS Window*)&window;
+  DMLA_LDS i32x4* pieces = (DMLA_LDS i32x4*)window.piece;
+  const unsigned base = lds_addr((DMLA_LDS char*)mem);
+  const Lds lds = {base, base + kSlots * kKeyBytes, base + kSlots * (kKeyBytes + kRopeBytes), (DMLA_LDS float*)stat, (DMLA_LDS float*)top,
+                   (DMLA_LDS int*)flag};
+  // Ranges that follow each other run on one XCD: they read the same keys.
+  auto my_range = [&] {
+    const int per_xcd = (arguments().n_ranges + 7) / 8;
+    return (int)(blockIdx.x % 8) * per_xcd + (int)(blockIdx.x / 8);
   };
-  DMLA_LDS int* pieces = (DMLA_LDS int*)win.piece;
-  piece(pieces);
+  if (my_range() >= arguments().n_ranges) return;
+  if (!cut(arguments(), win, my_range())) return;
+  next_piece(arguments(), win, pieces, my_range());
   bool have = false;
   for (int turn = 0;; turn ^= 1) {
-    DMLA_LDS int* now = pieces + turn * kPieceInts;
-    DMLA_LDS int* next = pieces + (turn ^ 1) * kPieceInts;
+    DMLA_LDS i32x4* now = pieces + 3 * turn;
+    DMLA_LDS i32x4* other = pieces + 3 * (turn ^ 1);
     __syncthreads();   // this piece is known, the one before it is read
-    if (uniform(now[2]) == 0) break;
-    Piece pc;
-    pc.s = Sequence{uniform(now[0]), uniform(now[3]), uniform(now[4])};
-    pc.row0 = uniform(now[1]);
-    pc.b = uniform(now[5]);
-    pc.t0 = uniform(now[6]);
-    pc.t1 = uniform(now[7]);
-    pc.slot = uniform(now[8]);
-    piece(next);
+    const i32x4 a = now[0], b = now[1];
+    if (uniform(a[2]) == 0) break;
+    next_piece(arguments(), win, other, my_range());
+    const ChunkParams p = arguments();
+    const Piece pc = {Sequence{uniform(a[0]), uniform(a[3]), uniform(b[0])}, uniform(b[1]), uniform(a[1]), uniform(b[2]), uniform(b[3]),
+                      uniform(now[2][0])};
+    const DMLA_LDS int* next = (const DMLA_LDS int*)other;
     Pass pass = {false, (int)0x80000000, 0x7fffffff};
-    const bool few = narrow(uniform(now[2]));
+    const bool few = narrow(uniform(a[2]));
     for (;;) {
       const bool again = few ? run_piece<true>(p, pc, lds, pass, have, next) : run_piece<false>(p, pc, lds, pass, have, next);
       have = true;
@@ -970,7 +972,6 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_kernel(ChunkParams p) {
       have = false;
     }
   }
-  if (tid == 0) p.links[range] = link;
 }
 
 // Row tiles that span ranges: o = sum_j w_j o_j / sum_j w_j with w_j = 2^(lse_j - max); and the queries behind the last
@@ -1079,11 +1080,14 @@ __global__ __launch_bounds__(256) void chunk_combine_kernel(ChunkParams p) {
   }
 }
 
+// At least the weight that the kernel adds up.
+int64_t chunk_weight(int64_t T, int64_t B, int64_t H, int64_t max_pages) {
+  const int64_t tiles = T * H / kRows + std::min(B, T);
+  return tiles * (kCost + 4 + max_pages * (2 * kPage / kTile));
+}
 // Ranges of a call: one per CU, as many as its work can fill at most.
 int64_t chunk_ranges(int64_t T, int64_t B, int64_t H, int64_t max_pages) {
-  const int64_t tiles = T * H / kRows + std::min(B, T);
-  const int64_t most = tiles * (kCost + 2 + max_pages * (2 * kPage / kTile)) + 4 * T;   // at least what the kernel adds up
-  return std::max<int64_t>(1, std::min<int64_t>(device_cu_count(), (most + kMinWidth - 1) / kMinWidth));
+  return std::max<int64_t>(1, std::min<int64_t>(device_cu_count(), (chunk_weight(T, B, H, max_pages) + kMinWidth - 1) / kMinWidth));
 }
 int64_t chunk_bytes(int64_t ranges) { return ranges * (2 * kRows * (int64_t)(kDv + 1) * 4 + (int64_t)sizeof(RangeLink)); }
 
@@ -1145,6 +1149,9 @@ extern "C" int dmla_chunk_paged(const void* q, const void* kv_pool, const int32_
   p.hdiv = make_fastdiv((unsigned)H);
   p.scale_log2 = softmax_scale * kLog2e;
   p.n_ranges = (int)chunk_ranges(T, B, H, max_pages_per_seq);
+  p.two_by_h = 2.0f / (float)H;
+  while (chunk_weight(T, B, H, max_pages_per_seq) >> p.weight_shift > (int64_t)1 << 30) ++p.weight_shift;
+  p.weight_scale = std::ldexp(1.0f, -p.weight_shift);
   if (B == 0) {   // nothing but queries behind the last sequence
     p.n_ranges = 0;
     hipLaunchKernelGGL(chunk_combine_kernel, dim3(256), dim3(256), 0, (hipStream_t)stream, p);
