@@ -64,6 +64,21 @@ struct ChunkParams {
   int weight_shift;
 };
 
+// A copy of the kernel's arguments, read again: kept in scalar registers from piece to piece, or over a tile loop that
+// needs a few of them, they would be spilled.
+struct ArgumentWords {
+  int w[sizeof(ChunkParams) / 4];
+};
+static_assert(sizeof(ArgumentWords) == sizeof(ChunkParams), "whole words");
+__device__ __forceinline__ ChunkParams arguments() {
+  auto a = (const __attribute__((address_space(4))) int*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(a));
+  ArgumentWords words;
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(ChunkParams) / 4); ++i) words.w[i] = a[i];
+  return __builtin_bit_cast(ChunkParams, words);
+}
+
 // A sequence's queries: q0 .. q0 + n - 1, the newest of its len tokens.
 struct Sequence {
   int q0, n, len;
@@ -161,8 +176,9 @@ __device__ __forceinline__ void copy_queries(const ChunkParams& p, const Lds& ld
 // Whether another pass has to follow.
 // have: the queries are on their way.  After it, those of the next piece's rows are.
 template <bool kNarrow>
-__device__ __forceinline__ bool run_piece(const ChunkParams& p, const Piece& pc, const Lds& lds, const Pass& pass, bool have,
+__device__ __forceinline__ bool run_piece(const Piece& pc, const Lds& lds, const Pass& pass, bool have,
                                           const DMLA_LDS int* next) {
+  const ChunkParams p = arguments();
   const int lane = fresh_lane_id();
   const int l32 = lane & 31, hl = lane >> 5;
   const int wave = uniform(threadIdx.x >> 6);
@@ -552,6 +568,7 @@ __device__ __forceinline__ bool run_piece(const ChunkParams& p, const Piece& pc,
   if constexpr (kNarrow) lsum = total_of(lsum, [](float a, float b) { return a + b; });
 
   // ---- output ----
+  const ChunkParams out = arguments();
   if constexpr (!kNarrow) lsum = half_sum(lsum);
   if (hl == 0 && (!kNarrow || wave == 0)) {
     if (!pass.careful) lds.top[first_row + l32] = mtrue;
@@ -565,20 +582,20 @@ __device__ __forceinline__ bool run_piece(const ChunkParams& p, const Piece& pc,
   auto written = [&](int row) {
     bool w = row < rows;
     if (pass.careful) {
-      const int l = limit_of(row);
+      const int l = out.causal ? pc.s.len - pc.s.n + fast_div(pc.row0 + min(row, rows - 1), out.hdiv) : pc.s.len - 1;
       w = w && l >= pass.from && l < pass.to;
     }
     return w;
   };
   auto place = [&](int row, int64_t st, int64_t sh) {   // of a row in o
-    const int r = pc.row0 + row, token = fast_div(r, p.hdiv);
-    return (pc.s.q0 + token) * st + (r - token * p.H) * sh;
+    const int r = pc.row0 + row, token = fast_div(r, out.hdiv);
+    return (pc.s.q0 + token) * st + (r - token * out.H) * sh;
   };
   if (hl == 0 && (!kNarrow || wave == 0) && written(first_row + l32)) {
     const float sum = lds.stat[first_row + l32];
     const float lse2 = sum == 0.f ? kNegInf : mref + __log2f(sum);
-    if (pc.slot >= 0) p.part_lse[(int64_t)pc.slot * kRows + first_row + l32] = lse2;
-    else if (p.lse != nullptr) p.lse[place(first_row + l32, p.H, 1)] = lse2 * kLn2;
+    if (pc.slot >= 0) out.part_lse[(int64_t)pc.slot * kRows + first_row + l32] = lse2;
+    else if (out.lse != nullptr) out.lse[place(first_row + l32, out.H, 1)] = lse2 * kLn2;
   }
   // Through LDS, so that a store covers whole lines: 256 bytes of each of 4 rows, or of a part 512 bytes of each of 2.
   // A wave has its own memory there.
@@ -598,14 +615,14 @@ __device__ __forceinline__ bool run_piece(const ChunkParams& p, const Piece& pc,
     const int g = lane >> 4, c = lane & 15;
     const unsigned get = lds_sum(256 * g + 16 * (c ^ g), mine);   // 8 columns of row g
     // Where rows follow each other evenly (contiguous outputs), offsets from the first one need no division.
-    const bool even = p.o_st == p.H * p.o_sh && p.o_sh < (1 << 20);
-    const int out_step = (int)p.o_sh;
-    bf16* first = p.o + pc.s.q0 * p.o_st + pc.row0 * p.o_sh + 128 * wave + (g * out_step + 8 * c);
-    const bool plain = even && rows == kRows && !pass.careful;
+    const bool even = out.o_st == out.H * out.o_sh && out.o_sh < (1 << 20);
+    const int out_step = (int)out.o_sh;
+    bf16* first = out.o + pc.s.q0 * out.o_st + pc.row0 * out.o_sh + 128 * wave + (g * out_step + 8 * c);
+    const bool plain = even && !pass.careful;
 #pragma unroll
     for (int n = 0; n < kRowBlocks; ++n) {
       const bf16* src = nullptr;
-      if (next_rows > 0) src = query_rows(p, wave, next_q0, next_row0, next_rows, n);
+      if (next_rows > 0) src = query_rows(out, wave, next_q0, next_row0, next_rows, n);
       auto ask = [&](int i) {
         if (next_rows > 0 && i < (narrow(next_rows) ? 3 : kQueryEarly))
           dma16_addr(src + query_dims(wave, next_rows, i), query_block(lds, wave, i) + n * 1024);
@@ -636,14 +653,13 @@ __device__ __forceinline__ bool run_piece(const ChunkParams& p, const Piece& pc,
       for (int r = 0; r < 8; ++r) v[r] = *lds_ptr<const bf16x8>((get ^ (64 * (r & 3))) + 1024 * r);
       if (plain) {
 #pragma unroll
-        for (int r = 0; r < 8; ++r) *reinterpret_cast<bf16x8*>(first + (32 * n + 4 * r) * out_step) = v[r];
+        for (int r = 0; r < 8; ++r)
+          if (32 * n + 4 * r + g < rows) *reinterpret_cast<bf16x8*>(first + (32 * n + 4 * r) * out_step) = v[r];
       } else {
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
           const int row = 32 * n + 4 * r + g;
-          if (!written(row)) continue;
-          if (even) *reinterpret_cast<bf16x8*>(first + (32 * n + 4 * r) * out_step) = v[r];
-          else *reinterpret_cast<bf16x8*>(p.o + place(row, p.o_st, p.o_sh) + 128 * wave + 8 * c) = v[r];
+          if (written(row)) *reinterpret_cast<bf16x8*>(out.o + place(row, out.o_st, out.o_sh) + 128 * wave + 8 * c) = v[r];
         }
       }
     }
@@ -652,7 +668,7 @@ __device__ __forceinline__ bool run_piece(const ChunkParams& p, const Piece& pc,
     const unsigned mine = lds.keys + wave * kKeyBytes;
     const unsigned put = lds_sum(512 * l32 + 16 * ((4 * hl) ^ l32), mine);
     const unsigned get = lds_sum(512 * hl + 16 * (l32 ^ hl), mine);     // 4 columns of row hl
-    float* part = p.part_o + (int64_t)pc.slot * kRows * kDv + 128 * wave;
+    float* part = out.part_o + (int64_t)pc.slot * kRows * kDv + 128 * wave;
 #pragma unroll
     for (int n = 0; n < kBlocks; ++n) {
       if (32 * n >= rows) break;
@@ -684,8 +700,8 @@ __device__ __forceinline__ bool run_piece(const ChunkParams& p, const Piece& pc,
   // The rest of the next queries, while the piece after that is worked out.
   const int next_q0 = uniform(next[0]), next_row0 = uniform(next[1]), next_rows = uniform(next[2]);
   if (next_rows > 0) {
-    if (pc.slot >= 0) copy_queries<0, kQueryEarly>(p, lds, wave, next_q0, next_row0, next_rows);
-    copy_queries<kQueryEarly, 3>(p, lds, wave, next_q0, next_row0, next_rows);
+    if (pc.slot >= 0) copy_queries<0, kQueryEarly>(out, lds, wave, next_q0, next_row0, next_rows);
+    copy_queries<kQueryEarly, 3>(out, lds, wave, next_q0, next_row0, next_rows);
   }
   return uniform(lds.flag[0] | lds.flag[1] | lds.flag[2] | lds.flag[3]) != 0;
 }
@@ -913,20 +929,6 @@ __device__ __forceinline__ void next_piece(const ChunkParams& p, DMLA_LDS Window
   }
 }
 
-// A copy of the kernel's arguments, read again: kept in scalar registers from piece to piece they would be spilled.
-struct ArgumentWords {
-  int w[sizeof(ChunkParams) / 4];
-};
-static_assert(sizeof(ArgumentWords) == sizeof(ChunkParams), "whole words");
-__device__ __forceinline__ ChunkParams arguments() {
-  auto a = (const __attribute__((address_space(4))) int*)__builtin_amdgcn_kernarg_segment_ptr();
-  asm volatile("" : "+s"(a));
-  ArgumentWords words;
-#pragma unroll
-  for (int i = 0; i < (int)(sizeof(ChunkParams) / 4); ++i) words.w[i] = a[i];
-  return __builtin_bit_cast(ChunkParams, words);
-}
-
 __global__ __launch_bounds__(kThreads, 1) void chunk_kernel(ChunkParams) {
   __shared__ __attribute__((aligned(1024))) char mem[kLdsBytes];
   __shared__ __attribute__((aligned(16))) float stat[kRows], top[kRows];
@@ -953,16 +955,16 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_kernel(ChunkParams) {
     const i32x4 a = now[0], b = now[1];
     if (uniform(a[2]) == 0) break;
     next_piece(arguments(), win, other, my_range());
-    const ChunkParams p = arguments();
     const Piece pc = {Sequence{uniform(a[0]), uniform(a[3]), uniform(b[0])}, uniform(b[1]), uniform(a[1]), uniform(b[2]), uniform(b[3]),
                       uniform(now[2][0])};
     const DMLA_LDS int* next = (const DMLA_LDS int*)other;
     Pass pass = {false, (int)0x80000000, 0x7fffffff};
     const bool few = narrow(uniform(a[2]));
     for (;;) {
-      const bool again = few ? run_piece<true>(p, pc, lds, pass, have, next) : run_piece<false>(p, pc, lds, pass, have, next);
+      const bool again = few ? run_piece<true>(pc, lds, pass, have, next) : run_piece<false>(pc, lds, pass, have, next);
       have = true;
       if (pass.careful ? pass.to == 0x7fffffff : !again) break;
+      const ChunkParams p = arguments();
       const int base = pc.s.len - pc.s.n, last = min(pc.row0 + kRows, pc.s.n * p.H) - 1;
       const int first_lim = p.causal ? base + fast_div(pc.row0, p.hdiv) : pc.s.len - 1;
       const int last_lim = p.causal ? base + fast_div(last, p.hdiv) : pc.s.len - 1;
