@@ -1,0 +1,186 @@
+"""Chunk attention where its cut into ranges can go wrong: hundreds of sequences with empty ones between, tables of
+a million pages, row tiles in two parts and in hundreds; and rows few enough that the waves share their scores."""
+import math
+import random
+
+import pytest
+import torch
+
+from paging import D_QK, D_V, PAGE, assert_attention, attention64, ints, pages, paged, starts
+
+pytestmark = pytest.mark.gpu
+SCALE = 1.0 / math.sqrt(192.0)
+
+
+def queries(T, H, seed, scale=0.5):
+    g = torch.Generator().manual_seed(1000 + seed)
+    return (torch.randn(T, H, D_QK, generator=g) * scale).to(torch.bfloat16)
+
+
+def check(q, o, lse, rows, lens, counts, causal=True, some=None, what=""):
+    """Against the plain form, of `some` queries or of all."""
+    at, o, lse = 0, o.cpu(), lse.cpu()
+    for r, N, n in zip(rows, lens, counts):
+        mine = [i for i in range(n) if some is None or at + i in some]
+        if mine:
+            at_these = [at + i for i in mine]
+            ref = attention64(q[at_these], r, [N - n + i + 1 if causal else N for i in mine], SCALE)
+            assert_attention(o[at_these], lse[at_these], ref, what or f"queries {at_these[0]} to {at_these[-1]}")
+        at += n
+
+
+def run(gpu, q, pool, table, lens, counts, causal=True):
+    from python import ops
+    return ops.flash_dmla_chunk_paged(q.to(gpu), pool, table, ints(lens, gpu), ints(starts(counts), gpu), softmax_scale=SCALE,
+                                      causal=causal, return_lse=True)
+
+
+@pytest.mark.parametrize("H", [1, 16, 128])
+@pytest.mark.parametrize("causal", [True, False])
+def test_hundreds_of_sequences(gpu, H, causal):
+    r = random.Random(H)
+    lens = [r.choice([0, 1, 31, 64, r.randint(1, 200)]) for _ in range(700)]
+    counts = [r.choice([0, 0, 1, 1, 2, 5]) for _ in lens]
+    pool, table, rows = paged(lens, gpu, seed=H)
+    q = queries(sum(counts), H, H)
+    o, lse = run(gpu, q, pool, table, lens, counts, causal)
+    check(q, o, lse, rows, lens, counts, causal)
+
+
+@pytest.mark.parametrize("B,only", [(257, 256), (600, 599), (600, 0), (1025, 512), (3000, 2047)])
+@pytest.mark.parametrize("H,n,N", [(16, 1, 70), (128, 3, 1000)])
+def test_one_sequence_among_empty_ones(gpu, B, only, H, n, N):
+    """A padded batch: the other sequences have neither tokens nor queries, or tokens alone."""
+    lens, counts = [0] * B, [0] * B
+    lens[only], counts[only] = N, n
+    if only > 3:
+        lens[3] = 100
+    pool, table, rows = paged(lens, gpu)
+    q = queries(n, H, 1)
+    o, lse = run(gpu, q, pool, table, lens, counts)
+    check(q, o, lse, rows, lens, counts)
+
+
+@pytest.mark.parametrize("B", [1, 255, 256, 257, 800])
+def test_batches_without_a_token(gpu, B):
+    pool, table, _ = paged([0] * B, gpu)
+    o, lse = run(gpu, queries(B, 16, 1), pool, table, [0] * B, [1] * B)
+    assert (o == 0).all() and (lse == float("-inf")).all()
+
+
+@pytest.mark.parametrize("H,lens,counts", [
+    (16, [300], [1]), (16, [900], [1]), (16, [2500, 2500], [1, 1]), (16, [20000], [1]), (16, [20000, 11], [2, 1]),
+    (128, [300], [1]), (128, [700, 900], [1, 1]), (128, [3000] * 9, [1] * 9), (128, [17000] * 3, [1] * 3), (128, [30000], [1]),
+    (20, [9000] * 5, [1, 2, 3, 9, 17]), (33, [4000, 1000], [3, 40]), (64, [1500] * 30, [2] * 30)])
+def test_row_tiles_in_parts(gpu, H, lens, counts):
+    """Two parts of a row tile and hundreds, of all 128 rows and of few."""
+    pool, table, rows = paged(lens, gpu, seed=H)
+    q = queries(sum(counts), H, H)
+    o, lse = run(gpu, q, pool, table, lens, counts)
+    check(q, o, lse, rows, lens, counts)
+
+
+@pytest.mark.parametrize("H", [16, 128])
+def test_parts_without_a_weight(gpu, H):
+    """Scores of minus infinity over many parts: a query sees the other tokens alone."""
+    N = 9000
+    pool, table, rows = paged([N], gpu)
+    q = queries(1, H, 2)
+    q[:, :, D_V] = q[:, :, D_V].abs() + 1
+    for gone in (range(0, 8000), range(100, 8991), range(1000, 9000)):
+        p = pool.clone()
+        for j in range(gone[0] // PAGE, gone[-1] // PAGE + 1):
+            a, b = max(gone[0] - PAGE * j, 0), min(gone[-1] + 1 - PAGE * j, PAGE)
+            p[table[0, j].item(), a:b, D_V] = float("-inf")
+        o, lse = run(gpu, q, p, table, [N], [1])
+        left = rows[0][[j for j in range(N) if j not in gone]]
+        ref = attention64(q, left, [len(left)], SCALE)
+        assert_attention(o, lse, ref, f"without {gone}")
+
+
+@pytest.mark.parametrize("H", [16, 128])
+def test_not_a_number_in_one_part_reaches_the_rows_that_see_it(gpu, H):
+    lens, counts = [9000, 5000], [3, 2]
+    pool, table, rows = paged(lens, gpu)
+    q = queries(5, H, 3)
+    for at in (0, 4000, 8998):
+        p = pool.clone()
+        p[table[0, at // PAGE].item(), at % PAGE, 7] = float("nan")
+        o, lse = run(gpu, q, p, table, lens, counts)
+        clean = [i for i in range(5) if i >= 3 or 8997 + i < at]
+        check(q, o, lse, rows, lens, counts, some=clean)
+        hit = [i for i in range(5) if i not in clean]
+        assert torch.isnan(o[hit]).any(2).all()
+
+
+def test_tables_of_a_million_pages(gpu):
+    """The weights of a row tile pass 32 bits where each may have a million pages: they are taken in larger units."""
+    lens, counts, H = [9000, 700], [8000, 200], 64
+    pool, table, rows = paged(lens, gpu)
+    wide = torch.full((2, 1 << 20), -1, dtype=torch.int32, device=gpu)
+    wide[:, :table.shape[1]] = table
+    q = queries(sum(counts), H, 4)
+    o, lse = run(gpu, q, pool, wide, lens, counts)
+    r = random.Random(1)
+    check(q, o, lse, rows, lens, counts, some=set([0, 7999, 8000, 8199] + r.sample(range(8200), 40)))
+    near, near_lse = run(gpu, q, pool, table, lens, counts)
+    # Two answers within a tolerance each, of outputs that are a mean of values up to 3 (0.5 x 6 standard deviations).
+    assert ((o.float() - near.float()).abs() <= 4 * 2.0 ** -8 * 3).all() and torch.isfinite(o).all()
+    assert ((lse - near_lse).abs() <= 2.0 ** -14 * (1 + lse.abs())).all()
+
+
+# ---- up to 32 rows: the waves share the scores ---------------------------------------------------------
+
+@pytest.mark.parametrize("H,n", [(1, 1), (1, 31), (1, 32), (1, 33), (2, 16), (4, 8), (16, 2), (11, 3), (31, 1), (32, 1), (33, 1)])
+@pytest.mark.parametrize("N", [33, 40, 64, 97, 1000])
+@pytest.mark.parametrize("causal", [True, False])
+def test_few_rows(gpu, H, n, N, causal):
+    lens, counts = [N, 1, N + 3], [n, 1, n]
+    pool, table, rows = paged(lens, gpu, seed=N)
+    q = queries(sum(counts), H, n)
+    o, lse = run(gpu, q, pool, table, lens, counts, causal)
+    check(q, o, lse, rows, lens, counts, causal)
+
+
+@pytest.mark.parametrize("H,n", [(16, 2), (1, 20), (5, 6)])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+def test_few_rows_and_what_they_do_not_attend(gpu, H, n, value):
+    N = 150
+    pool, table, rows = paged([N], gpu)
+    q = queries(n, H, 5)
+    for bad in ([N - 1], [N - n + 1, N - 1], [40]):
+        p = pool.clone()
+        for j in bad:
+            p[table[0, j // PAGE].item(), j % PAGE, 9] = value
+        o, lse = run(gpu, q, p, table, [N], [n])
+        clean = max(0, bad[0] - (N - n))
+        check(q, o, lse, rows, [N], [n], some=set(range(clean)))
+        assert not torch.isfinite(o[clean:, :, 9]).any()
+
+
+@pytest.mark.parametrize("H", [1, 16, 32])
+def test_few_rows_with_a_bad_page(gpu, H):
+    lens, counts = [200, 500, 64], [1, 1, 1]
+    pool, table, rows = paged(lens, gpu)
+    q = queries(3, H, 6)
+    table[1, 3] = pool.shape[0]
+    o, lse = run(gpu, q, pool, table, lens, counts)
+    check(q, o, lse, rows, lens, counts, some={0, 2})
+    assert torch.isnan(o[1]).all() and torch.isnan(lse[1]).all()
+
+
+@pytest.mark.parametrize("steepest", [4.0, 60.0])
+@pytest.mark.parametrize("H,N", [(16, 400), (32, 400), (16, 9000), (128, 9000)])
+def test_climbing_scores(gpu, H, N, steepest):
+    """Values of 2^110 under scores that climb by tens and by hundreds, within a part and over parts."""
+    rows = torch.zeros(N, D_QK)
+    rows[:, :D_V] = 2.0 ** 110
+    rows[:, D_V] = torch.linspace(0, 60, N)
+    rows = rows.to(torch.bfloat16)
+    pool = torch.zeros(pages(N), PAGE, D_QK, dtype=torch.bfloat16)
+    pool.view(-1, D_QK)[:N] = rows
+    q = torch.zeros(1, H, D_QK)
+    q[:, :, D_V] = torch.linspace(0.1, steepest, H)
+    q = q.to(torch.bfloat16)
+    o, lse = run(gpu, q, pool.to(gpu), ints([list(range(pages(N)))], gpu), [N], [1])
+    check(q, o, lse, [rows], [N], [1])
