@@ -45,17 +45,20 @@ constexpr float kHeadroom = 32.0f;                         // log2 headroom of P
 
 __device__ __forceinline__ int key_swz(int r) { return (r & 3) << 2 | (r >> 2 & 3); }
 
+// Pointers say that they are to global memory: taken out of a copy of the arguments, the compiler would not know.
+template <typename T>
+using Global = DMLA_GLOBAL T*;
+
 struct ChunkParams {
-  const bf16* q;
-  const char* kv;
-  const int32_t* block_table;
-  const int32_t* seqlens;
-  const int32_t* cu;     // nullable: one query per sequence
-  bf16* o;
-  float* lse;            // nullable
-  float* part_o;         // [2 ranges, 128 rows, 512] normalised partial outputs
-  float* part_lse;       // [2 ranges, 128 rows], log2 units
-  int4* links;           // [ranges] (RangeLink)
+  Global<const bf16> q;
+  Global<const char> kv;
+  Global<const int32_t> block_table, seqlens;
+  Global<const int32_t> cu;       // nullable: one query per sequence
+  Global<bf16> o;
+  Global<float> lse;              // nullable
+  Global<float> part_o;           // [2 ranges, 128 rows, 512] normalised partial outputs
+  Global<float> part_lse;         // [2 ranges, 128 rows], log2 units
+  Global<i32x4> links;            // [ranges] (RangeLink)
   int64_t q_st, q_sh, kv_sp, kv_ss, bt_sb, o_st, o_sh;   // kv strides in bytes
   int T, B, H, num_pages, max_pages, causal, n_ranges, groups;
   FastDiv hdiv;          // division by H
@@ -138,7 +141,7 @@ struct Pages {
     const bool off = page < 0 || page >= p.num_pages;
     bad = off ? min(bad, t / 2) : bad;
     page = off ? 0 : page;
-    return p.kv + page * p.kv_sp + (t & 1) * kTile * p.kv_ss;
+    return (const char*)(p.kv + page * p.kv_sp + (t & 1) * kTile * p.kv_ss);
   }
 };
 
@@ -160,7 +163,7 @@ __device__ __forceinline__ const bf16* query_rows(const ChunkParams& p, int wave
   const int ln = fresh_lane_id();
   const int r = row0 + min((narrow(rows) ? 0 : 32 * wave) + 8 * g + (ln >> 3), rows - 1);
   const int token = fast_div(r, p.hdiv), head = r - token * p.H;
-  return p.q + (q0 + token) * p.q_st + head * p.q_sh + 8 * ((ln & 7) ^ (ln >> 3));
+  return (const bf16*)(p.q + (q0 + token) * p.q_st + head * p.q_sh + 8 * ((ln & 7) ^ (ln >> 3)));
 }
 template <int kFirst, int kN>
 __device__ __forceinline__ void copy_queries(const ChunkParams& p, const Lds& lds, int wave, int q0, int row0, int rows) {
@@ -617,7 +620,7 @@ __device__ __forceinline__ bool run_piece(const Piece& pc, const Lds& lds, const
     // Where rows follow each other evenly (contiguous outputs), offsets from the first one need no division.
     const bool even = out.o_st == out.H * out.o_sh && out.o_sh < (1 << 20);
     const int out_step = (int)out.o_sh;
-    bf16* first = out.o + pc.s.q0 * out.o_st + pc.row0 * out.o_sh + 128 * wave + (g * out_step + 8 * c);
+    Global<bf16> first = out.o + pc.s.q0 * out.o_st + pc.row0 * out.o_sh + 128 * wave + (g * out_step + 8 * c);
     const bool plain = even && !pass.careful;
 #pragma unroll
     for (int n = 0; n < kRowBlocks; ++n) {
@@ -654,12 +657,12 @@ __device__ __forceinline__ bool run_piece(const Piece& pc, const Lds& lds, const
       if (plain) {
 #pragma unroll
         for (int r = 0; r < 8; ++r)
-          if (32 * n + 4 * r + g < rows) *reinterpret_cast<bf16x8*>(first + (32 * n + 4 * r) * out_step) = v[r];
+          if (32 * n + 4 * r + g < rows) *reinterpret_cast<Global<bf16x8>>(first + (32 * n + 4 * r) * out_step) = v[r];
       } else {
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
           const int row = 32 * n + 4 * r + g;
-          if (written(row)) *reinterpret_cast<bf16x8*>(out.o + place(row, out.o_st, out.o_sh) + 128 * wave + 8 * c) = v[r];
+          if (written(row)) *reinterpret_cast<Global<bf16x8>>(out.o + place(row, out.o_st, out.o_sh) + 128 * wave + 8 * c) = v[r];
         }
       }
     }
@@ -668,7 +671,7 @@ __device__ __forceinline__ bool run_piece(const Piece& pc, const Lds& lds, const
     const unsigned mine = lds.keys + wave * kKeyBytes;
     const unsigned put = lds_sum(512 * l32 + 16 * ((4 * hl) ^ l32), mine);
     const unsigned get = lds_sum(512 * hl + 16 * (l32 ^ hl), mine);     // 4 columns of row hl
-    float* part = out.part_o + (int64_t)pc.slot * kRows * kDv + 128 * wave;
+    Global<float> part = out.part_o + (int64_t)pc.slot * kRows * kDv + 128 * wave;
 #pragma unroll
     for (int n = 0; n < kBlocks; ++n) {
       if (32 * n >= rows) break;
@@ -688,7 +691,7 @@ __device__ __forceinline__ bool run_piece(const Piece& pc, const Lds& lds, const
       for (int r = 0; r < 16; ++r) {   // row 2 r + hl
         const f32x4 v = *lds_ptr<const f32x4>((get ^ (32 * r)) + 1024 * r);
         const int row = 32 * n + 2 * r + hl;
-        if (written(row)) *reinterpret_cast<f32x4*>(part + row * kDv + 4 * l32) = v;
+        if (written(row)) *reinterpret_cast<Global<f32x4>>(part + row * kDv + 4 * l32) = v;
       }
     }
   }
@@ -713,7 +716,7 @@ __device__ __forceinline__ Pass careful_pass(const ChunkParams& p, const Piece& 
   for (int j = max(from + 1, 0) + wave; j <= min(lim_last, pc.t1 * kTile - 1); j += kWaves) {
     const int page = uniform(p.block_table[pc.b * p.bt_sb + j / kPage]);
     if (page < 0 || page >= p.num_pages) continue;
-    const u32x4 v = *reinterpret_cast<const u32x4*>(p.kv + page * p.kv_sp + j % kPage * p.kv_ss + 16 * fresh_lane_id());
+    const u32x4 v = *reinterpret_cast<Global<const u32x4>>(p.kv + page * p.kv_sp + j % kPage * p.kv_ss + 16 * fresh_lane_id());
     bool odd = false;
 #pragma unroll
     for (int i = 0; i < 4; ++i) odd = odd || (v[i] & 0x7f80u) == 0x7f80u || (v[i] & 0x7f800000u) == 0x7f800000u;
@@ -800,7 +803,7 @@ __device__ __forceinline__ Place place_of(const ChunkParams& p, int b, const Seq
 
 // What the combine reads of a range: x the rows of a row tile that begins in it and goes on in the next (0: none), their
 // packed query q0 and first row, w how its first part goes on: 1 it ends here, 2 it does not.
-typedef int4 RangeLink;
+typedef i32x4 RangeLink;
 
 // The window from sequence b0 on; this thread's sequence.
 __device__ __forceinline__ Sequence load_window(const ChunkParams& p, DMLA_LDS Window* win, int b0) {
@@ -844,7 +847,7 @@ __device__ __forceinline__ bool cut(const ChunkParams& p, DMLA_LDS Window* win, 
   }
   const int width = max(max(1, kMinWidth >> p.weight_shift), (int)(((int64_t)total + p.n_ranges - 1) / p.n_ranges));
   const int x0 = (int)min((int64_t)range * width, (int64_t)total), x1 = (int)min((int64_t)x0 + width, (int64_t)total);
-  if (tid == 0) p.links[range] = make_int4(0, 0, 0, 0);
+  if (tid == 0) p.links[range] = i32x4{0, 0, 0, 0};
   if (x0 >= total) return false;
   // The places of x0 and x1, by the threads whose sequences hold them; x1 at the end of one is that end.
   for (int b0 = 0, before = 0; b0 < p.B && before < x1; b0 += kThreads, before += sum) {
@@ -916,13 +919,13 @@ __device__ __forceinline__ void next_piece(const ChunkParams& p, DMLA_LDS Window
     to[0] = i32x4{s.q0, row0, rows, s.n};
     to[1] = i32x4{s.len, at.b, at.t, whole ? key_tiles(p, s, at.rt) : end.t};
     to[2] = i32x4{at.t > 0 ? 2 * range : whole ? -1 : 2 * range + 1, 0, 0, 0};
-    RangeLink* link = p.links + range;
+    Global<RangeLink> link = p.links + range;
     if (at.t > 0) {
-      link->w = whole ? 1 : 2;
+      (*link)[3] = whole ? 1 : 2;
     } else if (!whole) {
-      link->x = rows;
-      link->y = s.q0;
-      link->z = row0;
+      (*link)[0] = rows;
+      (*link)[1] = s.q0;
+      (*link)[2] = row0;
     }
     win->at.b = at.b;
     win->at.rt = whole ? at.rt + 1 : at.rt;
@@ -1031,8 +1034,8 @@ __device__ __forceinline__ void join_rows(const ChunkParams& p, const Joined& t,
         for (int j = 0; j < kParts; ++j) {
           const int64_t at = t.place(min(j0 + j, t.parts - 1), min(row + r * step, t.rows - 1));
           l[r][j] = p.part_lse[at];
-          v0[r][j] = *reinterpret_cast<const f32x4*>(p.part_o + at * kDv + 8 * lane);
-          v1[r][j] = *reinterpret_cast<const f32x4*>(p.part_o + at * kDv + 8 * lane + 4);
+          v0[r][j] = *reinterpret_cast<Global<const f32x4>>(p.part_o + at * kDv + 8 * lane);
+          v1[r][j] = *reinterpret_cast<Global<const f32x4>>(p.part_o + at * kDv + 8 * lane + 4);
         }
 #pragma unroll
       for (int r = 0; r < kAt; ++r) {
@@ -1071,7 +1074,7 @@ __device__ __forceinline__ void join_rows(const ChunkParams& p, const Joined& t,
       }
       int head;
       const int64_t token = token_head(p, t, row + r * step, head);
-      *reinterpret_cast<bf16x8*>(p.o + token * p.o_st + head * p.o_sh + 8 * lane) = v;
+      *reinterpret_cast<Global<bf16x8>>(p.o + token * p.o_st + head * p.o_sh + 8 * lane) = v;
       if (lane == 0 && p.lse != nullptr) p.lse[token * p.H + head] = joined_lse(top[r], sum[r], odd[r]);
     }
   }
@@ -1104,7 +1107,7 @@ __device__ __forceinline__ void join_span(const ChunkParams& p, const Joined& t,
     for (int i = 0; i < kInFlight; ++i) {
       const int64_t at = t.place(min(j0 + 16 * i, t.parts - 1), row);
       l[i] = p.part_lse[at];
-      v[i] = *reinterpret_cast<const f32x4*>(p.part_o + at * kDv + column);
+      v[i] = *reinterpret_cast<Global<const f32x4>>(p.part_o + at * kDv + column);
     }
 #pragma unroll
     for (int i = 0; i < kInFlight; ++i) {
@@ -1132,7 +1135,7 @@ __device__ __forceinline__ void join_span(const ChunkParams& p, const Joined& t,
     for (int i = 0; i < 4; ++i) v[i] = (bf16)(a[i] * scale);
     int head;
     const int64_t token = token_head(p, t, row, head);
-    *reinterpret_cast<bf16x4*>(p.o + token * p.o_st + head * p.o_sh + column) = v;
+    *reinterpret_cast<Global<bf16x4>>(p.o + token * p.o_st + head * p.o_sh + column) = v;
     if (column == 0 && p.lse != nullptr) p.lse[token * p.H + head] = joined_lse(top, sum, odd);
   }
 }
@@ -1146,7 +1149,7 @@ __global__ __launch_bounds__(256) void chunk_combine_kernel(ChunkParams p) {
     i32x4 link[kWords];   // lane i: of ranges i, 64 + i, ..
 #pragma unroll
     for (int k = 0; k < kWords; ++k) {
-      const i32x4 v = reinterpret_cast<const i32x4*>(p.links)[min(64 * k + lane, p.n_ranges - 1)];
+      const i32x4 v = p.links[min(64 * k + lane, p.n_ranges - 1)];
       link[k] = 64 * k + lane < p.n_ranges ? v : i32x4{0, 0, 0, 0};
     }
     // The last range up to this one in which a row tile begins, if the ranges since are whole within it, and the first
@@ -1191,7 +1194,7 @@ __global__ __launch_bounds__(256) void chunk_combine_kernel(ChunkParams p) {
   const int64_t total = (int64_t)(p.T - behind) * p.H;
   for (int64_t u = (int64_t)blockIdx.x * 4 + wave; u < total; u += (int64_t)gridDim.x * 4) {
     const int token = behind + (int)(u / p.H), head = (int)(u % p.H);
-    *reinterpret_cast<bf16x8*>(p.o + token * p.o_st + head * p.o_sh + 8 * lane) = bf16x8{};
+    *reinterpret_cast<Global<bf16x8>>(p.o + token * p.o_st + head * p.o_sh + 8 * lane) = bf16x8{};
     if (lane == 0 && p.lse != nullptr) p.lse[(int64_t)token * p.H + head] = kNegInf;
   }
 }
@@ -1252,13 +1255,13 @@ extern "C" int dmla_chunk_paged(const void* q, const void* kv_pool, const int32_
   if (B > 0 && (num_pages == 0 || max_pages_per_seq == 0))
     return fail(DMLA_ERR_INVALID_ARG, "%s: empty page pool or block table", what);
   ChunkParams p = {};
-  p.q = static_cast<const bf16*>(q);
-  p.kv = static_cast<const char*>(kv_pool);
-  p.block_table = block_table;
-  p.seqlens = cache_seqlens;
-  p.cu = cu_seqlens_q;
-  p.o = static_cast<bf16*>(o);
-  p.lse = lse;
+  p.q = (Global<const bf16>)q;
+  p.kv = (Global<const char>)kv_pool;
+  p.block_table = (Global<const int32_t>)block_table;
+  p.seqlens = (Global<const int32_t>)cache_seqlens;
+  p.cu = (Global<const int32_t>)cu_seqlens_q;
+  p.o = (Global<bf16>)o;
+  p.lse = (Global<float>)lse;
   p.q_st = q_st; p.q_sh = q_sh; p.kv_sp = 2 * kv_sp; p.kv_ss = 2 * kv_ss; p.bt_sb = bt_sb; p.o_st = o_st; p.o_sh = o_sh;
   p.T = (int)T; p.B = (int)B; p.H = (int)H; p.num_pages = (int)num_pages; p.max_pages = (int)max_pages_per_seq;
   p.causal = causal ? 1 : 0;
@@ -1281,9 +1284,9 @@ extern "C" int dmla_chunk_paged(const void* q, const void* kv_pool, const int32_
     return fail(DMLA_ERR_WORKSPACE, "%s: workspace of %lld bytes needed (got %lld)", what, (long long)need,
                 (long long)workspace_bytes);
   if (!aligned16(workspace)) return fail(DMLA_ERR_INVALID_ARG, "%s: workspace must be 16-byte aligned", what);
-  p.part_o = static_cast<float*>(workspace);
+  p.part_o = (Global<float>)workspace;
   p.part_lse = p.part_o + (int64_t)p.n_ranges * 2 * kRows * kDv;
-  p.links = reinterpret_cast<int4*>(p.part_lse + (int64_t)p.n_ranges * 2 * kRows);
+  p.links = (Global<RangeLink>)(p.part_lse + (int64_t)p.n_ranges * 2 * kRows);
   hipLaunchKernelGGL(chunk_kernel, dim3((unsigned)((p.n_ranges + 7) / 8 * 8)), dim3(kThreads), 0, (hipStream_t)stream, p);
   hipLaunchKernelGGL(chunk_combine_kernel, dim3((unsigned)(p.n_ranges * p.groups)), dim3(256), 0, (hipStream_t)stream, p);
   return check_launch(what);
