@@ -739,17 +739,17 @@ __device__ __forceinline__ Pass careful_pass(const ChunkParams& p, const Piece& 
 // each, merged by chunk_combine_kernel: range r writes the part that it begins with to slot 2 r (a row tile that an
 // earlier range began) and the one that it ends with to slot 2 r + 1.
 //
-// Weights are estimates in closed form, in halves of what a key tile of 128 rows takes: a tile weighs u = 2, of a
-// sequence with up to kNarrowRows rows u = 1, a start and end c.  The first n row tiles of a sequence whose first query is
-// token `base` weigh A(n) = n (c + u (base + 31) / 32) + 2 u n (n + 1) / H (row tile i ends at token
-// base + 128 (i + 1) / H, causal).  A range's end is the next one's start by the same arithmetic, so nothing is lost
-// or done twice where they are off.  They are integers (of fp32 products, ascending in n whatever the rounding); where
-// the host finds that they could pass 2^30, all are taken in units of 2^weight_shift.
-// (Costs from 12 / 8 to 24 / 16 were within 4 % of each other over thirteen batches, least widths of 8 and 12 cost
-// single sequences of 16 heads 3 and 10 us.)
+// Weights are estimates in closed form, in key tiles (one of a few rows takes as long as one of 128: 32 sequences x
+// 16 heads, four of them with chunks of 460 tokens, 343 us, 506 when it weighed half).  The first n row tiles of a
+// sequence whose first query is token `base` weigh A(n) = n (c + (base + 31) / 32) + 2 n (n + 1) / H (row tile i ends
+// at token base + 128 (i + 1) / H, causal), where c is what a start and end cost.  A range's end is the next one's start
+// by the same arithmetic, so nothing is lost or done twice where they are off.  They are integers (of fp32 products,
+// ascending in n whatever the rounding); where the host finds that they could pass 2^30, all are taken in units of
+// 2^weight_shift.
+// (c of 9 and 1: four prompts of 4200 tokens x 128 heads take 818 us, 880 with 6 and 853 with 14.)
 constexpr int kMaxRanges = 256;
-constexpr int kCost = 20, kNarrowCost = 20;
-constexpr int kMinWidth = 6;    // of a range
+constexpr int kCost = 9, kNarrowCost = 6;
+constexpr int kMinWidth = 3;    // of a range
 constexpr int kSnap = 8;        // tiles: a cut this near to a row tile's end moves there, or a quarter of a range's width
 
 struct Place {   // in the row tiles and key tiles of all sequences
@@ -770,20 +770,20 @@ __device__ __forceinline__ int key_tiles(const ChunkParams& p, const Sequence& s
   return (max(end, 0) + kTile - 1) / kTile;
 }
 struct Weights {
-  int unit, cost;
+  int cost;
   float base, growth;   // of a row tile, and how much more each one weighs
 };
 __device__ __forceinline__ Weights weights(const ChunkParams& p, const Sequence& s) {
   const bool few = s.n * p.H <= kNarrowRows;
-  Weights w = {few ? 1 : 2, few ? kNarrowCost : kCost, 0.f, 0.f};
+  Weights w = {few ? kNarrowCost : kCost, 0.f, 0.f};
   const int tiles = ((p.causal ? max(s.len - s.n, 0) : s.len) + kTile - 1) / kTile;
-  w.base = (float)(w.cost + w.unit * tiles);
-  w.growth = p.causal ? w.unit * p.two_by_h : 0.f;
+  w.base = (float)(w.cost + tiles);
+  w.growth = p.causal ? p.two_by_h : 0.f;
   return w;
 }
-// A(n).
+// A(n), one more for each row tile: none is without a weight, or no range would hold it.
 __device__ __forceinline__ int weight(const ChunkParams& p, const Weights& w, int n) {
-  return (int)((float)n * (w.base + w.growth * (float)(n + 1)) * p.weight_scale);
+  return n + (int)((float)n * (w.base + w.growth * (float)(n + 1)) * p.weight_scale);
 }
 // The place at weight y of sequence b.
 __device__ __forceinline__ Place place_of(const ChunkParams& p, int b, const Sequence& s, int y, int width) {
@@ -793,9 +793,9 @@ __device__ __forceinline__ Place place_of(const ChunkParams& p, int b, const Seq
     const int mid = (lo + hi + 1) / 2;
     if (weight(p, w, mid) <= y) lo = mid; else hi = mid - 1;
   }
-  const int nt = key_tiles(p, s, lo), snap = min(kSnap, width >> (w.unit + 1) << p.weight_shift);
+  const int nt = key_tiles(p, s, lo), snap = min(kSnap, width >> 2 << p.weight_shift);
   const int64_t in = (int64_t)(y - weight(p, w, lo)) << p.weight_shift;
-  int t = (int)min((int64_t)nt, max((int64_t)0, in - w.cost) >> (w.unit - 1));
+  int t = (int)min((int64_t)nt, max((int64_t)0, in - w.cost));
   if (t <= snap) t = 0;
   if (t > 0 && nt - t <= snap) return Place{b, lo + 1, 0};
   return Place{b, lo, t};
@@ -845,10 +845,11 @@ __device__ __forceinline__ bool cut(const ChunkParams& p, DMLA_LDS Window* win, 
     upto = scan(mine, sum);
     total += sum;
   }
-  const int width = max(max(1, kMinWidth >> p.weight_shift), (int)(((int64_t)total + p.n_ranges - 1) / p.n_ranges));
-  const int x0 = (int)min((int64_t)range * width, (int64_t)total), x1 = (int)min((int64_t)x0 + width, (int64_t)total);
+  const int n = max(1, min(p.n_ranges, total / max(1, kMinWidth >> p.weight_shift)));
+  const int width = total / n, rest = total - width * n;
+  const int x0 = range * width + range * rest / n, x1 = (range + 1) * width + (range + 1) * rest / n;
   if (tid == 0) p.links[range] = i32x4{0, 0, 0, 0};
-  if (x0 >= total) return false;
+  if (range >= n || x0 >= x1) return false;
   // The places of x0 and x1, by the threads whose sequences hold them; x1 at the end of one is that end.
   for (int b0 = 0, before = 0; b0 < p.B && before < x1; b0 += kThreads, before += sum) {
     if (p.B > kThreads) {
@@ -1202,7 +1203,7 @@ __global__ __launch_bounds__(256) void chunk_combine_kernel(ChunkParams p) {
 // At least the weight that the kernel adds up.
 int64_t chunk_weight(int64_t T, int64_t B, int64_t H, int64_t max_pages) {
   const int64_t tiles = T * H / kRows + std::min(B, T);
-  return tiles * (kCost + 4 + max_pages * (2 * kPage / kTile));
+  return tiles * (kCost + 3 + max_pages * (kPage / kTile));
 }
 // Ranges of a call: one per CU, as many as its work can fill at most.
 int64_t chunk_ranges(int64_t T, int64_t B, int64_t H, int64_t max_pages) {

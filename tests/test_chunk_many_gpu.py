@@ -184,3 +184,20 @@ def test_climbing_scores(gpu, H, N, steepest):
     q = q.to(torch.bfloat16)
     o, lse = run(gpu, q, pool.to(gpu), ints([list(range(pages(N)))], gpu), [N], [1])
     check(q, o, lse, [rows], [N], [1])
+
+
+def test_short_sequences_beside_tables_of_a_million_pages(gpu):
+    """Sequences that weigh less than a unit of the cut are there all the same."""
+    lens, counts, H = [3, 1, 600, 2, 64, 1, 40, 9], [3, 1, 600, 1, 64, 1, 40, 2], 128
+    pool, table, rows = paged(lens, gpu)
+    wide = torch.full((len(lens), 1 << 20), -1, dtype=torch.int32, device=gpu)
+    wide[:, :table.shape[1]] = table
+    extra = 20000   # queries behind the last sequence, which the host counts as work that could be
+    q = queries(sum(counts), H, 4)
+    padded = torch.zeros(sum(counts) + extra, H, D_QK, dtype=torch.bfloat16, device=gpu)
+    padded[:sum(counts)] = q
+    o, lse = run(gpu, padded, pool, wide, lens, counts)
+    r = random.Random(1)
+    n = sum(counts)
+    check(q, o[:n], lse[:n], rows, lens, counts, some=set(list(range(10)) + list(range(n - 110, n)) + r.sample(range(n), 30)))
+    assert (o[n:] == 0).all() and (lse[n:] == float("-inf")).all()
