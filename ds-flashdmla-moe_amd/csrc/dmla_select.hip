@@ -106,7 +106,8 @@ struct ScoreArgs {
   Queries qs;
   float* scores;
   float2* stats;   // [chunks, T, H]: max (log2 units) and sum
-  int64_t q_st, q_sh, m_sp, bt_sb, s_st;
+  float* kept;     // [T, H, kept_sp]: the products q . mean, where they are kept
+  int64_t q_st, q_sh, m_sp, bt_sb, s_st, kept_sp;
   int H, num_pages;
   int blocks, passes;   // 16-row blocks of a query (at most kBlocks of a pass), passes over the heads
   int group;            // queries of a workgroup
@@ -123,13 +124,35 @@ constexpr int kCopies = 9;                                // of a wave and tile
 constexpr int kIdTiles = 64;                              // tiles whose table entries are in LDS
 constexpr int kQueryBytes = 32 * 2 * kD;                  // of a wave, in the tiles' memory
 static_assert(kScoreWaves * kQueryBytes == kRing * (kTileBytes + kRopeBytes), "the queries fill it");
-enum { kFused, kStats, kSum };
+enum { kFused, kStats, kKeep, kSum };
 
 // 16-byte unit u of row r of a tile lies at u ^ mean_swz(r): 16 rows' units at one place of a row lie in different banks.
 __device__ __forceinline__ int mean_swz(int r) { return r & 15; }
 
+// A head's largest score (0: none) and the inverse of its sum, over all chunks of the pages; of heads that are not there
+// such that every weight is 0.  (Apart: their product's logarithm would lose the digits of a large maximum.)
+__device__ __forceinline__ void head_sums(const ScoreArgs& a, int t, int head, float& top, float& inverse) {
+  float m = kNegInf, l = 0.f;
+  constexpr int kLoads = 4;   // in flight (one: 100000 tokens x 128 heads 28 us, four 21, sixteen 24)
+  for (int c0 = 0; c0 < a.chunks; c0 += kLoads) {
+    float2 s[kLoads];
+#pragma unroll
+    for (int c = 0; c < kLoads; ++c) s[c] = a.stats[((int64_t)min(c0 + c, a.chunks - 1) * a.qs.T + t) * a.H + min(head, a.H - 1)];
+#pragma unroll
+    for (int c = 0; c < kLoads; ++c) {
+      if (c0 + c >= a.chunks) break;
+      const float mm = fmaxf(m, s[c].x);
+      l = mm == kNegInf ? l + s[c].y : l * fast_exp2(m - mm) + s[c].y * fast_exp2(s[c].x - mm);   // (0 or not a number)
+      m = mm;
+    }
+  }
+  top = head >= a.H ? __builtin_inff() : m == kNegInf ? 0.f : m;
+  inverse = head >= a.H || l == 0.f ? 0.f : 1.f / l;
+}
+
 // kFused: one workgroup has all pages of its queries, their sums first and then the scores.  Else the pages are cut in
-// chunks over workgroups, kStats leaves each chunk's maxima and sums and kSum reads all of them.
+// chunks over workgroups: kStats leaves each chunk's maxima and sums and kSum reads all of them, with the products once
+// more; kKeep leaves the products too, for page_sums_kernel.
 //
 // A wave holds 32 rows (query, head) in registers, as chunk attention does, and tiles of 32 mean rows come through LDS,
 // three tiles ahead.  For the sums over pages the means are the MFMA's rows, so a lane has 16 pages of one head; for
@@ -179,17 +202,7 @@ __global__ void __launch_bounds__(kScoreThreads, 1) page_scores_kernel(ScoreArgs
     if constexpr (kMode == kSum) {
       for (int r = tid; r < 16 * kBlocks; r += kScoreThreads) {
         const int head = head0 + head_of(r), i = query_of(r);
-        float m = kNegInf, l = 0.f;
-        for (int c = 0; c < a.chunks; ++c) {
-          const float2 s = a.stats[((int64_t)c * a.qs.T + t0 + i) * a.H + min(head, a.H - 1)];
-          const float mm = fmaxf(m, s.x);
-          l = mm == kNegInf ? l + s.y : l * fast_exp2(m - mm) + s.y * fast_exp2(s.x - mm);   // (0 or not a number)
-          m = mm;
-        }
-        // (m and 1 / l apart: their product's logarithm would lose the digits of a large m.)
-        const bool head_there = head < a.H;
-        s_max[r] = !head_there ? __builtin_inff() : m == kNegInf ? 0.f : m;
-        s_inv[r] = !head_there || l == 0.f ? 0.f : 1.f / l;
+        head_sums(a, t0 + i, head, s_max[r], s_inv[r]);
       }
     }
     wait_vm<0>();
@@ -244,7 +257,7 @@ __global__ void __launch_bounds__(kScoreThreads, 1) page_scores_kernel(ScoreArgs
         for (int s = 0; s < n_tiles; ++s) {
           // Half the entries ahead of their use, into the half that every wave is past.
           if (s > 1 && s % (kIdTiles / 2) == 1 && s - 1 + kIdTiles / 2 < n_tiles) load_ids(s - 1 + kIdTiles / 2);
-          wait_vm<2 * kCopies>();   // tile s; those of two tiles more may be on their way
+          wait_vm<2 * kCopies>();   // tile s; those of two tiles more may be on their way (or stores of an earlier one)
           __syncthreads();          // tile s landed, tile s - 1 is read
           copy(s + 3);
           const unsigned key = lds_sum(kMeanRow * l32 + 16 * (hl ^ mean_swz(l32)), tiles + (unsigned)(s % kRing) * kTileBytes);
@@ -264,10 +277,23 @@ __global__ void __launch_bounds__(kScoreThreads, 1) page_scores_kernel(ScoreArgs
       if constexpr (kMode != kSum) {
         float m = kNegInf, l = 0.f;   // of row 32 wave + l32
         const int limit = rows_pages(32 * wave + l32);
+        const int r = 32 * wave + l32, i = query_of(r), head = head0 + head_of(r);
+        // (Rows behind the last query are its rows again.)
+        const bool own = i >= i0 && i < i1 && (multi || (r >> 4) / a.blocks < nt);
+        float* keep = nullptr;
+        if constexpr (kMode == kKeep)
+          if (own && head < a.H) keep = a.kept + ((int64_t)(t0 + i) * a.H + head) * a.kept_sp + c0 + 4 * hl;
         stream([&](int s, auto k, unsigned there) {
           f32x16 x = {};
 #pragma unroll
           for (int c = 0; c < kSteps; ++c) x = mfma32_bf16(k(c), q[c], x);
+          if constexpr (kMode == kKeep) {
+            if (keep != nullptr) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                *reinterpret_cast<f32x4*>(keep + kTile * s + 8 * j) = f32x4{x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]};
+            }
+          }
           const unsigned seen = (there & first_pages(s, limit)) >> (4 * hl);
 #pragma unroll
           for (int i = 0; i < 16; ++i) x[i] = seen >> (8 * (i >> 2) + (i & 3)) & 1 ? x[i] * a.scale_log2 : kNegInf;
@@ -282,11 +308,8 @@ __global__ void __launch_bounds__(kScoreThreads, 1) page_scores_kernel(ScoreArgs
           for (int i = 0; i < 16; ++i) l += fast_exp2(x[i] - ms);   // (not a number stays)
         });
         l = half_sum(l);
-        const int r = 32 * wave + l32, i = query_of(r), head = head0 + head_of(r);
-        // (Rows behind the last query are its rows again.)
-        const bool own = i >= i0 && i < i1 && (multi || (r >> 4) / a.blocks < nt);
         if (hl == 0 && own) {
-          if constexpr (kMode == kStats) {
+          if constexpr (kMode == kStats || kMode == kKeep) {
             if (head < a.H) a.stats[((int64_t)blockIdx.y * a.qs.T + t0 + i) * a.H + head] = make_float2(m, l);
           } else {
             s_max[r] = head >= a.H ? __builtin_inff() : m == kNegInf ? 0.f : m;
@@ -295,7 +318,7 @@ __global__ void __launch_bounds__(kScoreThreads, 1) page_scores_kernel(ScoreArgs
         }
         __syncthreads();
       }
-      if constexpr (kMode != kStats) {
+      if constexpr (kMode == kFused || kMode == kSum) {
         // Scores of tile s: the sums of each query's blocks, posted by the waves.
         auto put = [&](int s) {
           const int i = tid >> 5, p = c0 + kTile * s + (tid & 31);
@@ -348,6 +371,50 @@ __global__ void __launch_bounds__(kScoreThreads, 1) page_scores_kernel(ScoreArgs
       i0 = i1;
     }
   }
+}
+
+// The scores of a query's pages from what was kept of each head, 64 pages a wave (a lane has a page); with a.split > 1
+// that many waves share the heads of a page, their sums in a fixed order.
+// Bound: latency (what the first kernel kept is in the last-level cache).
+constexpr int kSumHeads = 128, kSumLoads = 16;
+__global__ void __launch_bounds__(kScoreThreads) page_sums_kernel(ScoreArgs a, int split) {
+  __shared__ float s_max[kSumHeads], s_inv[kSumHeads], s_part[kScoreWaves][64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+  const int t = blockIdx.y, p = 64 * ((int)blockIdx.x * (kScoreWaves / split) + wave / split) + lane;
+  const int b = sequence_of(a.qs, t), n = visible(a.qs, b, t);
+  const int pages = uniform(n > 0 ? (n - 1) / kPage : 0);
+  const bool any = 64 * (int)blockIdx.x * (kScoreWaves / split) < pages;   // of this workgroup's
+  bool there = false;
+  float v = 0.f;
+  if (any) {
+    if (p < pages) {
+      const int id = a.block_table[b * a.bt_sb + p];
+      there = id >= 0 && id < a.num_pages;
+    }
+    const float* x = a.kept + (int64_t)t * a.H * a.kept_sp + min(p, pages - 1);
+    for (int h0 = 0; h0 < a.H; h0 += kSumHeads) {
+      const int heads = min(kSumHeads, a.H - h0), each = (heads + split - 1) / split;
+      const int first = (wave % split) * each, last = min(first + each, heads);
+      __syncthreads();   // those before are read
+      for (int h = tid; h < heads; h += kScoreThreads) head_sums(a, t, h0 + h, s_max[h], s_inv[h]);
+      __syncthreads();
+      for (int h = first; h < last; h += kSumLoads) {
+        float k[kSumLoads];
+#pragma unroll
+        for (int i = 0; i < kSumLoads; ++i) k[i] = x[(int64_t)(h0 + min(h + i, last - 1)) * a.kept_sp];
+#pragma unroll
+        for (int i = 0; i < kSumLoads; ++i)
+          if (h + i < last) v += fast_exp2(__builtin_fmaf(k[i], a.scale_log2, -s_max[h + i])) * s_inv[h + i];
+      }
+    }
+  }
+  if (split > 1) {
+    s_part[wave][lane] = v;
+    __syncthreads();
+    if (wave % split != 0) return;
+    for (int w = 1; w < split; ++w) v += s_part[wave + w][lane];
+  }
+  if (p < a.qs.max_pages) a.scores[t * a.s_st + p] = there ? v : 0.f;
 }
 
 // ---- selection ----------------------------------------------------------------------------------------
@@ -502,7 +569,13 @@ int queries_validate(const char* what, const int32_t* cu, const int32_t* cache_s
 struct ScoreShape {
   int blocks, passes, group, chunk, chunks;
   int64_t groups;
+  int64_t kept_sp;   // 0: the products are not kept
+
+  int64_t stats_bytes(int64_t T, int64_t H) const { return (chunks > 1 ? chunks * T * H * (int64_t)sizeof(float2) : 0) + 15 & ~(int64_t)15; }
+  int64_t bytes(int64_t T, int64_t H) const { return stats_bytes(T, H) + T * H * kept_sp * (int64_t)sizeof(float); }
 };
+// Up to here the products are kept (64 queries x 128 heads x 500 / 8000 pages: 28 / 237 us, computed again 36 / 297).
+constexpr int64_t kKeepBytes = (int64_t)512 << 20;
 ScoreShape score_shape(int64_t T, int64_t H, int64_t max_pages, bool packed) {
   ScoreShape s;
   const int64_t blocks = (H + 15) / 16;
@@ -516,6 +589,7 @@ ScoreShape score_shape(int64_t T, int64_t H, int64_t max_pages, bool packed) {
   const int64_t each = (most + want - 1) / want;
   s.chunk = (int)(kTile * each);
   s.chunks = (int)((most + each - 1) / each);
+  s.kept_sp = s.chunks > 1 && T * H * most * kTile <= kKeepBytes / (int64_t)sizeof(float) ? most * kTile : 0;
   return s;
 }
 
@@ -567,7 +641,7 @@ extern "C" int64_t dmla_page_scores_workspace_bytes(int64_t T, int64_t H, int64_
       max_pages_per_seq > ((int64_t)1 << 24))
     return 0;
   const ScoreShape s = score_shape(T, H, max_pages_per_seq, packed != 0);
-  return s.chunks > 1 ? s.chunks * T * H * (int64_t)sizeof(float2) : 0;
+  return s.bytes(T, H);
 }
 
 extern "C" int dmla_page_scores(const void* q, const void* means, const int32_t* block_table, const int32_t* cache_seqlens,
@@ -594,7 +668,7 @@ extern "C" int dmla_page_scores(const void* q, const void* means, const int32_t*
   if (H == 0 || num_pages == 0) return fail(DMLA_ERR_INVALID_ARG, "%s: no heads or no pages", what);
   const ScoreShape s = score_shape(T, H, max_pages_per_seq, cu_seqlens_q != nullptr);
   if (s.groups > 0x7fffffff || s.chunks > 65535) return fail(DMLA_ERR_UNSUPPORTED, "%s: size too large", what);
-  const int64_t need = s.chunks > 1 ? s.chunks * T * H * (int64_t)sizeof(float2) : 0;
+  const int64_t need = s.bytes(T, H);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need))
     return fail(DMLA_ERR_WORKSPACE, "%s: workspace of %lld bytes needed (got %lld)", what, (long long)need,
                 (long long)workspace_bytes);
@@ -606,6 +680,8 @@ extern "C" int dmla_page_scores(const void* q, const void* means, const int32_t*
   a.qs = Queries{cu_seqlens_q, cache_seqlens, (int)B, (int)T, (int)max_pages_per_seq};
   a.scores = scores;
   a.stats = static_cast<float2*>(workspace);
+  a.kept = reinterpret_cast<float*>(static_cast<char*>(workspace) + s.stats_bytes(T, H));
+  a.kept_sp = s.kept_sp;
   a.q_st = q_st; a.q_sh = q_sh; a.m_sp = m_sp; a.bt_sb = bt_sb; a.s_st = s_st;
   a.H = (int)H; a.num_pages = (int)num_pages;
   a.blocks = s.blocks; a.passes = s.passes; a.group = s.group; a.chunk = s.chunk; a.chunks = s.chunks;
@@ -616,6 +692,15 @@ extern "C" int dmla_page_scores(const void* q, const void* means, const int32_t*
     return check_launch(what);
   };
   if (s.chunks == 1) return launch(page_scores_kernel<kFused>);
+  if (s.kept_sp > 0) {
+    const int kept = launch(page_scores_kernel<kKeep>);
+    if (kept != DMLA_OK) return kept;
+    const int split = H > kSumHeads / kScoreWaves ? kScoreWaves : 1;
+    const int64_t wide = 64 * (kScoreWaves / split);
+    hipLaunchKernelGGL(page_sums_kernel, dim3((unsigned)((max_pages_per_seq + wide - 1) / wide), (unsigned)T), dim3(kScoreThreads), 0,
+                       (hipStream_t)stream, a, split);   // (several chunks: no more than 1024 queries)
+    return check_launch(what);
+  }
   const int first = launch(page_scores_kernel<kStats>);
   return first != DMLA_OK ? first : launch(page_scores_kernel<kSum>);
 }

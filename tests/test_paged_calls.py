@@ -102,11 +102,13 @@ def test_workspace_sizes():
     assert lib.dmla_chunk_paged_workspace_bytes(1, 1, 16, 1) < lib.dmla_chunk_paged_workspace_bytes(1, 1, 16, 128)
     for bad in ((0, 1, 16, 1), (1, 0, 16, 1), (1, 1, 0, 1), (1, 1, 16, 0), (1, 1, 1 << 17, 1), (1 << 25, 1, 128, 1)):
         assert lib.dmla_chunk_paged_workspace_bytes(*bad) == 0
-    # Page scores: a maximum and a sum per query, head and chunk of pages; none where one workgroup has all pages.
+    # Page scores: a maximum and a sum per query, head and chunk of pages, and the products up to 512 MB; none where one
+    # workgroup has all pages.
     assert lib.dmla_page_scores_workspace_bytes(1, 128, 32, 1) == 0
     assert lib.dmla_page_scores_workspace_bytes(4096, 128, 512, 1) == 0
-    n = lib.dmla_page_scores_workspace_bytes(64, 128, 512, 0)
-    assert n > 0 and n % (64 * 128 * 8) == 0 and n // (64 * 128 * 8) <= 16
+    for pages, kept in ((512, 512), (16384, 16384), (16385, 0)):
+        n = lib.dmla_page_scores_workspace_bytes(64, 128, pages, 0) - 64 * 128 * kept * 4
+        assert n > 0 and n % (64 * 128 * 8) == 0 and n // (64 * 128 * 8) <= 16
     assert lib.dmla_page_scores_workspace_bytes(0, 128, 32, 1) == 0
 
 

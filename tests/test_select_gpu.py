@@ -260,3 +260,26 @@ def test_sparse_attention(gpu, q4, H, lens, counts):
                 assert len(keys) == sel_lens[t].item()
                 assert k < 64 or len(keys) == end
                 assert_attention(o[t:t + 1], lse[t:t + 1], attention64(q[t:t + 1], keys, [len(keys)], SCALE), f"query {t} of {b}")
+
+
+@pytest.mark.parametrize("H,lens,counts,width", [(16, [3000, 700], [400, 600], 8400), (300, [5000, 300], [100, 27], 3600),
+                                                 (128, [9000] * 5, [1] * 5, 270000)])
+def test_scores_under_tables_too_wide_to_keep_products(gpu, H, lens, counts, width):
+    """Past 512 MB of products the second kernel computes them once more: the same scores either way."""
+    from python import _lib, ops
+    pool, table, _ = paged(lens, gpu, seed=H)
+    means = (torch.randn(pool.shape[0], D_QK, generator=torch.Generator().manual_seed(H)) * 0.3).to(torch.bfloat16).to(gpu)
+    T = sum(counts)
+    q = (torch.randn(T, H, D_QK, generator=torch.Generator().manual_seed(H + 1))).to(torch.bfloat16).to(gpu)
+    wide = torch.full((len(lens), width), -1, dtype=torch.int32, device=gpu)
+    wide[:, :table.shape[1]] = table
+    assert 0 < _lib.lib().dmla_page_scores_workspace_bytes(T, H, width, 1) < 1 << 26
+    got = ops.flash_dmla_page_scores(q, means, wide, ints(lens, gpu), ints(starts(counts), gpu), SCALE)
+    kept = ops.flash_dmla_page_scores(q, means, table, ints(lens, gpu), ints(starts(counts), gpu), SCALE)
+    assert (got[:, table.shape[1]:] == 0).all()
+    at = starts(counts)
+    for b, (N, n) in enumerate(zip(lens, counts)):
+        some = sorted({0, n // 2, n - 1})
+        s, tol = scores64(q[[at[b] + i for i in some]], means, table[b].cpu(), [N - n + i + 1 for i in some])
+        for x in (got, kept):
+            assert ((x[[at[b] + i for i in some], :table.shape[1]].double().cpu() - s).abs() <= tol).all()
