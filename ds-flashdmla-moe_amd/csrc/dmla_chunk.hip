@@ -13,6 +13,20 @@
 //    (ds_read_b128), the value product 32 columns of 8 rows transposed (ds_read_b64_tr_b16).  The rope dims have
 //    rows of 128 bytes of their own, eight of them a copy.
 //  * Step s multiplies scores of tile s and values of tile s - 1; copies run two tiles ahead, four tiles fit.
+//  * Up to 32 rows (one token of 16 heads, say) would leave three waves without scores.  There every wave has all rows and
+//    a quarter of the dims, and the partial scores of four waves are added through LDS in a fixed order (512 sequences of
+//    2048 tokens x 16 heads: 264 -> 229 us).
+//  * One workgroup per CU takes an equal share of all work, whatever the lengths ("cutting the work" below), and
+//    a second kernel joins what was cut.
+//
+// Bound, by what a call is made of (MI355X, 1.2 PFLOP/s and 5 TB/s being what a large product and a large copy reach):
+//  * Chunks and prompts by the matrix cores: a tile of 32 keys takes 128 rows 1.7 us, 1.3 PFLOP/s over all CUs; 1024
+//    queries x 128 heads over 8192 tokens 1.78 ms (1.23 PFLOP/s).
+//  * Many single tokens by HBM: 512 sequences of 2048 tokens x 16 heads 229 us, 5.3 TB/s.
+//  * Short rows of keys by what a piece costs beside its tiles, 9 us: 3 us of queries through LDS (their copies, the
+//    first tile, the last tile's values) and 4 us of outputs, both at what a CU's vector memory path takes (some 27
+//    bytes a cycle).  Four prompts of 300 to 1900 tokens x 128 heads: 880 us, 0.99 PFLOP/s.
+//  * One token by latency: the cut, queries, tiles, the join: 31 us for 5000 tokens x 128 heads.
 #include <algorithm>
 #include <cmath>
 
@@ -848,8 +862,14 @@ __device__ __forceinline__ bool cut(const ChunkParams& p, DMLA_LDS Window* win, 
   const int n = max(1, min(p.n_ranges, total / max(1, kMinWidth >> p.weight_shift)));
   const int width = total / n, rest = total - width * n;
   const int x0 = range * width + range * rest / n, x1 = (range + 1) * width + (range + 1) * rest / n;
-  if (tid == 0) p.links[range] = i32x4{0, 0, 0, 0};
+  if (tid == 0) {
+    p.links[range] = i32x4{0, 0, 0, 0};
+    // (Starts that do not ascend can add up to anything; then there may be no place, and nothing to do.)
+    win->at.b = win->at.rt = win->at.t = 0;
+    win->end.b = win->end.rt = win->end.t = 0;
+  }
   if (range >= n || x0 >= x1) return false;
+  __syncthreads();
   // The places of x0 and x1, by the threads whose sequences hold them; x1 at the end of one is that end.
   for (int b0 = 0, before = 0; b0 < p.B && before < x1; b0 += kThreads, before += sum) {
     if (p.B > kThreads) {

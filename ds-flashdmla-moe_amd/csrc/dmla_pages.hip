@@ -334,7 +334,7 @@ extern "C" int dmla_kv_append_rows(void* kv_pool, const int32_t* slots, const vo
     return fail(DMLA_ERR_INVALID_ARG, "dmla_kv_append_rows: kv_pool and rows must be 16-byte aligned");
   if (!mult8(kv_sp) || !mult8(kv_ss) || !mult8(r_ss) || kv_ss < d || kv_sp < kPage * kv_ss || r_ss < d)
     return fail(DMLA_ERR_INVALID_ARG, "dmla_kv_append_rows: strides must be multiples of 8 and cover a row / page");
-  if (num_pages > ((int64_t)1 << 25) || d / 8 > 0x7fffffff || T * (d / 8) > 0x7fffffff)
+  if (num_pages > ((int64_t)1 << 25) || d / 8 > 0x7fffffff || T > 0x7fffffff || T * (d / 8) > 0x7fffffff)
     return fail(DMLA_ERR_UNSUPPORTED, "dmla_kv_append_rows: size too large");
   if (T == 0) return DMLA_OK;
   AppendRowsArgs a = {};

@@ -354,7 +354,8 @@ int dmla_kv_evict(void* kv_pool, const int32_t* block_table, const int32_t* cach
  * dmla_kv_release: the pages that a sequence of old_lens[b] tokens has and one of new_lens[b] does not need
  *   (entries ceil(new_lens[b] / 64) .. ceil(old_lens[b] / 64) - 1 of its row; new_lens[b] = 0: it has ended) go on
  *   the stack in order.  block_table keeps the entries.  An entry outside [0, num_pages), and pages past `capacity`
- *   (entries of free_pages), are left out and set *bad_index_flag to 1.
+ *   (entries of free_pages), are left out and set *bad_index_flag to 1.  A page goes there once for every row of
+ *   block_table that gives it back: of one that sequences share, only its last holder's row may.
  * dmla_kv_reserve: sequence b of cache_seqlens[b] tokens gets the pages that new_lens[b] more need, in order, into its
  *   row of block_table.  Its new rows are rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 of a packed array of num_rows.
  *   cu_seqlens [B + 1]  row starts: running sums of new_lens (at most num_rows)
