@@ -760,9 +760,9 @@ __device__ __forceinline__ Pass careful_pass(const ChunkParams& p, const Piece& 
 // by the same arithmetic, so nothing is lost or done twice where they are off.  They are integers (of fp32 products,
 // ascending in n whatever the rounding); where the host finds that they could pass 2^30, all are taken in units of
 // 2^weight_shift.
-// (c of 9 and 1: four prompts of 4200 tokens x 128 heads take 818 us, 880 with 6 and 853 with 14.)
+// (c of 7 and the one more: four prompts of 300 to 1900 tokens x 128 heads 814 us; 863 with 5, 829 with 9.)
 constexpr int kMaxRanges = 256;
-constexpr int kCost = 9, kNarrowCost = 6;
+constexpr int kCost = 7, kNarrowCost = 5;
 constexpr int kMinWidth = 3;    // of a range
 constexpr int kSnap = 8;        // tiles: a cut this near to a row tile's end moves there, or a quarter of a range's width
 
