@@ -764,7 +764,9 @@ __device__ __forceinline__ Pass careful_pass(const ChunkParams& p, const Piece& 
 constexpr int kMaxRanges = 256;
 constexpr int kCost = 7, kNarrowCost = 5;
 constexpr int kMinWidth = 3;    // of a range
-constexpr int kSnap = 8;        // tiles: a cut this near to a row tile's end moves there, or a quarter of a range's width
+// Tiles: a cut this near to a row tile's end moves there, or a quarter of a range's width.  (512 queries x 128 heads over
+// 32 pages each, two row tiles a range: 262 us, 288 with 8; 256 queries x 128 heads over 8192 tokens 514 us, 501 with 8.)
+constexpr int kSnap = 12;
 
 struct Place {   // in the row tiles and key tiles of all sequences
   int b, rt, t;
