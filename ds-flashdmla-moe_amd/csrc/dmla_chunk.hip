@@ -26,7 +26,7 @@
 //  * Short rows of keys by what a piece costs beside its tiles, 9 us: 3 us of queries through LDS (their copies, the
 //    first tile, the last tile's values) and 4 us of outputs, both at what a CU's vector memory path takes (some 27
 //    bytes a cycle).  Four prompts of 300 to 1900 tokens x 128 heads: 880 us, 0.99 PFLOP/s.
-//  * One token by latency: the cut, queries, tiles, the join: 31 us for 5000 tokens x 128 heads.
+//  * One token by latency: the cut, queries, tiles, the join: 27 us for 5000 tokens x 128 heads.
 #include <algorithm>
 #include <cmath>
 
@@ -113,11 +113,11 @@ __device__ __forceinline__ Sequence sequence(const ChunkParams& p, int b) {
   return s;
 }
 
-// 128 rows of a sequence from row0 on, the key tiles [t0, t1) of them, and where their output goes: slot < 0 to o, else
+// Up to 128 rows of a sequence from row0 on, the key tiles [t0, t1) of them, and where their output goes: slot < 0 to o, else
 // a part.
 struct Piece {
   Sequence s;
-  int b, row0, t0, t1, slot;
+  int b, row0, rows, t0, t1, slot;
 };
 
 // A piece runs once, against each row's largest score in the first tile.  Where scores have climbed more than kHeadroom
@@ -199,7 +199,7 @@ __device__ __forceinline__ bool run_piece(const Piece& pc, const Lds& lds, const
   const int lane = fresh_lane_id();
   const int l32 = lane & 31, hl = lane >> 5;
   const int wave = uniform(threadIdx.x >> 6);
-  const int rows = min(pc.s.n * p.H - pc.row0, kRows);
+  const int rows = pc.rows;
   constexpr int kBlocks = kNarrow ? 1 : kRowBlocks;   // of 32 rows
   const int first_row = kNarrow ? 0 : 32 * wave;      // of the wave's 32
   // Rows past the last one are the last one again, and not written.
@@ -764,6 +764,12 @@ __device__ __forceinline__ Pass careful_pass(const ChunkParams& p, const Piece& 
 constexpr int kMaxRanges = 256;
 constexpr int kCost = 7, kNarrowCost = 5;
 constexpr int kMinWidth = 3;    // of a range
+// Little work (a weight of kFine and less) is cut in row tiles of 32 rows: their queries and outputs take a
+// quarter of the time, and there are four times as many to spread (one token x 128 heads over 5000 / 20000 tokens: 27 / 36
+// us, 33 / 40 in row tiles of 128; over 40000, weight 1260, 50 and 45).
+constexpr int kFine = 900;
+constexpr int kRowsLog2 = 7, kNarrowLog2 = 5;
+static_assert(1 << kRowsLog2 == kRows && 1 << kNarrowLog2 == kNarrowRows, "row tiles");
 // Tiles: a cut this near to a row tile's end moves there, or a quarter of a range's width.  (512 queries x 128 heads over
 // 32 pages each, two row tiles a range: 262 us, 288 with 8; 256 queries x 128 heads over 8192 tokens 514 us, 501 with 8.)
 constexpr int kSnap = 12;
@@ -776,12 +782,14 @@ struct Window {   // the sequences of 256 at a time, and what the threads share
   int tmp[kWaves];
   Place at, end;        // where the next piece begins, and the range's end
   int first;            // sequence of the window
+  int rows_log2;        // rows of a row tile
   i32x4 piece[2][3];   // q0, row0, rows, n; len, b, t0, t1; slot: this one and the next
 };
 
-__device__ __forceinline__ int row_tiles(const ChunkParams& p, const Sequence& s) { return (s.n * p.H + kRows - 1) / kRows; }
-__device__ __forceinline__ int key_tiles(const ChunkParams& p, const Sequence& s, int rt) {
-  const int last = fast_div(min((rt + 1) * kRows, s.n * p.H) - 1, p.hdiv);
+// (Rows of a row tile: 2^rows_log2.)
+__device__ __forceinline__ int row_tiles(const ChunkParams& p, const Sequence& s, int rows_log2) { return (s.n * p.H + (1 << rows_log2) - 1) >> rows_log2; }
+__device__ __forceinline__ int key_tiles(const ChunkParams& p, const Sequence& s, int rt, int rows_log2) {
+  const int last = fast_div(min((rt + 1) << rows_log2, s.n * p.H) - 1, p.hdiv);
   const int end = p.causal ? s.len - s.n + last + 1 : s.len;
   return (max(end, 0) + kTile - 1) / kTile;
 }
@@ -789,12 +797,12 @@ struct Weights {
   int cost;
   float base, growth;   // of a row tile, and how much more each one weighs
 };
-__device__ __forceinline__ Weights weights(const ChunkParams& p, const Sequence& s) {
-  const bool few = s.n * p.H <= kNarrowRows;
+__device__ __forceinline__ Weights weights(const ChunkParams& p, const Sequence& s, int rows_log2) {
+  const bool few = s.n * p.H <= kNarrowRows || rows_log2 == kNarrowLog2;
   Weights w = {few ? kNarrowCost : kCost, 0.f, 0.f};
   const int tiles = ((p.causal ? max(s.len - s.n, 0) : s.len) + kTile - 1) / kTile;
   w.base = (float)(w.cost + tiles);
-  w.growth = p.causal ? p.two_by_h : 0.f;
+  w.growth = !p.causal ? 0.f : rows_log2 == kNarrowLog2 ? 0.25f * p.two_by_h : p.two_by_h;
   return w;
 }
 // A(n), one more for each row tile: none is without a weight, or no range would hold it.
@@ -802,14 +810,14 @@ __device__ __forceinline__ int weight(const ChunkParams& p, const Weights& w, in
   return n + (int)((float)n * (w.base + w.growth * (float)(n + 1)) * p.weight_scale);
 }
 // The place at weight y of sequence b.
-__device__ __forceinline__ Place place_of(const ChunkParams& p, int b, const Sequence& s, int y, int width) {
-  const Weights w = weights(p, s);
-  int lo = 0, hi = row_tiles(p, s) - 1;   // the last row tile that begins at or before y
+__device__ __forceinline__ Place place_of(const ChunkParams& p, int b, const Sequence& s, int y, int width, int rows_log2) {
+  const Weights w = weights(p, s, rows_log2);
+  int lo = 0, hi = row_tiles(p, s, rows_log2) - 1;   // the last row tile that begins at or before y
   while (lo < hi) {
     const int mid = (lo + hi + 1) / 2;
     if (weight(p, w, mid) <= y) lo = mid; else hi = mid - 1;
   }
-  const int nt = key_tiles(p, s, lo), snap = min(kSnap, width >> 2 << p.weight_shift);
+  const int nt = key_tiles(p, s, lo, rows_log2), snap = min(kSnap, width >> 2 << p.weight_shift);
   const int64_t in = (int64_t)(y - weight(p, w, lo)) << p.weight_shift;
   int t = (int)min((int64_t)nt, max((int64_t)0, in - w.cost));
   if (t <= snap) t = 0;
@@ -853,13 +861,18 @@ __device__ __forceinline__ bool cut(const ChunkParams& p, DMLA_LDS Window* win, 
     }
     return v;
   };
-  int total = 0, upto = 0, mine = 0, sum = 0;
+  int total = 0, upto = 0, mine = 0, sum = 0, rows_log2 = kRowsLog2;
   Sequence s = {0, 0, 0};
   for (int b0 = 0; b0 < p.B; b0 += kThreads) {
     s = load_window(p, win, b0);
-    mine = weight(p, weights(p, s), row_tiles(p, s));
+    mine = weight(p, weights(p, s, rows_log2), row_tiles(p, s, rows_log2));
     upto = scan(mine, sum);
     total += sum;
+  }
+  if (total <= kFine && p.B <= kThreads && p.weight_shift == 0) {
+    rows_log2 = kNarrowLog2;
+    mine = weight(p, weights(p, s, rows_log2), row_tiles(p, s, rows_log2));
+    upto = scan(mine, total);
   }
   const int n = max(1, min(p.n_ranges, total / max(1, kMinWidth >> p.weight_shift)));
   const int width = total / n, rest = total - width * n;
@@ -869,6 +882,7 @@ __device__ __forceinline__ bool cut(const ChunkParams& p, DMLA_LDS Window* win, 
     // (Starts that do not ascend can add up to anything; then there may be no place, and nothing to do.)
     win->at.b = win->at.rt = win->at.t = 0;
     win->end.b = win->end.rt = win->end.t = 0;
+    win->rows_log2 = rows_log2;
   }
   if (range >= n || x0 >= x1) return false;
   __syncthreads();
@@ -876,7 +890,7 @@ __device__ __forceinline__ bool cut(const ChunkParams& p, DMLA_LDS Window* win, 
   for (int b0 = 0, before = 0; b0 < p.B && before < x1; b0 += kThreads, before += sum) {
     if (p.B > kThreads) {
       s = load_window(p, win, b0);
-      mine = weight(p, weights(p, s), row_tiles(p, s));
+      mine = weight(p, weights(p, s, rows_log2), row_tiles(p, s, rows_log2));
       upto = scan(mine, sum);
     }
     const int lo = before + upto - mine, hi = before + upto;
@@ -885,8 +899,8 @@ __device__ __forceinline__ bool cut(const ChunkParams& p, DMLA_LDS Window* win, 
       to->rt = v.rt;
       to->t = v.t;
     };
-    if (lo <= x0 && x0 < hi) put(&win->at, place_of(p, b0 + tid, s, x0 - lo, width));
-    if (lo < x1 && x1 <= hi) put(&win->end, x1 == hi ? Place{b0 + tid, row_tiles(p, s), 0} : place_of(p, b0 + tid, s, x1 - lo, width));
+    if (lo <= x0 && x0 < hi) put(&win->at, place_of(p, b0 + tid, s, x0 - lo, width, rows_log2));
+    if (lo < x1 && x1 <= hi) put(&win->end, x1 == hi ? Place{b0 + tid, row_tiles(p, s, rows_log2), 0} : place_of(p, b0 + tid, s, x1 - lo, width, rows_log2));
   }
   __syncthreads();
   const int b = uniform(win->at.b), first = uniform(win->first);
@@ -902,6 +916,7 @@ __device__ __forceinline__ bool cut(const ChunkParams& p, DMLA_LDS Window* win, 
 __device__ __forceinline__ void next_piece(const ChunkParams& p, DMLA_LDS Window* win, DMLA_LDS i32x4* to, int range) {
   const int tid = threadIdx.x, lane = tid & 63;
   Place at = {uniform(win->at.b), uniform(win->at.rt), uniform(win->at.t)};
+  const int rows_log2 = uniform(win->rows_log2);
   const Place end = {uniform(win->end.b), uniform(win->end.rt), uniform(win->end.t)};
   Sequence s;
   for (;;) {
@@ -911,7 +926,7 @@ __device__ __forceinline__ void next_piece(const ChunkParams& p, DMLA_LDS Window
     }
     int first = uniform(win->first);
     s = known(win, at.b - first);
-    if (at.rt < row_tiles(p, s)) break;
+    if (at.rt < row_tiles(p, s, rows_log2)) break;
     // The next sequence with queries (there is one, end.b at the latest): 256 looked at together.
     int b = at.b + 1;
     for (;; b = first + kThreads) {
@@ -935,12 +950,12 @@ __device__ __forceinline__ void next_piece(const ChunkParams& p, DMLA_LDS Window
     }
     at = Place{uniform(b), 0, 0};
   }
-  const int row0 = at.rt * kRows, rows = min(s.n * p.H - row0, kRows);
+  const int row0 = at.rt << rows_log2, rows = min(s.n * p.H - row0, 1 << rows_log2);
   const bool whole = !(at.b == end.b && at.rt == end.rt);   // to its end
   __syncthreads();   // the place is read
   if (tid == 0) {
     to[0] = i32x4{s.q0, row0, rows, s.n};
-    to[1] = i32x4{s.len, at.b, at.t, whole ? key_tiles(p, s, at.rt) : end.t};
+    to[1] = i32x4{s.len, at.b, at.t, whole ? key_tiles(p, s, at.rt, rows_log2) : end.t};
     to[2] = i32x4{at.t > 0 ? 2 * range : whole ? -1 : 2 * range + 1, 0, 0, 0};
     Global<RangeLink> link = p.links + range;
     if (at.t > 0) {
@@ -982,17 +997,17 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_kernel(ChunkParams) {
     const i32x4 a = now[0], b = now[1];
     if (uniform(a[2]) == 0) break;
     next_piece(arguments(), win, other, my_range());
-    const Piece pc = {Sequence{uniform(a[0]), uniform(a[3]), uniform(b[0])}, uniform(b[1]), uniform(a[1]), uniform(b[2]), uniform(b[3]),
+    const Piece pc = {Sequence{uniform(a[0]), uniform(a[3]), uniform(b[0])}, uniform(b[1]), uniform(a[1]), uniform(a[2]), uniform(b[2]), uniform(b[3]),
                       uniform(now[2][0])};
     const DMLA_LDS int* next = (const DMLA_LDS int*)other;
     Pass pass = {false, (int)0x80000000, 0x7fffffff};
-    const bool few = narrow(uniform(a[2]));
+    const bool few = narrow(pc.rows);
     for (;;) {
       const bool again = few ? run_piece<true>(pc, lds, pass, have, next) : run_piece<false>(pc, lds, pass, have, next);
       have = true;
       if (pass.careful ? pass.to == 0x7fffffff : !again) break;
       const ChunkParams p = arguments();
-      const int base = pc.s.len - pc.s.n, last = min(pc.row0 + kRows, pc.s.n * p.H) - 1;
+      const int base = pc.s.len - pc.s.n, last = pc.row0 + pc.rows - 1;
       const int first_lim = p.causal ? base + fast_div(pc.row0, p.hdiv) : pc.s.len - 1;
       const int last_lim = p.causal ? base + fast_div(last, p.hdiv) : pc.s.len - 1;
       pass = careful_pass(p, pc, lds, pass.careful ? pass.to : first_lim, last_lim);
@@ -1222,14 +1237,15 @@ __global__ __launch_bounds__(256) void chunk_combine_kernel(ChunkParams p) {
   }
 }
 
-// At least the weight that the kernel adds up.
-int64_t chunk_weight(int64_t T, int64_t B, int64_t H, int64_t max_pages) {
-  const int64_t tiles = T * H / kRows + std::min(B, T);
+// At least the weight that the kernel adds up, in row tiles of `rows` rows.
+int64_t chunk_weight(int64_t T, int64_t B, int64_t H, int64_t max_pages, int64_t rows) {
+  const int64_t tiles = T * H / rows + std::min(B, T);
   return tiles * (kCost + 3 + max_pages * (kPage / kTile));
 }
 // Ranges of a call: one per CU, as many as its work can fill at most.
 int64_t chunk_ranges(int64_t T, int64_t B, int64_t H, int64_t max_pages) {
-  return std::max<int64_t>(1, std::min<int64_t>(std::min(device_cu_count(), kMaxRanges), (chunk_weight(T, B, H, max_pages) + kMinWidth - 1) / kMinWidth));
+  const int64_t most = chunk_weight(T, B, H, max_pages, kNarrowRows);
+  return std::max<int64_t>(1, std::min<int64_t>(std::min(device_cu_count(), kMaxRanges), (most + kMinWidth - 1) / kMinWidth));
 }
 int64_t chunk_bytes(int64_t ranges) { return ranges * (2 * kRows * (int64_t)(kDv + 1) * 4 + (int64_t)sizeof(RangeLink)); }
 
@@ -1292,7 +1308,7 @@ extern "C" int dmla_chunk_paged(const void* q, const void* kv_pool, const int32_
   p.scale_log2 = softmax_scale * kLog2e;
   p.n_ranges = (int)chunk_ranges(T, B, H, max_pages_per_seq);
   p.two_by_h = 2.0f / (float)H;
-  while (chunk_weight(T, B, H, max_pages_per_seq) >> p.weight_shift > (int64_t)1 << 30) ++p.weight_shift;
+  while (chunk_weight(T, B, H, max_pages_per_seq, kRows) >> p.weight_shift > (int64_t)1 << 30) ++p.weight_shift;
   p.weight_scale = std::ldexp(1.0f, -p.weight_shift);
   // A combine workgroup holds 110 registers a lane, so 4 per CU run at once; a call of few row tiles takes 8 (one of
   // 100000 tokens x 128 heads 17.8 -> 15.3 us), more would only queue (64 sequences x 16 heads 6.9 with 4, 10.9 with 8).

@@ -201,3 +201,96 @@ def test_short_sequences_beside_tables_of_a_million_pages(gpu):
     n = sum(counts)
     check(q, o[:n], lse[:n], rows, lens, counts, some=set(list(range(10)) + list(range(n - 110, n)) + r.sample(range(n), 30)))
     assert (o[n:] == 0).all() and (lse[n:] == float("-inf")).all()
+
+
+# ---- row tiles of 128 rows: a call with less than 900 tiles of 32 keys is cut in row tiles of 32 --------
+
+LONG = 29000   # tokens of a sequence that makes a call large
+
+
+@pytest.mark.parametrize("H,lens,counts", [
+    (128, [1], [1]), (128, [5], [5]), (16, [33, 200, 7], [33, 9, 2]), (1, [300, 64], [290, 64]), (5, [97, 31, 1000], [50, 31, 3]),
+    (20, [129, 0, 63], [17, 0, 1]), (96, [70, 40], [3, 40]), (128, [2000], [3]), (128, [191, 640], [64, 2]), (130, [100], [3]),
+    (300, [66], [2]), (64, [33] * 40, [1] * 40), (33, [40], [1]), (32, [40, 50], [1, 2])])
+@pytest.mark.parametrize("causal", [True, False])
+def test_large_calls(gpu, H, lens, counts, causal):
+    lens, counts = lens + [LONG], counts + [1]
+    pool, table, rows = paged(lens, gpu, seed=H)
+    q = queries(sum(counts), H, H)
+    o, lse = run(gpu, q, pool, table, lens, counts, causal)
+    check(q, o, lse, rows, lens, counts, causal)
+
+
+@pytest.mark.parametrize("H", [1, 16, 48, 128])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+def test_large_calls_and_what_a_query_does_not_attend(gpu, H, value):
+    lens, counts = [90, LONG], [60, 1]
+    pool, table, rows = paged(lens, gpu)
+    q = queries(61, H, 3)
+    for bad in ([45], [31, 32, 77], list(range(60, 90))):
+        p = pool.clone()
+        for j in bad:
+            p[table[0, j // PAGE].item(), j % PAGE, 5] = value
+        o, lse = run(gpu, q, p, table, lens, counts)
+        clean = max(0, bad[0] - 30)   # query i is token 30 + i
+        check(q, o, lse, rows, lens, counts, some=set(range(clean)) | {60})
+        assert not torch.isfinite(o[clean:60, :, 5]).any(), "a query that attends it"
+
+
+@pytest.mark.parametrize("H", [16, 128])
+def test_large_calls_with_bad_pages(gpu, H):
+    lens, counts = [200, 130, LONG], [200, 2, 1]
+    pool, table, rows = paged(lens, gpu)
+    q = queries(203, H, 5)
+    for bad in (-1, pool.shape[0], 2 ** 31 - 1):
+        t = table.clone()
+        t[0, 2] = bad
+        o, lse = run(gpu, q, pool, t, lens, counts)
+        check(q, o, lse, rows, lens, counts, some=set(range(128)) | {200, 201, 202})
+        assert torch.isnan(o[128:200]).all() and torch.isnan(lse[128:200]).all()
+
+
+@pytest.mark.parametrize("steepest", [4.0, 60.0])
+@pytest.mark.parametrize("H", [16, 128])
+def test_large_calls_with_climbing_scores(gpu, H, steepest):
+    N = 400
+    pool, table, rows = paged([N, LONG], gpu)
+    climb = torch.zeros(N, D_QK)
+    climb[:, :D_V] = 2.0 ** 110
+    climb[:, D_V] = torch.linspace(0, 60, N)
+    rows[0] = climb.to(torch.bfloat16)
+    for j in range(pages(N)):
+        part = rows[0][PAGE * j:PAGE * (j + 1)]
+        pool[table[0, j].item(), :len(part)] = part.to(gpu)
+    q = torch.zeros(10, H, D_QK)
+    q[:, :, D_V] = torch.linspace(0.1, steepest, H)
+    q = q.to(torch.bfloat16)
+    o, lse = run(gpu, q, pool, table, [N, LONG], [9, 1])
+    check(q, o, lse, rows, [N, LONG], [9, 1])
+
+
+def test_large_calls_with_strides(gpu):
+    from python import ops
+    lens, counts, H = [150, 20, LONG], [40, 20, 1], 16
+    pool, table, rows = paged(lens, gpu)
+    q = queries(61, H, 4)
+    q2 = torch.full((61, H + 3, D_QK + 8), float("nan"), dtype=torch.bfloat16, device=gpu)
+    q2[:, :H, :D_QK] = q.to(gpu)
+    p2 = torch.full((pool.shape[0], PAGE + 2, D_QK + 24), float("nan"), dtype=torch.bfloat16, device=gpu)
+    p2[:, :PAGE, :D_QK] = pool
+    by_head = q.transpose(0, 1).contiguous().to(gpu).transpose(0, 1)
+    want = run(gpu, q, pool, table, lens, counts)
+    check(q, *want, rows, lens, counts)
+    for x, y in ((q2[:, :H, :D_QK], p2[:, :PAGE, :D_QK]), (by_head, pool)):
+        got = ops.flash_dmla_chunk_paged(x, y, table, ints(lens, gpu), ints(starts(counts), gpu), softmax_scale=SCALE,
+                                         return_lse=True)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("N", [28300, 28500, 28544, 28576, 28608, 28700])
+@pytest.mark.parametrize("H,n", [(128, 1), (40, 2)])
+def test_where_row_tiles_change_their_size(gpu, N, H, n):
+    pool, table, rows = paged([N], gpu)
+    q = queries(n, H, 7)
+    o, lse = run(gpu, q, pool, table, [N], [n])
+    check(q, o, lse, rows, [N], [n])
