@@ -10,6 +10,7 @@
 #include <algorithm>
 
 #include "dmla_host.h"
+#include "dmla_pipe.h"
 #include "dmla_q4.h"
 
 namespace dmla {
@@ -158,8 +159,9 @@ __device__ __forceinline__ void head_sums(const ScoreArgs& a, int t, int head, f
 // three tiles ahead.  For the sums over pages the means are the MFMA's rows, so a lane has 16 pages of one head; for
 // the sums over heads they are its columns, so a lane has 16 heads of one page.  Both sums are then in-lane, in a
 // fixed order.
-// Bound: latency (a launch, queries, the first tile); the rates would allow 3 us for the means of 64 sequences of 8192 to
-// 32768 tokens and their queries.  The first version held the queries in LDS, 147 KB for each 64 pages.
+// Bound: a few tiles a workgroup by latency (a launch, 147 KB of queries 3 us, the first tile 2); a tile takes 1.2 us, the
+// LDS reads of four waves that each need all of it; long tables by HBM (64 queries x 128 heads x 2000 pages, 280 MB with the
+// products: 58 us).
 template <int kMode>
 __global__ void __launch_bounds__(kScoreThreads, 1) page_scores_kernel(ScoreArgs a) {
   __shared__ __attribute__((aligned(1024))) char mem[kRing * (kTileBytes + kRopeBytes)];
@@ -226,7 +228,7 @@ __global__ void __launch_bounds__(kScoreThreads, 1) page_scores_kernel(ScoreArgs
         const int i = query_of(r);
         return i >= i0 && i < i1 ? s_pages[i] : 0;
       };
-      // Tiles in order, each through each(s, k, there): operand reader and a bit per page in the pool.
+      // Tiles in order, each through each(s, k, there, beside): operand reader, a bit per page in the pool, what runs after product c.
       auto stream = [&](auto each) {
         if (n_tiles == 0) return;
         // Table entries of tiles [s, s + kIdTiles / 2), -1 where there is no page of the pool.
@@ -237,37 +239,58 @@ __global__ void __launch_bounds__(kScoreThreads, 1) page_scores_kernel(ScoreArgs
             s_ids[(kTile * s + k) % (kTile * kIdTiles)] = id < a.num_pages ? id : -1;
           }
         };
-        auto copy = [&](int s) {   // (past the end: the last tile once more, so that the copies count the same)
-          const int t = min(s, n_tiles - 1);
+        // Tile s's pages of this wave (past the end: the last tile once more, so that the copies count the same), and copy i
+        // of kCopies.
+        auto pages_of = [&](int s) {
+          return max(s_ids[(kTile * min(s, n_tiles - 1)) % (kTile * kIdTiles) + 8 * wave + (lane >> 3)], 0);   // not there: page 0, masked
+        };
+        auto copy = [&](int s, int id, int i) {
           const unsigned slot = (unsigned)(s % kRing);
-          const int id = max(s_ids[(kTile * t) % (kTile * kIdTiles) + 8 * wave + (lane >> 3)], 0);   // not there: page 0, masked
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int r = 8 * wave + i;
-            dma16(a.means + __builtin_amdgcn_readlane(id, 8 * i) * a.m_sp, 16 * (lane ^ mean_swz(r)), tiles + slot * kTileBytes + r * kMeanRow);
-          }
-          dma16_addr(a.means + id * a.m_sp + kLat + 8 * ((lane & 7) ^ (lane >> 3)), ropes + slot * kRopeBytes + wave * 1024);
+          const int r = 8 * wave + i;
+          if (i < 8) dma16(a.means + __builtin_amdgcn_readlane(id, 8 * i) * a.m_sp, 16 * (lane ^ mean_swz(r)), tiles + slot * kTileBytes + r * kMeanRow);
+          else dma16_addr(a.means + id * a.m_sp + kLat + 8 * ((lane & 7) ^ (lane >> 3)), ropes + slot * kRopeBytes + wave * 1024);
         };
         load_ids(0);
         if (n_tiles > kIdTiles / 2) load_ids(kIdTiles / 2);
         __syncthreads();
-        copy(0);
-        copy(1);
-        copy(2);
+        for (int s = 0; s < 3; ++s) {
+          const int id = pages_of(s);
+#pragma unroll
+          for (int i = 0; i < kCopies; ++i) copy(s, id, i);
+        }
         for (int s = 0; s < n_tiles; ++s) {
           // Half the entries ahead of their use, into the half that every wave is past.
           if (s > 1 && s % (kIdTiles / 2) == 1 && s - 1 + kIdTiles / 2 < n_tiles) load_ids(s - 1 + kIdTiles / 2);
           wait_vm<2 * kCopies>();   // tile s; those of two tiles more may be on their way (or stores of an earlier one)
           __syncthreads();          // tile s landed, tile s - 1 is read
-          copy(s + 3);
+          const int id = pages_of(s + 3);
           const unsigned key = lds_sum(kMeanRow * l32 + 16 * (hl ^ mean_swz(l32)), tiles + (unsigned)(s % kRing) * kTileBytes);
           const unsigned rope = lds_sum(128 * l32 + 16 * (hl ^ (l32 & 7)), ropes + (unsigned)(s % kRing) * kRopeBytes);
           each(s, [&](int c) {
             return *lds_ptr<const bf16x8>(c < kLatSteps ? (key ^ (32 * (c & 7))) + 256 * (c >> 3) : rope ^ (32 * (c - kLatSteps)));
-          }, (unsigned)__ballot(s_ids[(kTile * s) % (kTile * kIdTiles) + l32] >= 0));
+          }, (unsigned)__ballot(s_ids[(kTile * s) % (kTile * kIdTiles) + l32] >= 0), [&](int c) {   // between its products
+            if (c % 4 == 1) copy(s + 3, id, c / 4);
+          });
         }
         wait_vm<0>();
         __syncthreads();   // the last tile is read, no copy is on its way
+      };
+      // A tile's products; operands are read kDepth MFMAs ahead (left to the compiler, each waits for its own: 3800
+      // cycles a tile instead of 2800).
+      auto product = [&](auto k, auto beside, auto multiply) {
+        constexpr int kDepth = 8;
+        bf16x8 mean[kDepth];
+#pragma unroll
+        for (int c = 0; c < kDepth; ++c) mean[c] = k(c);
+        f32x16 x = {};
+        static_for<kSteps>([&](auto c_tag) {
+          constexpr int c = decltype(c_tag)::value;
+          x = multiply(mean[c % kDepth], q[c], x);
+          if constexpr (c + kDepth < kSteps) mean[c % kDepth] = k(c + kDepth);
+          beside(c);
+          in_order();
+        });
+        return x;
       };
       // Bit k: page k of tile s is one of the first n of the sequence.
       auto first_pages = [&](int s, int n) {
@@ -283,10 +306,8 @@ __global__ void __launch_bounds__(kScoreThreads, 1) page_scores_kernel(ScoreArgs
         float* keep = nullptr;
         if constexpr (kMode == kKeep)
           if (own && head < a.H) keep = a.kept + ((int64_t)(t0 + i) * a.H + head) * a.kept_sp + c0 + 4 * hl;
-        stream([&](int s, auto k, unsigned there) {
-          f32x16 x = {};
-#pragma unroll
-          for (int c = 0; c < kSteps; ++c) x = mfma32_bf16(k(c), q[c], x);
+        stream([&](int s, auto k, unsigned there, auto beside) {
+          f32x16 x = product(k, beside, [](const bf16x8& mean, const bf16x8& row, const f32x16& x) { return mfma32_bf16(mean, row, x); });
           if constexpr (kMode == kKeep) {
             if (keep != nullptr) {
 #pragma unroll
@@ -341,11 +362,9 @@ __global__ void __launch_bounds__(kScoreThreads, 1) page_scores_kernel(ScoreArgs
           }
         }
         const int limit0 = rows_pages(32 * wave), limit1 = rows_pages(32 * wave + 16);
-        stream([&](int s, auto k, unsigned there) {
+        stream([&](int s, auto k, unsigned there, auto beside) {
           if (s > 0) put(s - 1);
-          f32x16 x = {};
-#pragma unroll
-          for (int c = 0; c < kSteps; ++c) x = mfma32_bf16(q[c], k(c), x);
+          const f32x16 x = product(k, beside, [](const bf16x8& mean, const bf16x8& row, const f32x16& x) { return mfma32_bf16(row, mean, x); });
           float v0 = 0.f, v1 = 0.f;
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
