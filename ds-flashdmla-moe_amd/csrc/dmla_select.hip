@@ -593,7 +593,7 @@ struct ScoreShape {
   int64_t stats_bytes(int64_t T, int64_t H) const { return (chunks > 1 ? chunks * T * H * (int64_t)sizeof(float2) : 0) + 15 & ~(int64_t)15; }
   int64_t bytes(int64_t T, int64_t H) const { return stats_bytes(T, H) + T * H * kept_sp * (int64_t)sizeof(float); }
 };
-// Up to here the products are kept (64 queries x 128 heads x 500 / 8000 pages: 28 / 237 us, computed again 36 / 297).
+// Up to here the products are kept (64 queries x 128 heads x 500 / 8000 pages: 26 / 234 us, computed again 31 / 247).
 constexpr int64_t kKeepBytes = (int64_t)512 << 20;
 ScoreShape score_shape(int64_t T, int64_t H, int64_t max_pages, bool packed) {
   ScoreShape s;
