@@ -148,14 +148,15 @@ struct Pages {
     pages = i < (pc.t1 + 1) / 2 ? p.block_table[pc.b * p.bt_sb + i] : 0;
     asm volatile("" : "+v"(pages));   // waited for here, in the rare branch, and not by every reader
   }
-  // Address of a key tile; tiles come in ascending order.  A bad page reads page 0 instead.
-  __device__ __forceinline__ const char* tile(const ChunkParams& p, const Piece& pc, int t) {
-    if (t / 2 - first >= 64) fetch(p, pc, first + 64);
-    int page = __builtin_amdgcn_readlane(pages, uniform((t / 2 - first) & 63));
-    const bool off = page < 0 || page >= p.num_pages;
-    bad = off ? min(bad, t / 2) : bad;
-    page = off ? 0 : page;
-    return (const char*)(p.kv + page * p.kv_sp + (t & 1) * kTile * p.kv_ss);
+  // The page of index i; they come in ascending order.  A bad page reads page 0 instead.
+  __device__ __forceinline__ void reach(const ChunkParams& p, const Piece& pc, int i) {
+    if (i - first >= 64) fetch(p, pc, first + 64);
+  }
+  __device__ __forceinline__ int page(const ChunkParams& p, int i) {
+    const int page = __builtin_amdgcn_readlane(pages, uniform((i - first) & 63));
+    const bool off = (unsigned)page >= (unsigned)p.num_pages;
+    bad = off ? min(bad, i) : bad;
+    return off ? 0 : page;
   }
 };
 
@@ -219,14 +220,26 @@ __device__ __forceinline__ bool run_piece(const Piece& pc, const Lds& lds, const
   int copy_more = 0;                // rows behind it
   unsigned copy_keys = 0, copy_rope = 0, copy_lane = 0;
   const int row_step = uniform((int)p.kv_ss);
-  auto copy_begin = [&](int s) {
-    copy_lane = 16 * (fresh_lane_id() ^ key_swz(8 * wave));
-    const int t = min(pc.t0 + s, t1 - 1);   // past the end: the last tile, which nobody counts
-    const int last = uniform(min(key_end - t * kTile, kTile) - 1), row = min(8 * wave, last);
-    copy_src = pages.tile(p, pc, t) + row * row_step;
-    copy_more = last - row;
-    copy_keys = lds.keys + (unsigned)(s % kSlots) * kKeyBytes + wave * 8 * kKeyRow;
-    copy_rope = lds.rope + (unsigned)(s % (kNarrow ? kNarrowRopes : kSlots)) * kRopeBytes + wave * 1024;
+  // What the copies of a tile need, in kBegins parts for the gaps between MFMAs (an MFMA hides about six instructions).
+  constexpr int kBegins = 4;
+  int copy_t = 0, copy_row = 0;
+  auto copy_begin = [&](int s, int part) {
+    if (part == 0) {
+      copy_t = min(pc.t0 + s, t1 - 1);   // past the end: the last tile, which nobody counts
+      pages.reach(p, pc, copy_t >> 1);
+    } else if (part == 1) {
+      const int last = uniform(min(key_end - copy_t * kTile, kTile) - 1);
+      copy_row = min(8 * wave, last);
+      copy_more = last - copy_row;
+      copy_row += (copy_t & 1) * kTile;   // of the page
+    } else if (part == 2) {
+      copy_src = (const char*)(p.kv + pages.page(p, copy_t >> 1) * p.kv_sp);
+    } else {
+      copy_src += copy_row * row_step;
+      copy_lane = 16 * (fresh_lane_id() ^ key_swz(8 * wave));
+      copy_keys = lds.keys + (unsigned)(s % kSlots) * kKeyBytes + wave * 8 * kKeyRow;
+      copy_rope = lds.rope + (unsigned)(s % (kNarrow ? kNarrowRopes : kSlots)) * kRopeBytes + wave * 1024;
+    }
   };
   auto copy = [&](int i) {
     if (i < 8) {   // key_swz(8 wave + i) is key_swz(8 wave) ^ key_swz(i)
@@ -238,7 +251,8 @@ __device__ __forceinline__ bool run_piece(const Piece& pc, const Lds& lds, const
     }
   };
   auto copy_tile = [&](int s) {
-    copy_begin(s);
+#pragma unroll
+    for (int i = 0; i < kBegins; ++i) copy_begin(s, i);
 #pragma unroll
     for (int i = 0; i < kCopies; ++i) copy(i);
   };
@@ -325,6 +339,12 @@ __device__ __forceinline__ bool run_piece(const Piece& pc, const Lds& lds, const
     for (int i = 1; i < 16; ++i) mx = fmaxf(mx, x[i]);
     return half_max(mx) * p.scale_log2;   // scale > 0
   };
+  // (fmaxf would quiet each operand first, an instruction more for each.)
+  auto max3 = [](float a, float b, float c) {
+    float v;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(v) : "v"(a), "v"(b), "v"(c));
+    return v;
+  };
   // The softmax of a tile in kPieces pieces, which the value product of another tile takes between its
   // MFMAs: the maximum, then an element at a time.
   constexpr int kPieces = 21;
@@ -333,9 +353,9 @@ __device__ __forceinline__ bool run_piece(const Piece& pc, const Lds& lds, const
   auto softmax_piece = [&](const f32x16& x, auto i_tag) {
     constexpr int i = decltype(i_tag)::value;
     if constexpr (i < 4) {
-      mx_part[i] = fmaxf(fmaxf(x[4 * i], x[4 * i + 1]), fmaxf(x[4 * i + 2], x[4 * i + 3]));
+      mx_part[i] = max3(max3(x[4 * i], x[4 * i + 1], x[4 * i + 2]), x[4 * i + 3], x[4 * i + 3]);
     } else if constexpr (i == 4) {
-      const float mx = half_max(fmaxf(fmaxf(mx_part[0], mx_part[1]), fmaxf(mx_part[2], mx_part[3])));
+      const float mx = half_max(max3(max3(mx_part[0], mx_part[1], mx_part[2]), mx_part[3], mx_part[3]));
       mtrue = fmaxf(mtrue, mx * p.scale_log2);   // scale > 0
       ms = mref == kNegInf ? 0.f : mref;
     } else if constexpr (i < kPieces) {
@@ -513,7 +533,8 @@ __device__ __forceinline__ bool run_piece(const Piece& pc, const Lds& lds, const
       for (int c = 0; c < kDepth; ++c) read_key(c);
       f32x16 x0 = scores([&](auto m_tag) {
         constexpr int m = decltype(m_tag)::value;
-        if constexpr (m % 18 == 0) copy_begin(1 + m / 18);
+        if constexpr (m % 18 == 0)
+          for (int i = 0; i < kBegins; ++i) copy_begin(1 + m / 18, i);
         if constexpr (m % 2 == 1) copy(m % 18 / 2);
       });
       score_done(x0);
@@ -538,8 +559,9 @@ __device__ __forceinline__ bool run_piece(const Piece& pc, const Lds& lds, const
       for (int s = 1; s < n_steps; ++s) {
         f32x16 x = scores([&](auto m_tag) {
           constexpr int m = decltype(m_tag)::value;
-          if constexpr (m == 1) copy_begin(s + 2);
-          if constexpr (m % 7 == 2) copy(m / 7);
+          if constexpr (m >= 1 && m <= kBegins) copy_begin(s + 2, m - 1);
+          // (A copy takes a CU some 90 cycles for four waves, three MFMAs; beside the softmax there is no room for them.)
+          if constexpr (m >= 6 && m % 3 == 0 && m != 24) copy(m < 24 ? m / 3 - 2 : m / 3 - 3);
           if constexpr (m == 22) {
             wait_lds<7>();   // P is posted; reads of later keys may be on their way
             barrier();       // A
@@ -550,7 +572,6 @@ __device__ __forceinline__ bool run_piece(const Piece& pc, const Lds& lds, const
         });
         values([&](auto i_tag) {
           constexpr int i = decltype(i_tag)::value;
-          if constexpr (i % 6 == 1 && i < 20) copy(5 + i / 6);
           if constexpr (i == 2) {
             asm("s_nop 7" : "+v"(x));
             mask(x, s);
