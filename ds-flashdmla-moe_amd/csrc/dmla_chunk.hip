@@ -299,7 +299,7 @@ __device__ __forceinline__ bool run_piece(const Piece& pc, const Lds& lds, const
 
   // ---- scores: S^T[key 8 (i / 4) + 4 hl + i % 4][row l32] of step s's tile ----
   bf16x8 rope[4];
-  constexpr int kDepth = 8;   // operands in flight
+  constexpr int kDepth = 6;   // operands in flight
   unsigned key_addr = 0;
   bf16x8 k[kDepth];
   auto read_rope = [&](int s) {
@@ -586,7 +586,7 @@ __device__ __forceinline__ bool run_piece(const Piece& pc, const Lds& lds, const
           } else if constexpr (i == 26) {
             read_rope(s + 1);
             scores_begin(s + 1);
-          } else if constexpr (i > 26 && i < 31) {
+          } else if constexpr (i > 26 && i <= 26 + kDepth / 2) {
             read_key(2 * (i - 27));
             read_key(2 * (i - 27) + 1);
           }
