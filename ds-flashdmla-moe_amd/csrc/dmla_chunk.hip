@@ -20,12 +20,13 @@
 //    a second kernel joins what was cut.
 //
 // Bound, by what a call is made of (MI355X, 1.2 PFLOP/s and 5 TB/s being what a large product and a large copy reach):
-//  * Chunks and prompts by the matrix cores: a tile of 32 keys takes 128 rows 1.7 us, 1.3 PFLOP/s over all CUs; 1024
-//    queries x 128 heads over 8192 tokens 1.78 ms (1.23 PFLOP/s).
-//  * Many single tokens by HBM: 512 sequences of 2048 tokens x 16 heads 229 us, 5.3 TB/s.
+//  * Chunks and prompts by the matrix cores: a tile of 32 keys takes 128 rows 1.6 us, 1.4 PFLOP/s over all CUs; 1024
+//    queries x 128 heads over 8192 tokens 1.69 ms (1.30 PFLOP/s, a large library product 1.36).  68 MFMAs are 2200 of a
+//    tile's 3400 cycles; an MFMA hides about six other instructions, and what is more of them shows.
+//  * Many single tokens by HBM: 512 sequences of 2048 tokens x 16 heads 227 us, 5.3 TB/s.
 //  * Short rows of keys by what a piece costs beside its tiles, 9 us: 3 us of queries through LDS (their copies, the
 //    first tile, the last tile's values) and 4 us of outputs, both at what a CU's vector memory path takes (some 27
-//    bytes a cycle).  Four prompts of 300 to 1900 tokens x 128 heads: 880 us, 0.99 PFLOP/s.
+//    bytes a cycle).  Four prompts of 200 to 2000 tokens x 128 heads: 837 us, 1.04 PFLOP/s.
 //  * One token by latency: the cut, queries, tiles, the join: 27 us for 5000 tokens x 128 heads.
 #include <algorithm>
 #include <cmath>
