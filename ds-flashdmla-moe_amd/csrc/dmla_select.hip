@@ -29,44 +29,71 @@ struct MeansArgs {
   int B, num_pages, max_pages;
 };
 
-// A page per workgroup at a time: thread (g, c) adds rows 8 g .. 8 g + 7 of the 8 columns of piece c, the eight
-// groups meet in LDS, in order.
-// Bound: HBM, the pages' rows; a decode step has at most one new full page per sequence and is a launch.
-constexpr int kMeanGroups = 8, kMeanThreads = kMeanGroups * (kD / 8);   // 576, nine waves
+// A page per workgroup at a time: thread (g, c) adds the rows of group g in piece c, the groups meet in LDS, in order.
+// Pieces are 16 bytes of a row: of bf16 rows 8 columns, of 4-bit rows 32 columns (16 of those, and eight of the rope's).
+// Bound: of bf16 rows HBM (64 sequences of 500 pages 461 us, 5.1 TB/s), of 4-bit rows conversions and additions (271 us, 3.0
+// TB/s; a word of codes and a byte of scale a load took 684); a decode step has at most one new full page per sequence
+// and is a launch.
 template <bool kQ4>
-__global__ void __launch_bounds__(kMeanThreads) page_means_kernel(MeansArgs a) {
-  __shared__ __attribute__((aligned(16))) float part[kMeanGroups][kD];
-  const int g = threadIdx.x / (kD / 8), c = threadIdx.x % (kD / 8);
+struct MeanShape {
+  static constexpr int kPieces = kQ4 ? kLat / 32 + (kD - kLat) / 8 : kD / 8;
+  static constexpr int kGroups = kQ4 ? 16 : 8, kThreads = kGroups * kPieces, kRows = kPage / kGroups;   // 384 or 576 threads
+};
+template <bool kQ4>
+__global__ void __launch_bounds__(MeanShape<kQ4>::kThreads) page_means_kernel(MeansArgs a) {
+  using Shape = MeanShape<kQ4>;
+  __shared__ __attribute__((aligned(16))) float part[Shape::kGroups][kD];
+  const int g = threadIdx.x / Shape::kPieces, c = threadIdx.x % Shape::kPieces;
+  const bool codes = kQ4 && c < kLat / 32;
+  const int offset = !kQ4 || codes ? 16 * c : kQ4RopeOff + 16 * (c - kLat / 32);
   for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
     const int64_t len = min((int64_t)a.seqlens[b], (int64_t)a.max_pages * kPage);
     const int first = a.starts != nullptr ? max(a.starts[b], 0) / kPage : 0;
     for (int64_t p = first + blockIdx.y; p < len / kPage; p += gridDim.y) {
       const int page = a.block_table[b * a.bt_sb + p];
       if (page < 0 || page >= a.num_pages) continue;   // (uniform)
-      float x[8] = {};
+      u32x4 v[Shape::kRows];
+      int scale[Shape::kRows] = {};
 #pragma unroll
-      for (int r = 0; r < kPage / kMeanGroups; ++r) {
-        const char* row = a.pool + page * a.kv_sp + (g * (kPage / kMeanGroups) + r) * a.kv_ss;
-        bf16x8 v;
-        if constexpr (!kQ4) v = *reinterpret_cast<const bf16x8*>(row + 16 * c);
-        else if (c >= kLat / 8) v = *reinterpret_cast<const bf16x8*>(row + kQ4RopeOff + 16 * (c - kLat / 8));
-        else v = q4_octet(*reinterpret_cast<const unsigned*>(row + 4 * c), q4_scale((uint8_t)row[kQ4ScaleOff + c / 4]));
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] += (float)v[i];
+      for (int r = 0; r < Shape::kRows; ++r) {
+        const char* row = a.pool + page * a.kv_sp + (g * Shape::kRows + r) * a.kv_ss;
+        v[r] = *reinterpret_cast<const u32x4*>(row + offset);
+        if (codes) scale[r] = (uint8_t)row[kQ4ScaleOff + c];
       }
+      if (codes) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) part[g][8 * c + i] = x[i];
-      __syncthreads();
-      if (g == 0) {
-        bf16x8 v;
+        for (int w = 0; w < 4; ++w) {
+          float x[8] = {};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          float s = x[i];
+          for (int r = 0; r < Shape::kRows; ++r) {
+            const bf16x8 o = q4_octet(v[r][w], q4_scale(scale[r]));
 #pragma unroll
-          for (int o = 1; o < kMeanGroups; ++o) s += part[o][8 * c + i];
-          v[i] = (bf16)(s * (1.0f / kPage));
+            for (int i = 0; i < 8; ++i) x[i] += (float)o[i];
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) part[g][32 * c + 8 * w + i] = x[i];
         }
-        *reinterpret_cast<bf16x8*>(a.means + page * a.m_sp + 8 * c) = v;
+      } else {
+        float x[8] = {};
+#pragma unroll
+        for (int r = 0; r < Shape::kRows; ++r) {
+          const bf16x8 o = __builtin_bit_cast(bf16x8, v[r]);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] += (float)o[i];
+        }
+        const int column = kQ4 ? kLat + 8 * (c - kLat / 32) : 8 * c;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) part[g][column + i] = x[i];
+      }
+      __syncthreads();
+      if (threadIdx.x < kD / 4) {
+        f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int o = 0; o < Shape::kGroups; ++o) sum += *reinterpret_cast<const f32x4*>(&part[o][4 * threadIdx.x]);
+        bf16x4 m;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m[i] = (bf16)(sum[i] * (1.0f / kPage));
+        *reinterpret_cast<bf16x4*>(a.means + page * a.m_sp + 4 * threadIdx.x) = m;
       }
       __syncthreads();
     }
@@ -647,11 +674,9 @@ extern "C" int dmla_page_means(const void* kv_pool, const int32_t* block_table, 
   a.B = (int)B; a.num_pages = (int)num_pages; a.max_pages = (int)max_pages_per_seq;
   const int64_t wgs = 8 * device_cu_count();
   const int64_t x = std::min(B, wgs), y = std::min<int64_t>(std::max<int64_t>(1, wgs / x), max_pages_per_seq);
-  auto launch = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)x, (unsigned)y), dim3(kMeanThreads), 0, (hipStream_t)stream, a);
-  };
-  if (q4) launch(page_means_kernel<true>);
-  else launch(page_means_kernel<false>);
+  const dim3 grid((unsigned)x, (unsigned)y);
+  if (q4) hipLaunchKernelGGL(page_means_kernel<true>, grid, dim3(MeanShape<true>::kThreads), 0, (hipStream_t)stream, a);
+  else hipLaunchKernelGGL(page_means_kernel<false>, grid, dim3(MeanShape<false>::kThreads), 0, (hipStream_t)stream, a);
   return check_launch(what);
 }
 
