@@ -201,6 +201,7 @@ __device__ __forceinline__ bool cut(const ChunkParams& p, DMLA_LDS Window* win, 
   // Inclusive sum over the threads and their total.
   auto scan = [&](int v, int& sum) {
     v = lane_scan(v);
+    __syncthreads();   // every wave has read the sums of a scan before
     if (lane == 63) win->tmp[wave] = v;
     __syncthreads();
     sum = 0;
