@@ -89,6 +89,7 @@ __device__ __forceinline__ Pass careful_pass(const ChunkParams& p, const Piece& 
       break;
     }
   }
+  __syncthreads();   // every wave has read from these words that a pass follows
   if (fresh_lane_id() == 0) flag[wave] = to;
   __syncthreads();
   to = uniform(min(min(flag[0], flag[1]), min(flag[2], flag[3])));

@@ -116,3 +116,30 @@ def watched(tmp_path_factory):
 def test_the_cut_has_no_races(watched, H, lens, counts):
     """Little work (cut twice), much, several rounds of 256 sequences, a range that begins behind the first of them."""
     assert_all_done_once(cut_of(watched, H, lens, counts, n_ranges=3), H, lens, counts)
+
+
+# ---- the rows of a careful pass ------------------------------------------------------------------------
+
+END = 0x7fffffff   # no row is left out
+
+
+def careful(exe, begin, last, odd=(), table=(3, 1, 2, 0), pages=4, end=8):
+    """The pass of the rows whose last tokens are from `begin` on up to `last`, of a piece that ends at key tile `end`;
+    odd: tokens that hold an infinity."""
+    at = [table[j // 64] * 64 + j % 64 for j in odd]
+    out, = ask(exe, ["careful", pages, begin, last, end, len(at), len(table), *at, *table])
+    assert out[:2] == [1, begin]
+    return out[2]
+
+
+@pytest.mark.parametrize("begin,last,odd,to", [
+    (10, 90, [], END), (10, 90, [10], END), (10, 90, [11], 11), (10, 90, [91], END), (10, 90, [90, 33, 64], 33), (-1, 20, [0], 0),
+    (-5, 20, [0, 3], 0), (-1, 20, [], END), (200, 200, [100], END)])
+def test_where_rows_are_cut(checked, begin, last, odd, to):
+    assert careful(checked, begin, last, odd) == to
+
+
+def test_a_careful_pass_has_no_races(watched):
+    """Its waves post where they would cut in the words in which they have just read that a pass has to follow."""
+    assert careful(watched, -1, 20, [0]) == 0
+    assert careful(watched, 10, 90, []) == END
