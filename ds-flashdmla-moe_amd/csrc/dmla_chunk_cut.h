@@ -66,20 +66,25 @@ struct Piece {
 // A piece runs once, against each row's largest score in the first tile.  Where scores have climbed more than kHeadroom
 // above it, or an output is not a number or infinite, it runs the careful way: a row's reference is the largest score
 // that was seen, and a row sees nothing of later tokens, as a probability of 0 times a latent that is not a number is
-// none either.  So the rows are cut where a later row's token holds such a latent, and the rows before it run
-// without it.  Both are rare, and the loop holds neither rescaling nor tests.
+// none either.  So the rows are cut where a later row's token holds such a latent or begins a page outside the pool, and
+// the rows before it run without it.  Both are rare, and the loop holds neither rescaling nor tests.
 struct Pass {
   bool careful;
   int from, to;   // rows with a limit in [from, to) are written
 };
 
-// The next rows to run the careful way, from the limit `from` on: up to a later token whose latents are not all finite.
+// The next rows to run the careful way, from the limit `from` on: up to a later token whose latents are not all finite,
+// or the first one of a page outside the pool.
 __device__ __forceinline__ Pass careful_pass(const ChunkParams& p, const Piece& pc, DMLA_LDS int* flag, int from, int lim_last) {
   const int wave = uniform(threadIdx.x >> 6);
   int to = 0x7fffffff;
   for (int j = max(from + 1, 0) + wave; j <= min(lim_last, pc.t1 * kTile - 1); j += kWaves) {
     const int page = uniform(p.block_table[pc.b * p.bt_sb + j / kPage]);
-    if (page < 0 || page >= p.num_pages) continue;
+    if (page < 0 || page >= p.num_pages) {   // page 0 stands in for it; its first token's row and all behind see it
+      if (j % kPage != 0) continue;
+      to = j;
+      break;
+    }
     const u32x4 v = *reinterpret_cast<Global<const u32x4>>(p.kv + page * p.kv_sp + j % kPage * p.kv_ss + 16 * fresh_lane_id());
     bool odd = false;
 #pragma unroll

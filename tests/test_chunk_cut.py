@@ -143,3 +143,13 @@ def test_a_careful_pass_has_no_races(watched):
     """Its waves post where they would cut in the words in which they have just read that a pass has to follow."""
     assert careful(watched, -1, 20, [0]) == 0
     assert careful(watched, 10, 90, []) == END
+
+
+@pytest.mark.parametrize("bad", [-1, 4, 2 ** 31 - 1])
+@pytest.mark.parametrize("begin,last,odd,page,to", [
+    (10, 90, [], 1, 64), (63, 90, [], 1, 64), (64, 90, [], 1, END), (70, 90, [], 1, END), (10, 90, [33], 1, 33), (33, 90, [33], 1, 64),
+    (64, 140, [], 1, END), (64, 140, [129], 1, 129), (-3, 20, [], 0, 0), (10, 60, [], 1, END), (100, 190, [], 2, 128)])
+def test_rows_are_cut_where_a_bad_page_begins(checked, bad, begin, last, odd, page, to):
+    """What stands in for its tokens reaches none of the rows before them; the rows behind its first token all see it."""
+    table = [bad if i == page else p for i, p in enumerate((3, 1, 2, 0))]
+    assert careful(checked, begin, last, odd, table) == to

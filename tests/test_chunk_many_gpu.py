@@ -294,3 +294,39 @@ def test_where_row_tiles_change_their_size(gpu, N, H, n):
     q = queries(n, H, 7)
     o, lse = run(gpu, q, pool, table, [N], [n])
     check(q, o, lse, rows, [N], [n])
+
+
+# ---- row tiles with rows before a page outside the pool and behind ---------------------------------------
+
+@pytest.mark.parametrize("H", [1, 5, 48])
+@pytest.mark.parametrize("large", [False, True])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+def test_rows_before_a_bad_page(gpu, H, large, value):
+    """Page 0 stands in for a page outside the pool: whatever it holds, rows of tokens before that page see nothing of it."""
+    lens, counts = [200, 70], [150, 9]
+    if large:
+        lens, counts = lens + [LONG], counts + [1]
+    pool, table, rows = paged(lens, gpu, seed=H)
+    pool = torch.cat([torch.full_like(pool[:1], value), pool])
+    q = queries(sum(counts), H, 8)
+    for b, page in ((0, 1), (0, 2), (1, 1)):
+        at = starts(counts)[b]
+        first = at + PAGE * page - (lens[b] - counts[b])   # the first query that attends the page
+        seen = range(first, at + counts[b])
+        for bad in (-1, pool.shape[0]):
+            t = torch.where(table < 0, table, table + 1)
+            t[b, page] = bad
+            o, lse = run(gpu, q, pool, t, lens, counts)
+            check(q, o, lse, rows, lens, counts, some=set(range(sum(counts))) - set(seen))
+            assert torch.isnan(o[first:seen[-1] + 1]).all() and torch.isnan(lse[first:seen[-1] + 1]).all()
+
+
+@pytest.mark.parametrize("H", [16, 48])
+def test_queries_without_a_token_before_a_bad_page(gpu, H):
+    """The first page is outside the pool: NaN for those that have tokens, the others have none."""
+    from python import ops
+    pool = torch.full((3, PAGE, D_QK), float("nan"), dtype=torch.bfloat16, device=gpu)
+    o, lse = ops.flash_dmla_chunk_paged(queries(9, H, 9).to(gpu), pool, ints([[3]], gpu), ints([4], gpu), ints([0, 9], gpu),
+                                        softmax_scale=SCALE, return_lse=True)
+    assert (o[:5] == 0).all() and (lse[:5] == float("-inf")).all()
+    assert torch.isnan(o[5:]).all() and torch.isnan(lse[5:]).all()
