@@ -112,7 +112,8 @@ __device__ __forceinline__ Pass careful_pass(const ChunkParams& p, const Piece& 
 // Weights are estimates in closed form, in key tiles (one of a few rows takes as long as one of 128: 32 sequences x
 // 16 heads, four of them with chunks of 460 tokens, 343 us, 506 when it weighed half).  The first n row tiles of a
 // sequence whose first query is token `base` weigh A(n) = n (c + (base + 31) / 32) + 2 n (n + 1) / H (row tile i ends
-// at token base + 128 (i + 1) / H, causal), where c is what a start and end cost.  A range's end is the next one's start
+// at token base + 128 (i + 1) / H, causal), where c is what a start and end cost; of more queries than tokens the first row
+// tiles weigh c alone, and the growth starts behind them.  A range's end is the next one's start
 // by the same arithmetic, so nothing is lost or done twice where they are off.  They are integers (of fp32 products,
 // ascending in n whatever the rounding); where the host finds that they could pass 2^30, all are taken in units of
 // 2^weight_shift.
@@ -150,20 +151,22 @@ __device__ __forceinline__ int key_tiles(const ChunkParams& p, const Sequence& s
   return (max(end, 0) + kTile - 1) / kTile;
 }
 struct Weights {
-  int cost;
-  float base, growth;   // of a row tile, and how much more each one weighs
+  int cost, none;       // none: row tiles before the first that has a token
+  float base, growth;   // of a row tile, and how much more each one behind those weighs
 };
 __device__ __forceinline__ Weights weights(const ChunkParams& p, const Sequence& s, int rows_log2) {
   const bool few = s.n * p.H <= kNarrowRows || rows_log2 == kNarrowLog2;
-  Weights w = {few ? kNarrowCost : kCost, 0.f, 0.f};
+  Weights w = {few ? kNarrowCost : kCost, 0, 0.f, 0.f};
   const int tiles = ((p.causal ? max(s.len - s.n, 0) : s.len) + kTile - 1) / kTile;
   w.base = (float)(w.cost + tiles);
+  w.none = p.causal ? max(s.n - s.len, 0) * p.H >> rows_log2 : 0;
   w.growth = !p.causal ? 0.f : rows_log2 == kNarrowLog2 ? 0.25f * p.two_by_h : p.two_by_h;
   return w;
 }
 // A(n), one more for each row tile: none is without a weight, or no range would hold it.
 __device__ __forceinline__ int weight(const ChunkParams& p, const Weights& w, int n) {
-  return n + (int)((float)n * (w.base + w.growth * (float)(n + 1)) * p.weight_scale);
+  const int m = max(n - w.none, 0);
+  return n + (int)(((float)m * (w.base + w.growth * (float)(m + 1)) + (float)(n - m) * w.base) * p.weight_scale);
 }
 // The place at weight y of sequence b.
 __device__ __forceinline__ Place place_of(const ChunkParams& p, int b, const Sequence& s, int y, int width, int rows_log2) {
@@ -328,7 +331,8 @@ __device__ __forceinline__ void next_piece(const ChunkParams& p, DMLA_LDS Window
   }
 }
 
-// At least the weight that the kernel adds up, in row tiles of `rows` rows.
+// At least the weight that the kernel adds up, in row tiles of `rows` rows (but for two a row tile, from roundings up): a
+// row tile has no more keys than the table, however many queries have no token.
 inline int64_t chunk_weight(int64_t T, int64_t B, int64_t H, int64_t max_pages, int64_t rows) {
   const int64_t tiles = T * H / rows + std::min(B, T);
   return tiles * (kCost + 3 + max_pages * (kPage / kTile));

@@ -95,6 +95,42 @@ def test_hundreds_of_sequences(checked, B, H):
     assert_all_done_once(cut_of(checked, H, lens, counts, n_ranges=3), H, lens, counts)
 
 
+@pytest.mark.parametrize("H,n,N", [(1, 1 << 22, 64), (16, 1 << 21, 1), (128, 1 << 18, 0), (1, 1 << 20, 1 << 19)])
+def test_many_more_queries_than_tokens(checked, H, n, N):
+    """The weights' sum stays within 32 bits, and ranges follow each other up to the last row."""
+    some = [0, 1, 254, 255]
+    pieces = cut_of(checked, H, [N], [n], n_ranges=256, ranges=some)
+    by_range = {r: [x for x in pieces if x[0] == r] for r in some}
+    for r in some:
+        assert by_range[r], "a range without work"
+        for x, y in zip(by_range[r], by_range[r][1:]):
+            assert y[2] == x[2] + x[3] and y[5] == 0
+    last = by_range[255][-1]
+    assert by_range[0][0][2] == 0 and last[2] + last[3] == n * H
+    for r in (0, 254):
+        x, y = by_range[r][-1], by_range[r + 1][0]
+        assert (y[2], y[5]) in ((x[2] + x[3], 0), (x[2], x[6]))
+
+
+def test_the_hosts_bound_of_the_weight(checked):
+    """In units of 2^shift the sum stays within 32 bits whatever the lengths; ascending with the row tiles."""
+    r = random.Random(5)
+    lines, bounds = [], []
+    for _ in range(400):
+        H, B = r.choice([1, 2, 5, 16, 128, 300, 1 << 16]), r.choice([1, 2, 7])
+        pages = int(2 ** r.uniform(0, 20))
+        T = int(2 ** r.uniform(0, 30 - (H - 1).bit_length()))
+        at = sorted(r.randint(0, T) for _ in range(B - 1))
+        cu = [0, *at, T]
+        lens = [r.choice([0, 1, 64 * pages, r.randint(0, 64 * pages), min(64 * pages, cu[i + 1] - cu[i])]) for i in range(B)]
+        lines.append(["weight", T, B, H, pages, r.choice([0, 1]), *lens, *cu])
+        bounds.append((T * H // ROWS + min(B, T)) * (10 + 2 * pages))
+    for line, bound, (total, shift, ascending) in zip(lines, bounds, ask(checked, *lines)):
+        assert ascending, line
+        row_tiles = line[1] * line[3] // ROWS + line[2]
+        assert total <= min((bound >> shift) + 2 * row_tiles + 1, 2 ** 31 - 1), line
+
+
 # ---- what waves read and write between barriers --------------------------------------------------------
 
 @pytest.fixture(scope="module")

@@ -330,3 +330,19 @@ def test_queries_without_a_token_before_a_bad_page(gpu, H):
                                         softmax_scale=SCALE, return_lse=True)
     assert (o[:5] == 0).all() and (lse[:5] == float("-inf")).all()
     assert torch.isnan(o[5:]).all() and torch.isnan(lse[5:]).all()
+
+
+@pytest.mark.parametrize("H,n", [(1, 1 << 22), (16, 70000)])
+def test_many_more_queries_than_tokens(gpu, H, n):
+    """Millions of queries without a token before the few that have one, and an ordinary sequence behind them."""
+    from python import ops
+    lens, counts = [50, 400], [n, 30]
+    pool, table, rows = paged(lens, gpu)
+    q = queries(80, H, 10)
+    few = torch.zeros(1, 1, D_QK, dtype=torch.bfloat16, device=gpu).expand(n - 50, H, D_QK)
+    all_q = torch.cat([few, q.to(gpu)])
+    stale = torch.full((sum(counts), H, D_V), float("nan"), dtype=torch.bfloat16, device=gpu)   # what the output's memory may hold
+    del stale
+    o, lse = ops.flash_dmla_chunk_paged(all_q, pool, table, ints(lens, gpu), ints(starts(counts), gpu), softmax_scale=SCALE, return_lse=True)
+    assert (o[:n - 50] == 0).all() and (lse[:n - 50] == float("-inf")).all()
+    check(q, o[n - 50:], lse[n - 50:], rows, lens, [50, 30])
