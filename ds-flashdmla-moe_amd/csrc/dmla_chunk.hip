@@ -27,7 +27,7 @@
 //  * Short rows of keys by what a piece costs beside its tiles, 9 us: 3 us of queries through LDS (their copies, the
 //    first tile, the last tile's values) and 4 us of outputs, both at what a CU's vector memory path takes (some 27
 //    bytes a cycle).  Four prompts of 200 to 2000 tokens x 128 heads: 837 us, 1.04 PFLOP/s.
-//  * One token by latency: the cut, queries, tiles, the join: 27 us for 5000 tokens x 128 heads.
+//  * One token by latency: the cut, queries, tiles, the join: 26 us for 5000 tokens x 128 heads.
 #include <algorithm>
 #include <cmath>
 

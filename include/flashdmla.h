@@ -400,7 +400,7 @@ int dmla_kv_append_rows_q4(void* kv_pool, const int32_t* slots, const void* rows
  * attends a page outside [0, num_pages) NaN.  What a query does not attend does not reach it, whatever it holds.
  * Probabilities enter the value product as bf16, sums stay in fp32.
  * The workspace (16-byte aligned, contents ignored) is of dmla_chunk_paged_workspace_bytes of the same sizes on the
- * current device.  Supported: d_qk = 576, d_v = 512, T * H <= 2^30.
+ * current device: 525 KB for each CU that the call may use, 134 MB on 256 CUs for all but the smallest sizes.  Supported: d_qk = 576, d_v = 512, T * H <= 2^30.
  */
 int64_t dmla_chunk_paged_workspace_bytes(int64_t T, int64_t B, int64_t H, int64_t max_pages_per_seq);
 int dmla_chunk_paged(const void* q, const void* kv_pool, const int32_t* block_table, const int32_t* cache_seqlens,

@@ -33,7 +33,7 @@ def checked(tmp_path_factory):
 def ask(exe, *lines):
     env = dict(os.environ, TSAN_OPTIONS="halt_on_error=1")
     run = subprocess.run([exe], env=env, input="\n".join(" ".join(str(x) for x in line) for line in lines) + "\n", capture_output=True,
-                         text=True, timeout=60)
+                         text=True, timeout=120)
     assert run.returncode == 0, run.stderr[-3000:]
     return [[int(x) for x in line.split()] for line in run.stdout.splitlines()]
 
